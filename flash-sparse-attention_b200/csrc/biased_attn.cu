@@ -1,0 +1,225 @@
+// Attention with changed scores (capped by a tanh, biased by distance) under causal, window, document and prefix masks, packed
+// sequences: the limits of every token and the entry points.  The kernels are those of range attention (range_dense.cu,
+// range_bwd_dkdv.cu) compiled for changed scores: under each of these masks a token sees one stretch of K/V rows.
+#include "../../include/fsa_sm100.h"
+
+#include "range_bwd.cuh"
+#include "range_fwd.cuh"
+
+namespace fsa {
+
+int make_tile_map(CUtensorMap* map, const void* base, int dtype, int64_t rows, int64_t cols, int64_t row_stride, int box_rows);
+int make_tile_map_3d_box(CUtensorMap* map, const void* base, int dtype, int64_t d0, int64_t d1, int64_t d2, int64_t stride1,
+                         int64_t stride2, int box1, int box2);
+int cuda_failed(cudaError_t e);
+
+// What the forward leaves for the backward: a status word, and for every token the first and last K/V row that it sees and its own place.
+struct BiasedLimits {
+    int *status, *lo, *hi, *pos;
+    BiasedLimits(void* ws, int64_t N) : status((int*)ws), lo(status + 16), hi(lo + N), pos(hi + N) {}
+    static int64_t bytes(int64_t N) { return (16 + 3 * N) * 4; }
+};
+
+constexpr int kLimThreads = 256;
+
+// Last row j <= row of [first, row] that begins a document: whose id differs from that of the row before, or `first` itself.  All lanes of a
+// warp call it; 512 ids a step (one load is as long on its way as sixteen).
+__device__ __forceinline__ int document_start(const int32_t* __restrict__ ids, int first, int row, int lane) {
+    const int id = __ldg(ids + row);
+    for (int end = row; end > first; end -= 512) {      // rows [end - 512, end) are looked at
+        int found = -1;                                 // last row of another document among them
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            const int j = end - 1 - (i * 32 + lane);
+            if (j >= first && __ldg(ids + j) != id) found = max(found, j);
+        }
+        found = __reduce_max_sync(0xffffffffu, found);
+        if (found >= 0) return found + 1;
+    }
+    return first;
+}
+
+// One thread per token.  Tokens of one sequence stand at consecutive K/V rows, the last of them at the sequence's last row.  Documents: a token
+// whose row does not begin one sees from where the token before it does, so a warp scans its tokens and searches only for those
+// that no such token precedes in it.  Rows behind the last sequence become zeros (lse: -inf).
+__global__ void __launch_bounds__(kLimThreads) biased_limits(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
+                                                             const int32_t* __restrict__ doc_ids, const int32_t* __restrict__ prefix_lens, int B, int64_t N,
+                                                             int window, int Hq, int D, BiasedLimits out, uint4* __restrict__ o, float* __restrict__ lse) {
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int64_t n0 = (int64_t)blockIdx.x * kLimThreads, n = n0 + tid;
+    if (n == 0) *out.status = kStatusOk;
+    const int used = __ldg(cu_q + B);
+    int lo = 0, hi = -1, pos = 0, seq = -1;
+    if (n < used && n < N) {
+        seq = find_seq(cu_q, B, (int)n);
+        const int k0 = __ldg(cu_k + seq), k1 = __ldg(cu_k + seq + 1);
+        pos = (int)n + k1 - __ldg(cu_q + seq + 1);
+        if (pos >= k0) {            // (else the sequence has fewer keys than queries, and this one precedes them)
+            lo = window >= 0 ? max(k0, pos - window) : k0;
+            hi = prefix_lens ? max(pos, min(k0 + __ldg(prefix_lens + seq), k1) - 1) : pos;
+        }
+    }
+    if (doc_ids) {
+        const bool in = hi >= 0;
+        const int k0 = in ? __ldg(cu_k + seq) : 0, id = in ? __ldg(doc_ids + pos) : -1;
+        const bool begins = !in || pos == k0 || __ldg(doc_ids + pos - 1) != id;
+        const int seq_before = __shfl_up_sync(0xffffffffu, seq, 1);
+        int start = begins ? pos : -1;                  // of the document, where it is known
+        const bool head = lane == 0 || seq_before != seq;
+        for (unsigned todo = __ballot_sync(0xffffffffu, head && !begins); todo; todo &= todo - 1) {
+            const int src = __ffs(todo) - 1;
+            const int found = document_start(doc_ids, __shfl_sync(0xffffffffu, k0, src), __shfl_sync(0xffffffffu, pos, src), lane);
+            if (lane == src) start = found;
+        }
+        // the nearest lane at or below this one that knows
+        const unsigned known = __ballot_sync(0xffffffffu, start >= 0) & (0xffffffffu >> (31 - lane));
+        start = __shfl_sync(0xffffffffu, start, known ? 31 - __clz(known) : lane);
+        if (in) {
+            if (id < 0) hi = -1;
+            else lo = max(lo, start);
+        }
+    }
+    if (n < N) {
+        out.lo[n] = hi >= 0 ? lo : 0;
+        out.hi[n] = hi;
+        out.pos[n] = pos;
+    }
+    const int64_t tail = max(n0, (int64_t)used), end = min(n0 + kLimThreads, N), chunks = (int64_t)Hq * D / 8;
+    for (int64_t i = tail * chunks + tid; i < end * chunks; i += kLimThreads) o[i] = make_uint4(0u, 0u, 0u, 0u);
+    if (n >= tail && n < N)
+        for (int h = 0; h < Hq; ++h) lse[(int64_t)h * N + n] = -INFINITY;
+}
+
+static int biased_shape(int64_t N, int64_t Nk, int B, int Hq, int Hk, int D, SelShape* s) {
+    if (N < 0 || Nk < 0 || B < 1 || Hq <= 0 || Hk <= 0 || Hq % Hk) return FSA_ERR_BAD_ARG;
+    if ((D != 64 && D != 128) || Hq / Hk > 32 || Hk > 65535 || N >= kMaxTokens || Nk >= kMaxTokens || B >= kMaxTokens ||
+        N * Hq >= ((int64_t)1 << 31)) return FSA_ERR_UNSUPPORTED;
+    *s = SelShape{};
+    s->N = N; s->Nk = Nk; s->B = B; s->Hq = Hq; s->Hk = Hk; s->G = Hq / Hk; s->D = D;
+    s->TPT = (kTileRows / s->G) & ~3;
+    return FSA_OK;
+}
+
+static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
+
+static int biased_mod(float sm_scale, float softcap, const float* slopes, const int32_t* doc_ids, int ahead, ScoreMod* m, int* which) {
+    if (!(sm_scale > 0.f) || !(softcap >= 0.f)) return FSA_ERR_BAD_ARG;
+    *which = (softcap > 0.f ? kModCap : 0) | (slopes ? kModBias : 0);
+    *m = ScoreMod{};
+    if (softcap > 0.f) { m->x_scale = sm_scale / softcap; m->cap_log2 = softcap * kLog2e; }
+    m->slopes = slopes; m->key_ids = doc_ids; m->ahead = ahead;
+    return FSA_OK;
+}
+
+}  // namespace fsa
+
+using namespace fsa;
+
+extern "C" int fsa_biased_attn_limits_bytes(int64_t N, int64_t* bytes_out) {
+    if (!bytes_out || N < 0) return FSA_ERR_BAD_ARG;
+    *bytes_out = BiasedLimits::bytes(N);
+    return FSA_OK;
+}
+
+extern "C" int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                                   const int32_t* doc_ids, const int32_t* prefix_lens, const float* slopes, int64_t N, int64_t Nk, int B, int Hq, int Hk,
+                                   int D, int dtype, int64_t q_sn, int64_t q_sh, int64_t k_sn, int64_t v_sn, float sm_scale, float softcap, int window,
+                                   void* o, float* lse, void* limits, int64_t limits_bytes, void* stream_) {
+    SelShape s;
+    int rc = biased_shape(N, Nk, B, Hq, Hk, D, &s);
+    if (rc) return rc;
+    if (dtype != FSA_DTYPE_BF16 && dtype != FSA_DTYPE_FP16) return FSA_ERR_BAD_ARG;
+    // under these pairs a token would not see one stretch of rows
+    if (prefix_lens && (window >= 0 || doc_ids)) return FSA_ERR_UNSUPPORTED;
+    RangeDenseLaunch l = {};
+    int which;
+    if ((rc = biased_mod(sm_scale, softcap, slopes, doc_ids, prefix_lens != nullptr, &l.mod, &which))) return rc;
+    if (N == 0) return FSA_OK;
+    if (!q || !k || !v || !cu_seqlens_q || !cu_seqlens_k || !o || !lse || !limits || Nk == 0) return FSA_ERR_BAD_ARG;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(limits)) return FSA_ERR_BAD_ARG;
+    if ((q_sn % 8) || (q_sh % 8) || (k_sn % 8) || (v_sn % 8) || k_sn < (int64_t)Hk * D || v_sn < (int64_t)Hk * D) return FSA_ERR_BAD_ARG;
+    if (limits_bytes < BiasedLimits::bytes(N)) return FSA_ERR_WORKSPACE;
+    (void)cudaGetLastError();
+    if ((rc = ensure_context())) return rc;
+    if ((rc = make_tile_map_3d_box(&l.q[0], q, dtype, D, N, Hq, q_sn, q_sh, s.TPT, s.G))) return rc;
+    if ((rc = make_tile_map_3d_box(&l.o[0], o, dtype, D, N, Hq, (int64_t)Hq * D, D, s.TPT, s.G))) return rc;
+    if ((rc = make_tile_map(&l.k[0], k, dtype, Nk, (int64_t)Hk * D, k_sn, 64))) return rc;
+    if ((rc = make_tile_map(&l.v[0], v, dtype, Nk, (int64_t)Hk * D, v_sn, 64))) return rc;
+    cudaStream_t stream = (cudaStream_t)stream_;
+    const BiasedLimits lim(limits, N);
+    biased_limits<<<(unsigned)((N + kLimThreads - 1) / kLimThreads), kLimThreads, 0, stream>>>(cu_seqlens_q, cu_seqlens_k, doc_ids, prefix_lens, B, N, window,
+                                                                                            Hq, D, lim, (uint4*)o, lse);
+    cudaError_t e = cudaGetLastError();
+    if (e != cudaSuccess) return cuda_failed(e);
+    l.mod.pos = lim.pos;
+    RangeDenseParams& p = l.p[0];
+    p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.kv_lo = lim.lo; p.kv_hi = lim.hi;
+    p.N = N; p.Nk = Nk; p.B = B; p.Hq = Hq; p.Hk = Hk; p.G = s.G; p.TPT = s.TPT;
+    p.scale_log2 = sm_scale * kLog2e;
+    p.o = o; p.o_sn = (int64_t)Hq * D; p.o_sh = D; p.lse = lse; p.status = lim.status;
+    e = launch_range_fwd_mod(D, dtype, which, l, (int)((N + s.TPT - 1) / s.TPT) + B, stream);
+    return e == cudaSuccess ? FSA_OK : cuda_failed(e);
+}
+
+extern "C" int fsa_biased_attn_bwd_bytes(int64_t N, int64_t Nk, int B, int Hq, int Hk, int D, int64_t* bytes_out) {
+    SelShape s;
+    const int rc = biased_shape(N, Nk, B, Hq, Hk, D, &s);
+    if (rc) return rc;
+    if (!bytes_out) return FSA_ERR_BAD_ARG;
+    *bytes_out = align_up(N * Hq * 4, 1024) + align_up(range_kv_plan_bytes(s), 1024) + range_kv_slab_bytes(s);
+    return FSA_OK;
+}
+
+extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o,
+                                   const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* doc_ids, int has_prefix, const float* slopes,
+                                   int64_t N, int64_t Nk, int B, int Hq, int Hk, int D, int dtype, int64_t q_sn, int64_t q_sh, int64_t k_sn, int64_t v_sn,
+                                   int64_t do_sn, int64_t do_sh, float sm_scale, float softcap, void* dq, void* dk, void* dv, void* limits,
+                                   int64_t limits_bytes, void* scratch, int64_t scratch_bytes, void* stream_) {
+    SelShape s;
+    int rc = biased_shape(N, Nk, B, Hq, Hk, D, &s);
+    if (rc) return rc;
+    if (dtype != FSA_DTYPE_BF16 && dtype != FSA_DTYPE_FP16) return FSA_ERR_BAD_ARG;
+    ScoreMod mod;
+    int which;
+    if ((rc = biased_mod(sm_scale, softcap, slopes, doc_ids, has_prefix, &mod, &which))) return rc;
+    if (N == 0) return FSA_OK;
+    if (!q || !k || !v || !o || !lse || !d_o || !cu_seqlens_q || !cu_seqlens_k || !dq || !dk || !dv || !limits || !scratch || Nk == 0) return FSA_ERR_BAD_ARG;
+    for (const void* x : {q, k, v, o, d_o, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)limits, (const void*)scratch})
+        if (!aligned16(x)) return FSA_ERR_BAD_ARG;
+    if ((q_sn % 8) || (q_sh % 8) || (k_sn % 8) || (v_sn % 8) || (do_sn % 8) || (do_sh % 8) || k_sn < (int64_t)Hk * D || v_sn < (int64_t)Hk * D) return FSA_ERR_BAD_ARG;
+    int64_t need = 0;
+    if ((rc = fsa_biased_attn_bwd_bytes(N, Nk, B, Hq, Hk, D, &need))) return rc;
+    if (limits_bytes < BiasedLimits::bytes(N) || scratch_bytes < need) return FSA_ERR_WORKSPACE;
+    (void)cudaGetLastError();
+    if ((rc = ensure_context())) return rc;
+    CUtensorMap kmap, vmap;
+    if ((rc = make_tile_map(&kmap, k, dtype, Nk, (int64_t)Hk * D, k_sn, 64))) return rc;
+    if ((rc = make_tile_map(&vmap, v, dtype, Nk, (int64_t)Hk * D, v_sn, 64))) return rc;
+    cudaStream_t stream = (cudaStream_t)stream_;
+    const BiasedLimits lim(limits, N);
+    mod.pos = lim.pos;
+    char* sp = (char*)scratch;
+    SelBwdArgs a = {};
+    a.q = q; a.d_o = d_o; a.o = o;
+    a.q_sn = q_sn; a.q_sh = q_sh; a.do_sn = do_sn; a.do_sh = do_sh; a.o_sn = (int64_t)Hq * D; a.o_sh = D;
+    a.lse = lse; a.cu = cu_seqlens_q; a.sm_scale = sm_scale;
+    a.delta = (float*)sp;           sp += align_up(N * Hq * 4, 1024);
+    a.bd = SelBounds{cu_seqlens_k, lim.lo, lim.hi};
+    a.dq = dq; a.dk = dk; a.dv = dv;
+    RangeKvPlan plan = {};
+    plan.cu_q = cu_seqlens_q; plan.cu_k = cu_seqlens_k; plan.kv_lo = lim.lo; plan.kv_hi = lim.hi;
+    plan.N = N; plan.Nk = Nk; plan.B = B; plan.Hk = Hk; plan.TPT = s.TPT; plan.aim = range_kv_items();
+    plan.max_tiles = (int)range_kv_max_tiles(s);
+    plan.D = D; plan.Hq = Hq; plan.dq = (uint4*)dq;
+    plan.counts = (int*)sp;
+    plan.tiles = (int4*)(sp + 256);
+    plan.multi = plan.tiles + plan.max_tiles;
+    plan.items = plan.multi + plan.max_tiles;
+    sp += align_up(range_kv_plan_bytes(s), 1024);
+    a.slabs = (float*)sp;
+    cudaError_t e = launch_range_bwd_plan(plan, a, lim.status, stream);
+    if (e == cudaSuccess) e = launch_sel_bwd_delta(dtype, a, s, stream);
+    if (e == cudaSuccess) e = launch_range_bwd_dq(dtype, a, s, kmap, vmap, lim.status, stream, &mod, which);
+    if (e == cudaSuccess) e = launch_range_bwd_dkdv(dtype, plan, a, s, kmap, vmap, lim.status, stream, &mod, which);
+    return e == cudaSuccess ? FSA_OK : cuda_failed(e);
+}

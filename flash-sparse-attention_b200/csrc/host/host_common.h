@@ -69,5 +69,6 @@ void check_status(const void* word, const Tensor& like, const char* what);
 void bind_sel(pybind11::module& m);
 void bind_decode(pybind11::module& m);
 void bind_layer(pybind11::module& m);
+void bind_biased(pybind11::module& m);
 
 }  // namespace fsa_host

@@ -1,5 +1,6 @@
 // Shared by the range-attention backward's kernels (range_bwd_dkdv.cu) and their callers (fsa_api.cu, sel_bwd.cu).
 #pragma once
+#include "score.cuh"
 #include "sel_launch.cuh"
 
 namespace fsa {
@@ -14,6 +15,9 @@ struct RangeKvPlan {
     const int32_t* kv_hi;
     int64_t N, Nk;
     int B, Hk, TPT, max_tiles;
+    int D;
+    uint4* dq;          // rows behind the last sequence are zeroed here (or null)
+    int Hq;
     int aim;            // range_kv_items()
     int* counts;        // [0] items, [1] tiles cut into several items
     int4* tiles;        // [max_tiles] first K/V row, rows, first and last token that see one of them
@@ -29,10 +33,10 @@ inline int64_t range_kv_max_cut(const SelShape& s) {
     return a < b ? a : b;
 }
 inline int64_t range_kv_plan_bytes(const SelShape& s) { return 256 + 16 * (3 * range_kv_max_tiles(s) + range_kv_max_cut(s)); }
-inline int64_t range_kv_slab_bytes(const SelShape& s) { return range_kv_max_cut(s) * s.Hk * (2 * 128 * 128 * 4); }
+inline int64_t range_kv_slab_bytes(const SelShape& s) { return range_kv_max_cut(s) * s.Hk * (2 * 128 * (int64_t)s.D * 4); }
 
 cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream);
 cudaError_t launch_range_bwd_dkdv(int dtype, const RangeKvPlan& p, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap,
-                                  const CUtensorMap& vmap, int* status, cudaStream_t stream);
+                                  const CUtensorMap& vmap, int* status, cudaStream_t stream, const ScoreMod* mod = nullptr, int which = 0);
 
 }  // namespace fsa

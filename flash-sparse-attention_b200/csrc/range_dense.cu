@@ -22,7 +22,8 @@
 #include "../../include/fsa_sm100.h"
 #include <climits>
 
-#include "sel_launch.cuh"
+#include "range_bwd.cuh"
+#include "range_fwd.cuh"
 
 namespace fsa {
 
@@ -31,47 +32,30 @@ int make_tile_map_3d_box(CUtensorMap* map, const void* base, int dtype, int64_t 
                          int64_t stride2, int box1, int box2);
 int device_sm_count(int* out);
 
-struct RangeDenseParams {
-    const int32_t* cu_q;    // [B + 1]
-    const int32_t* cu_k;    // [B + 1] first K/V row of every sequence
-    const int32_t* kv_lo;   // [N] lowest visible K/V row of every token, or null (the sequence's first row)
-    const int32_t* kv_hi;   // [N] highest visible K/V row, lower than kv_lo when the token sees nothing
-    int64_t N, Nk;
-    int B, Hq, Hk, G, TPT;
-    float scale_log2;
-    void* o;  int64_t o_sn, o_sh;     // [N, Hq, D]
-    float* lse;                       // [Hq, N] log2 units
-    int* status;
-};
-
-// Up to three problems in one launch (blockIdx.z): branches of a layer that do not wait for one another.  A short prompt has fewer tiles
-// than the SMs hold CTAs, and each launch of its own left most of them empty (517 tokens, 32 / 8 heads: 3 x 11 us, together 19: prefill 158 -> 138 us).
-constexpr int kRdProblems = 3;
-struct RangeDenseLaunch {
-    CUtensorMap q[kRdProblems], k[kRdProblems], v[kRdProblems], o[kRdProblems];
-    RangeDenseParams p[kRdProblems];
-};
-
 constexpr int kRdThreads = 192;
 constexpr int kRdBK = 64;
 constexpr float kRdLazy = 8.0f;       // raise a row's reference max only when exceeded by more than this (log2 units)
 
-__device__ __forceinline__ float rd_ex2(float x) {
-    float y;
-    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-    return y;
-}
-
 // One item: a tile of tokens x one KV head of problem z.
 struct RdItem {
-    int z, h, seq, tok0, ne, row_lo, nblk;
+    int z, h, seq, tok0, ne, row_lo, nblk, row_hi;     // row_hi: last K/V row that a row of the item sees
 };
 
 // The K/V rows that a row of the item sees: [x, y].
+template <int MOD>
 __device__ __forceinline__ int2 rd_row(const RangeDenseLaunch& launch, const RdItem& m, bool valid, int e) {
     if (m.z < 0 || !valid) return make_int2(0, -1);
-    const RangeDenseParams& p = launch.p[m.z];
+    const RangeDenseParams& p = launch.p[(MOD & kModSplit) ? 0 : m.z];
     return make_int2(p.kv_lo ? __ldg(p.kv_lo + m.tok0 + e) : __ldg(p.cu_k + m.seq), __ldg(p.kv_hi + m.tok0 + e));
+}
+
+// kModBias: the slope of the row's head (log2 units) and its token's place as a K/V row.
+template <int MOD>
+__device__ __forceinline__ void rd_bias(const RangeDenseLaunch& launch, const RdItem& m, bool valid, int g, int e, float& slope, int& pos) {
+    slope = 0.f; pos = 0;
+    if (!(MOD & kModBias) || m.z < 0 || !valid) return;
+    slope = __ldg(launch.mod.slopes + m.h * launch.p[0].G + g) * kLog2e;
+    pos = __ldg(launch.mod.pos + m.tok0 + e);
 }
 
 // Takes over a CTA of this launch that has not started yet (cluster launch control): 16 bytes of answer at dst, with bar as the
@@ -94,7 +78,8 @@ __device__ __forceinline__ bool claimed_cta(uint32_t src, int& x, int& y, int& z
     return yes != 0;
 }
 
-template <int D, typename ET>
+// MOD (score.cuh): changed scores, rows that nobody sees, chunks of K/V rows with partial results.
+template <int D, int MOD, typename ET>
 __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_constant__ RangeDenseLaunch launch) {
     constexpr int BK = kRdBK;
     constexpr int kQ = kTileRows * D * 2;
@@ -129,7 +114,8 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
     int* status = reinterpret_cast<int*>(bars + 30) + 1;     // of this CTA
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const uint32_t limit = wait_limit(launch.p[blockIdx.z].status);
+    constexpr bool kSplit = (MOD & kModSplit) != 0;
+    const uint32_t limit = wait_limit(launch.p[kSplit ? 0 : blockIdx.z].status);
     const int G = launch.p[0].G, TPT = launch.p[0].TPT;      // (the same for all problems)
     if (tid == 0) {
         *status = kStatusOk;
@@ -153,7 +139,7 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
         const int4 x = s_item[(n & 1) * 2], y = s_item[(n & 1) * 2 + 1];
         RdItem m;
         m.z = x.x; m.h = x.y; m.seq = x.z; m.tok0 = x.w;
-        m.ne = y.x; m.row_lo = y.y; m.nblk = y.z;
+        m.ne = y.x; m.row_lo = y.y; m.nblk = y.z; m.row_hi = y.w;
         return m;
     };
     auto take_item = [&](int n, bool& ok) {
@@ -171,7 +157,7 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
         int n = 0, claims = 0, qi = 0, c = 0;           // items, claims, non-empty items, K/V tiles so far
         int bx = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
         while (ok) {
-            const RangeDenseParams& p = launch.p[z];
+            const RangeDenseParams& p = launch.p[kSplit ? 0 : z];
             bool asked = false;
             auto ask = [&]() {
                 mbar_expect_tx(claim, 16);
@@ -198,23 +184,29 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 }
                 lo = max(lo, 0);
                 hi = min(hi, (int)p.Nk - 1);
-                const int nblk = hi >= lo ? (hi - lo) / BK + 1 : 0;
+                int nblk = hi >= lo ? (hi - lo) / BK + 1 : 0;
+                if constexpr (kSplit) {
+                    const int per = (nblk + launch.nchunk - 1) / launch.nchunk, b0 = min(z * per, nblk);
+                    nblk = min(per, nblk - b0);
+                    lo += b0 * BK;
+                    hi = min(hi, lo + nblk * BK - 1);
+                }
                 if (n > 0) ok = ok && mbar_wait(it_empty, (n - 1) & 1, status, limit);
                 ok = warp_ok(ok);
                 if (ok && lane == 0) {
                     s_item[(n & 1) * 2] = make_int4(z, h, seq, tok0);
-                    s_item[(n & 1) * 2 + 1] = make_int4(ne, lo, nblk, 0);
+                    s_item[(n & 1) * 2 + 1] = make_int4(ne, lo, nblk, hi);
                     mbar_arrive(it_full);
                 }
                 ++n;
                 if (lane == 0 && nblk > 0) {
-                    const CUtensorMap *kmap = &launch.k[z], *vmap = &launch.v[z];
+                    const CUtensorMap *kmap = &launch.k[kSplit ? 0 : z], *vmap = &launch.v[kSplit ? 0 : z];
                     ok = ok && mbar_wait(q_empty, (qi & 1) ^ 1, status, limit);
                     ask();                  // not earlier: a CTA is to be one item ahead, not to take the share of others
                     if (ok) {
                         mbar_expect_tx(q_full, (uint32_t)(KH * 128 * TPT * G));
 #pragma unroll
-                        for (int b = 0; b < KH; ++b) tma_load_3d(smem_u32(sQ + b * (kTileRows * 128)), &launch.q[z], b * 64, tok0, h * G, q_full);
+                        for (int b = 0; b < KH; ++b) tma_load_3d(smem_u32(sQ + b * (kTileRows * 128)), &launch.q[kSplit ? 0 : z], b * 64, tok0, h * G, q_full);
                     }
                     // K tile j and V tile j are loaded in the order the MMA warp needs them: K(0), K(1), V(0), K(2), V(1), ...
                     for (int step = 0; step < nblk + 1 && ok; ++step) {
@@ -327,11 +319,17 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
         bool ok = true;
         int n = 0, c = 0;
         RdItem m = take_item(n, ok);
-        int2 sees = rd_row(launch, m, g < G && e < m.ne, e);
+        int2 sees = rd_row<MOD>(launch, m, g < G && e < m.ne, e);
+        float slope;
+        int pos;
+        rd_bias<MOD>(launch, m, g < G && e < m.ne, g, e, slope, pos);
         // (the four warps leave the loop together: they meet at barriers in it)
         for (ok = bar_all(1, 128, ok); ok && m.z >= 0;) {
-            const float scale_log2 = launch.p[0].scale_log2;                 // (the same for all problems)
-            const int lo_r = sees.x - m.row_lo, hi_r = min(sees.y, (int)launch.p[m.z].Nk - 1) - m.row_lo;      // rows past the end of K/V do not exist
+            // from what the loop below has in v to log2 units (the same for all problems)
+            const float scale_log2 = (MOD & kModBias) ? 1.f : (MOD & kModCap) ? launch.mod.cap_log2 : launch.p[0].scale_log2;
+            const int lo_r = sees.x - m.row_lo, hi_r = min(sees.y, (int)launch.p[kSplit ? 0 : m.z].Nk - 1) - m.row_lo;      // rows past the end of K/V do not exist
+            const float slope_r = slope;
+            const int pos_r = pos - m.row_lo;
             const int nblk = m.nblk;
             float m_ref = -INFINITY, l_run = 0.f;
             for (int j = 0; j < nblk; ++j, ++c) {          // (left by all lanes at the vote below)
@@ -343,6 +341,10 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 tmem_ld32(tbase + lane_off + cS + st * BK, *reinterpret_cast<uint32_t (*)[32]>(&v[0]));
                 tmem_ld32(tbase + lane_off + cS + st * BK + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
                 tmem_ld_wait();
+                if constexpr (MOD & kModCap) cap_scores(v, launch.mod.x_scale);
+                if constexpr (MOD & kModBias)
+                    bias_scores(v, (MOD & kModCap) ? launch.mod.cap_log2 : launch.p[0].scale_log2, slope_r, (float)(pos_r - j * BK),
+                                launch.mod.ahead && __any_sync(0xffffffffu, j * BK + c_hi - 1 > pos_r));
                 if (c_lo > 0 || c_hi < BK) {
                     // bit i: column i is seen
                     const int v_hi = max(c_hi, 0), v_lo = min(c_lo, BK);
@@ -365,7 +367,7 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 float alpha = 1.f;
                 const bool raise = m_blk > m_ref + kRdLazy;     // false when m_blk is -inf; true when m_ref is -inf and m_blk finite
                 if (raise) {
-                    alpha = m_ref == -INFINITY ? 0.f : rd_ex2(m_ref - m_blk);
+                    alpha = m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - m_blk);
                     m_ref = m_blk;
                 }
                 // accumulator rows already hold products (j > 0): rescale them when any row of the warp changes reference
@@ -390,10 +392,10 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 uint32_t pk[BK / 2];
 #pragma unroll
                 for (int i = 0; i < BK; i += 4) {
-                    const float p0 = rd_ex2(fmaf(__uint_as_float(v[i]), scale_log2, -m_use));
-                    const float p1 = rd_ex2(fmaf(__uint_as_float(v[i + 1]), scale_log2, -m_use));
-                    const float p2 = rd_ex2(fmaf(__uint_as_float(v[i + 2]), scale_log2, -m_use));
-                    const float p3 = rd_ex2(fmaf(__uint_as_float(v[i + 3]), scale_log2, -m_use));
+                    const float p0 = ex2_approx(fmaf(__uint_as_float(v[i]), scale_log2, -m_use));
+                    const float p1 = ex2_approx(fmaf(__uint_as_float(v[i + 1]), scale_log2, -m_use));
+                    const float p2 = ex2_approx(fmaf(__uint_as_float(v[i + 2]), scale_log2, -m_use));
+                    const float p3 = ex2_approx(fmaf(__uint_as_float(v[i + 3]), scale_log2, -m_use));
                     ls[0] += p0; ls[1] += p1; ls[2] += p2; ls[3] += p3;
                     pk[i >> 1] = ElemTraits<ET>::pack2(p0, p1);
                     pk[(i >> 1) + 1] = ElemTraits<ET>::pack2(p2, p3);
@@ -401,22 +403,62 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
                 tmem_st32(tbase + lane_off + cS + st * BK, *reinterpret_cast<uint32_t (*)[32]>(&pk[0]));
                 tmem_st_wait();
+                if constexpr (MOD & kModGuard) {
+                    // V rows that no row of the item sees are multiplied by p = 0, but 0 x NaN is NaN: zeros take their place.  Every thread
+                    // has half of one of the 64 rows.
+                    const int row = m.row_lo + j * BK + (r & (BK - 1));
+                    const bool unseen = row > m.row_hi || (launch.mod.key_ids && __ldg(launch.mod.key_ids + row) < 0);
+                    if (__any_sync(0xffffffffu, unseen)) {
+                        ok = ok && mbar_wait(&v_full[st], (c >> 1) & 1, status, limit);
+                        if (unseen && ok)
+#pragma unroll
+                            for (int i = 0; i < D / 16; ++i) {
+                                const int chunk = (r >> 6) * (D / 16) + i;
+                                *reinterpret_cast<uint4*>(sV + st * kKt + (chunk >> 3) * (BK * 128) + sw128_chunk_off(r & (BK - 1), chunk & 7)) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                            }
+                        fence_async_smem();
+                    }
+                }
                 tc_fence_before();
                 mbar_arrive(&p_full[st]);
             }
             m = read_item(n);
-            const RangeDenseParams& p = launch.p[m.z];
+            const RangeDenseParams& p = launch.p[kSplit ? 0 : m.z];
             const bool row_valid = g < G && e < m.ne;
             const int tok = m.tok0 + e;
             // the next item's numbers arrive under this item's epilogue
             const RdItem next = take_item(++n, ok);
-            sees = rd_row(launch, next, g < G && e < next.ne, e);
+            sees = rd_row<MOD>(launch, next, g < G && e < next.ne, e);
+            rd_bias<MOD>(launch, next, g < G && e < next.ne, g, e, slope, pos);
             // ---- epilogue
             if (m.nblk > 0) {
                 ok = ok && mbar_wait(&pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1, status, limit);
                 tc_fence_after();
             }
             ok = bar_all(1, 128, ok);
+            if constexpr (kSplit) {
+                const int64_t part = ((int64_t)tok * p.Hq + m.h * G + g) * launch.P + m.z;
+                const bool some = m.nblk > 0 && l_run > 0.f;
+                if (row_valid && ok) launch.ml[part] = some ? make_float2(m_ref, l_run) : make_float2(-INFINITY, 0.f);
+#pragma unroll
+                for (int c0 = 0; c0 < D; c0 += 32) {
+                    uint32_t a[32];
+                    if (m.nblk == 0) break;
+                    tmem_ld32(tbase + lane_off + cO + c0, a);
+                    tmem_ld_wait();
+                    if (c0 + 32 == D) {
+                        tc_fence_before();
+                        mbar_arrive(o_free);            // the accumulator may take the next item
+                    }
+                    if (row_valid && some && ok)
+#pragma unroll
+                        for (int i = 0; i < 32; i += 4)
+                            *reinterpret_cast<uint4*>(launch.o_part + part * D + c0 + i) = make_uint4(a[i], a[i + 1], a[i + 2], a[i + 3]);
+                }
+                m = next;
+                continue;
+            }
             const float inv_l = l_run > 0.f ? 1.f / l_run : 0.f;
             if (row_valid && ok) p.lse[(int64_t)(m.h * G + g) * p.N + tok] = l_run > 0.f ? m_ref + log2f(l_run) : -INFINITY;
             const bool full_tile = m.ne == TPT && G * TPT == kTileRows;      // whole box inside the sequence, every row staged
@@ -470,10 +512,10 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
     if (tid < kRdProblems && *status != kStatusOk && launch.p[tid].status) atomicMax(launch.p[tid].status, *status);
 }
 
-template <int D, typename ET>
+template <int D, int MOD, typename ET>
 static cudaError_t launch_rd(const RangeDenseLaunch& l, int num, int max_tiles, cudaStream_t stream) {
     constexpr int smem = kTileRows * D * 2 + 4 * kRdBK * D * 2 + kTileRows * 128 + 256;
-    auto kern = range_fwd_dense<D, ET>;
+    auto kern = range_fwd_dense<D, MOD, ET>;
     cudaError_t e = allow_smem((const void*)kern, smem);
     if (e != cudaSuccess) return e;
     prof_begin(FSA_KERNEL_RANGE_DENSE, stream);
@@ -482,6 +524,24 @@ static cudaError_t launch_rd(const RangeDenseLaunch& l, int num, int max_tiles, 
     return cudaGetLastError();
 }
 
+template <int D, typename ET>
+static cudaError_t launch_rd_mod(int mod, const RangeDenseLaunch& l, int max_tiles, cudaStream_t stream) {
+    switch (mod) {
+#define FSA_CASE(M) case M: return launch_rd<D, (M) | kModGuard, ET>(l, 1, max_tiles, stream);
+        FSA_CASE(0) FSA_CASE(1) FSA_CASE(2) FSA_CASE(3)
+#undef FSA_CASE
+#define FSA_CASE(M) case M | kModSplit: return launch_rd<D, (M) | kModSplit | kModGuard, ET>(l, l.nchunk, max_tiles, stream);
+        FSA_CASE(0) FSA_CASE(1) FSA_CASE(2) FSA_CASE(3)
+#undef FSA_CASE
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+cudaError_t launch_range_fwd_mod(int D, int dtype, int mod, const RangeDenseLaunch& l, int max_tiles, cudaStream_t stream) {
+    if (D == 128)
+        return dtype == kBF16 ? launch_rd_mod<128, __nv_bfloat16>(mod, l, max_tiles, stream) : launch_rd_mod<128, __half>(mod, l, max_tiles, stream);
+    return dtype == kBF16 ? launch_rd_mod<64, __nv_bfloat16>(mod, l, max_tiles, stream) : launch_rd_mod<64, __half>(mod, l, max_tiles, stream);
+}
 
 // ------------------------------------------------------------------------------------------------ dQ, query-tile-major
 // dQ of range attention with the same tiling as the forward above: per K/V tile S = Q K^T and dP = dO V^T, then
@@ -514,6 +574,7 @@ struct RangeDqParams {
     const float* delta;     // [Hq, N] sum_d o dO
     void* dq;               // [N, Hq, D] contiguous
     int* status;
+    ScoreMod mod;
 };
 
 constexpr int kDqThreads = 384;     // producer, S/dP issuer, 8 row warps, dQ issuer, item warp
@@ -526,7 +587,7 @@ static_assert(kMaxTokens / kRdBK * kDqTileClocks + FSA_WAIT_CLOCKS < (int64_t)1 
 
 // One work item of the dQ kernel: a tile of tokens x one KV head.
 struct DqItem {
-    int seq, tok0, ne, row_lo, nblk, h;
+    int seq, tok0, ne, row_lo, nblk, h, row_hi;
 };
 
 // Work item w of the list (heaviest tiles first).  Warp-collective: all 32 lanes call it and get the same answer.
@@ -534,7 +595,7 @@ __device__ __forceinline__ DqItem dq_item(const RangeDqParams& p, int ntiles, in
     DqItem m;
     m.h = w % p.Hk;
     const int want = ntiles - 1 - w / p.Hk;
-    m.row_lo = 0; m.nblk = 0;
+    m.row_lo = 0; m.nblk = 0; m.row_hi = -1;
     find_seq_tile(p.cu_q, p.B, p.TPT, want, lane, m.seq, m.tok0, m.ne);
     if (m.seq < 0) return m;
     int lo = INT_MAX, hi = -1;
@@ -551,18 +612,18 @@ __device__ __forceinline__ DqItem dq_item(const RangeDqParams& p, int ntiles, in
     }
     lo = max(lo, 0);
     hi = min(hi, (int)p.Nk - 1);
-    m.row_lo = lo;
+    m.row_lo = lo; m.row_hi = hi;
     m.nblk = hi >= lo ? (hi - lo) / kRdBK + 1 : 0;
     return m;
 }
 
-template <typename ET>
+template <int D, int MOD, typename ET>
 __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeDqParams p, const __grid_constant__ CUtensorMap qmap,
                                                                    const __grid_constant__ CUtensorMap domap,
                                                                    const __grid_constant__ CUtensorMap kmap,
                                                                    const __grid_constant__ CUtensorMap vmap,
                                                                    const __grid_constant__ CUtensorMap dqmap) {
-    constexpr int D = 128, BK = kRdBK, KH = D / 64;
+    constexpr int BK = kRdBK, KH = D / 64;
     constexpr int kQ = kTileRows * D * 2;            // Q tile, same for dO
     constexpr int kKt = BK * D * 2;
     constexpr int kOut = kTileRows * 128;            // 64 columns of the dQ tile on their way out
@@ -621,7 +682,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
         ok = warp_ok(ok);
         if (lane == 0) mbar_arrive(&it_empty[n % kDqItems]);
         DqItem m;
-        m.seq = x.x; m.tok0 = x.y; m.ne = x.z; m.row_lo = x.w; m.nblk = y.x; m.h = y.y;
+        m.seq = x.x; m.tok0 = x.y; m.ne = x.z; m.row_lo = x.w; m.nblk = y.x; m.h = y.y; m.row_hi = y.z;
         if (!ok) m.ne = m.nblk = 0;
         return m;
     };
@@ -637,7 +698,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
             longest = max(longest, m.nblk);
             if (ok && lane == 0) {
                 s_item[(n % kDqItems) * 2] = make_int4(m.seq, m.tok0, m.ne, m.row_lo);
-                s_item[(n % kDqItems) * 2 + 1] = make_int4(m.nblk, m.h, 0, 0);
+                s_item[(n % kDqItems) * 2 + 1] = make_int4(m.nblk, m.h, m.row_hi, 0);
                 mbar_arrive(&it_full[n % kDqItems]);
             }
         }
@@ -767,27 +828,31 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
             ok = ok && mbar_wait(qd_full, qi & 1, status);
             ++qi;
             const uint8_t* src = sb ? sDO : sQ;
-            uint32_t x[2][32];
+            uint32_t x[KH][32];
 #pragma unroll
             for (int i = 0; i < D / 8; ++i)
                 *reinterpret_cast<uint4*>(&x[i >> 3][(i & 7) * 4]) = *reinterpret_cast<const uint4*>(src + (i >> 3) * (kTileRows * 128) + sw128_chunk_off(r, i & 7));
-            tmem_st32(tbase + lane_off + (sb ? cDO : cQ), x[0]);
-            tmem_st32(tbase + lane_off + (sb ? cDO : cQ) + 32, x[1]);
+#pragma unroll
+            for (int b = 0; b < KH; ++b) tmem_st32(tbase + lane_off + (sb ? cDO : cQ) + b * 32, x[b]);
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(qd_empty);
             mbar_arrive(qt_full);
         };
         // This row's numbers, loaded an item ahead: item numbers and loads of their own between two items were a third of the kernel.
-        struct Row { int lo, hi; float lse, delta; };
+        struct Row { int lo, hi; float lse, delta, slope; int pos; };
         auto load_numbers = [&](const DqItem& m) {
-            Row x = {0, -1, 0.f, 0.f};
+            Row x = {0, -1, 0.f, 0.f, 0.f, 0};
             if (g < p.G && e < m.ne) {
                 x.lo = p.kv_lo ? __ldg(p.kv_lo + m.tok0 + e) : __ldg(p.cu_k + m.seq);
                 x.hi = __ldg(p.kv_hi + m.tok0 + e);
                 const int64_t idx = (int64_t)(m.h * p.G + g) * p.N + m.tok0 + e;
                 x.lse = __ldg(p.lse + idx);
                 x.delta = __ldg(p.delta + idx);
+                if constexpr (MOD & kModBias) {
+                    x.slope = __ldg(p.mod.slopes + m.h * p.G + g) * kLog2e;
+                    x.pos = __ldg(p.mod.pos + m.tok0 + e);
+                }
             }
             return x;
         };
@@ -804,7 +869,8 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
             const bool row_valid = g < p.G && e < m.ne;
             const int tok = m.tok0 + e;
             const int lo_r = row.lo;
-            const float lse_r = row.lse, delta_s = row.delta * p.scale;
+            const float lse_r = row.lse, delta_s = row.delta * p.scale, slope_r = row.slope;
+            const int pos_r = row.pos;
             int hi_r = min(row.hi, (int)p.Nk - 1);              // rows past the end of K/V do not exist
             if (!(lse_r > -INFINITY)) hi_r = lo_r - 1;          // a row that saw nothing in the forward sees nothing here
             DqItem next;
@@ -828,22 +894,55 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
                     tc_fence_before();
                     mbar_arrive(&sdp_free[b]);       // both rows are in registers: the buffer may take tile c + 2
                     if (j + 1 == m.nblk && next.nblk > 0) take_row();      // the next item's S / dP run under this item's end
-                    if (all_visible) {
+                    // bit i: column cb + i is seen
+                    const int v_lo = min(max(c_lo - cb, 0), HC), v_hi = min(max(c_hi - cb, 0), HC);
+                    const uint32_t vis = v_hi > v_lo ? (0xffffffffu >> (HC - v_hi + v_lo)) << v_lo : 0u;
+                    if constexpr (MOD != 0) {
+                        if constexpr (MOD & kModCap) cap_scores(sv, p.mod.x_scale);
+                        const float to_log2 = (MOD & kModCap) ? p.mod.cap_log2 : p.scale_log2;
+                        const uint64_t s2 = f32x2(to_log2, to_log2), g2 = f32x2(p.scale, p.scale), d2 = f32x2(-delta_s, -delta_s), one2 = f32x2(1.f, 1.f);
+                        const float rel = (float)(pos_r - R0 - cb);
+                        const float base = (MOD & kModBias) ? fmaf(-slope_r, rel, -lse_r) : -lse_r;
+                        // dS of two columns; BOTH: keys behind the token's place are seen too, ALL: no mask
+                        auto pairs = [&](auto both, auto all) {
+#pragma unroll
+                            for (int i = 0; i < 32; i += 2) {
+                                float b0 = base, b1 = base;
+                                if constexpr (MOD & kModBias) {
+                                    b0 = decltype(both)::on ? fmaf(-slope_r, fabsf(rel - (float)i), -lse_r) : fmaf(slope_r, (float)i, base);
+                                    b1 = decltype(both)::on ? fmaf(-slope_r, fabsf(rel - (float)(i + 1)), -lse_r) : fmaf(slope_r, (float)(i + 1), base);
+                                }
+                                const uint64_t x = f32x2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+                                const float2 s = f32x2_get(fma_f32x2(x, s2, f32x2(b0, b1)));
+                                uint64_t gr = fma_f32x2(f32x2(__uint_as_float(dv[i]), __uint_as_float(dv[i + 1])), g2, d2);
+                                // d tanh(x) = 1 - tanh(x)^2
+                                if constexpr (MOD & kModCap) gr = mul_f32x2(gr, fma_f32x2(f32x2(-__uint_as_float(sv[i]), -__uint_as_float(sv[i + 1])), x, one2));
+                                const float2 ds = f32x2_get(mul_f32x2(f32x2(ex2_approx(s.x), ex2_approx(s.y)), gr));
+                                dd[i >> 1] = decltype(all)::on ? ElemTraits<ET>::pack2(ds.x, ds.y)
+                                                 : ElemTraits<ET>::pack2(vis >> i & 1u ? ds.x : 0.f, vis >> (i + 1) & 1u ? ds.y : 0.f);
+                            }
+                        };
+                        if constexpr (MOD & kModBias) {
+                            if (p.mod.ahead && __any_sync(0xffffffffu, hi_r > pos_r)) pairs(Flag<true>{}, Flag<false>{});
+                            else if (all_visible) pairs(Flag<false>{}, Flag<true>{});
+                            else pairs(Flag<false>{}, Flag<false>{});
+                        } else {
+                            if (all_visible) pairs(Flag<false>{}, Flag<true>{});
+                            else pairs(Flag<false>{}, Flag<false>{});
+                        }
+                    } else if (all_visible) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
-                            const float p0 = rd_ex2(fmaf(__uint_as_float(sv[i]), p.scale_log2, -lse_r));
-                            const float p1 = rd_ex2(fmaf(__uint_as_float(sv[i + 1]), p.scale_log2, -lse_r));
+                            const float p0 = ex2_approx(fmaf(__uint_as_float(sv[i]), p.scale_log2, -lse_r));
+                            const float p1 = ex2_approx(fmaf(__uint_as_float(sv[i + 1]), p.scale_log2, -lse_r));
                             dd[i >> 1] = ElemTraits<ET>::pack2(p0 * fmaf(__uint_as_float(dv[i]), p.scale, -delta_s),
                                                                p1 * fmaf(__uint_as_float(dv[i + 1]), p.scale, -delta_s));
                         }
                     } else {
-                        // bit i: column cb + i is seen
-                        const int v_lo = min(max(c_lo - cb, 0), HC), v_hi = min(max(c_hi - cb, 0), HC);
-                        const uint32_t vis = v_hi > v_lo ? (0xffffffffu >> (HC - v_hi + v_lo)) << v_lo : 0u;
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
-                            const float p0 = rd_ex2(fmaf(__uint_as_float(sv[i]), p.scale_log2, -lse_r));
-                            const float p1 = rd_ex2(fmaf(__uint_as_float(sv[i + 1]), p.scale_log2, -lse_r));
+                            const float p0 = ex2_approx(fmaf(__uint_as_float(sv[i]), p.scale_log2, -lse_r));
+                            const float p1 = ex2_approx(fmaf(__uint_as_float(sv[i + 1]), p.scale_log2, -lse_r));
                             const float d0 = (vis >> i & 1u) && p0 > 0.f ? p0 * fmaf(__uint_as_float(dv[i]), p.scale, -delta_s) : 0.f;
                             const float d1 = (vis >> (i + 1) & 1u) && p1 > 0.f ? p1 * fmaf(__uint_as_float(dv[i + 1]), p.scale, -delta_s) : 0.f;
                             dd[i >> 1] = ElemTraits<ET>::pack2(d0, d1);
@@ -852,26 +951,44 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
                 }
                 tmem_st16(tbase + lane_off + b * 128 + BK + cb, dd);
                 tmem_st_wait();
+                if constexpr (MOD & kModGuard) {
+                    // K rows that no row of the item sees are multiplied by dS = 0: zeros take the place of what may be NaN (the tile's S is
+                    // done).  Every thread has a quarter of one of the 64 rows.
+                    const int kr = R0 + (r & (BK - 1)), part = sb * 2 + (r >> 6);
+                    const bool unseen = kr > m.row_hi || (p.mod.key_ids && __ldg(p.mod.key_ids + kr) < 0);
+                    if (__any_sync(0xffffffffu, unseen)) {
+                        if (unseen && ok)
+#pragma unroll
+                            for (int i = 0; i < D / 32; ++i) {
+                                const int chunk = part * (D / 32) + i;
+                                *reinterpret_cast<uint4*>(sKV + (c % kDqStages) * 2 * kKt + (chunk >> 3) * (BK * 128) + sw128_chunk_off(r & (BK - 1), chunk & 7)) =
+                                    make_uint4(0u, 0u, 0u, 0u);
+                            }
+                        fence_async_smem();
+                    }
+                }
                 tc_fence_before();
                 mbar_arrive(&ds_full[b]);
             }
             if (m.nblk == 0 && next.nblk > 0) take_row();
             // ---- epilogue of the item: this group's 64 of the 128 dQ columns
-            const bool full_tile = m.ne == p.TPT && p.G * p.TPT == kTileRows && m.nblk > 0;
+            // (at head size 64 a group has 32 columns, whose 64 bytes a row go out as plain stores)
+            constexpr int kOwn = D / 2;
+            const bool full_tile = D == 128 && m.ne == p.TPT && p.G * p.TPT == kTileRows && m.nblk > 0;
             if (m.nblk > 0) {
                 ok = ok && mbar_wait(&ds_empty[(c - 1) & 1], ((c - 1) >> 1) & 1, status);      // the item's last dQ product is done
                 tc_fence_after();
             }
-            ET* drow = reinterpret_cast<ET*>(p.dq) + ((int64_t)tok * p.Hq + (m.h * p.G + g)) * D + sb * 64;
+            ET* drow = reinterpret_cast<ET*>(p.dq) + ((int64_t)tok * p.Hq + (m.h * p.G + g)) * D + sb * kOwn;
             uint8_t* stage = sOut + sb * kOut;
             // the slab of the item before has left its place; and the four warps go on, or give up, together
             if (quarter == 0 && lane == 0) bulk_wait_read0();
             ok = bar_all(1 + sb, 128, ok);
 #pragma unroll
-            for (int c0 = 0; c0 < 64; c0 += 32) {
+            for (int c0 = 0; c0 < kOwn; c0 += 32) {
                 uint32_t a[32];
                 if (m.nblk > 0) {
-                    tmem_ld32(tbase + lane_off + cDQ + sb * 64 + c0, a);
+                    tmem_ld32(tbase + lane_off + cDQ + sb * kOwn + c0, a);
                     tmem_ld_wait();
                 } else {
 #pragma unroll
@@ -914,40 +1031,52 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
     if (warp == 0) tmem_dealloc(tbase, kCols);
 }
 
-// dQ of a range-attention backward (head_dim 128).  q / dO strided, dq contiguous [N, Hq, 128].
+template <int D, int MOD, typename ET>
+static cudaError_t launch_dq(const RangeDqParams& p, const CUtensorMap* maps, unsigned grid, cudaStream_t stream) {
+    constexpr int smem = 2 * kTileRows * D * 2 + kDqStages * 2 * kRdBK * D * 2 + 2 * kTileRows * kRdBK * 2 + 256 + kDqItems * 32;
+    auto kern = range_bwd_dq_dense<D, MOD, ET>;
+    const cudaError_t e = allow_smem((const void*)kern, smem);
+    if (e != cudaSuccess) return e;
+    prof_begin(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
+    kern<<<grid, kDqThreads, smem, stream>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4]);
+    prof_end(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
+    return cudaGetLastError();
+}
+
+template <int D, typename ET>
+static cudaError_t launch_dq_mod(int mod, const RangeDqParams& p, const CUtensorMap* maps, unsigned grid, cudaStream_t stream) {
+    switch (mod) {
+        case 0: return launch_dq<D, kModGuard, ET>(p, maps, grid, stream);
+        case 1: return launch_dq<D, 1 | kModGuard, ET>(p, maps, grid, stream);
+        case 2: return launch_dq<D, 2 | kModGuard, ET>(p, maps, grid, stream);
+        case 3: return launch_dq<D, 3 | kModGuard, ET>(p, maps, grid, stream);
+        default: return cudaErrorInvalidValue;
+    }
+}
+
+// dQ of a range-attention backward.  q / dO strided, dq contiguous [N, Hq, D].  mod null: plain scores, head_dim 128.
 cudaError_t launch_range_bwd_dq(int dtype, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap, const CUtensorMap& vmap,
-                                int* status, cudaStream_t stream) {
-    CUtensorMap qmap, domap, dqmap;
-    if (make_tile_map_3d_box(&qmap, a.q, dtype, 128, s.N, s.Hq, a.q_sn, a.q_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
-    if (make_tile_map_3d_box(&domap, a.d_o, dtype, 128, s.N, s.Hq, a.do_sn, a.do_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
-    if (make_tile_map_3d_box(&dqmap, a.dq, dtype, 128, s.N, s.Hq, (int64_t)s.Hq * 128, 128, s.TPT, s.G)) return cudaErrorInvalidValue;
+                                int* status, cudaStream_t stream, const ScoreMod* mod, int which) {
+    const int D = mod ? s.D : 128;
+    CUtensorMap maps[5];        // Q, dO, K, V, dQ
+    if (make_tile_map_3d_box(&maps[0], a.q, dtype, D, s.N, s.Hq, a.q_sn, a.q_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
+    if (make_tile_map_3d_box(&maps[1], a.d_o, dtype, D, s.N, s.Hq, a.do_sn, a.do_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
+    maps[2] = kmap; maps[3] = vmap;
+    if (make_tile_map_3d_box(&maps[4], a.dq, dtype, D, s.N, s.Hq, (int64_t)s.Hq * D, D, s.TPT, s.G)) return cudaErrorInvalidValue;
     RangeDqParams p;
     p.cu_q = a.cu; p.cu_k = a.bd.cu_k ? a.bd.cu_k : a.cu; p.kv_lo = a.bd.kv_lo; p.kv_hi = a.bd.kv_hi;
     p.N = s.N; p.Nk = s.Nk; p.B = s.B; p.Hq = s.Hq; p.Hk = s.Hk; p.G = s.G; p.TPT = s.TPT;
     p.scale = a.sm_scale; p.scale_log2 = a.sm_scale * 1.4426950408889634f;
     p.lse = a.lse; p.delta = a.delta; p.dq = a.dq; p.status = status;
-    constexpr int smem = 2 * kTileRows * 128 * 2 + kDqStages * 2 * kRdBK * 128 * 2 + 2 * kTileRows * kRdBK * 2 + 256 + kDqItems * 32;
+    p.mod = mod ? *mod : ScoreMod{};
     const int64_t max_items = ((s.N + s.TPT - 1) / s.TPT + s.B) * (int64_t)s.Hk;
     int sms = 0;
     if (device_sm_count(&sms) != 0 || sms <= 0) return cudaErrorInvalidValue;
     const unsigned grid = (unsigned)(max_items < sms ? max_items : sms);
-    cudaError_t e;
-    if (dtype == kBF16) {
-        auto kern = range_bwd_dq_dense<__nv_bfloat16>;
-        e = allow_smem((const void*)kern, smem);
-        if (e != cudaSuccess) return e;
-        prof_begin(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
-        kern<<<grid, kDqThreads, smem, stream>>>(p, qmap, domap, kmap, vmap, dqmap);
-        prof_end(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
-    } else {
-        auto kern = range_bwd_dq_dense<__half>;
-        e = allow_smem((const void*)kern, smem);
-        if (e != cudaSuccess) return e;
-        prof_begin(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
-        kern<<<grid, kDqThreads, smem, stream>>>(p, qmap, domap, kmap, vmap, dqmap);
-        prof_end(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
-    }
-    return cudaGetLastError();
+    const bool bf16 = dtype == kBF16;
+    if (!mod) return bf16 ? launch_dq<128, 0, __nv_bfloat16>(p, maps, grid, stream) : launch_dq<128, 0, __half>(p, maps, grid, stream);
+    if (D == 128) return bf16 ? launch_dq_mod<128, __nv_bfloat16>(which, p, maps, grid, stream) : launch_dq_mod<128, __half>(which, p, maps, grid, stream);
+    return bf16 ? launch_dq_mod<64, __nv_bfloat16>(which, p, maps, grid, stream) : launch_dq_mod<64, __half>(which, p, maps, grid, stream);
 }
 
 }  // namespace fsa
@@ -992,8 +1121,8 @@ extern "C" int fsa_range_attn_fwd_dense_several(int num, const fsa_range_problem
     }
     if (used == 0) return FSA_OK;
     cudaStream_t stream = (cudaStream_t)stream_;
-    const cudaError_t e = dtype == FSA_DTYPE_BF16 ? (D == 128 ? launch_rd<128, __nv_bfloat16>(l, used, max_tiles, stream) : launch_rd<64, __nv_bfloat16>(l, used, max_tiles, stream))
-                                                  : (D == 128 ? launch_rd<128, __half>(l, used, max_tiles, stream) : launch_rd<64, __half>(l, used, max_tiles, stream));
+    const cudaError_t e = dtype == FSA_DTYPE_BF16 ? (D == 128 ? launch_rd<128, 0, __nv_bfloat16>(l, used, max_tiles, stream) : launch_rd<64, 0, __nv_bfloat16>(l, used, max_tiles, stream))
+                                                  : (D == 128 ? launch_rd<128, 0, __half>(l, used, max_tiles, stream) : launch_rd<64, 0, __half>(l, used, max_tiles, stream));
     return e == cudaSuccess ? FSA_OK : FSA_ERR_CUDA;
 }
 

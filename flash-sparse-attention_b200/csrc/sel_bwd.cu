@@ -554,6 +554,20 @@ __global__ void __launch_bounds__(256) sel_bwd_convert(const float* __restrict__
 
 constexpr int64_t kReduceFew = 24000;      // output rows up to which both reductions go in one launch (more: resident merges take dq)
 
+template <typename ET>
+static cudaError_t launch_delta(const SelBwdArgs& a, const SelShape& s, cudaStream_t stream) {
+    const int64_t rows = s.N * s.Hq, rows_per_cta = 2 * (256 / (s.D / 8));
+    const cudaError_t e = prefer_l1((const void*)sel_bwd_delta<ET>);
+    if (e != cudaSuccess) return e;
+    sel_bwd_delta<ET><<<(unsigned)((rows + rows_per_cta - 1) / rows_per_cta), 256, 0, stream>>>((const ET*)a.o, a.o_sn, a.o_sh, (const ET*)a.d_o, a.do_sn,
+                                                                                               a.do_sh, s.N, s.Hq, s.D, a.delta);
+    return cudaGetLastError();
+}
+
+cudaError_t launch_sel_bwd_delta(int dtype, const SelBwdArgs& a, const SelShape& s, cudaStream_t stream) {
+    return dtype == kBF16 ? launch_delta<__nv_bfloat16>(a, s, stream) : launch_delta<__half>(a, s, stream);
+}
+
 template <int D, typename ET>
 static cudaError_t launch_sel_bwd(const SelBwdArgs& a, const SelShape& s, const SelIndex& ix, const CUtensorMap& kmap,
                                   const CUtensorMap& vmap, int num_sms, cudaStream_t stream) {
@@ -573,14 +587,7 @@ static cudaError_t launch_sel_bwd(const SelBwdArgs& a, const SelShape& s, const 
         e = cudaMemsetAsync(a.dk_acc, 0, kv_elems * 4 * 2, stream);   // dk_acc and dv_acc are adjacent
         if (e != cudaSuccess) return e;
     }
-    if (rows > 0 && !a.have_delta) {
-        const int64_t rows_per_cta = 2 * (256 / (D / 8));
-        unsigned grid = (unsigned)((rows + rows_per_cta - 1) / rows_per_cta);
-        e = prefer_l1((const void*)sel_bwd_delta<ET>);
-        if (e != cudaSuccess) return e;
-        sel_bwd_delta<ET><<<grid, 256, 0, stream>>>((const ET*)a.o, a.o_sn, a.o_sh, (const ET*)a.d_o, a.do_sn, a.do_sh,
-                                                    s.N, s.Hq, D, a.delta);
-    }
+    if (rows > 0 && !a.have_delta && (e = launch_delta<ET>(a, s, stream)) != cudaSuccess) return e;
     if (a.plan) {
         e = launch_range_bwd_dq(dt, a, s, kmap, vmap, ix.header, stream);
         return e == cudaSuccess ? launch_range_bwd_dkdv(dt, *a.plan, a, s, kmap, vmap, ix.header, stream) : e;

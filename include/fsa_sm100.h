@@ -201,6 +201,32 @@ typedef struct {
 int fsa_range_attn_fwd_dense_several(int num, const fsa_range_problem* problems, int batch, int num_q_heads, int num_kv_heads, int head_dim, int dtype,
                                      float sm_scale, void* stream);
 int fsa_range_attn_bwd_indexed(int head_dim);
+
+/* Attention with changed scores, packed sequences (no counterpart in the reference; next to the sliding-window branch):
+ *   s = sm_scale q.k;  s = softcap tanh(s / softcap) (softcap > 0);  s = s - slopes[h] |t - j| (slopes not null);  o = softmax(s) v
+ * over the keys j that token t may see.  The tokens of a sequence are its last ones: token i of Lq stands at place t = Lk - Lq + i of the
+ * sequence's Lk keys, and sees the keys j <= t, of them with
+ *   window >= 0      those with j >= t - window;
+ *   doc_ids          (int32 per K/V row) those of its document: the stretch of equal ids around t.  Rows with a negative id are padding:
+ *                    they see nothing (o = 0, lse = -inf) and nobody sees them;
+ *   prefix_lens      (int32 per sequence; not with window or doc_ids) and the sequence's first prefix_lens[b] keys besides.
+ * k, v: head stride head_dim.  o [N, Hq, D] contiguous, lse [Hq, N] (log2 units); rows behind the last sequence become 0 / -inf.  K/V
+ * rows that no token sees, and q and d_o rows of tokens that see nothing, may hold anything, NaN included.  limits: workspace of
+ * fsa_biased_attn_limits_bytes bytes, kept for the backward; its first word is the status word (fsa_read_status).
+ * head_dim 64 or 128, up to 32 query heads a kv head, fewer than 2^25 tokens and K/V rows, N * num_q_heads below 2^31. */
+int fsa_biased_attn_limits_bytes(int64_t total_tokens, int64_t* bytes_out);
+int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
+                        const int32_t* doc_ids, const int32_t* prefix_lens, const float* slopes, int64_t total_tokens, int64_t total_kv_rows, int batch,
+                        int num_q_heads, int num_kv_heads, int head_dim, int dtype, int64_t q_stride_n, int64_t q_stride_h, int64_t k_stride_n,
+                        int64_t v_stride_n, float sm_scale, float softcap, int window, void* o, float* lse, void* limits, int64_t limits_bytes, void* stream);
+/* dq, dk, dv contiguous; every row of them is written.  has_prefix: the forward was given prefix_lens.  Bit-reproducible. */
+int fsa_biased_attn_bwd_bytes(int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads, int head_dim, int64_t* bytes_out);
+int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens_q,
+                        const int32_t* cu_seqlens_k, const int32_t* doc_ids, int has_prefix, const float* slopes, int64_t total_tokens, int64_t total_kv_rows,
+                        int batch, int num_q_heads, int num_kv_heads, int head_dim, int dtype, int64_t q_stride_n, int64_t q_stride_h, int64_t k_stride_n,
+                        int64_t v_stride_n, int64_t do_stride_n, int64_t do_stride_h, float sm_scale, float softcap, void* dq, void* dk, void* dv,
+                        void* limits, int64_t limits_bytes, void* scratch, int64_t scratch_bytes, void* stream);
+
 int fsa_range_attn_index(const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* kv_lo, const int32_t* kv_hi,
                          int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads,
                          int max_blocks, int block_size, void* index_ws, int64_t index_ws_bytes, void* stream);
