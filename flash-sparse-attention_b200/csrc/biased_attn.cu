@@ -1,6 +1,6 @@
 // Attention with changed scores (capped by a tanh, biased by distance) under causal, window, document and prefix masks, packed
-// sequences: the limits of every token and the entry points.  The kernels are those of range attention (range_dense.cu,
-// range_bwd_dkdv.cu) compiled for changed scores: under each of these masks a token sees one stretch of K/V rows.
+// sequences: the limits of every token and the entry points.  Under each of these masks a token sees one stretch of
+// K/V rows.  Forward: biased_fwd.cu; backward: the kernels of range attention (range_dense.cu, range_bwd_dkdv.cu) compiled for changed scores.
 #include "../../include/fsa_sm100.h"
 
 #include "range_bwd.cuh"
@@ -106,7 +106,11 @@ static int biased_mod(float sm_scale, float softcap, const float* slopes, const 
     if (!(sm_scale > 0.f) || !(softcap >= 0.f)) return FSA_ERR_BAD_ARG;
     *which = (softcap > 0.f ? kModCap : 0) | (slopes ? kModBias : 0);
     *m = ScoreMod{};
-    if (softcap > 0.f) { m->x_scale = sm_scale / softcap; m->cap_log2 = softcap * kLog2e; }
+    if (softcap > 0.f) {
+        m->x_scale = sm_scale / softcap;
+        m->cap_log2 = softcap * kLog2e;
+        near_coefficients(m);
+    }
     m->slopes = slopes; m->key_ids = doc_ids; m->ahead = ahead;
     return FSA_OK;
 }
@@ -131,20 +135,19 @@ extern "C" int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, 
     if (dtype != FSA_DTYPE_BF16 && dtype != FSA_DTYPE_FP16) return FSA_ERR_BAD_ARG;
     // under these pairs a token would not see one stretch of rows
     if (prefix_lens && (window >= 0 || doc_ids)) return FSA_ERR_UNSUPPORTED;
-    RangeDenseLaunch l = {};
+    BiasedFwdLaunch l = {};
     int which;
     if ((rc = biased_mod(sm_scale, softcap, slopes, doc_ids, prefix_lens != nullptr, &l.mod, &which))) return rc;
     if (N == 0) return FSA_OK;
     if (!q || !k || !v || !cu_seqlens_q || !cu_seqlens_k || !o || !lse || !limits || Nk == 0) return FSA_ERR_BAD_ARG;
-    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(o) || !aligned16(limits)) return FSA_ERR_BAD_ARG;
+    if (!aligned16(q) || !aligned16(k) || !aligned16(v) || ((uintptr_t)o & 31) || !aligned16(limits)) return FSA_ERR_BAD_ARG;
     if ((q_sn % 8) || (q_sh % 8) || (k_sn % 8) || (v_sn % 8) || k_sn < (int64_t)Hk * D || v_sn < (int64_t)Hk * D) return FSA_ERR_BAD_ARG;
     if (limits_bytes < BiasedLimits::bytes(N)) return FSA_ERR_WORKSPACE;
     (void)cudaGetLastError();
     if ((rc = ensure_context())) return rc;
-    if ((rc = make_tile_map_3d_box(&l.q[0], q, dtype, D, N, Hq, q_sn, q_sh, s.TPT, s.G))) return rc;
-    if ((rc = make_tile_map_3d_box(&l.o[0], o, dtype, D, N, Hq, (int64_t)Hq * D, D, s.TPT, s.G))) return rc;
-    if ((rc = make_tile_map(&l.k[0], k, dtype, Nk, (int64_t)Hk * D, k_sn, 64))) return rc;
-    if ((rc = make_tile_map(&l.v[0], v, dtype, Nk, (int64_t)Hk * D, v_sn, 64))) return rc;
+    if ((rc = make_tile_map_3d_box(&l.q, q, dtype, D, N, Hq, q_sn, q_sh, s.TPT, s.G))) return rc;
+    if ((rc = make_tile_map(&l.k, k, dtype, Nk, (int64_t)Hk * D, k_sn, 64))) return rc;
+    if ((rc = make_tile_map(&l.v, v, dtype, Nk, (int64_t)Hk * D, v_sn, 64))) return rc;
     cudaStream_t stream = (cudaStream_t)stream_;
     const BiasedLimits lim(limits, N);
     biased_limits<<<(unsigned)((N + kLimThreads - 1) / kLimThreads), kLimThreads, 0, stream>>>(cu_seqlens_q, cu_seqlens_k, doc_ids, prefix_lens, B, N, window,
@@ -152,12 +155,12 @@ extern "C" int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, 
     cudaError_t e = cudaGetLastError();
     if (e != cudaSuccess) return cuda_failed(e);
     l.mod.pos = lim.pos;
-    RangeDenseParams& p = l.p[0];
+    RangeDenseParams& p = l.p;
     p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.kv_lo = lim.lo; p.kv_hi = lim.hi;
     p.N = N; p.Nk = Nk; p.B = B; p.Hq = Hq; p.Hk = Hk; p.G = s.G; p.TPT = s.TPT;
     p.scale_log2 = sm_scale * kLog2e;
-    p.o = o; p.o_sn = (int64_t)Hq * D; p.o_sh = D; p.lse = lse; p.status = lim.status;
-    e = launch_range_fwd_mod(D, dtype, which, l, (int)((N + s.TPT - 1) / s.TPT) + B, stream);
+    p.o = o; p.lse = lse; p.status = lim.status;
+    e = launch_biased_fwd(D, dtype, which, false, l, (int)((N + s.TPT - 1) / s.TPT) + B, stream);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
 }
 

@@ -423,6 +423,8 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
         const int key = quarter * 32 + lane;
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
         const uint32_t tS = tbase + lane_off + cS + grp * 64, tP = tbase + lane_off + cP + grp * 64;
+        const NearTanh near(p.mod, 1.f);
+        bool far = false;               // the tile before had scores near the cap
         const int g_first = grp * 64 / TPT, e_first = grp * 64 - g_first * TPT;      // head and token of the group's first column
         bool ok = true;
         int c = 0, qi = 0;
@@ -444,35 +446,62 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
                 tmem_ld_wait();
                 uint32_t pk[32];
                 if constexpr (MOD != 0) {
-                    // v: P (1 - tanh^2), what dS takes; pk: P
-                    if constexpr (MOD & kModCap) cap_scores(v, p.mod.x_scale);
+                    // v: P (1 - tanh^2), what dS takes; pk: P.  NEAR: products whose tanh is near's (looked at afterwards), else v has been changed
+                    // already
                     const float to_log2 = (MOD & kModCap) ? p.mod.cap_log2 : p.scale_log2;
                     const uint64_t s2 = f32x2(to_log2, to_log2), one2 = f32x2(1.f, 1.f);
-                    int e4 = e_first, g4 = g_first;
+                    float big[2] = {0.f, 0.f};
+                    auto pairs = [&](auto is_near) {
+                        int e4 = e_first, g4 = g_first;
 #pragma unroll
-                    for (int j = 0; j < 16; ++j) {
-                        const float4 l = lse4[j];
-                        float c[4] = {-l.x, -l.y, -l.z, -l.w};
-                        if constexpr (MOD & kModBias) {
-                            // four columns: consecutive tokens of one head
-                            const float slope = __ldg(p.mod.slopes + m.h * p.G + min(g4, p.G - 1)) * kLog2e, d = (float)(key_rel - i * TPT - e4);
+                        for (int j = 0; j < 16; ++j) {
+                            const float4 l = lse4[j];
+                            float c[4] = {-l.x, -l.y, -l.z, -l.w};
+                            if constexpr (MOD & kModBias) {
+                                // four columns: consecutive tokens of one head
+                                const float slope = __ldg(p.mod.slopes + m.h * p.G + min(g4, p.G - 1)) * kLog2e, d = (float)(key_rel - i * TPT - e4);
 #pragma unroll
-                            for (int q = 0; q < 4; ++q) c[q] = p.mod.ahead ? fmaf(-slope, fabsf(d - (float)q), c[q]) : fmaf(slope, d - (float)q, c[q]);
-                            e4 += 4;
-                            if (e4 == TPT) { e4 = 0; ++g4; }
+                                for (int q = 0; q < 4; ++q) c[q] = p.mod.ahead ? fmaf(-slope, fabsf(d - (float)q), c[q]) : fmaf(slope, d - (float)q, c[q]);
+                                e4 += 4;
+                                if (e4 == TPT) { e4 = 0; ++g4; }
+                            }
+#pragma unroll
+                            for (int q = 0; q < 4; q += 2) {
+                                const int k = 4 * j + q;
+                                uint64_t x = f32x2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+                                if constexpr (decltype(is_near)::on) {
+                                    big[(k >> 1) & 1] = max3_abs(big[(k >> 1) & 1], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
+                                    x = mul_f32x2(x, near.slope(x));
+                                }
+                                const float2 s = f32x2_get(fma_f32x2(x, s2, f32x2(c[q], c[q + 1])));
+                                float2 pr = make_float2(ex2_approx(s.x), ex2_approx(s.y));
+                                pk[k >> 1] = ElemTraits<ET>::pack2(pr.x, pr.y);
+                                if constexpr (MOD & kModCap) {
+                                    const float2 th = f32x2_get(x);
+                                    pr = f32x2_get(mul_f32x2(f32x2(pr.x, pr.y), fma_f32x2(f32x2(-th.x, -th.y), x, one2)));
+                                }
+                                v[k] = __float_as_uint(pr.x);
+                                v[k + 1] = __float_as_uint(pr.y);
+                            }
                         }
-#pragma unroll
-                        for (int q = 0; q < 4; q += 2) {
-                            const int k = 4 * j + q;
-                            const uint64_t x = f32x2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]));
-                            const float2 s = f32x2_get(fma_f32x2(x, s2, f32x2(c[q], c[q + 1])));
-                            float2 pr = make_float2(ex2_approx(s.x), ex2_approx(s.y));
-                            pk[k >> 1] = ElemTraits<ET>::pack2(pr.x, pr.y);
-                            if constexpr (MOD & kModCap)
-                                pr = f32x2_get(mul_f32x2(f32x2(pr.x, pr.y), fma_f32x2(f32x2(-__uint_as_float(v[k]), -__uint_as_float(v[k + 1])), x, one2)));
-                            v[k] = __float_as_uint(pr.x);
-                            v[k + 1] = __float_as_uint(pr.y);
+                    };
+                    if constexpr (MOD & kModCap) {
+                        bool is_far = far;
+                        if (!is_far) {
+                            pairs(Flag<true>{});
+                            is_far = __any_sync(0xffffffffu, !(fmaxf(big[0], big[1]) <= p.mod.near_v));
+                            if (is_far) {
+                                tmem_ld32(tS, *reinterpret_cast<uint32_t (*)[32]>(&v[0]));
+                                tmem_ld32(tS + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
+                                tmem_ld_wait();
+                            }
                         }
+                        if (is_far) {
+                            far = cap_scores(v, p.mod.x_scale, p.mod.near_v);
+                            pairs(Flag<false>{});
+                        }
+                    } else {
+                        pairs(Flag<false>{});
                     }
                 } else {
 #pragma unroll

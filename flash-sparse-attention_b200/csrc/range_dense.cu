@@ -33,53 +33,21 @@ int make_tile_map_3d_box(CUtensorMap* map, const void* base, int dtype, int64_t 
 int device_sm_count(int* out);
 
 constexpr int kRdThreads = 192;
-constexpr int kRdBK = 64;
 constexpr float kRdLazy = 8.0f;       // raise a row's reference max only when exceeded by more than this (log2 units)
 
 // One item: a tile of tokens x one KV head of problem z.
 struct RdItem {
-    int z, h, seq, tok0, ne, row_lo, nblk, row_hi;     // row_hi: last K/V row that a row of the item sees
+    int z, h, seq, tok0, ne, row_lo, nblk;
 };
 
 // The K/V rows that a row of the item sees: [x, y].
-template <int MOD>
 __device__ __forceinline__ int2 rd_row(const RangeDenseLaunch& launch, const RdItem& m, bool valid, int e) {
     if (m.z < 0 || !valid) return make_int2(0, -1);
-    const RangeDenseParams& p = launch.p[(MOD & kModSplit) ? 0 : m.z];
+    const RangeDenseParams& p = launch.p[m.z];
     return make_int2(p.kv_lo ? __ldg(p.kv_lo + m.tok0 + e) : __ldg(p.cu_k + m.seq), __ldg(p.kv_hi + m.tok0 + e));
 }
 
-// kModBias: the slope of the row's head (log2 units) and its token's place as a K/V row.
-template <int MOD>
-__device__ __forceinline__ void rd_bias(const RangeDenseLaunch& launch, const RdItem& m, bool valid, int g, int e, float& slope, int& pos) {
-    slope = 0.f; pos = 0;
-    if (!(MOD & kModBias) || m.z < 0 || !valid) return;
-    slope = __ldg(launch.mod.slopes + m.h * launch.p[0].G + g) * kLog2e;
-    pos = __ldg(launch.mod.pos + m.tok0 + e);
-}
-
-// Takes over a CTA of this launch that has not started yet (cluster launch control): 16 bytes of answer at dst, with bar as the
-// transaction barrier.  Not to be called again once the answer was no.
-__device__ __forceinline__ void claim_next_cta(uint32_t dst, uint64_t* bar) {
-    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(dst),
-                 "r"(smem_u32(bar)) : "memory");
-}
-__device__ __forceinline__ bool claimed_cta(uint32_t src, int& x, int& y, int& z) {
-    uint32_t yes, cx, cy, cz;
-    asm volatile(
-        "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t"
-        "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
-        "ld.shared.b128 a, [%4];\n\t"
-        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
-        "selp.u32 %0, 1, 0, p;\n\t"
-        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, a;\n\t}"
-        : "=r"(yes), "=r"(cx), "=r"(cy), "=r"(cz) : "r"(src) : "memory");
-    x = (int)cx; y = (int)cy; z = (int)cz;
-    return yes != 0;
-}
-
-// MOD (score.cuh): changed scores, rows that nobody sees, chunks of K/V rows with partial results.
-template <int D, int MOD, typename ET>
+template <int D, typename ET>
 __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_constant__ RangeDenseLaunch launch) {
     constexpr int BK = kRdBK;
     constexpr int kQ = kTileRows * D * 2;
@@ -114,8 +82,7 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
     int* status = reinterpret_cast<int*>(bars + 30) + 1;     // of this CTA
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    constexpr bool kSplit = (MOD & kModSplit) != 0;
-    const uint32_t limit = wait_limit(launch.p[kSplit ? 0 : blockIdx.z].status);
+    const uint32_t limit = wait_limit(launch.p[blockIdx.z].status);
     const int G = launch.p[0].G, TPT = launch.p[0].TPT;      // (the same for all problems)
     if (tid == 0) {
         *status = kStatusOk;
@@ -139,7 +106,7 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
         const int4 x = s_item[(n & 1) * 2], y = s_item[(n & 1) * 2 + 1];
         RdItem m;
         m.z = x.x; m.h = x.y; m.seq = x.z; m.tok0 = x.w;
-        m.ne = y.x; m.row_lo = y.y; m.nblk = y.z; m.row_hi = y.w;
+        m.ne = y.x; m.row_lo = y.y; m.nblk = y.z;
         return m;
     };
     auto take_item = [&](int n, bool& ok) {
@@ -157,7 +124,7 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
         int n = 0, claims = 0, qi = 0, c = 0;           // items, claims, non-empty items, K/V tiles so far
         int bx = blockIdx.x, h = blockIdx.y, z = blockIdx.z;
         while (ok) {
-            const RangeDenseParams& p = launch.p[kSplit ? 0 : z];
+            const RangeDenseParams& p = launch.p[z];
             bool asked = false;
             auto ask = [&]() {
                 mbar_expect_tx(claim, 16);
@@ -184,29 +151,23 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 }
                 lo = max(lo, 0);
                 hi = min(hi, (int)p.Nk - 1);
-                int nblk = hi >= lo ? (hi - lo) / BK + 1 : 0;
-                if constexpr (kSplit) {
-                    const int per = (nblk + launch.nchunk - 1) / launch.nchunk, b0 = min(z * per, nblk);
-                    nblk = min(per, nblk - b0);
-                    lo += b0 * BK;
-                    hi = min(hi, lo + nblk * BK - 1);
-                }
+                const int nblk = hi >= lo ? (hi - lo) / BK + 1 : 0;
                 if (n > 0) ok = ok && mbar_wait(it_empty, (n - 1) & 1, status, limit);
                 ok = warp_ok(ok);
                 if (ok && lane == 0) {
                     s_item[(n & 1) * 2] = make_int4(z, h, seq, tok0);
-                    s_item[(n & 1) * 2 + 1] = make_int4(ne, lo, nblk, hi);
+                    s_item[(n & 1) * 2 + 1] = make_int4(ne, lo, nblk, 0);
                     mbar_arrive(it_full);
                 }
                 ++n;
                 if (lane == 0 && nblk > 0) {
-                    const CUtensorMap *kmap = &launch.k[kSplit ? 0 : z], *vmap = &launch.v[kSplit ? 0 : z];
+                    const CUtensorMap *kmap = &launch.k[z], *vmap = &launch.v[z];
                     ok = ok && mbar_wait(q_empty, (qi & 1) ^ 1, status, limit);
                     ask();                  // not earlier: a CTA is to be one item ahead, not to take the share of others
                     if (ok) {
                         mbar_expect_tx(q_full, (uint32_t)(KH * 128 * TPT * G));
 #pragma unroll
-                        for (int b = 0; b < KH; ++b) tma_load_3d(smem_u32(sQ + b * (kTileRows * 128)), &launch.q[kSplit ? 0 : z], b * 64, tok0, h * G, q_full);
+                        for (int b = 0; b < KH; ++b) tma_load_3d(smem_u32(sQ + b * (kTileRows * 128)), &launch.q[z], b * 64, tok0, h * G, q_full);
                     }
                     // K tile j and V tile j are loaded in the order the MMA warp needs them: K(0), K(1), V(0), K(2), V(1), ...
                     for (int step = 0; step < nblk + 1 && ok; ++step) {
@@ -319,17 +280,11 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
         bool ok = true;
         int n = 0, c = 0;
         RdItem m = take_item(n, ok);
-        int2 sees = rd_row<MOD>(launch, m, g < G && e < m.ne, e);
-        float slope;
-        int pos;
-        rd_bias<MOD>(launch, m, g < G && e < m.ne, g, e, slope, pos);
+        int2 sees = rd_row(launch, m, g < G && e < m.ne, e);
         // (the four warps leave the loop together: they meet at barriers in it)
         for (ok = bar_all(1, 128, ok); ok && m.z >= 0;) {
-            // from what the loop below has in v to log2 units (the same for all problems)
-            const float scale_log2 = (MOD & kModBias) ? 1.f : (MOD & kModCap) ? launch.mod.cap_log2 : launch.p[0].scale_log2;
-            const int lo_r = sees.x - m.row_lo, hi_r = min(sees.y, (int)launch.p[kSplit ? 0 : m.z].Nk - 1) - m.row_lo;      // rows past the end of K/V do not exist
-            const float slope_r = slope;
-            const int pos_r = pos - m.row_lo;
+            const float scale_log2 = launch.p[0].scale_log2;                 // (the same for all problems)
+            const int lo_r = sees.x - m.row_lo, hi_r = min(sees.y, (int)launch.p[m.z].Nk - 1) - m.row_lo;      // rows past the end of K/V do not exist
             const int nblk = m.nblk;
             float m_ref = -INFINITY, l_run = 0.f;
             for (int j = 0; j < nblk; ++j, ++c) {          // (left by all lanes at the vote below)
@@ -341,10 +296,6 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 tmem_ld32(tbase + lane_off + cS + st * BK, *reinterpret_cast<uint32_t (*)[32]>(&v[0]));
                 tmem_ld32(tbase + lane_off + cS + st * BK + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
                 tmem_ld_wait();
-                if constexpr (MOD & kModCap) cap_scores(v, launch.mod.x_scale);
-                if constexpr (MOD & kModBias)
-                    bias_scores(v, (MOD & kModCap) ? launch.mod.cap_log2 : launch.p[0].scale_log2, slope_r, (float)(pos_r - j * BK),
-                                launch.mod.ahead && __any_sync(0xffffffffu, j * BK + c_hi - 1 > pos_r));
                 if (c_lo > 0 || c_hi < BK) {
                     // bit i: column i is seen
                     const int v_hi = max(c_hi, 0), v_lo = min(c_lo, BK);
@@ -403,62 +354,22 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 l_run += (ls[0] + ls[1]) + (ls[2] + ls[3]);
                 tmem_st32(tbase + lane_off + cS + st * BK, *reinterpret_cast<uint32_t (*)[32]>(&pk[0]));
                 tmem_st_wait();
-                if constexpr (MOD & kModGuard) {
-                    // V rows that no row of the item sees are multiplied by p = 0, but 0 x NaN is NaN: zeros take their place.  Every thread
-                    // has half of one of the 64 rows.
-                    const int row = m.row_lo + j * BK + (r & (BK - 1));
-                    const bool unseen = row > m.row_hi || (launch.mod.key_ids && __ldg(launch.mod.key_ids + row) < 0);
-                    if (__any_sync(0xffffffffu, unseen)) {
-                        ok = ok && mbar_wait(&v_full[st], (c >> 1) & 1, status, limit);
-                        if (unseen && ok)
-#pragma unroll
-                            for (int i = 0; i < D / 16; ++i) {
-                                const int chunk = (r >> 6) * (D / 16) + i;
-                                *reinterpret_cast<uint4*>(sV + st * kKt + (chunk >> 3) * (BK * 128) + sw128_chunk_off(r & (BK - 1), chunk & 7)) =
-                                    make_uint4(0u, 0u, 0u, 0u);
-                            }
-                        fence_async_smem();
-                    }
-                }
                 tc_fence_before();
                 mbar_arrive(&p_full[st]);
             }
             m = read_item(n);
-            const RangeDenseParams& p = launch.p[kSplit ? 0 : m.z];
+            const RangeDenseParams& p = launch.p[m.z];
             const bool row_valid = g < G && e < m.ne;
             const int tok = m.tok0 + e;
             // the next item's numbers arrive under this item's epilogue
             const RdItem next = take_item(++n, ok);
-            sees = rd_row<MOD>(launch, next, g < G && e < next.ne, e);
-            rd_bias<MOD>(launch, next, g < G && e < next.ne, g, e, slope, pos);
+            sees = rd_row(launch, next, g < G && e < next.ne, e);
             // ---- epilogue
             if (m.nblk > 0) {
                 ok = ok && mbar_wait(&pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1, status, limit);
                 tc_fence_after();
             }
             ok = bar_all(1, 128, ok);
-            if constexpr (kSplit) {
-                const int64_t part = ((int64_t)tok * p.Hq + m.h * G + g) * launch.P + m.z;
-                const bool some = m.nblk > 0 && l_run > 0.f;
-                if (row_valid && ok) launch.ml[part] = some ? make_float2(m_ref, l_run) : make_float2(-INFINITY, 0.f);
-#pragma unroll
-                for (int c0 = 0; c0 < D; c0 += 32) {
-                    uint32_t a[32];
-                    if (m.nblk == 0) break;
-                    tmem_ld32(tbase + lane_off + cO + c0, a);
-                    tmem_ld_wait();
-                    if (c0 + 32 == D) {
-                        tc_fence_before();
-                        mbar_arrive(o_free);            // the accumulator may take the next item
-                    }
-                    if (row_valid && some && ok)
-#pragma unroll
-                        for (int i = 0; i < 32; i += 4)
-                            *reinterpret_cast<uint4*>(launch.o_part + part * D + c0 + i) = make_uint4(a[i], a[i + 1], a[i + 2], a[i + 3]);
-                }
-                m = next;
-                continue;
-            }
             const float inv_l = l_run > 0.f ? 1.f / l_run : 0.f;
             if (row_valid && ok) p.lse[(int64_t)(m.h * G + g) * p.N + tok] = l_run > 0.f ? m_ref + log2f(l_run) : -INFINITY;
             const bool full_tile = m.ne == TPT && G * TPT == kTileRows;      // whole box inside the sequence, every row staged
@@ -512,10 +423,10 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
     if (tid < kRdProblems && *status != kStatusOk && launch.p[tid].status) atomicMax(launch.p[tid].status, *status);
 }
 
-template <int D, int MOD, typename ET>
+template <int D, typename ET>
 static cudaError_t launch_rd(const RangeDenseLaunch& l, int num, int max_tiles, cudaStream_t stream) {
     constexpr int smem = kTileRows * D * 2 + 4 * kRdBK * D * 2 + kTileRows * 128 + 256;
-    auto kern = range_fwd_dense<D, MOD, ET>;
+    auto kern = range_fwd_dense<D, ET>;
     cudaError_t e = allow_smem((const void*)kern, smem);
     if (e != cudaSuccess) return e;
     prof_begin(FSA_KERNEL_RANGE_DENSE, stream);
@@ -524,24 +435,6 @@ static cudaError_t launch_rd(const RangeDenseLaunch& l, int num, int max_tiles, 
     return cudaGetLastError();
 }
 
-template <int D, typename ET>
-static cudaError_t launch_rd_mod(int mod, const RangeDenseLaunch& l, int max_tiles, cudaStream_t stream) {
-    switch (mod) {
-#define FSA_CASE(M) case M: return launch_rd<D, (M) | kModGuard, ET>(l, 1, max_tiles, stream);
-        FSA_CASE(0) FSA_CASE(1) FSA_CASE(2) FSA_CASE(3)
-#undef FSA_CASE
-#define FSA_CASE(M) case M | kModSplit: return launch_rd<D, (M) | kModSplit | kModGuard, ET>(l, l.nchunk, max_tiles, stream);
-        FSA_CASE(0) FSA_CASE(1) FSA_CASE(2) FSA_CASE(3)
-#undef FSA_CASE
-        default: return cudaErrorInvalidValue;
-    }
-}
-
-cudaError_t launch_range_fwd_mod(int D, int dtype, int mod, const RangeDenseLaunch& l, int max_tiles, cudaStream_t stream) {
-    if (D == 128)
-        return dtype == kBF16 ? launch_rd_mod<128, __nv_bfloat16>(mod, l, max_tiles, stream) : launch_rd_mod<128, __half>(mod, l, max_tiles, stream);
-    return dtype == kBF16 ? launch_rd_mod<64, __nv_bfloat16>(mod, l, max_tiles, stream) : launch_rd_mod<64, __half>(mod, l, max_tiles, stream);
-}
 
 // ------------------------------------------------------------------------------------------------ dQ, query-tile-major
 // dQ of range attention with the same tiling as the forward above: per K/V tile S = Q K^T and dP = dO V^T, then
@@ -591,12 +484,13 @@ struct DqItem {
 };
 
 // Work item w of the list (heaviest tiles first).  Warp-collective: all 32 lanes call it and get the same answer.
+template <int MOD>
 __device__ __forceinline__ DqItem dq_item(const RangeDqParams& p, int ntiles, int w, int lane) {
     DqItem m;
     m.h = w % p.Hk;
-    const int want = ntiles - 1 - w / p.Hk;
     m.row_lo = 0; m.nblk = 0; m.row_hi = -1;
-    find_seq_tile(p.cu_q, p.B, p.TPT, want, lane, m.seq, m.tok0, m.ne);
+    if constexpr (MOD != 0) find_ranked_tile(p.cu_q, p.cu_k, p.B, p.TPT, w / p.Hk, lane, m.seq, m.tok0, m.ne);
+    else find_seq_tile(p.cu_q, p.B, p.TPT, ntiles - 1 - w / p.Hk, lane, m.seq, m.tok0, m.ne);
     if (m.seq < 0) return m;
     int lo = INT_MAX, hi = -1;
     const int k0 = __ldg(p.cu_k + m.seq);
@@ -692,7 +586,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
         bool ok = true;
         int n = 0, longest = 0;
         for (int w = blockIdx.x; w < nitems && ok; w += gridDim.x, ++n) {
-            const DqItem m = dq_item(p, ntiles, w, lane);
+            const DqItem m = dq_item<MOD>(p, ntiles, w, lane);
             ok = ok && mbar_wait(&it_empty[n % kDqItems], ((n / kDqItems) & 1) ^ 1, status, FSA_WAIT_CLOCKS + longest * kDqTileClocks);
             ok = warp_ok(ok);
             longest = max(longest, m.nblk);
@@ -856,6 +750,8 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
             }
             return x;
         };
+        const NearTanh near(p.mod, 1.f);
+        bool far = false;               // the tile before had scores near the cap
         DqItem m;
         m.nblk = m.ne = 0;
         int n = 0;
@@ -898,13 +794,14 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
                     const int v_lo = min(max(c_lo - cb, 0), HC), v_hi = min(max(c_hi - cb, 0), HC);
                     const uint32_t vis = v_hi > v_lo ? (0xffffffffu >> (HC - v_hi + v_lo)) << v_lo : 0u;
                     if constexpr (MOD != 0) {
-                        if constexpr (MOD & kModCap) cap_scores(sv, p.mod.x_scale);
                         const float to_log2 = (MOD & kModCap) ? p.mod.cap_log2 : p.scale_log2;
                         const uint64_t s2 = f32x2(to_log2, to_log2), g2 = f32x2(p.scale, p.scale), d2 = f32x2(-delta_s, -delta_s), one2 = f32x2(1.f, 1.f);
                         const float rel = (float)(pos_r - R0 - cb);
                         const float base = (MOD & kModBias) ? fmaf(-slope_r, rel, -lse_r) : -lse_r;
-                        // dS of two columns; BOTH: keys behind the token's place are seen too, ALL: no mask
-                        auto pairs = [&](auto both, auto all) {
+                        float big[2] = {0.f, 0.f};
+                        // dS of the columns, two at a time.  NEAR: products whose tanh is near's (looked at afterwards), else sv has been changed
+                        // already; BOTH: keys behind the token's place are seen too; ALL: no mask
+                        auto pairs = [&](auto is_near, auto both, auto all) {
 #pragma unroll
                             for (int i = 0; i < 32; i += 2) {
                                 float b0 = base, b1 = base;
@@ -912,23 +809,34 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
                                     b0 = decltype(both)::on ? fmaf(-slope_r, fabsf(rel - (float)i), -lse_r) : fmaf(slope_r, (float)i, base);
                                     b1 = decltype(both)::on ? fmaf(-slope_r, fabsf(rel - (float)(i + 1)), -lse_r) : fmaf(slope_r, (float)(i + 1), base);
                                 }
-                                const uint64_t x = f32x2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+                                uint64_t x = f32x2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+                                if constexpr (decltype(is_near)::on) {
+                                    big[(i >> 1) & 1] = max3_abs(big[(i >> 1) & 1], __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
+                                    x = mul_f32x2(x, near.slope(x));
+                                }
                                 const float2 s = f32x2_get(fma_f32x2(x, s2, f32x2(b0, b1)));
                                 uint64_t gr = fma_f32x2(f32x2(__uint_as_float(dv[i]), __uint_as_float(dv[i + 1])), g2, d2);
                                 // d tanh(x) = 1 - tanh(x)^2
-                                if constexpr (MOD & kModCap) gr = mul_f32x2(gr, fma_f32x2(f32x2(-__uint_as_float(sv[i]), -__uint_as_float(sv[i + 1])), x, one2));
+                                if constexpr (MOD & kModCap) {
+                                    const float2 th = f32x2_get(x);
+                                    gr = mul_f32x2(gr, fma_f32x2(f32x2(-th.x, -th.y), x, one2));
+                                }
                                 const float2 ds = f32x2_get(mul_f32x2(f32x2(ex2_approx(s.x), ex2_approx(s.y)), gr));
                                 dd[i >> 1] = decltype(all)::on ? ElemTraits<ET>::pack2(ds.x, ds.y)
-                                                 : ElemTraits<ET>::pack2(vis >> i & 1u ? ds.x : 0.f, vis >> (i + 1) & 1u ? ds.y : 0.f);
+                                                               : ElemTraits<ET>::pack2(vis >> i & 1u ? ds.x : 0.f, vis >> (i + 1) & 1u ? ds.y : 0.f);
                             }
                         };
-                        if constexpr (MOD & kModBias) {
-                            if (p.mod.ahead && __any_sync(0xffffffffu, hi_r > pos_r)) pairs(Flag<true>{}, Flag<false>{});
-                            else if (all_visible) pairs(Flag<false>{}, Flag<true>{});
-                            else pairs(Flag<false>{}, Flag<false>{});
-                        } else {
-                            if (all_visible) pairs(Flag<false>{}, Flag<true>{});
-                            else pairs(Flag<false>{}, Flag<false>{});
+                        const bool both = (MOD & kModBias) && p.mod.ahead && __any_sync(0xffffffffu, hi_r > pos_r);
+                        bool is_far = both || far;
+                        if (!is_far) {
+                            if (all_visible) pairs(Flag<(MOD & kModCap) != 0>{}, Flag<false>{}, Flag<true>{});
+                            else pairs(Flag<(MOD & kModCap) != 0>{}, Flag<false>{}, Flag<false>{});
+                            if constexpr (MOD & kModCap) is_far = __any_sync(0xffffffffu, !(fmaxf(big[0], big[1]) <= p.mod.near_v));
+                        }
+                        if (is_far) {
+                            if constexpr (MOD & kModCap) far = cap_scores(sv, p.mod.x_scale, p.mod.near_v);
+                            if (both) pairs(Flag<false>{}, Flag<true>{}, Flag<false>{});
+                            else pairs(Flag<false>{}, Flag<false>{}, Flag<false>{});
                         }
                     } else if (all_visible) {
 #pragma unroll
@@ -1121,8 +1029,8 @@ extern "C" int fsa_range_attn_fwd_dense_several(int num, const fsa_range_problem
     }
     if (used == 0) return FSA_OK;
     cudaStream_t stream = (cudaStream_t)stream_;
-    const cudaError_t e = dtype == FSA_DTYPE_BF16 ? (D == 128 ? launch_rd<128, 0, __nv_bfloat16>(l, used, max_tiles, stream) : launch_rd<64, 0, __nv_bfloat16>(l, used, max_tiles, stream))
-                                                  : (D == 128 ? launch_rd<128, 0, __half>(l, used, max_tiles, stream) : launch_rd<64, 0, __half>(l, used, max_tiles, stream));
+    const cudaError_t e = dtype == FSA_DTYPE_BF16 ? (D == 128 ? launch_rd<128, __nv_bfloat16>(l, used, max_tiles, stream) : launch_rd<64, __nv_bfloat16>(l, used, max_tiles, stream))
+                                                  : (D == 128 ? launch_rd<128, __half>(l, used, max_tiles, stream) : launch_rd<64, __half>(l, used, max_tiles, stream));
     return e == cudaSuccess ? FSA_OK : FSA_ERR_CUDA;
 }
 

@@ -1,9 +1,11 @@
-// The forward of range attention (range_dense.cu) for its callers: one problem or several, plain scores or changed ones (score.cuh).
+// The forwards of range attention (range_dense.cu) and of attention with changed scores (biased_fwd.cu) for their callers.
 #pragma once
 #include "score.cuh"
 #include "sel_launch.cuh"
 
 namespace fsa {
+
+constexpr int kRdBK = 64;
 
 struct RangeDenseParams {
     const int32_t* cu_q;    // [B + 1]
@@ -24,15 +26,19 @@ constexpr int kRdProblems = 3;
 struct RangeDenseLaunch {
     CUtensorMap q[kRdProblems], k[kRdProblems], v[kRdProblems], o[kRdProblems];
     RangeDenseParams p[kRdProblems];
-    // kernels with a MOD: one problem
+};
+
+// Attention with changed scores: the same problem, one a launch.
+struct BiasedFwdLaunch {
+    CUtensorMap q, k, v;
+    RangeDenseParams p;     // (o_sn and o_sh are not used: o is contiguous)
     ScoreMod mod;
-    // kModSplit: the K/V rows of every tile are cut into nchunk chunks (blockIdx.z); chunk c of a row writes partial c of P
+    // kModSplit: the K/V rows of every tile are cut into nchunk chunks (blockIdx.y); chunk c of a row writes partial c of P
     float* o_part;          // [N, Hq, P, D] unnormalised
     float2* ml;             // [N, Hq, P] reference maximum (log2 units) and sum
     int P, nchunk;
 };
-
-// The forward with changed scores (range_dense.cu): l.p[0] and l.mod, tiles of l.p[0].TPT tokens; nchunk > 0: kModSplit.
-cudaError_t launch_range_fwd_mod(int D, int dtype, int mod, const RangeDenseLaunch& l, int max_tiles, cudaStream_t stream);
+// which: kModCap, kModBias; split: with kModSplit.  l.p.TPT tokens a tile, max_tiles tiles at most.
+cudaError_t launch_biased_fwd(int D, int dtype, int which, bool split, const BiasedFwdLaunch& l, int max_tiles, cudaStream_t stream);
 
 }  // namespace fsa

@@ -14,6 +14,8 @@ constexpr int kModScore = kModCap | kModBias;
 
 struct ScoreMod {
     float x_scale;              // scale / cap: from a product to the argument of the tanh
+    float near_v;               // products up to this size have the tanh v (near[0] + near[1] v^2 + ...)
+    float near[4];
     float cap_log2;             // cap log2(e): from the tanh to a score in log2 units
     const float* slopes;        // [Hq]
     const int32_t* pos;         // [N] place of every token, as a K/V row
@@ -40,27 +42,34 @@ __device__ __forceinline__ float rcp_approx(float x) {
 // makes 1e-5 of a score.  tanh.approx would take one special-function step instead of two, but is off by 5e-4 of the score.
 __device__ __forceinline__ float tanh_any(float v, float k) { return fmaf(-2.f, rcp_approx(1.f + ex2_approx(v * k)), 1.f); }
 
-// v <- tanh(x_scale v), N scores of a row (all lanes of a warp call it).  The special-function unit gives 16 results a cycle and SM, and the
+// tanh_near: of two values no larger than 3/4; cap_scores: v <- tanh(x_scale v), N scores of a row (all lanes of a warp
+// call it; whether some |v| was above near_v).  The special-function unit gives 16 results a cycle and SM, and the
 // softmax needs one for each score already; with two more the capped forward would be bound by it, three times as long as its products.
 // Where no |x| of the warp's 32 rows is above 3/4 (scores below 37 at a cap of 50), tanh(x) = x p(x^2) with p of degree 4: the
 // polynomial that is nearest to tanh(x) / x on [0, 9/16] in relative error, 6e-7 (fitted on Chebyshev points); two scores an instruction.
 constexpr float kTanhNear = 0.75f;
+__device__ __forceinline__ uint64_t tanh_near(uint64_t x) {
+    constexpr float c[5] = {0.999999463558197f, -0.3332825005054474f, 0.13258983194828033f, -0.050056297332048416f, 0.012929627671837807f};
+    const uint64_t u = mul_f32x2(x, x);
+    uint64_t p = f32x2(c[4], c[4]);
+#pragma unroll
+    for (int i = 3; i >= 0; --i) p = fma_f32x2(p, u, f32x2(c[i], c[i]));
+    return mul_f32x2(x, p);
+}
 template <int N>
-__device__ __forceinline__ void cap_scores(uint32_t (&v)[N], float x_scale) {
+__device__ __forceinline__ bool cap_scores(uint32_t (&v)[N], float x_scale, float near_v) {
     float a[2] = {0.f, 0.f};
 #pragma unroll
-    for (int i = 0; i < N; i += 2) {        // (a NaN stays out of a maximum: it is masked, or makes the row NaN either way)
-        a[0] = fmaxf(a[0], fabsf(__uint_as_float(v[i])));
-        a[1] = fmaxf(a[1], fabsf(__uint_as_float(v[i + 1])));
+    for (int i = 0; i < N; i += 4) {        // (a NaN stays out of a maximum: it is masked, or makes the row NaN either way)
+        a[0] = max3_abs(a[0], __uint_as_float(v[i]), __uint_as_float(v[i + 1]));
+        a[1] = max3_abs(a[1], __uint_as_float(v[i + 2]), __uint_as_float(v[i + 3]));
     }
-    if (__all_sync(0xffffffffu, fmaxf(a[0], a[1]) * x_scale <= kTanhNear)) {
-        const uint64_t xs = f32x2(x_scale, x_scale), c0 = f32x2(0.999999463558197f, 0.999999463558197f),
-                       c1 = f32x2(-0.3332825005054474f, -0.3332825005054474f), c2 = f32x2(0.13258983194828033f, 0.13258983194828033f),
-                       c3 = f32x2(-0.050056297332048416f, -0.050056297332048416f), c4 = f32x2(0.012929627671837807f, 0.012929627671837807f);
+    const float most = fmaxf(a[0], a[1]);
+    if (__all_sync(0xffffffffu, most * x_scale <= kTanhNear)) {
+        const uint64_t xs = f32x2(x_scale, x_scale);
 #pragma unroll
         for (int i = 0; i < N; i += 2) {
-            const uint64_t x = mul_f32x2(f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), xs), u = mul_f32x2(x, x);
-            const float2 t = f32x2_get(mul_f32x2(x, fma_f32x2(fma_f32x2(fma_f32x2(fma_f32x2(c4, u, c3), u, c2), u, c1), u, c0)));
+            const float2 t = f32x2_get(tanh_near(mul_f32x2(f32x2(__uint_as_float(v[i]), __uint_as_float(v[i + 1])), xs)));
             v[i] = __float_as_uint(t.x);
             v[i + 1] = __float_as_uint(t.y);
         }
@@ -69,6 +78,32 @@ __device__ __forceinline__ void cap_scores(uint32_t (&v)[N], float x_scale) {
 #pragma unroll
         for (int i = 0; i < N; ++i) v[i] = __float_as_uint(tanh_any(__uint_as_float(v[i]), k));
     }
+    return __any_sync(0xffffffffu, most > near_v);
+}
+
+// Of products no larger than near_v, half a cap: tanh(x_scale v) = v p(v^2), p of degree 3 with the scale in its coefficients (host: near_coefficients);
+// 6e-7 of the value as well.  f: what every coefficient is multiplied with.
+struct NearTanh {
+    uint64_t c[4];
+    __device__ __forceinline__ NearTanh(const ScoreMod& m, float f) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = f32x2(m.near[i] * f, m.near[i] * f);
+    }
+    // the factor of v
+    __device__ __forceinline__ uint64_t slope(uint64_t v) const {
+        const uint64_t w = mul_f32x2(v, v);
+        return fma_f32x2(fma_f32x2(fma_f32x2(c[3], w, c[2]), w, c[1]), w, c[0]);
+    }
+};
+inline void near_coefficients(ScoreMod* m) {
+    // nearest to tanh(x) / x on x^2 in [0, 1/4] in relative error.  Scales whose powers leave the normal numbers do without.
+    constexpr double c[4] = {0.999999463558197, -0.33326318860054016, 0.13190296292304993, -0.04440222308039665};
+    const double x = m->x_scale;
+    m->near_v = 0.f;
+    if (!(x >= 1e-4 && x <= 1e4)) return;
+    m->near_v = (float)(0.5 / x);
+    double pow = x;
+    for (int i = 0; i < 4; ++i, pow *= x * x) m->near[i] = (float)(c[i] * pow);
 }
 
 // v <- scale v - slope |rel - i|, N scores of a row against keys i = 0, 1, ... of a tile; rel: the token's place among them.  both (the

@@ -261,6 +261,36 @@ __device__ __forceinline__ void find_seq_tile(const int32_t* __restrict__ cu_q, 
     }
 }
 
+// The same list, longest rows of keys first, for up to 32 sequences (others: from its end): a tile's tokens see about as many keys as precede
+// them in their sequence, cu_k's included, which is what tiles are ranked by.  Sequence after sequence, a long one that comes late in the list
+// is still at work when everybody else is done: two sequences of 8192 tokens, 8 / 4 heads, took 28 % longer a tile than one of 16384.
+__device__ __forceinline__ void find_ranked_tile(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, int B, int TPT, int rank, int lane,
+                                                int& seq, int& tok0, int& ne) {
+    if (B > 32) {
+        find_seq_tile(cu_q, B, TPT, count_seq_tiles(cu_q, B, TPT, lane) - 1 - rank, lane, seq, tok0, ne);
+        return;
+    }
+    const int s0 = lane < B ? __ldg(cu_q + lane) : 0, s1 = lane < B ? __ldg(cu_q + lane + 1) : 0;
+    const int nt = (s1 - s0 + TPT - 1) / TPT;
+    const int first = lane < B ? max(0, __ldg(cu_k + lane + 1) - __ldg(cu_k + lane) - (s1 - s0)) / TPT : 0;      // level of its first tile
+    // tiles of level t and above
+    auto above = [&](int t) { return __reduce_add_sync(0xffffffffu, max(0, first + nt - max(t, first))); };
+    seq = -1; tok0 = 0; ne = 0;
+    if (rank >= above(0)) return;
+    int lo = 0, hi = __reduce_max_sync(0xffffffffu, first + nt);       // above(lo) > rank >= above(hi)
+    while (hi - lo > 1) {
+        const int mid = (lo + hi) >> 1;
+        if (above(mid) > rank) lo = mid; else hi = mid;
+    }
+    const int place = rank - above(lo + 1);
+    const unsigned here = __ballot_sync(0xffffffffu, lo >= first && lo < first + nt);
+    const bool me = (here >> lane & 1u) && __popc(here & ((1u << lane) - 1)) == place;
+    seq = __ffs(__ballot_sync(0xffffffffu, me)) - 1;
+    const int t0 = __shfl_sync(0xffffffffu, s0 + (lo - first) * TPT, seq);
+    tok0 = t0;
+    ne = min(TPT, __shfl_sync(0xffffffffu, s1, seq) - t0);
+}
+
 // One tile of the list, read from its record: no searching, and the address depends only on the
 // tile index, so records and entries can be prefetched any number of tiles ahead.
 struct TileInfo {

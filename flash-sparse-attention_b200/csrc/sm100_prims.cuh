@@ -173,6 +173,27 @@ __device__ __forceinline__ bool bar_all(int id, int threads, bool v) {
     return all != 0;
 }
 
+// ---------------------------------------------------------------- cluster launch control
+// Takes over a CTA of this launch that has not started yet (cluster launch control): 16 bytes of answer at dst, with bar as the
+// transaction barrier.  Not to be called again once the answer was no.
+__device__ __forceinline__ void claim_next_cta(uint32_t dst, uint64_t* bar) {
+    asm volatile("clusterlaunchcontrol.try_cancel.async.shared::cta.mbarrier::complete_tx::bytes.b128 [%0], [%1];" ::"r"(dst),
+                 "r"(smem_u32(bar)) : "memory");
+}
+__device__ __forceinline__ bool claimed_cta(uint32_t src, int& x, int& y, int& z) {
+    uint32_t yes, cx, cy, cz;
+    asm volatile(
+        "{\n\t.reg .pred p;\n\t.reg .b128 a;\n\t"
+        "mov.u32 %1, 0;\n\tmov.u32 %2, 0;\n\tmov.u32 %3, 0;\n\t"
+        "ld.shared.b128 a, [%4];\n\t"
+        "clusterlaunchcontrol.query_cancel.is_canceled.pred.b128 p, a;\n\t"
+        "selp.u32 %0, 1, 0, p;\n\t"
+        "@p clusterlaunchcontrol.query_cancel.get_first_ctaid.v4.b32.b128 {%1, %2, %3, _}, a;\n\t}"
+        : "=r"(yes), "=r"(cx), "=r"(cy), "=r"(cz) : "r"(src) : "memory");
+    x = (int)cx; y = (int)cy; z = (int)cz;
+    return yes != 0;
+}
+
 // ---------------------------------------------------------------- proxies / fences
 // Generic-proxy writes to shared memory (st.shared, cp.async) must be made visible to the
 // async proxy (TMA, tcgen05.mma operand reads) before those engines read them.
@@ -196,6 +217,12 @@ __device__ __forceinline__ void cp_async_wait() { asm volatile("cp.async.wait_gr
 
 // A hint: the line of p into L2.
 __device__ __forceinline__ void prefetch_l2(const void* p) { asm volatile("prefetch.global.L2 [%0];" ::"l"(p)); }
+
+// 32 bytes (a whole sector) from registers; dst 32-byte aligned
+__device__ __forceinline__ void st_global32(void* dst, const uint32_t* x) {
+    asm volatile("st.global.v8.b32 [%0], {%1, %2, %3, %4, %5, %6, %7, %8};" ::"l"(dst), "r"(x[0]), "r"(x[1]), "r"(x[2]), "r"(x[3]), "r"(x[4]),
+                 "r"(x[5]), "r"(x[6]), "r"(x[7]) : "memory");
+}
 
 // ---------------------------------------------------------------- TMA
 // 2-D tiled load: box of the tensor map starting at (x = innermost element, y = row).
@@ -417,6 +444,18 @@ __device__ __forceinline__ uint64_t mul_f32x2(uint64_t a, uint64_t b) {
     uint64_t r;
     asm("mul.rn.f32x2 %0, %1, %2;" : "=l"(r) : "l"(a), "l"(b));
     return r;
+}
+
+// the largest of three, and of three magnitudes, in one instruction (a NaN stays out)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float d;
+    asm("max.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
+}
+__device__ __forceinline__ float max3_abs(float a, float b, float c) {
+    float d;
+    asm("max.abs.f32 %0, %1, %2, %3;" : "=f"(d) : "f"(a), "f"(b), "f"(c));
+    return d;
 }
 
 // ---------------------------------------------------------------- element types
