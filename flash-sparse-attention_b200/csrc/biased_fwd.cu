@@ -70,6 +70,22 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
     const RangeDenseParams& p = launch.p;
     const uint32_t limit = wait_limit(p.status);
     const int G = p.G, TPT = p.TPT;
+    // First and last K/V row that a token sees, and its place.  kModSplit: a token is a sequence of the batch, whose own rows follow the shared ones.
+    struct Sees { int lo, hi, pos; };
+    auto limits = [&](int seq, int tok) {
+        Sees x;
+        if constexpr (kSplit) {
+            const int k0 = __ldg(p.cu_k + seq), k1 = __ldg(p.cu_k + seq + 1), len = __ldg(launch.seq_len + tok);
+            x.pos = k1 + len - 1;
+            x.lo = launch.window >= 0 ? max(k0, x.pos - launch.window) : k0;
+            x.hi = len > 0 ? k1 - 1 : -1;
+        } else {
+            x.lo = __ldg(p.kv_lo + tok);
+            x.hi = __ldg(p.kv_hi + tok);
+            x.pos = (MOD & kModBias) ? __ldg(launch.mod.pos + tok) : 0;
+        }
+        return x;
+    };
     if (tid == 0) {
         *status = kStatusOk;
         mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(k_full, 1); mbar_init(k_empty, 1); mbar_init(s_full, 1);
@@ -119,15 +135,16 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                 // lowest and highest K/V row any token of the tile sees
                 int lo = INT_MAX, hi = -1;
                 for (int e = lane; e < ne; e += 32) {
-                    const int l = __ldg(p.kv_lo + tok0 + e), u = __ldg(p.kv_hi + tok0 + e);
-                    if (u >= l) { lo = min(lo, l); hi = max(hi, u); }
+                    const Sees x = limits(seq, tok0 + e);
+                    if (x.hi >= x.lo) { lo = min(lo, x.lo); hi = max(hi, x.hi); }
                 }
                 lo = max(__reduce_min_sync(0xffffffffu, lo), 0);
                 hi = min(__reduce_max_sync(0xffffffffu, hi), (int)p.Nk - 1);
                 int nblk = hi >= lo ? (hi - lo) / BK + 1 : 0;
                 if constexpr (kSplit) {
-                    const int per = (nblk + launch.nchunk - 1) / launch.nchunk, b0 = min(z * per, nblk);
-                    nblk = min(per, nblk - b0);
+                    // chunks of one size (the last one takes what is left), so that long shared rows are cut more often than short ones
+                    const int b0 = min(z * launch.chunk, nblk);
+                    nblk = z + 1 < launch.nchunk ? min(launch.chunk, nblk - b0) : nblk - b0;
                     lo += b0 * BK;
                     hi = min(hi, lo + nblk * BK - 1);
                 }
@@ -265,11 +282,11 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
         auto load_row = [&](const BfItem& m) {
             Row x = {0, INT_MAX, 0.f, INT_MAX};
             if (m.z >= 0 && g < G && e < m.ne) {
-                x.lo = __ldg(p.kv_lo + m.tok0 + e);
-                x.hi = __ldg(p.kv_hi + m.tok0 + e);
+                const Sees s = limits(m.seq, m.tok0 + e);
+                x.lo = s.lo; x.hi = s.hi;
                 if constexpr (MOD & kModBias) {
                     x.slope = __ldg(launch.mod.slopes + m.h * G + g) * kLog2e;
-                    x.pos = __ldg(launch.mod.pos + m.tok0 + e);
+                    x.pos = s.pos;
                 }
             }
             return x;

@@ -155,6 +155,67 @@ std::tuple<Tensor, Tensor> biased_attention(const Tensor& q, const Tensor& k, co
     return {o, lse};
 }
 
-void bind_biased(pybind11::module& m) { m.def("biased_attention", &biased_attention); }
+// A cache of rows [rows, Hk, D] as it is read in place.  (None is copied: a copy of the cache at every step would be slower than all the rest.)
+static void check_cache(const Tensor& t, const char* name) {
+    TORCH_CHECK_VALUE(t.stride(2) == 1 && (t.size(1) == 1 || t.stride(1) == t.size(2)) && (t.size(0) <= 1 || (t.stride(0) % 8 == 0 && t.stride(0) >= t.size(1) * t.size(2))) &&
+                          ((uintptr_t)t.data_ptr() & 15) == 0,
+                      name, ": the heads of a row have to be adjacent, rows and memory aligned to 16 bytes; got strides ", t.strides());
+}
+static int64_t row_stride(const Tensor& t) { return t.size(0) <= 1 ? t.size(1) * t.size(2) : t.stride(0); }
+
+std::tuple<Tensor, Tensor> biased_decode(const Tensor& q_, const Tensor& k, const Tensor& v, const Tensor& seq_len, const Tensor& row0, const MaybeTensor& pk,
+                                         const MaybeTensor& pv, const MaybeTensor& cu_prefix, const MaybeTensor& cu_group, const MaybeTensor& slopes_, double scale,
+                                         double cap, int64_t window, int64_t max_len, int64_t max_prefix) {
+    check_qkv(q_, k, v);
+    const int64_t B = q_.size(0), Hq = q_.size(1), D = q_.size(2), Hk = k.size(1);
+    check_lengths(seq_len, q_, B, "seq_len");
+    check_lengths(row0, q_, B, "seq_row0");
+    int64_t groups = 0, prefix_rows = 0;
+    if (pk) {
+        check_qkv(q_, *pk, *pv);
+        TORCH_CHECK_VALUE(pk->size(1) == Hk, "prefix_k has ", pk->size(1), " heads, k ", Hk);
+        TORCH_CHECK_VALUE(cu_prefix->dim() == 1 && cu_prefix->size(0) >= 2, "cu_prefix has to have an entry more than there are prefixes, and there is one at least");
+        groups = cu_prefix->size(0) - 1;
+        check_lengths(*cu_prefix, q_, groups + 1, "cu_prefix");
+        check_lengths(*cu_group, q_, groups + 1, "cu_group");
+        prefix_rows = pk->size(0);
+    }
+    TORCH_CHECK_VALUE(window >= -1 && window <= INT32_MAX, "window_size has to be 0 or more (or None)");
+    TORCH_CHECK_VALUE(max_len >= 0 && max_prefix >= 0, "max_len and max_prefix have to be 0 or more");
+    const Tensor slopes = check_slopes(slopes_, q_);
+    check_scores(q_, scale, cap);
+    check_cache(k, "k");
+    check_cache(v, "v");
+    if (pk) {
+        check_cache(*pk, "prefix_k");
+        check_cache(*pv, "prefix_v");
+    }
+    c10::cuda::CUDAGuard guard(q_.device());
+    Tensor q = q_.contiguous();
+    if (((uintptr_t)q.data_ptr() & 15) != 0) q = q.clone(at::MemoryFormat::Contiguous);
+    if (B == 0) return {fresh({B, Hq, D}, q), f32({B, Hq}, q)};
+    TORCH_CHECK_VALUE(k.size(0) > 0, "the cache has no rows");
+    int64_t nb = 0;
+    check(fsa_biased_decode_bytes((int)B, (int)Hq, (int)Hk, (int)D, (int)groups, max_len, max_prefix, (int)window, &nb), "fsa_biased_decode_bytes");
+    const Tensor scratch = bytes(nb, q), lens = seq_len.contiguous(), rows = row0.contiguous(), cp = cu_prefix ? cu_prefix->contiguous() : Tensor(),
+                 cg = cu_group ? cu_group->contiguous() : Tensor();
+    Tensor o = fresh({B, Hq, D}, q), lse = f32({B, Hq}, q);
+    check(fsa_biased_decode(ptr(q), ptr(k), ptr(v), k.size(0), row_stride(k), row_stride(v), iptr(lens), iptr(rows), pk ? ptr(*pk) : nullptr, pk ? ptr(*pv) : nullptr,
+                            prefix_rows, pk ? row_stride(*pk) : 0, pk ? row_stride(*pv) : 0, iptr(cp), iptr(cg), (int)groups,
+                            slopes.defined() ? slopes.data_ptr<float>() : nullptr, (int)B, (int)Hq, (int)Hk, (int)D, dtype_code(q), (float)scale, (float)cap,
+                            (int)window, max_len, max_prefix, ptr(o), lse.data_ptr<float>(), ptr(scratch), scratch.numel(), stream_of(q)),
+          "fsa_biased_decode");
+    if (checking_status()) {
+        int st = 0;
+        check(fsa_biased_decode_read_status(&st), "fsa_biased_decode status");
+        TORCH_CHECK(st == 0, "fsa_biased_decode status: a kernel recorded a device-side failure (", st, ")");
+    }
+    return {o, lse};
+}
+
+void bind_biased(pybind11::module& m) {
+    m.def("biased_attention", &biased_attention);
+    m.def("biased_decode", &biased_decode);
+}
 
 }  // namespace fsa_host

@@ -33,10 +33,13 @@ struct BiasedFwdLaunch {
     CUtensorMap q, k, v;
     RangeDenseParams p;     // (o_sn and o_sh are not used: o is contiguous)
     ScoreMod mod;
-    // kModSplit: the K/V rows of every tile are cut into nchunk chunks (blockIdx.y); chunk c of a row writes partial c of P
+    // kModSplit: rows that several sequences share, a "token" is a sequence of the batch (kv_lo and kv_hi are not used).  The K/V rows of every
+    // tile are cut into nchunk chunks (blockIdx.y) of `chunk` tiles; chunk c of a row writes partial c of P
+    const int32_t* seq_len; // [N] own tokens of every sequence, the new one among them
+    int window;             // -1: none
     float* o_part;          // [N, Hq, P, D] unnormalised
     float2* ml;             // [N, Hq, P] reference maximum (log2 units) and sum
-    int P, nchunk;
+    int P, nchunk, chunk;
 };
 // which: kModCap, kModBias; split: with kModSplit.  l.p.TPT tokens a tile, max_tiles tiles at most.
 cudaError_t launch_biased_fwd(int D, int dtype, int which, bool split, const BiasedFwdLaunch& l, int max_tiles, cudaStream_t stream);

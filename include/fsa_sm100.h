@@ -219,7 +219,23 @@ int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, const int32
                         const int32_t* doc_ids, const int32_t* prefix_lens, const float* slopes, int64_t total_tokens, int64_t total_kv_rows, int batch,
                         int num_q_heads, int num_kv_heads, int head_dim, int dtype, int64_t q_stride_n, int64_t q_stride_h, int64_t k_stride_n,
                         int64_t v_stride_n, float sm_scale, float softcap, int window, void* o, float* lse, void* limits, int64_t limits_bytes, void* stream);
-/* dq, dk, dv contiguous; every row of them is written.  has_prefix: the forward was given prefix_lens.  Bit-reproducible. */
+/* The same scores for one new token of every sequence, the last of its seq_len[b] tokens, which the cache rows seq_row0[b] .. hold (next to
+ * fsa_decode_attn_partial).  Sequences may follow rows that they share: group i is the sequences cu_group[i] .. cu_group[i + 1] - 1, in front of
+ * whose own tokens stand the rows cu_shared[i] .. cu_shared[i + 1] - 1 of shared_k / shared_v, read once for all of them (num_groups 0: none; sequences
+ * behind the last group share nothing).  window: keys at least seq's length - 1 - window.  seq_len[b] <= 0: an idle place, o = 0, lse = -inf.
+ * q, o [B, Hq, D] contiguous, lse [B, Hq].  max_len, max_shared: how long the longest are, by which the work is cut; longer ones are
+ * read all the same.  Rows behind a sequence may hold anything.  scratch 32-byte aligned, of fsa_biased_decode_bytes bytes for the same sizes.
+ * Limits as above (batch, shared_rows and num_groups below 2^25, cache rows below 2^31). */
+int fsa_biased_decode_bytes(int batch, int num_q_heads, int num_kv_heads, int head_dim, int num_groups, int64_t max_len, int64_t max_shared, int window,
+                            int64_t* bytes_out);
+int fsa_biased_decode(const void* q, const void* k, const void* v, int64_t kv_rows, int64_t k_stride_n, int64_t v_stride_n, const int32_t* seq_len,
+                      const int32_t* seq_row0, const void* shared_k, const void* shared_v, int64_t shared_rows, int64_t shared_k_stride_n,
+                      int64_t shared_v_stride_n, const int32_t* cu_shared, const int32_t* cu_group, int num_groups, const float* slopes, int batch,
+                      int num_q_heads, int num_kv_heads, int head_dim, int dtype, float sm_scale, float softcap, int window, int64_t max_len,
+                      int64_t max_shared, void* o, float* lse, void* scratch, int64_t scratch_bytes, void* stream);
+/* What the waits of these kernels left: 0, or that one ran out (synchronises). */
+int fsa_biased_decode_read_status(int* status_out);
+/* fsa_biased_attn_fwd's gradient.  dq, dk, dv contiguous; every row of them is written.  has_prefix: the forward was given prefix_lens.  Bit-reproducible. */
 int fsa_biased_attn_bwd_bytes(int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads, int head_dim, int64_t* bytes_out);
 int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens_q,
                         const int32_t* cu_seqlens_k, const int32_t* doc_ids, int has_prefix, const float* slopes, int64_t total_tokens, int64_t total_kv_rows,
