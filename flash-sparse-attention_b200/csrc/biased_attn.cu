@@ -13,11 +13,27 @@ int make_tile_map_3d_box(CUtensorMap* map, const void* base, int dtype, int64_t 
                          int64_t stride2, int box1, int box2);
 int cuda_failed(cudaError_t e);
 
-// What the forward leaves for the backward: a status word, and for every token the first and last K/V row that it sees and its own place.
+// Set (atomicMax) by a kernel of these operators whose bounded wait ran out; read with fsa_biased_read_status.
+static __device__ int g_biased_status;
+
+// Its address on the current device (once per thread and device: a driver call).
+cudaError_t biased_status_word(int** out) {
+    static thread_local struct { int dev = -1; int* word = nullptr; } seen;
+    int dev = 0;
+    cudaError_t e = cudaGetDevice(&dev);
+    if (e == cudaSuccess && seen.dev != dev) {
+        void* p = nullptr;
+        if ((e = cudaGetSymbolAddress(&p, g_biased_status)) == cudaSuccess) { seen.dev = dev; seen.word = (int*)p; }
+    }
+    *out = seen.word;
+    return e;
+}
+
+// For every token the first and last K/V row that it sees and its own place.
 struct BiasedLimits {
-    int *status, *lo, *hi, *pos;
-    BiasedLimits(void* ws, int64_t N) : status((int*)ws), lo(status + 16), hi(lo + N), pos(hi + N) {}
-    static int64_t bytes(int64_t N) { return (16 + 3 * N) * 4; }
+    int *lo, *hi, *pos;
+    BiasedLimits(void* ws, int64_t N) : lo((int*)ws), hi(lo + N), pos(hi + N) {}
+    static int64_t bytes(int64_t N) { return 3 * N * 4; }
 };
 
 constexpr int kLimThreads = 256;
@@ -25,13 +41,13 @@ constexpr int kLimThreads = 256;
 // Last row j <= row of [first, row] that begins a document: whose id differs from that of the row before, or `first` itself.  All lanes of a
 // warp call it; 512 ids a step (one load is as long on its way as sixteen).
 __device__ __forceinline__ int document_start(const int32_t* __restrict__ ids, int first, int row, int lane) {
-    const int id = __ldg(ids + row);
+    const int id = __ldcg(ids + row);
     for (int end = row; end > first; end -= 512) {      // rows [end - 512, end) are looked at
         int found = -1;                                 // last row of another document among them
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             const int j = end - 1 - (i * 32 + lane);
-            if (j >= first && __ldg(ids + j) != id) found = max(found, j);
+            if (j >= first && __ldcg(ids + j) != id) found = max(found, j);
         }
         found = __reduce_max_sync(0xffffffffu, found);
         if (found >= 0) return found + 1;
@@ -39,55 +55,52 @@ __device__ __forceinline__ int document_start(const int32_t* __restrict__ ids, i
     return first;
 }
 
-// One thread per token.  Tokens of one sequence stand at consecutive K/V rows, the last of them at the sequence's last row.  Documents: a token
-// whose row does not begin one sees from where the token before it does, so a warp scans its tokens and searches only for those
-// that no such token precedes in it.  Rows behind the last sequence become zeros (lse: -inf).
+// One thread per token.  Tokens of one sequence stand at consecutive K/V rows.  Documents: a token whose row does not begin one sees from where the
+// token before it does, so a warp scans its tokens and searches only for those that no such token precedes in it.
 __global__ void __launch_bounds__(kLimThreads) biased_limits(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
                                                              const int32_t* __restrict__ doc_ids, const int32_t* __restrict__ prefix_lens, int B, int64_t N,
-                                                             int window, int Hq, int D, BiasedLimits out, uint4* __restrict__ o, float* __restrict__ lse) {
+                                                             int window, BiasedLimits out) {
     const int tid = threadIdx.x, lane = tid & 31;
-    const int64_t n0 = (int64_t)blockIdx.x * kLimThreads, n = n0 + tid;
-    if (n == 0) *out.status = kStatusOk;
-    const int used = __ldg(cu_q + B);
-    int lo = 0, hi = -1, pos = 0, seq = -1;
+    const int64_t n = (int64_t)blockIdx.x * kLimThreads + tid;
+    follow();
+    const int used = __ldcg(cu_q + B);
+    int seq = -1, k0 = 0;
+    Sees x = {0, -1, 0};
     if (n < used && n < N) {
-        seq = find_seq(cu_q, B, (int)n);
-        const int k0 = __ldg(cu_k + seq), k1 = __ldg(cu_k + seq + 1);
-        pos = (int)n + k1 - __ldg(cu_q + seq + 1);
-        if (pos >= k0) {            // (else the sequence has fewer keys than queries, and this one precedes them)
-            lo = window >= 0 ? max(k0, pos - window) : k0;
-            hi = prefix_lens ? max(pos, min(k0 + __ldg(prefix_lens + seq), k1) - 1) : pos;
-        }
+        seq = find_seq<true>(cu_q, B, (int)n);
+        k0 = __ldcg(cu_k + seq);
+        x = place_limits((int)n, k0, __ldcg(cu_k + seq + 1), __ldcg(cu_q + seq + 1), window, prefix_lens ? __ldcg(prefix_lens + seq) : 0);
     }
     if (doc_ids) {
-        const bool in = hi >= 0;
-        const int k0 = in ? __ldg(cu_k + seq) : 0, id = in ? __ldg(doc_ids + pos) : -1;
-        const bool begins = !in || pos == k0 || __ldg(doc_ids + pos - 1) != id;
+        const bool in = x.hi >= 0;
+        const int id = in ? __ldcg(doc_ids + x.pos) : -1;
+        const bool begins = !in || x.pos == k0 || __ldcg(doc_ids + x.pos - 1) != id;
         const int seq_before = __shfl_up_sync(0xffffffffu, seq, 1);
-        int start = begins ? pos : -1;                  // of the document, where it is known
+        int start = begins ? x.pos : -1;                // of the document, where it is known
         const bool head = lane == 0 || seq_before != seq;
         for (unsigned todo = __ballot_sync(0xffffffffu, head && !begins); todo; todo &= todo - 1) {
             const int src = __ffs(todo) - 1;
-            const int found = document_start(doc_ids, __shfl_sync(0xffffffffu, k0, src), __shfl_sync(0xffffffffu, pos, src), lane);
+            const int found = document_start(doc_ids, __shfl_sync(0xffffffffu, k0, src), __shfl_sync(0xffffffffu, x.pos, src), lane);
             if (lane == src) start = found;
         }
         // the nearest lane at or below this one that knows
         const unsigned known = __ballot_sync(0xffffffffu, start >= 0) & (0xffffffffu >> (31 - lane));
         start = __shfl_sync(0xffffffffu, start, known ? 31 - __clz(known) : lane);
         if (in) {
-            if (id < 0) hi = -1;
-            else lo = max(lo, start);
+            if (id < 0) x.hi = -1;
+            else x.lo = max(x.lo, start);
         }
     }
     if (n < N) {
-        out.lo[n] = hi >= 0 ? lo : 0;
-        out.hi[n] = hi;
-        out.pos[n] = pos;
+        out.lo[n] = x.hi >= 0 ? x.lo : 0;
+        out.hi[n] = x.hi;
+        out.pos[n] = x.pos;
     }
-    const int64_t tail = max(n0, (int64_t)used), end = min(n0 + kLimThreads, N), chunks = (int64_t)Hq * D / 8;
-    for (int64_t i = tail * chunks + tid; i < end * chunks; i += kLimThreads) o[i] = make_uint4(0u, 0u, 0u, 0u);
-    if (n >= tail && n < N)
-        for (int h = 0; h < Hq; ++h) lse[(int64_t)h * N + n] = -INFINITY;
+}
+
+static cudaError_t launch_limits(const int32_t* cu_q, const int32_t* cu_k, const int32_t* doc_ids, const int32_t* prefix_lens, int B, int64_t N, int window,
+                                 const BiasedLimits& out, cudaStream_t stream) {
+    return launch_dependent(biased_limits, dim3((unsigned)((N + kLimThreads - 1) / kLimThreads)), kLimThreads, 0, stream, 1, cu_q, cu_k, doc_ids, prefix_lens, B, N, window, out);
 }
 
 static int biased_shape(int64_t N, int64_t Nk, int B, int Hq, int Hk, int D, SelShape* s) {
@@ -150,16 +163,19 @@ extern "C" int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, 
     if ((rc = make_tile_map(&l.v, v, dtype, Nk, (int64_t)Hk * D, v_sn, 64))) return rc;
     cudaStream_t stream = (cudaStream_t)stream_;
     const BiasedLimits lim(limits, N);
-    biased_limits<<<(unsigned)((N + kLimThreads - 1) / kLimThreads), kLimThreads, 0, stream>>>(cu_seqlens_q, cu_seqlens_k, doc_ids, prefix_lens, B, N, window,
-                                                                                            Hq, D, lim, (uint4*)o, lse);
-    cudaError_t e = cudaGetLastError();
-    if (e != cudaSuccess) return cuda_failed(e);
-    l.mod.pos = lim.pos;
+    cudaError_t e;
     RangeDenseParams& p = l.p;
-    p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k; p.kv_lo = lim.lo; p.kv_hi = lim.hi;
+    if ((e = biased_status_word(&p.status)) != cudaSuccess) return cuda_failed(e);
+    p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k;
+    l.window = window; l.prefix_lens = prefix_lens;
+    if (doc_ids) {          // (else the kernel works them out for itself)
+        if ((e = launch_limits(cu_seqlens_q, cu_seqlens_k, doc_ids, nullptr, B, N, window, lim, stream)) != cudaSuccess) return cuda_failed(e);
+        p.kv_lo = lim.lo; p.kv_hi = lim.hi;
+        l.mod.pos = lim.pos;
+    }
     p.N = N; p.Nk = Nk; p.B = B; p.Hq = Hq; p.Hk = Hk; p.G = s.G; p.TPT = s.TPT;
     p.scale_log2 = sm_scale * kLog2e;
-    p.o = o; p.lse = lse; p.status = lim.status;
+    p.o = o; p.lse = lse;
     e = launch_biased_fwd(D, dtype, which, false, l, (int)((N + s.TPT - 1) / s.TPT) + B, stream);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
 }
@@ -174,9 +190,9 @@ extern "C" int fsa_biased_attn_bwd_bytes(int64_t N, int64_t Nk, int B, int Hq, i
 }
 
 extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o,
-                                   const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* doc_ids, int has_prefix, const float* slopes,
+                                   const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* doc_ids, const int32_t* prefix_lens, const float* slopes,
                                    int64_t N, int64_t Nk, int B, int Hq, int Hk, int D, int dtype, int64_t q_sn, int64_t q_sh, int64_t k_sn, int64_t v_sn,
-                                   int64_t do_sn, int64_t do_sh, float sm_scale, float softcap, void* dq, void* dk, void* dv, void* limits,
+                                   int64_t do_sn, int64_t do_sh, float sm_scale, float softcap, int window, void* dq, void* dk, void* dv, void* limits,
                                    int64_t limits_bytes, void* scratch, int64_t scratch_bytes, void* stream_) {
     SelShape s;
     int rc = biased_shape(N, Nk, B, Hq, Hk, D, &s);
@@ -184,7 +200,7 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     if (dtype != FSA_DTYPE_BF16 && dtype != FSA_DTYPE_FP16) return FSA_ERR_BAD_ARG;
     ScoreMod mod;
     int which;
-    if ((rc = biased_mod(sm_scale, softcap, slopes, doc_ids, has_prefix, &mod, &which))) return rc;
+    if ((rc = biased_mod(sm_scale, softcap, slopes, doc_ids, prefix_lens != nullptr, &mod, &which))) return rc;
     if (N == 0) return FSA_OK;
     if (!q || !k || !v || !o || !lse || !d_o || !cu_seqlens_q || !cu_seqlens_k || !dq || !dk || !dv || !limits || !scratch || Nk == 0) return FSA_ERR_BAD_ARG;
     for (const void* x : {q, k, v, o, d_o, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)limits, (const void*)scratch})
@@ -220,9 +236,18 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     plan.items = plan.multi + plan.max_tiles;
     sp += align_up(range_kv_plan_bytes(s), 1024);
     a.slabs = (float*)sp;
-    cudaError_t e = launch_range_bwd_plan(plan, a, lim.status, stream);
+    // with documents the forward has left the limits
+    cudaError_t e = doc_ids ? cudaSuccess : launch_limits(cu_seqlens_q, cu_seqlens_k, nullptr, prefix_lens, B, N, window, lim, stream);
+    int* status = nullptr;
+    if (e == cudaSuccess) e = biased_status_word(&status);
+    if (e == cudaSuccess) e = launch_range_bwd_plan(plan, a, nullptr, stream, true);
     if (e == cudaSuccess) e = launch_sel_bwd_delta(dtype, a, s, stream);
-    if (e == cudaSuccess) e = launch_range_bwd_dq(dtype, a, s, kmap, vmap, lim.status, stream, &mod, which);
-    if (e == cudaSuccess) e = launch_range_bwd_dkdv(dtype, plan, a, s, kmap, vmap, lim.status, stream, &mod, which);
+    if (e == cudaSuccess) e = launch_range_bwd_dq(dtype, a, s, kmap, vmap, status, stream, &mod, which);
+    if (e == cudaSuccess) e = launch_range_bwd_dkdv(dtype, plan, a, s, kmap, vmap, status, stream, &mod, which);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
+}
+
+extern "C" int fsa_biased_read_status(int* status_out) {
+    if (!status_out) return FSA_ERR_BAD_ARG;
+    return cudaMemcpyFromSymbol(status_out, g_biased_status, sizeof(int)) == cudaSuccess ? FSA_OK : FSA_ERR_CUDA;
 }

@@ -18,9 +18,7 @@ int make_tile_map_3d_box(CUtensorMap* map, const void* base, int dtype, int64_t 
                          int64_t stride2, int box1, int box2);
 int device_sm_count(int* out);
 int cuda_failed(cudaError_t e);
-
-// Set (atomicMax) by a kernel whose bounded wait ran out; read with fsa_biased_decode_read_status.
-static __device__ int g_biased_decode_status;
+cudaError_t biased_status_word(int** out);      // biased_attn.cu
 
 constexpr int kBdKT = 64;           // rows of a stage
 constexpr int kBdStages = 3;
@@ -38,6 +36,7 @@ struct BiasedDecodeParams {
     ScoreMod mod;
     float* o_part;              // [B, Hq, P, D]
     float2* ml;                 // [B, Hq, P]
+    int* status;
 };
 
 template <int D, bool HI, int MOD, typename ET>
@@ -50,7 +49,7 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
     constexpr int NK = D / 16;                           // k-steps of Q K^T
     constexpr int NO = D / 8;                            // 8-column output tiles of P V
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t limit = wait_limit(&g_biased_decode_status);
+    const uint32_t limit = wait_limit(p.status);
     uint64_t* full = reinterpret_cast<uint64_t*>(base + (size_t)kBdStages * STAGE_BYTES);
     uint64_t* empty = full + kBdStages;
     float* smm = reinterpret_cast<float*>(empty + kBdStages);    // [4][16]
@@ -91,7 +90,7 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
             const int row = p.row0[b] + lo;
             for (int it = 0; it * kBdKT < n; ++it) {
                 const int s = it % kBdStages;
-                if (it >= kBdStages && !mbar_wait(&empty[s], ((it / kBdStages) - 1) & 1, &g_biased_decode_status, limit)) break;
+                if (it >= kBdStages && !mbar_wait(&empty[s], ((it / kBdStages) - 1) & 1, p.status, limit)) break;
                 mbar_expect_tx(&full[s], STAGE_BYTES);
                 const uint32_t kb = sbase + s * STAGE_BYTES;
 #pragma unroll
@@ -131,7 +130,7 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
         bool ok = true;
         for (int it = 0; it * kBdKT < n; ++it) {
             const int s = it % kBdStages;
-            ok = mbar_wait(&full[s], (it / kBdStages) & 1, &g_biased_decode_status, limit);
+            ok = mbar_wait(&full[s], (it / kBdStages) & 1, p.status, limit);
             if (!warp_stays(ok)) break;
             const int k0 = it * kBdKT + warp * 16;               // first key of this warp's tile
             if (k0 < n) {
@@ -272,53 +271,72 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
 }
 
 // o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, lse = M + log2 of the latter, over the P partials of every row; 0 and -inf for a row that saw
-// nothing.  A sequence behind the last group (*grouped is their number) has no shared partials.  WARPS warps a row: a row's partials arrive in
-// P / (4 WARPS) rounds of loads.
+// nothing.  A sequence behind the last group (*grouped is their number) has no shared partials.  WARPS warps a row: what it takes is round trips to L2, so
+// all maxima and sums, and the first 16 partials of every warp, are asked for at once (1 x 8191 tokens, 32 heads, 64 partials a row: 12 us with
+// a round trip for every four partials of a warp).
+constexpr int kMgThreads = 128, kMgAhead = 16;
 template <int D, int WARPS, typename ET>
-__global__ void __launch_bounds__(128) biased_decode_merge(const float* o_part, const float2* ml, int64_t rows, int Hq, int P, int nshared, const int32_t* grouped,
-                                                           ET* __restrict__ o, float* __restrict__ lse) {
+__global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const float* o_part, const float2* ml, int64_t rows, int Hq, int P, int nshared, const int32_t* grouped,
+                                                                  ET* __restrict__ o, float* __restrict__ lse) {
     constexpr int V = D / 32;           // columns of a lane
-    __shared__ float4 s_acc[WARPS > 1 ? 4 : 1][32];
+    __shared__ float s_m[4], s_l[4];
+    __shared__ float4 s_acc[4][32];
     const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-    const int64_t row = (int64_t)blockIdx.x * (4 / WARPS) + warp / WARPS;
     const int w = warp % WARPS;
+    const int64_t row = (int64_t)blockIdx.x * (4 / WARPS) + warp / WARPS;
     follow();
-    if (row >= rows) return;            // (all warps of a row, and with WARPS > 1 the whole CTA)
-    const float2* mlr = ml + row * P;
+    if (row >= rows) return;            // (with WARPS = 4 there is no such CTA)
     const int first = nshared > 0 && row / Hq >= *grouped ? nshared : 0;
-    float M = -INFINITY;
-    for (int i = first + lane; i < P; i += 32) {
-        const float2 v = __ldcg(mlr + i);
-        if (v.y > 0.f) M = fmaxf(M, v.x);
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) M = fmaxf(M, __shfl_xor_sync(0xffffffffu, M, d));
-    float L = 0.f;
-    for (int i = first + lane; i < P; i += 32) {
-        const float2 v = __ldcg(mlr + i);
-        if (v.y > 0.f) L += ex2_approx(v.x - M) * v.y;
-    }
-#pragma unroll
-    for (int d = 16; d; d >>= 1) L += __shfl_xor_sync(0xffffffffu, L, d);
-    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    const float2* mlr = ml + row * P;
     const float* src = o_part + row * P * D + lane * V;
-    for (int i0 = first + w; i0 < P; i0 += 4 * WARPS) {
-        float x[4][4], f[4];
+    auto load = [&](int i, float (&x)[4]) {
+        x[2] = x[3] = 0.f;
+        if constexpr (V == 4) *reinterpret_cast<float4*>(x) = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)i * D));
+        else *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(src + (int64_t)i * D));
+    };
+    float x[kMgAhead][4];
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            const int i = i0 + j * WARPS;
-            const float2 v = i < P ? __ldcg(mlr + i) : make_float2(0.f, 0.f);
-            f[j] = v.y > 0.f ? ex2_approx(v.x - M) : 0.f;           // (a partial without keys has no o)
-            x[j][0] = x[j][1] = x[j][2] = x[j][3] = 0.f;
-            if (v.y > 0.f) {
-                if constexpr (V == 4) *reinterpret_cast<float4*>(x[j]) = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)i * D));
-                else *reinterpret_cast<float2*>(x[j]) = __ldcg(reinterpret_cast<const float2*>(src + (int64_t)i * D));
-            }
+    for (int j = 0; j < kMgAhead; ++j)
+        if (first + w + WARPS * j < P) load(first + w + WARPS * j, x[j]);
+    float M = -INFINITY, L = 0.f;
+    for (int i = first + w * 32 + lane; i < P; i += 32 * WARPS) {
+        const float2 v = __ldcg(mlr + i);
+        if (v.y > 0.f) {
+            const float m = fmaxf(M, v.x);
+            L = L * ex2_approx(M - m) + v.y * ex2_approx(v.x - m);
+            M = m;
         }
+    }
+    auto join = [&](float m2, float l2) {
+        const float m = fmaxf(M, m2), use = m == -INFINITY ? 0.f : m;
+        L = L * ex2_approx(M - use) + l2 * ex2_approx(m2 - use);
+        M = m;
+    };
 #pragma unroll
-        for (int j = 0; j < 4; ++j)
+    for (int d = 16; d; d >>= 1) join(__shfl_xor_sync(0xffffffffu, M, d), __shfl_xor_sync(0xffffffffu, L, d));
+    if constexpr (WARPS > 1) {
+        if (lane == 0) { s_m[warp] = M; s_l[warp] = L; }
+        __syncthreads();
+        M = -INFINITY; L = 0.f;
 #pragma unroll
-            for (int k = 0; k < V; ++k) acc[k] = fmaf(f[j], x[j][k], acc[k]);
+        for (int i = 0; i < WARPS; ++i) join(s_m[i], s_l[i]);
+    }
+    float acc[4] = {0.f, 0.f, 0.f, 0.f};
+    auto add = [&](int i, const float (&y)[4]) {
+        const float2 v = __ldcg(mlr + i);
+        if (v.y > 0.f) {                // (a partial without keys has no o)
+            const float f = ex2_approx(v.x - M);
+#pragma unroll
+            for (int k = 0; k < V; ++k) acc[k] = fmaf(f, y[k], acc[k]);
+        }
+    };
+#pragma unroll
+    for (int j = 0; j < kMgAhead; ++j)
+        if (first + w + WARPS * j < P) add(first + w + WARPS * j, x[j]);
+    for (int i = first + w + WARPS * kMgAhead; i < P; i += WARPS) {
+        float y[4];
+        load(i, y);
+        add(i, y);
     }
     if constexpr (WARPS > 1) {
         s_acc[warp][lane] = make_float4(acc[0], acc[1], acc[2], acc[3]);
@@ -334,7 +352,7 @@ __global__ void __launch_bounds__(128) biased_decode_merge(const float* o_part, 
     ET* dst = o + row * D + lane * V;
     if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(ElemTraits<ET>::pack2(acc[0] * inv, acc[1] * inv), ElemTraits<ET>::pack2(acc[2] * inv, acc[3] * inv));
     else *reinterpret_cast<uint32_t*>(dst) = ElemTraits<ET>::pack2(acc[0] * inv, acc[1] * inv);
-    if (lane == 0 && w == 0) lse[row] = L > 0.f ? M + log2f(L) : -INFINITY;
+    if (lane == 0) lse[row] = L > 0.f ? M + log2f(L) : -INFINITY;
 }
 
 template <int D, bool HI, int MOD, typename ET>
@@ -360,31 +378,37 @@ static cudaError_t launch_bd_which(int which, const BiasedDecodeParams& p, const
 template <int D, typename ET>
 static cudaError_t launch_merge(const float* o_part, const float2* ml, int64_t rows, int Hq, int P, int nshared, const int32_t* grouped, void* o, float* lse,
                                 cudaStream_t stream) {
-    // four warps a row while that many still run at once
-    if (rows <= 2048)
-        return launch_dependent(biased_decode_merge<D, 4, ET>, dim3((unsigned)rows), 128, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, grouped, (ET*)o, lse);
-    return launch_dependent(biased_decode_merge<D, 1, ET>, dim3((unsigned)((rows + 3) / 4)), 128, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, grouped, (ET*)o, lse);
+    // a CTA per row while all of them still run at once
+    if (rows <= 4 * sm_count())
+        return launch_dependent(biased_decode_merge<D, 4, ET>, dim3((unsigned)rows), kMgThreads, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, grouped, (ET*)o, lse);
+    return launch_dependent(biased_decode_merge<D, 1, ET>, dim3((unsigned)((rows + 3) / 4)), kMgThreads, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, grouped, (ET*)o,
+                            lse);
 }
 
-// How a decode call is cut: partials of the shared rows, of the own ones.  Own rows: chunks as long as they may be (few partials, a ring that stays
-// full) while about four CTAs an SM are left, up to 1024 rows.  Shared rows: about two items an SM (what runs at once), at least two tiles each.
+// How a decode call is cut: partials of the shared rows, of the own ones.  Own rows: as many chunks as run at once, two CTAs an SM, and chunks of up to
+// 1024 rows where there is more to read than that.  Shared rows: as many items as run at once as well, of at least two tiles.
 struct DecodeCut {
-    int parts, own, nown, tiles, nshared;       // own: rows of a chunk; tiles: 64-row tiles of a shared chunk
+    int parts, own, nown, tiles, nshared, mtiles;       // own: rows of a chunk; tiles: 64-row tiles of a shared chunk; mtiles: tiles of 128 queries at most
     DecodeCut(int B, int Hk, int G, int TPT, int groups, int64_t max_len, int64_t max_shared, int window) {
         const int sms = sm_count();
         parts = (G + 15) / 16;
         int64_t rows = max_len < 1 ? 1 : max_len;
         if (window >= 0 && rows > (int64_t)window + 1) rows = (int64_t)window + 1;
-        const int64_t ctas = 4 * sms, per = (rows * B * Hk * parts + ctas - 1) / ctas;
-        int64_t c = (per + kBdKT - 1) / kBdKT * kBdKT;
+        const int64_t heads = (int64_t)B * Hk * parts, each = heads > 0 ? 2 * sms / heads : 1;      // chunks of a sequence and kv head
+        int64_t c = each > 0 ? (rows + each - 1) / each : 1024;
+        // (more sequences and kv heads than run at once, of unlike lengths: about four turns)
+        if (each == 0 && rows * heads < 8 * (int64_t)sms * 1024) c = (rows * heads + 8 * sms - 1) / (8 * sms);
+        c = (c + kBdKT - 1) / kBdKT * kBdKT;
         c = c < kBdKT ? kBdKT : c > 1024 ? 1024 : c;
         own = (int)c;
         nown = (int)((rows + c - 1) / c);
-        tiles = nshared = 0;
+        tiles = nshared = mtiles = 0;
         if (groups > 0) {
-            const int64_t mtiles = (int64_t)(B + TPT - 1) / TPT > groups ? (B + TPT - 1) / TPT : groups;
+            // (a group's last tile has one sequence at least; a place in the grid that no tile takes would hold up one that does)
+            mtiles = B > groups ? (B - groups) / TPT + groups : B > 0 ? B : 1;
             const int64_t blocks = max_shared < 1 ? 1 : (max_shared + kRdBK - 1) / kRdBK;
-            int64_t n = (2 * sms + mtiles * Hk - 1) / (mtiles * Hk);
+            int64_t n = 2 * sms / ((int64_t)mtiles * Hk);
+            if (n < 1) n = 1;
             if (n > (blocks + 1) / 2) n = (blocks + 1) / 2;
             if (n > 256) n = 256;
             tiles = (int)((blocks + n - 1) / n);
@@ -393,19 +417,6 @@ struct DecodeCut {
     }
     int partials() const { return nshared + nown; }
 };
-
-// The status word's address on the current device (once per thread and device: a driver call).
-static cudaError_t status_word(int** out) {
-    static thread_local struct { int dev = -1; int* word = nullptr; } seen;
-    int dev = 0;
-    cudaError_t e = cudaGetDevice(&dev);
-    if (e == cudaSuccess && seen.dev != dev) {
-        void* p = nullptr;
-        if ((e = cudaGetSymbolAddress(&p, g_biased_decode_status)) == cudaSuccess) { seen.dev = dev; seen.word = (int*)p; }
-    }
-    *out = seen.word;
-    return e;
-}
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
 
@@ -465,28 +476,11 @@ extern "C" int fsa_biased_decode(const void* q, const void* k, const void* v, in
     }
     mod.slopes = slopes;
     cudaError_t e;
-    if (has_shared) {
-        int* status = nullptr;
-        if ((e = status_word(&status)) != cudaSuccess) return cuda_failed(e);
-        BiasedFwdLaunch l = {};
-        if ((rc = make_tile_map_3d_box(&l.q, q, dtype, D, B, Hq, (int64_t)Hq * D, D, TPT, G))) return rc;
-        if ((rc = make_tile_map(&l.k, shared_k, dtype, shared_rows, packed, shared_k_stride_n, kRdBK))) return rc;
-        if ((rc = make_tile_map(&l.v, shared_v, dtype, shared_rows, packed, shared_v_stride_n, kRdBK))) return rc;
-        RangeDenseParams& p = l.p;
-        p.cu_q = cu_group; p.cu_k = cu_shared;
-        p.N = B; p.Nk = shared_rows; p.B = num_groups; p.Hq = Hq; p.Hk = Hk; p.G = G; p.TPT = TPT;
-        p.scale_log2 = sm_scale * kLog2e;
-        p.status = status;
-        l.mod = mod;
-        l.seq_len = seq_len; l.window = window;
-        l.o_part = o_part; l.ml = ml; l.P = P; l.nchunk = cut.nshared; l.chunk = cut.tiles;
-        e = launch_biased_fwd(D, dtype, which, true, l, (B + TPT - 1) / TPT + num_groups, stream);
-        if (e != cudaSuccess) return cuda_failed(e);
-    }
     BiasedDecodeParams p = {};
     p.q = q; p.seq_len = seq_len; p.row0 = seq_row0;
     p.B = B; p.Hq = Hq; p.Hk = Hk; p.G = G; p.parts = cut.parts; p.window = window; p.chunk = cut.own; p.nchunk = cut.nown; p.P = P; p.p0 = cut.nshared;
     p.scale_log2 = sm_scale * kLog2e; p.mod = mod; p.o_part = o_part; p.ml = ml;
+    if ((e = biased_status_word(&p.status)) != cudaSuccess) return cuda_failed(e);
     CUtensorMap kmap, vmap;
     if ((rc = make_tile_map(&kmap, k, dtype, kv_rows, packed, k_stride_n, kBdKT))) return rc;
     if ((rc = make_tile_map(&vmap, v, dtype, kv_rows, packed, v_stride_n, kBdKT))) return rc;
@@ -494,14 +488,26 @@ extern "C" int fsa_biased_decode(const void* q, const void* k, const void* v, in
     if (D == 128) e = bf16 ? launch_bd_which<128, __nv_bfloat16>(which, p, kmap, vmap, stream) : launch_bd_which<128, __half>(which, p, kmap, vmap, stream);
     else e = bf16 ? launch_bd_which<64, __nv_bfloat16>(which, p, kmap, vmap, stream) : launch_bd_which<64, __half>(which, p, kmap, vmap, stream);
     if (e != cudaSuccess) return cuda_failed(e);
+    // (beside the own rows' kernel: neither needs anything of the other)
+    if (has_shared) {
+        BiasedFwdLaunch l = {};
+        if ((rc = make_tile_map_3d_box(&l.q, q, dtype, D, B, Hq, (int64_t)Hq * D, D, TPT, G))) return rc;
+        if ((rc = make_tile_map(&l.k, shared_k, dtype, shared_rows, packed, shared_k_stride_n, kRdBK))) return rc;
+        if ((rc = make_tile_map(&l.v, shared_v, dtype, shared_rows, packed, shared_v_stride_n, kRdBK))) return rc;
+        RangeDenseParams& r = l.p;
+        r.cu_q = cu_group; r.cu_k = cu_shared;
+        r.N = B; r.Nk = shared_rows; r.B = num_groups; r.Hq = Hq; r.Hk = Hk; r.G = G; r.TPT = TPT;
+        r.scale_log2 = sm_scale * kLog2e;
+        r.status = p.status;
+        l.mod = mod;
+        l.seq_len = seq_len; l.window = window;
+        l.o_part = o_part; l.ml = ml; l.P = P; l.nchunk = cut.nshared; l.chunk = cut.tiles;
+        e = launch_biased_fwd(D, dtype, which, true, l, cut.mtiles, stream);
+        if (e != cudaSuccess) return cuda_failed(e);
+    }
     const int32_t* grouped = has_shared ? cu_group + num_groups : nullptr;
     auto merge = [&](auto run) { return run(o_part, ml, rows, Hq, P, cut.nshared, grouped, o, lse, stream); };
     if (D == 128) e = bf16 ? merge(launch_merge<128, __nv_bfloat16>) : merge(launch_merge<128, __half>);
     else e = bf16 ? merge(launch_merge<64, __nv_bfloat16>) : merge(launch_merge<64, __half>);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
-}
-
-extern "C" int fsa_biased_decode_read_status(int* status_out) {
-    if (!status_out) return FSA_ERR_BAD_ARG;
-    return cudaMemcpyFromSymbol(status_out, g_biased_decode_status, sizeof(int)) == cudaSuccess ? FSA_OK : FSA_ERR_CUDA;
 }

@@ -38,67 +38,80 @@ template <int D, int MOD, typename ET>
 __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constant__ BiasedFwdLaunch launch) {
     constexpr int BK = kRdBK, KH = D / 64;
     constexpr int kQ = kTileRows * D * 2;
-    constexpr int kSlabQ = kTileRows * 128;          // 64 columns of the Q tile, and of two K tiles
+    constexpr int kSlabQ = kTileRows * 128;          // 64 columns of the Q tile
     constexpr int kKt = BK * D * 2;                  // one K (or V) tile
     constexpr uint32_t kCols = 256;
     constexpr int cS = 0, cO = 2 * BK;
     constexpr bool kSplit = (MOD & kModSplit) != 0;
     extern __shared__ __align__(1024) uint8_t smem[];
     uint8_t* sQ = smem;
-    uint8_t* sK = sQ + kQ;                           // two tiles: the lower rows first
+    uint8_t* sK = sQ + kQ;                           // [2]
     uint8_t* sV = sK + 2 * kKt;                      // [kBfV]
     uint64_t* bars = reinterpret_cast<uint64_t*>(sV + kBfV * kKt);
     uint64_t* q_full = bars;
     uint64_t* q_empty = bars + 1;       // the item's last S product is done
-    uint64_t* k_full = bars + 2;
-    uint64_t* k_empty = bars + 3;       // S of a pair of tiles is done with K
-    uint64_t* s_full = bars + 4;        // ... and there to be read
-    uint64_t* p_full = bars + 5;        // [2] P of a pair's lower / upper tile is in its place
-    uint64_t* pv_done = bars + 7;       // [2] ... and has been multiplied
-    uint64_t* v_full = bars + 9;        // [kBfV]
+    uint64_t* k_full = bars + 2;        // [2]
+    uint64_t* k_empty = bars + 4;       // [2] S of the tile is done with K
+    uint64_t* s_full = bars + 6;        // [2] ... and there to be read
+    uint64_t* p_full = bars + 8;        // [2] P is in its place
+    uint64_t* pv_done = bars + 10;      // [2] ... and has been multiplied
+    uint64_t* v_full = bars + 12;       // [kBfV]
     uint64_t* v_empty = v_full + kBfV;  // [kBfV]
     uint64_t* o_free = v_empty + kBfV;  // the 128 row threads have read an item's accumulator
     uint64_t* it_full = o_free + 1;     // the next item is known
     uint64_t* it_empty = o_free + 2;    // ... has been taken by the five other warps
     uint64_t* claim = o_free + 3;       // the answer to a claim has arrived
-    int* s_claim = reinterpret_cast<int*>(bars + 20);    // 16 bytes
-    int4* s_item = reinterpret_cast<int4*>(bars + 22);   // [2 items][2]
-    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 30);
-    int* status = reinterpret_cast<int*>(bars + 30) + 1;     // of this CTA
+    int* s_claim = reinterpret_cast<int*>(bars + 22);    // 16 bytes
+    int4* s_item = reinterpret_cast<int4*>(bars + 24);   // [2 items][2]
+    uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(bars + 32);
+    int* status = reinterpret_cast<int*>(bars + 32) + 1;     // of this CTA
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const RangeDenseParams& p = launch.p;
     const uint32_t limit = wait_limit(p.status);
     const int G = p.G, TPT = p.TPT;
     // First and last K/V row that a token sees, and its place.  kModSplit: a token is a sequence of the batch, whose own rows follow the shared ones.
-    struct Sees { int lo, hi, pos; };
     auto limits = [&](int seq, int tok) {
         Sees x;
         if constexpr (kSplit) {
-            const int k0 = __ldg(p.cu_k + seq), k1 = __ldg(p.cu_k + seq + 1), len = __ldg(launch.seq_len + tok);
+            const int k0 = __ldcg(p.cu_k + seq), k1 = __ldcg(p.cu_k + seq + 1), len = __ldcg(launch.seq_len + tok);
             x.pos = k1 + len - 1;
             x.lo = launch.window >= 0 ? max(k0, x.pos - launch.window) : k0;
             x.hi = len > 0 ? k1 - 1 : -1;
+        } else if (p.kv_lo) {
+            x.lo = __ldcg(p.kv_lo + tok);
+            x.hi = __ldcg(p.kv_hi + tok);
+            x.pos = (MOD & kModBias) ? __ldcg(launch.mod.pos + tok) : 0;
         } else {
-            x.lo = __ldg(p.kv_lo + tok);
-            x.hi = __ldg(p.kv_hi + tok);
-            x.pos = (MOD & kModBias) ? __ldg(launch.mod.pos + tok) : 0;
+            const int k0 = __ldcg(p.cu_k + seq), k1 = __ldcg(p.cu_k + seq + 1);
+            x = place_limits(tok, k0, k1, __ldcg(p.cu_q + seq + 1), launch.window, launch.prefix_lens ? __ldcg(launch.prefix_lens + seq) : 0);
         }
         return x;
     };
+    if constexpr (!kSplit) follow_late();
     if (tid == 0) {
         *status = kStatusOk;
-        mbar_init(q_full, 1); mbar_init(q_empty, 1); mbar_init(k_full, 1); mbar_init(k_empty, 1); mbar_init(s_full, 1);
-        for (int i = 0; i < 2; ++i) { mbar_init(&p_full[i], 128); mbar_init(&pv_done[i], 1); }
+        mbar_init(q_full, 1); mbar_init(q_empty, 1);
+        for (int i = 0; i < 2; ++i) {
+            mbar_init(&k_full[i], 1); mbar_init(&k_empty[i], 1); mbar_init(&s_full[i], 1);
+            mbar_init(&p_full[i], 128); mbar_init(&pv_done[i], 1);
+        }
         for (int i = 0; i < kBfV; ++i) { mbar_init(&v_full[i], 1); mbar_init(&v_empty[i], 1); }
         mbar_init(o_free, 128); mbar_init(it_full, 1); mbar_init(it_empty, 5); mbar_init(claim, 1);
         mbar_init_fence();
     }
-    if (warp == 0) tmem_alloc(&tmem_slot, kCols);
-    tc_fence_before();
-    __syncthreads();
-    tc_fence_after();
-    const uint32_t tbase = tmem_slot;
+    // (warp 0 has set the barriers up itself and needs no TMEM: it goes on to find its item)
+    if (warp == 0) {
+        __syncwarp();
+        asm volatile("bar.arrive 2, 192;" ::: "memory");
+    } else {
+        if (warp == 1) tmem_alloc(&tmem_slot, kCols);
+        tc_fence_before();
+        asm volatile("bar.sync 2, 192;" ::: "memory");
+        tc_fence_after();
+        if constexpr (!kSplit) let_next_start();
+    }
+    const uint32_t tbase = warp ? tmem_slot : 0u;
     // Item n of this CTA.  Each of the five other warps takes every item once, in order; z < 0 ends the list.
     auto read_item = [&](int n) {
         const int4 x = s_item[(n & 1) * 2], y = s_item[(n & 1) * 2 + 1];
@@ -119,7 +132,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
     if (warp == 0) {
         // ------------------------------------------------------------------ items and TMA producer
         bool ok = true;
-        int n = 0, claims = 0, qi = 0, pc = 0, c = 0;           // items, claims, non-empty items, pairs and tiles of K/V rows so far
+        int n = 0, claims = 0, qi = 0, c = 0;           // items, claims, non-empty items, K/V tiles so far
         int bx = blockIdx.x, z = blockIdx.y;
         while (ok) {
             bool asked = false;
@@ -158,37 +171,48 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                 ++n;
                 if (lane == 0 && nblk > 0) {
                     ok = ok && mbar_wait(q_empty, (qi & 1) ^ 1, status, limit);
-                    ask();                  // not earlier: a CTA is to be one item ahead, not to take the share of others
+                    if constexpr (!kSplit) ask();       // not earlier: a CTA is to be one item ahead, not to take the share of others
                     if (ok) {
                         mbar_expect_tx(q_full, (uint32_t)(KH * 128 * TPT * G));
 #pragma unroll
                         for (int b = 0; b < KH; ++b) tma_load_3d(smem_u32(sQ + b * kSlabQ), &launch.q, b * 64, tok0, h * G, q_full);
                     }
-                    int vc = c;
-                    for (int t = nblk - 1, i = pc; t >= 0 && ok; t -= 2, ++i) {
-                        const int t0 = max(t - 1, 0);            // lower tile of the pair
-                        ok = ok && mbar_wait(k_empty, (i & 1) ^ 1, status, limit);
-                        if (!ok) break;
-                        mbar_expect_tx(k_full, (uint32_t)((t - t0 + 1) * kKt));
-                        for (int u = t0; u <= t; ++u)
+                    // K and V tiles in the order that the MMA warp needs them: K(0), K(1), V(0), K(2), V(1), ...
+                    for (int step = 0; step < nblk + 1 && ok; ++step) {
+                        const int jk = c + step, jv = jk - 1;
+                        if (step < nblk) {
+                            const int st = jk & 1;
+                            ok = ok && mbar_wait(&k_empty[st], ((jk >> 1) & 1) ^ 1, status, limit);
+                            if (!ok) break;
+                            mbar_expect_tx(&k_full[st], (uint32_t)kKt);
 #pragma unroll
                             for (int b = 0; b < KH; ++b)
-                                tma_load_2d(smem_u32(sK + b * kSlabQ + (u - t0) * (BK * 128)), &launch.k, h * D + b * 64, lo + u * BK, k_full);
-                        for (int u = t; u >= t0 && ok; --u, ++vc) {
-                            const int st = vc % kBfV;
-                            ok = ok && mbar_wait(&v_empty[st], ((vc / kBfV) & 1) ^ 1, status, limit);
+                                tma_load_2d(smem_u32(sK + st * kKt + b * (BK * 128)), &launch.k, h * D + b * 64, lo + (nblk - 1 - step) * BK, &k_full[st]);
+                        }
+                        if (step > 0) {
+                            const int st = jv % kBfV;
+                            ok = ok && mbar_wait(&v_empty[st], ((jv / kBfV) & 1) ^ 1, status, limit);
                             if (!ok) break;
                             mbar_expect_tx(&v_full[st], (uint32_t)kKt);
 #pragma unroll
                             for (int b = 0; b < KH; ++b)
-                                tma_load_2d(smem_u32(sV + st * kKt + b * (BK * 128)), &launch.v, h * D + b * 64, lo + u * BK, &v_full[st]);
+                                tma_load_2d(smem_u32(sV + st * kKt + b * (BK * 128)), &launch.v, h * D + b * 64, lo + (nblk - step) * BK, &v_full[st]);
                         }
                     }
                 }
                 c += nblk;
-                pc += (nblk + 1) / 2;
                 qi += nblk > 0;
+            } else if constexpr (!kSplit) {
+                // There are max_tiles >= N / TPT + B places in the list and at most used / TPT + B tiles: those left over clear the rows behind the
+                // last sequence, TPT tokens each.
+                const int64_t t0 = (int64_t)__ldcg(p.cu_q + p.B) + (int64_t)tok0 * TPT;
+                const int nt = (int)min((int64_t)TPT, p.N - t0);
+                for (int i = lane; i < nt * G; i += 32) p.lse[(int64_t)(h * G + i % G) * p.N + t0 + i / G] = -INFINITY;
+                for (int i = lane; i < nt * (G * D / 8); i += 32)
+                    reinterpret_cast<uint4*>(p.o)[((t0 + i / (G * D / 8)) * p.Hq + h * G) * (D / 8) + i % (G * D / 8)] = make_uint4(0u, 0u, 0u, 0u);
             }
+            // (chunks: an item a CTA.  Beside another kernel some CTAs start late, and the early ones would have taken their items: twice the time)
+            if constexpr (kSplit) break;
             if (lane == 0 && !asked) ask();
             // (the answer is in shared memory before this CTA may end, whatever happened above)
             const bool answered = mbar_wait(claim, claims & 1, status, limit);
@@ -210,60 +234,59 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
     } else if (warp == 1) {
         // ------------------------------------------------------------------ MMA issuer
         const bool leader = elect_one();
-        constexpr uint32_t idesc_two = umma_idesc(ElemTraits<ET>::kIsBF16, 128, 2 * BK, false, false);
-        constexpr uint32_t idesc_one = umma_idesc(ElemTraits<ET>::kIsBF16, 128, BK, false, false);
+        constexpr uint32_t idesc_s = umma_idesc(ElemTraits<ET>::kIsBF16, 128, BK, false, false);
         constexpr uint32_t idesc_o = umma_idesc(ElemTraits<ET>::kIsBF16, 128, D, false, true);
         constexpr uint32_t hi_1024 = umma_desc_hi(1024);
         const uint32_t q_lo = umma_desc_lo(smem_u32(sQ), 16);
         const uint32_t k_lo = umma_desc_lo(smem_u32(sK), 16);
         const uint32_t v_lo = umma_desc_lo(smem_u32(sV), BK * 128);     // MN-major: LBO = slab stride
         bool ok = true;
-        int n = 0, qi = 0, pc = 0, hc = 0, c = 0;              // hc: pairs of two tiles so far
+        int n = 0, qi = 0, c = 0;
+        // S(t) takes the place of P(t - 2): products of two shapes may run in another order than they were issued, so it waits for the one that
+        // reads P(t - 2)
+        auto issue_s = [&](int t, bool last) {
+            const int st = t & 1;
+            ok = ok && mbar_wait(&k_full[st], (t >> 1) & 1, status, limit);
+            if (t >= 2) ok = ok && mbar_wait(&pv_done[st], ((t - 2) >> 1) & 1, status, limit);
+            ok = warp_ok(ok);
+            if (!ok) return;
+            tc_fence_after();
+            if (leader) {
+                constexpr int kSlabB = (BK * 128) >> 4;
+                const uint32_t b_lo = k_lo + (uint32_t)(st * (kKt >> 4));
+#pragma unroll
+                for (int ks = 0; ks < D / 16; ++ks)
+                    umma_ss(tbase + cS + st * BK, umma_desc_pack(q_lo + (ks >> 2) * (kSlabQ >> 4) + (ks & 3) * 2, hi_1024),
+                            umma_desc_pack(b_lo + (ks >> 2) * kSlabB + (ks & 3) * 2, hi_1024), idesc_s, ks > 0);
+                umma_commit(&k_empty[st]);
+                umma_commit(&s_full[st]);
+                if (last) umma_commit(q_empty);
+            }
+            __syncwarp();
+        };
         for (BfItem m = take_item(n, ok); m.z >= 0; m = take_item(++n, ok)) {
             if (m.nblk == 0) continue;
             ok = ok && mbar_wait(q_full, qi & 1, status, limit);
-            ok = warp_ok(ok);
-            for (int t = m.nblk - 1; t >= 0 && ok; t -= 2, ++pc) {
-                const bool two = t > 0;
-                ok = ok && mbar_wait(k_full, pc & 1, status, limit);
-                // S takes the place of P of the pair before (products of two shapes may run in another order than they were issued); of its upper
-                // tile too, whose product is before the lower one's: both have the same shape and accumulator
-                if (pc > 0) ok = ok && mbar_wait(&pv_done[0], (pc - 1) & 1, status, limit);
+            issue_s(c, m.nblk == 1);
+            for (int j = 0; j < m.nblk && ok; ++j, ++c) {
+                const int st = c & 1, sv = c % kBfV;
+                if (j + 1 < m.nblk) issue_s(c + 1, j + 2 == m.nblk);
+                if (j == 0 && qi > 0) ok = ok && mbar_wait(o_free, (qi - 1) & 1, status, limit);
+                ok = ok && mbar_wait(&p_full[st], (c >> 1) & 1, status, limit);
+                ok = ok && mbar_wait(&v_full[sv], (c / kBfV) & 1, status, limit);
                 ok = warp_ok(ok);
                 if (!ok) break;
                 tc_fence_after();
                 if (leader) {
+                    const uint32_t b_lo = v_lo + (uint32_t)(sv * (kKt >> 4));
 #pragma unroll
-                    for (int ks = 0; ks < D / 16; ++ks) {
-                        const uint32_t off = (ks >> 2) * (kSlabQ >> 4) + (ks & 3) * 2;
-                        umma_ss(tbase + cS, umma_desc_pack(q_lo + off, hi_1024), umma_desc_pack(k_lo + off, hi_1024), two ? idesc_two : idesc_one, ks > 0);
-                    }
-                    umma_commit(k_empty);
-                    umma_commit(s_full);
-                    if (t <= 1) umma_commit(q_empty);
+                    for (int ks = 0; ks < BK / 16; ++ks)
+                        umma_ts(tbase + cO, tbase + cS + st * BK + ks * 8, umma_desc_pack(b_lo + ks * (2048 >> 4), hi_1024), idesc_o,
+                                (j > 0 || ks > 0) ? 1u : 0u);
+                    umma_commit(&v_empty[sv]);
+                    umma_commit(&pv_done[st]);
                 }
                 __syncwarp();
-                for (int half = two; half >= 0 && ok; --half, ++c) {
-                    const int st = c % kBfV;
-                    const bool first = t == m.nblk - 1 && half == two;
-                    if (first && qi > 0) ok = ok && mbar_wait(o_free, (qi - 1) & 1, status, limit);
-                    ok = ok && mbar_wait(&p_full[half], (half ? hc : pc) & 1, status, limit);
-                    ok = ok && mbar_wait(&v_full[st], (c / kBfV) & 1, status, limit);
-                    ok = warp_ok(ok);
-                    if (!ok) break;
-                    tc_fence_after();
-                    if (leader) {
-                        const uint32_t b_lo = v_lo + (uint32_t)(st * (kKt >> 4));
-#pragma unroll
-                        for (int ks = 0; ks < BK / 16; ++ks)
-                            umma_ts(tbase + cO, tbase + cS + half * BK + ks * 8, umma_desc_pack(b_lo + ks * (2048 >> 4), hi_1024), idesc_o,
-                                    (!first || ks > 0) ? 1u : 0u);
-                        umma_commit(&v_empty[st]);
-                        umma_commit(&pv_done[half]);
-                    }
-                    __syncwarp();
-                }
-                hc += two;
             }
             ++qi;
         }
@@ -285,14 +308,14 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                 const Sees s = limits(m.seq, m.tok0 + e);
                 x.lo = s.lo; x.hi = s.hi;
                 if constexpr (MOD & kModBias) {
-                    x.slope = __ldg(launch.mod.slopes + m.h * G + g) * kLog2e;
+                    x.slope = __ldcg(launch.mod.slopes + m.h * G + g) * kLog2e;
                     x.pos = s.pos;
                 }
             }
             return x;
         };
         bool ok = true, far = false;
-        int n = 0, pc = 0, hc = 0;
+        int n = 0, c = 0;
         BfItem m = take_item(n, ok);
         Row row = load_row(m);
         // (the four warps leave the loop together: they meet at barriers in it)
@@ -306,12 +329,11 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
             const int whole_lo = __reduce_max_sync(0xffffffffu, (max(lo_r, 0) + BK - 1) / BK);
             const int whole_hi = __reduce_min_sync(0xffffffffu, (((MOD & kModBias) && launch.mod.ahead ? min(hi_r, pos_r) : hi_r) + 1 >> 6) - 1);
             bool fresh = true;                             // some row of the warp has no reference yet
-            for (int t = nblk - 1; t >= 0; --t) {          // (left by all lanes at the vote below)
-                const int half = (nblk - 1 - t) & 1 ? 0 : t > 0;       // its place: the upper tile of a pair, the lower one, one alone
-                const bool begins = half == 1 || ((nblk - 1 - t) & 1) == 0;
-                if (begins) ok = ok && mbar_wait(s_full, pc & 1, status, limit);
+            for (int t = nblk - 1; t >= 0; --t, ++c) {     // (left by all lanes at the vote below)
+                const int st = c & 1;
+                ok = ok && mbar_wait(&s_full[st], (c >> 1) & 1, status, limit);
                 tc_fence_after();
-                const uint32_t tS = tbase + lane_off + cS + half * BK;
+                const uint32_t tS = tbase + lane_off + cS + st * BK;
                 uint32_t v[BK], pk[BK / 2];
                 tmem_ld32(tS, *reinterpret_cast<uint32_t (*)[32]>(&v[0]));
                 tmem_ld32(tS + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
@@ -375,8 +397,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                     // accumulator rows already hold products: rescale them when any row of the warp changes reference
                     const bool scale_acc = __any_sync(0xffffffffu, (raise && t < nblk - 1) || !ok);
                     if (scale_acc) {
-                        // the product of the tile before is done when this pair's S is, or is this pair's upper one
-                        if (!begins) ok = ok && mbar_wait(&pv_done[1], hc & 1, status, limit);
+                        ok = ok && mbar_wait(&pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1, status, limit);
                         if (!warp_stays(ok)) break;
                         tc_fence_after();
 #pragma unroll 1
@@ -404,26 +425,22 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                     // V rows that no row of the item sees are multiplied by p = 0, but 0 x NaN is NaN: zeros take their place.  Every thread
                     // has half of one of the 64 rows.
                     const int kr = m.row_lo + t * BK + (r & (BK - 1));
-                    const bool unseen = kr > m.row_hi || (launch.mod.key_ids && __ldg(launch.mod.key_ids + kr) < 0);
+                    const bool unseen = kr > m.row_hi || (launch.mod.key_ids && __ldcg(launch.mod.key_ids + kr) < 0);
                     if (__any_sync(0xffffffffu, unseen)) {
-                        const int vc = pc + hc + (begins ? 0 : 1), st = vc % kBfV;
-                        ok = ok && mbar_wait(&v_full[st], (vc / kBfV) & 1, status, limit);
+                        const int sv = c % kBfV;
+                        ok = ok && mbar_wait(&v_full[sv], (c / kBfV) & 1, status, limit);
                         if (unseen && ok)
 #pragma unroll
                             for (int i = 0; i < D / 16; ++i) {
                                 const int chunk = (r >> 6) * (D / 16) + i;
-                                *reinterpret_cast<uint4*>(sV + st * kKt + (chunk >> 3) * (BK * 128) + sw128_chunk_off(r & (BK - 1), chunk & 7)) =
+                                *reinterpret_cast<uint4*>(sV + sv * kKt + (chunk >> 3) * (BK * 128) + sw128_chunk_off(r & (BK - 1), chunk & 7)) =
                                     make_uint4(0u, 0u, 0u, 0u);
                             }
                         fence_async_smem();
                     }
                 }
                 tc_fence_before();
-                mbar_arrive(&p_full[half]);
-                if (half == 0) {
-                    ++pc;
-                    hc += !begins;
-                }
+                mbar_arrive(&p_full[st]);
             }
             m = read_item(n);
             const bool row_valid = g < G && e < m.ne;
@@ -433,7 +450,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
             row = load_row(next);
             // ---- epilogue
             if (m.nblk > 0) {
-                ok = ok && mbar_wait(&pv_done[0], (pc - 1) & 1, status, limit);
+                ok = ok && mbar_wait(&pv_done[(c - 1) & 1], ((c - 1) >> 1) & 1, status, limit);
                 tc_fence_after();
             }
             ok = bar_all(1, 128, ok);
@@ -479,18 +496,19 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
     }
     tc_fence_before();
     __syncthreads();
-    if (warp == 0) tmem_dealloc(tbase, kCols);
+    if (warp == 1) tmem_dealloc(tbase, kCols);
+    if constexpr (kSplit) follow_late();
     if (tid == 0 && *status != kStatusOk && p.status) atomicMax(p.status, *status);
 }
 
 template <int D, int MOD, typename ET>
 static cudaError_t launch_bf(const BiasedFwdLaunch& l, int max_tiles, cudaStream_t stream) {
-    constexpr int smem = kTileRows * D * 2 + (2 + kBfV) * kRdBK * D * 2 + 256;
+    constexpr int smem = kTileRows * D * 2 + (2 + kBfV) * kRdBK * D * 2 + 512;
     auto kern = biased_fwd<D, MOD, ET>;
     const cudaError_t e = allow_smem((const void*)kern, smem);
     if (e != cudaSuccess) return e;
-    kern<<<dim3((unsigned)max_tiles * (unsigned)l.p.Hk, (MOD & kModSplit) ? (unsigned)l.nchunk : 1u), kBfThreads, smem, stream>>>(l);
-    return cudaGetLastError();
+    // (kModSplit: beside the kernel before it, which is the one of the own rows, biased_decode.cu)
+    return launch_dependent(kern, dim3((unsigned)max_tiles * (unsigned)l.p.Hk, (MOD & kModSplit) ? (unsigned)l.nchunk : 1u), kBfThreads, smem, stream, 1, l);
 }
 
 template <int D, typename ET>

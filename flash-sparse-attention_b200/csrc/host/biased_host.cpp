@@ -36,6 +36,13 @@ struct BiasedArgs {
     int64_t window;         // -1: none
 };
 
+static void check_biased_status(const char* what) {
+    if (!checking_status()) return;
+    int st = 0;
+    check(fsa_biased_read_status(&st), what);
+    check(st == 0 ? FSA_OK : FSA_ERR_DEVICE_STATUS, what);
+}
+
 static void check_lengths(const Tensor& t, const Tensor& q, int64_t n, const char* name) {
     TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " has to be int32, got ", t.scalar_type());
     TORCH_CHECK_VALUE(t.dim() == 1 && (n < 0 || t.size(0) == n), name, " has to have ", n, " entries, got a tensor of shape ", t.sizes());
@@ -85,7 +92,7 @@ static std::tuple<Tensor, Tensor, Tensor> biased_fwd(const Tensor& q_, const Ten
                               dtype_code(q_), q.sn, q.sh, k.sn, v.sn, (float)a.scale, (float)a.cap, (int)a.window, ptr(o), lse.data_ptr<float>(), ptr(limits),
                               limits.numel(), stream_of(q_)),
           "fsa_biased_attn_fwd");
-    check_status(ptr(limits), q_, "fsa_biased_attn_fwd status");
+    check_biased_status("fsa_biased_attn_fwd status");
     return {o, lse, limits};
 }
 
@@ -104,11 +111,11 @@ static std::tuple<Tensor, Tensor, Tensor> biased_bwd(const Tensor& q_, const Ten
     const Tensor scratch = bytes(nb, q_);
     Tensor dq = fresh({N, Hq, D}, q_), dk = fresh({Nk, Hk, D}, q_), dv = fresh_like(dk);
     check(fsa_biased_attn_bwd(ptr(q.t), ptr(k.t), ptr(v.t), ptr(o), lse.data_ptr<float>(), ptr(dout.t), iptr(a.cu_q), iptr(a.cu_k), iptr(a.docs),
-                              a.prefix.defined(), a.slopes.defined() ? a.slopes.data_ptr<float>() : nullptr, N, Nk, B, (int)Hq, (int)Hk, (int)D,
-                              dtype_code(q_), q.sn, q.sh, k.sn, v.sn, dout.sn, dout.sh, (float)a.scale, (float)a.cap, ptr(dq), ptr(dk), ptr(dv), ptr(limits),
+                              iptr(a.prefix), a.slopes.defined() ? a.slopes.data_ptr<float>() : nullptr, N, Nk, B, (int)Hq, (int)Hk, (int)D,
+                              dtype_code(q_), q.sn, q.sh, k.sn, v.sn, dout.sn, dout.sh, (float)a.scale, (float)a.cap, (int)a.window, ptr(dq), ptr(dk), ptr(dv), ptr(limits),
                               limits.numel(), ptr(scratch), scratch.numel(), stream_of(q_)),
           "fsa_biased_attn_bwd");
-    check_status(ptr(limits), q_, "fsa_biased_attn_bwd status");
+    check_biased_status("fsa_biased_attn_bwd status");
     return {dq, dk, dv};
 }
 
@@ -205,11 +212,7 @@ std::tuple<Tensor, Tensor> biased_decode(const Tensor& q_, const Tensor& k, cons
                             slopes.defined() ? slopes.data_ptr<float>() : nullptr, (int)B, (int)Hq, (int)Hk, (int)D, dtype_code(q), (float)scale, (float)cap,
                             (int)window, max_len, max_prefix, ptr(o), lse.data_ptr<float>(), ptr(scratch), scratch.numel(), stream_of(q)),
           "fsa_biased_decode");
-    if (checking_status()) {
-        int st = 0;
-        check(fsa_biased_decode_read_status(&st), "fsa_biased_decode status");
-        TORCH_CHECK(st == 0, "fsa_biased_decode status: a kernel recorded a device-side failure (", st, ")");
-    }
+    check_biased_status("fsa_biased_decode status");
     return {o, lse};
 }
 

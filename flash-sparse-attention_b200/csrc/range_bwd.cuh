@@ -35,7 +35,8 @@ inline int64_t range_kv_max_cut(const SelShape& s) {
 inline int64_t range_kv_plan_bytes(const SelShape& s) { return 256 + 16 * (3 * range_kv_max_tiles(s) + range_kv_max_cut(s)); }
 inline int64_t range_kv_slab_bytes(const SelShape& s) { return range_kv_max_cut(s) * s.Hk * (2 * 128 * (int64_t)s.D * 4); }
 
-cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream);
+// dependent: as part of a chain of dependent launches, which leaves the status word (may be null) alone
+cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream, bool dependent = false);
 cudaError_t launch_range_bwd_dkdv(int dtype, const RangeKvPlan& p, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap,
                                   const CUtensorMap& vmap, int* status, cudaStream_t stream, const ScoreMod* mod = nullptr, int which = 0);
 

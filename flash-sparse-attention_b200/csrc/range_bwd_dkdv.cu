@@ -44,8 +44,9 @@ constexpr int kRkUnits = 5;             // Q / dO tiles in the ring
 __global__ void __launch_bounds__(512) range_key_tiles(const RangeKvPlan p, uint4* __restrict__ dk, uint4* __restrict__ dv, int* __restrict__ status) {
     __shared__ int s_lo[16], s_hi[16];
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
+    follow();
     if (blockIdx.x == gridDim.x - 1) {
-        if (tid == 0) *status = kStatusOk;
+        if (tid == 0 && status) *status = kStatusOk;
         const int64_t row16 = (int64_t)p.Hk * p.D / 8;
         for (int64_t i = (int64_t)__ldg(p.cu_k + p.B) * row16 + tid; i < p.Nk * row16; i += blockDim.x) {
             dk[i] = make_uint4(0u, 0u, 0u, 0u);
@@ -69,8 +70,8 @@ __global__ void __launch_bounds__(512) range_key_tiles(const RangeKvPlan p, uint
 #pragma unroll
         for (int j = 0; j < 8; ++j) {
             const int t = base + j * 512;
-            l[j] = t < t1 ? (p.kv_lo ? __ldg(p.kv_lo + t) : k0) : 0;
-            u[j] = t < t1 ? __ldg(p.kv_hi + t) : -1;
+            l[j] = t < t1 ? (p.kv_lo ? __ldcg(p.kv_lo + t) : k0) : 0;
+            u[j] = t < t1 ? __ldcg(p.kv_hi + t) : -1;
         }
 #pragma unroll
         for (int j = 0; j < 8; ++j)
@@ -96,6 +97,7 @@ __global__ void __launch_bounds__(1024) range_plan_items(const RangeKvPlan p) {
     const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     auto row_tiles = [&](const int4& t) { return t.w >= 0 ? (t.w - t.z + p.TPT) / p.TPT : 0; };
     if (tid == 0) total = 0;
+    follow();
     __syncthreads();
     int mine = 0;
     for (int i = tid; i < p.max_tiles; i += 1024) mine += row_tiles(p.tiles[i]);
@@ -138,6 +140,7 @@ __global__ void __launch_bounds__(1024) range_plan_items(const RangeKvPlan p) {
 // dk / dv rows of the K/V tiles that were cut: the sum of the slabs in order.  Slab: [dV, dK][column / 4][row] float4.
 template <int D, typename ET>
 __global__ void __launch_bounds__(256) range_dkdv_reduce(const RangeKvPlan p, const float4* __restrict__ slabs, ET* __restrict__ dk, ET* __restrict__ dv) {
+    follow();
     constexpr int kChunks = D / 8, kParts = 2 * kChunks * 128 / 256;
     const int64_t units = (int64_t)__ldg(p.counts + 1) * p.Hk * kParts;       // 2 x kChunks x 128 chunks of 8 columns per tile and head, 256 a CTA
     for (int64_t w = blockIdx.x; w < units; w += gridDim.x) {
@@ -644,9 +647,14 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
     tc_fence_before();
     __syncthreads();
     if (warp == 0) tmem_dealloc(tbase, 512);
+    if constexpr (MOD != 0) follow_late();      // it runs beside the dQ kernel, of which it needs nothing
 }
 
-cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream) {
+cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream, bool dependent) {
+    if (dependent) {
+        const cudaError_t e = launch_dependent(range_key_tiles, dim3((unsigned)p.max_tiles + 1), 512, 0, stream, 1, p, (uint4*)a.dk, (uint4*)a.dv, status);
+        return e == cudaSuccess ? launch_dependent(range_plan_items, dim3(1), 1024, 0, stream, 1, p) : e;
+    }
     range_key_tiles<<<(unsigned)p.max_tiles + 1, 512, 0, stream>>>(p, (uint4*)a.dk, (uint4*)a.dv, status);
     range_plan_items<<<1, 1024, 0, stream>>>(p);
     return cudaGetLastError();
@@ -658,8 +666,15 @@ static cudaError_t launch_rk(const RangeKvParams& p, const CUtensorMap* maps, in
     auto kern = range_bwd_dkdv<D, MOD, ET>;
     cudaError_t e = allow_smem((const void*)kern, smem);
     if (e != cudaSuccess) return e;
+    const unsigned grid = (unsigned)(max_items < sms ? max_items : sms);
+    if constexpr (MOD != 0) {
+        e = launch_dependent(kern, dim3(grid), kRkThreads, smem, stream, 1, p, maps[0], maps[1], maps[2], maps[3]);
+        if (e == cudaSuccess) e = prefer_l1((const void*)range_dkdv_reduce<D, ET>);
+        if (e != cudaSuccess) return e;
+        return launch_dependent(range_dkdv_reduce<D, ET>, dim3((unsigned)(4 * sms)), 256, 0, stream, 1, p.plan, (const float4*)p.slabs, (ET*)p.dk, (ET*)p.dv);
+    }
     prof_begin(FSA_KERNEL_SEL_BWD_MAIN, stream);
-    kern<<<(unsigned)(max_items < sms ? max_items : sms), kRkThreads, smem, stream>>>(p, maps[0], maps[1], maps[2], maps[3]);
+    kern<<<grid, kRkThreads, smem, stream>>>(p, maps[0], maps[1], maps[2], maps[3]);
     prof_end(FSA_KERNEL_SEL_BWD_MAIN, stream);
     e = prefer_l1((const void*)range_dkdv_reduce<D, ET>);
     if (e != cudaSuccess) return e;

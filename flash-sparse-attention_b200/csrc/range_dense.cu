@@ -546,6 +546,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int* status = p.status;
+    if constexpr (MOD != 0) follow_late();
     if (tid == 0) {
         mbar_init(qd_full, 1); mbar_init(qd_empty, 256);
         for (int i = 0; i < kDqStages; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
@@ -567,6 +568,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
     __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tmem_slot;
+    if constexpr (MOD != 0) let_next_start();
     const int ntiles = count_seq_tiles(p.cu_q, p.B, p.TPT, lane);
     const int nitems = ntiles * p.Hk;
     // Entry n of this CTA's items: every warp but the one that fills the ring takes each of them once, in order.
@@ -742,7 +744,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
                 x.hi = __ldg(p.kv_hi + m.tok0 + e);
                 const int64_t idx = (int64_t)(m.h * p.G + g) * p.N + m.tok0 + e;
                 x.lse = __ldg(p.lse + idx);
-                x.delta = __ldg(p.delta + idx);
+                x.delta = MOD ? __ldcg(p.delta + idx) : __ldg(p.delta + idx);        // (MOD: the kernel before wrote it)
                 if constexpr (MOD & kModBias) {
                     x.slope = __ldg(p.mod.slopes + m.h * p.G + g) * kLog2e;
                     x.pos = __ldg(p.mod.pos + m.tok0 + e);
@@ -945,6 +947,7 @@ static cudaError_t launch_dq(const RangeDqParams& p, const CUtensorMap* maps, un
     auto kern = range_bwd_dq_dense<D, MOD, ET>;
     const cudaError_t e = allow_smem((const void*)kern, smem);
     if (e != cudaSuccess) return e;
+    if constexpr (MOD != 0) return launch_dependent(kern, dim3(grid), kDqThreads, smem, stream, 1, p, maps[0], maps[1], maps[2], maps[3], maps[4]);
     prof_begin(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
     kern<<<grid, kDqThreads, smem, stream>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4]);
     prof_end(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);

@@ -28,15 +28,28 @@ struct RangeDenseLaunch {
     RangeDenseParams p[kRdProblems];
 };
 
+// First and last K/V row that token `tok` of a sequence sees, and its place, without documents.  The sequence has the rows [k0, k1); its last token is
+// the one before q1 and stands at row k1 - 1.  window: -1 for none; prefix: rows at its beginning that all tokens see.
+struct Sees { int lo, hi, pos; };
+__device__ __forceinline__ Sees place_limits(int tok, int k0, int k1, int q1, int window, int prefix) {
+    Sees x;
+    x.pos = tok + k1 - q1;
+    const bool in = x.pos >= k0;            // (else the sequence has fewer keys than queries, and this one precedes them)
+    x.lo = in && window >= 0 ? max(k0, x.pos - window) : k0;
+    x.hi = in ? max(x.pos, min(k0 + prefix, k1) - 1) : -1;
+    return x;
+}
+
 // Attention with changed scores: the same problem, one a launch.
 struct BiasedFwdLaunch {
     CUtensorMap q, k, v;
-    RangeDenseParams p;     // (o_sn and o_sh are not used: o is contiguous)
+    RangeDenseParams p;     // (o_sn and o_sh are not used: o is contiguous; kv_lo null: place_limits)
     ScoreMod mod;
+    int window;                     // -1: none
+    const int32_t* prefix_lens;     // [B] or null
     // kModSplit: rows that several sequences share, a "token" is a sequence of the batch (kv_lo and kv_hi are not used).  The K/V rows of every
     // tile are cut into nchunk chunks (blockIdx.y) of `chunk` tiles; chunk c of a row writes partial c of P
     const int32_t* seq_len; // [N] own tokens of every sequence, the new one among them
-    int window;             // -1: none
     float* o_part;          // [N, Hq, P, D] unnormalised
     float2* ml;             // [N, Hq, P] reference maximum (log2 units) and sum
     int P, nchunk, chunk;

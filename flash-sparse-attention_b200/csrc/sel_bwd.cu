@@ -345,6 +345,7 @@ template <typename ET>
 __global__ void __launch_bounds__(256) sel_bwd_delta(const ET* __restrict__ o, int64_t o_sn, int64_t o_sh,
                                                      const ET* __restrict__ d_o, int64_t do_sn, int64_t do_sh,
                                                      int64_t N, int Hq, int D, float* __restrict__ delta) {
+    follow();
     const int tpr = D >> 3;                                  // threads per row: 8, 16 or 32 (a power of two)
     const int rpc = 256 / tpr;                               // rows per pass of the CTA
     const int part = threadIdx.x & (tpr - 1), rloc = threadIdx.x / tpr;
@@ -555,17 +556,19 @@ __global__ void __launch_bounds__(256) sel_bwd_convert(const float* __restrict__
 constexpr int64_t kReduceFew = 24000;      // output rows up to which both reductions go in one launch (more: resident merges take dq)
 
 template <typename ET>
-static cudaError_t launch_delta(const SelBwdArgs& a, const SelShape& s, cudaStream_t stream) {
+static cudaError_t launch_delta(const SelBwdArgs& a, const SelShape& s, cudaStream_t stream, bool dependent = false) {
     const int64_t rows = s.N * s.Hq, rows_per_cta = 2 * (256 / (s.D / 8));
     const cudaError_t e = prefer_l1((const void*)sel_bwd_delta<ET>);
     if (e != cudaSuccess) return e;
-    sel_bwd_delta<ET><<<(unsigned)((rows + rows_per_cta - 1) / rows_per_cta), 256, 0, stream>>>((const ET*)a.o, a.o_sn, a.o_sh, (const ET*)a.d_o, a.do_sn,
-                                                                                               a.do_sh, s.N, s.Hq, s.D, a.delta);
+    const unsigned grid = (unsigned)((rows + rows_per_cta - 1) / rows_per_cta);
+    if (dependent)
+        return launch_dependent(sel_bwd_delta<ET>, dim3(grid), 256, 0, stream, 1, (const ET*)a.o, a.o_sn, a.o_sh, (const ET*)a.d_o, a.do_sn, a.do_sh, s.N, s.Hq, s.D, a.delta);
+    sel_bwd_delta<ET><<<grid, 256, 0, stream>>>((const ET*)a.o, a.o_sn, a.o_sh, (const ET*)a.d_o, a.do_sn, a.do_sh, s.N, s.Hq, s.D, a.delta);
     return cudaGetLastError();
 }
 
 cudaError_t launch_sel_bwd_delta(int dtype, const SelBwdArgs& a, const SelShape& s, cudaStream_t stream) {
-    return dtype == kBF16 ? launch_delta<__nv_bfloat16>(a, s, stream) : launch_delta<__half>(a, s, stream);
+    return dtype == kBF16 ? launch_delta<__nv_bfloat16>(a, s, stream, true) : launch_delta<__half>(a, s, stream, true);
 }
 
 template <int D, typename ET>

@@ -114,12 +114,17 @@ inline SelIndex sel_index_carve(void* ws, const SelShape& s) {
     ix.pos = (int*)p;
     return ix;
 }
+// A load for kernels launched as dependents (sm100_prims.cuh): CG, through L2, or the non-coherent one.
+template <bool CG>
+__device__ __forceinline__ int ld_cg(const int32_t* p) { return CG ? __ldcg(p) : __ldg(p); }
+
 // sequence of token n: largest b with cu[b] <= n
+template <bool CG = false>
 __device__ __forceinline__ int find_seq(const int* __restrict__ cu, int B, int n) {
     int lo = 0, hi = B;   // invariant: cu[lo] <= n < cu[hi]
     while (hi - lo > 1) {
         int mid = (lo + hi) >> 1;
-        if (__ldg(cu + mid) <= n) lo = mid; else hi = mid;
+        if (ld_cg<CG>(cu + mid) <= n) lo = mid; else hi = mid;
     }
     return lo;
 }
@@ -220,11 +225,12 @@ struct TileCursorT {
 
 // Query-tile-major kernels cut every sequence into tiles of TPT consecutive tokens.  Both helpers are warp-collective (every lane calls them and gets the same
 // answer) and walk the sequences 32 at a time, so that a packed batch of thousands of short sequences costs B / 32 steps.
+template <bool CG = false>
 __device__ __forceinline__ int count_seq_tiles(const int32_t* __restrict__ cu_q, int B, int TPT, int lane) {
     int total = 0;
     for (int b0 = 0; b0 < B; b0 += 32) {
         const int b = b0 + lane;
-        int nt = b < B ? (__ldg(cu_q + b + 1) - __ldg(cu_q + b) + TPT - 1) / TPT : 0;
+        int nt = b < B ? (ld_cg<CG>(cu_q + b + 1) - ld_cg<CG>(cu_q + b) + TPT - 1) / TPT : 0;
 #pragma unroll
         for (int d = 16; d > 0; d >>= 1) nt += __shfl_xor_sync(0xffffffffu, nt, d);
         total += nt;
@@ -232,6 +238,7 @@ __device__ __forceinline__ int count_seq_tiles(const int32_t* __restrict__ cu_q,
     return total;
 }
 // tile `want` of the list: its sequence (-1 if there is no such tile), first token and number of tokens
+template <bool CG = false>
 __device__ __forceinline__ void find_seq_tile(const int32_t* __restrict__ cu_q, int B, int TPT, int want, int lane, int& seq, int& tok0,
                                              int& ne) {
     seq = -1; tok0 = 0; ne = 0;
@@ -239,7 +246,7 @@ __device__ __forceinline__ void find_seq_tile(const int32_t* __restrict__ cu_q, 
     int acc = 0;
     for (int b0 = 0; b0 < B; b0 += 32) {
         const int b = b0 + lane;
-        const int s0 = b < B ? __ldg(cu_q + b) : 0, L = b < B ? __ldg(cu_q + b + 1) - s0 : 0;
+        const int s0 = b < B ? ld_cg<CG>(cu_q + b) : 0, L = b < B ? ld_cg<CG>(cu_q + b + 1) - s0 : 0;
         const int nt = (L + TPT - 1) / TPT;
         int incl = nt;                                   // inclusive prefix over the 32 sequences
 #pragma unroll
@@ -261,22 +268,25 @@ __device__ __forceinline__ void find_seq_tile(const int32_t* __restrict__ cu_q, 
     }
 }
 
-// The same list, longest rows of keys first, for up to 32 sequences (others: from its end): a tile's tokens see about as many keys as precede
+// The same list (behind its end: seq -1, tok0 how far), longest rows of keys first, for up to 32 sequences (others: from its end): a tile's tokens see about as many keys as precede
 // them in their sequence, cu_k's included, which is what tiles are ranked by.  Sequence after sequence, a long one that comes late in the list
 // is still at work when everybody else is done: two sequences of 8192 tokens, 8 / 4 heads, took 28 % longer a tile than one of 16384.
 __device__ __forceinline__ void find_ranked_tile(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, int B, int TPT, int rank, int lane,
                                                 int& seq, int& tok0, int& ne) {
     if (B > 32) {
-        find_seq_tile(cu_q, B, TPT, count_seq_tiles(cu_q, B, TPT, lane) - 1 - rank, lane, seq, tok0, ne);
+        const int total = count_seq_tiles<true>(cu_q, B, TPT, lane);
+        find_seq_tile<true>(cu_q, B, TPT, total - 1 - rank, lane, seq, tok0, ne);
+        if (seq < 0) tok0 = rank - total;
         return;
     }
-    const int s0 = lane < B ? __ldg(cu_q + lane) : 0, s1 = lane < B ? __ldg(cu_q + lane + 1) : 0;
+    const int s0 = lane < B ? __ldcg(cu_q + lane) : 0, s1 = lane < B ? __ldcg(cu_q + lane + 1) : 0;
     const int nt = (s1 - s0 + TPT - 1) / TPT;
-    const int first = lane < B ? max(0, __ldg(cu_k + lane + 1) - __ldg(cu_k + lane) - (s1 - s0)) / TPT : 0;      // level of its first tile
+    const int first = lane < B ? max(0, __ldcg(cu_k + lane + 1) - __ldcg(cu_k + lane) - (s1 - s0)) / TPT : 0;      // level of its first tile
     // tiles of level t and above
     auto above = [&](int t) { return __reduce_add_sync(0xffffffffu, max(0, first + nt - max(t, first))); };
-    seq = -1; tok0 = 0; ne = 0;
-    if (rank >= above(0)) return;
+    const int total = above(0);
+    seq = -1; tok0 = rank - total; ne = 0;
+    if (rank >= total) return;
     int lo = 0, hi = __reduce_max_sync(0xffffffffu, first + nt);       // above(lo) > rank >= above(hi)
     while (hi - lo > 1) {
         const int mid = (lo + hi) >> 1;

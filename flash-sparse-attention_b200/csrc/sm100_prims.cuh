@@ -86,6 +86,13 @@ __device__ __forceinline__ void follow() {
     asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// The wait alone.  A kernel that needs nothing of the one before it may run beside it: it calls this before it returns instead of follow(), so that
+// whoever waits for it has waited for both.  What comes before the kernel before it is there: that one has called follow().
+__device__ __forceinline__ void follow_late() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+// The other half.  A kernel that takes TMEM waits before it does so, and lets the next one start afterwards: CTAs of two kernels on one SM, one
+// with the TMEM that the other needs to end and waiting for that end, would stand there for good.
+__device__ __forceinline__ void let_next_start() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
 // ---------------------------------------------------------------- mbarrier
 __device__ __forceinline__ void mbar_init(uint64_t* bar, uint32_t count) {
     asm volatile("mbarrier.init.shared::cta.b64 [%0], %1;" ::"r"(smem_u32(bar)), "r"(count) : "memory");

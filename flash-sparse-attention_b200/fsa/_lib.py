@@ -83,14 +83,14 @@ SIGNATURES = {
     "fsa_biased_attn_bwd_bytes": (c_int, [c_int64] * 2 + [c_int] * 4 + [POINTER(c_int64)]),
     "fsa_biased_attn_bwd": (
         c_int,
-        [c_void_p] * 9 + [c_int, c_void_p] + [c_int64] * 2 + [c_int] * 5 + [c_int64] * 6 + [c_float] * 2 + [c_void_p] * 4
+        [c_void_p] * 11 + [c_int64] * 2 + [c_int] * 5 + [c_int64] * 6 + [c_float] * 2 + [c_int] + [c_void_p] * 4
         + [c_int64, c_void_p, c_int64, c_void_p]),
     "fsa_biased_decode_bytes": (c_int, [c_int] * 5 + [c_int64, c_int64, c_int, POINTER(c_int64)]),
     "fsa_biased_decode": (
         c_int,
         [c_void_p] * 3 + [c_int64] * 3 + [c_void_p] * 4 + [c_int64] * 3 + [c_void_p] * 2 + [c_int, c_void_p] + [c_int] * 5 + [c_float] * 2
         + [c_int] + [c_int64] * 2 + [c_void_p] * 3 + [c_int64, c_void_p]),
-    "fsa_biased_decode_read_status": (c_int, [POINTER(c_int)]),
+    "fsa_biased_read_status": (c_int, [POINTER(c_int)]),
     "fsa_linear_compress_fwd": (
         c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "fsa_compress_bias_scratch_bytes": (c_int64, [c_int, c_int]),

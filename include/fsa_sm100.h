@@ -212,7 +212,7 @@ int fsa_range_attn_bwd_indexed(int head_dim);
  *   prefix_lens      (int32 per sequence; not with window or doc_ids) and the sequence's first prefix_lens[b] keys besides.
  * k, v: head stride head_dim.  o [N, Hq, D] contiguous, lse [Hq, N] (log2 units); rows behind the last sequence become 0 / -inf.  K/V
  * rows that no token sees, and q and d_o rows of tokens that see nothing, may hold anything, NaN included.  limits: workspace of
- * fsa_biased_attn_limits_bytes bytes, kept for the backward; its first word is the status word (fsa_read_status).
+ * fsa_biased_attn_limits_bytes bytes, kept for the backward.
  * head_dim 64 or 128, up to 32 query heads a kv head, fewer than 2^25 tokens and K/V rows, N * num_q_heads below 2^31. */
 int fsa_biased_attn_limits_bytes(int64_t total_tokens, int64_t* bytes_out);
 int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
@@ -233,14 +233,14 @@ int fsa_biased_decode(const void* q, const void* k, const void* v, int64_t kv_ro
                       int64_t shared_v_stride_n, const int32_t* cu_shared, const int32_t* cu_group, int num_groups, const float* slopes, int batch,
                       int num_q_heads, int num_kv_heads, int head_dim, int dtype, float sm_scale, float softcap, int window, int64_t max_len,
                       int64_t max_shared, void* o, float* lse, void* scratch, int64_t scratch_bytes, void* stream);
-/* What the waits of these kernels left: 0, or that one ran out (synchronises). */
-int fsa_biased_decode_read_status(int* status_out);
-/* fsa_biased_attn_fwd's gradient.  dq, dk, dv contiguous; every row of them is written.  has_prefix: the forward was given prefix_lens.  Bit-reproducible. */
+/* What the waits of these operators' kernels left on the current device: 0, or that one ran out (synchronises). */
+int fsa_biased_read_status(int* status_out);
+/* fsa_biased_attn_fwd's gradient.  dq, dk, dv contiguous; every row of them is written.  limits: what the forward left.  Bit-reproducible. */
 int fsa_biased_attn_bwd_bytes(int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads, int head_dim, int64_t* bytes_out);
 int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens_q,
-                        const int32_t* cu_seqlens_k, const int32_t* doc_ids, int has_prefix, const float* slopes, int64_t total_tokens, int64_t total_kv_rows,
+                        const int32_t* cu_seqlens_k, const int32_t* doc_ids, const int32_t* prefix_lens, const float* slopes, int64_t total_tokens, int64_t total_kv_rows,
                         int batch, int num_q_heads, int num_kv_heads, int head_dim, int dtype, int64_t q_stride_n, int64_t q_stride_h, int64_t k_stride_n,
-                        int64_t v_stride_n, int64_t do_stride_n, int64_t do_stride_h, float sm_scale, float softcap, void* dq, void* dk, void* dv,
+                        int64_t v_stride_n, int64_t do_stride_n, int64_t do_stride_h, float sm_scale, float softcap, int window, void* dq, void* dk, void* dv,
                         void* limits, int64_t limits_bytes, void* scratch, int64_t scratch_bytes, void* stream);
 
 int fsa_range_attn_index(const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k, const int32_t* kv_lo, const int32_t* kv_hi,
