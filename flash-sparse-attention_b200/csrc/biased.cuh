@@ -1,31 +1,23 @@
-// The forwards of range attention (range_dense.cu) and of attention with changed scores (biased_fwd.cu) for their callers.
+// Attention with changed scores: its kernels (biased_fwd.cu, biased_bwd_dq.cu, biased_bwd_dkdv.cu) for their callers (biased_attn.cu, biased_decode.cu).
 #pragma once
 #include "score.cuh"
 #include "sel_launch.cuh"
 
 namespace fsa {
 
-constexpr int kRdBK = 64;
+constexpr int kBiasedBK = 64;       // K/V rows of a tile
 
-struct RangeDenseParams {
+struct BiasedFwdParams {
     const int32_t* cu_q;    // [B + 1]
     const int32_t* cu_k;    // [B + 1] first K/V row of every sequence
-    const int32_t* kv_lo;   // [N] lowest visible K/V row of every token, or null (the sequence's first row)
-    const int32_t* kv_hi;   // [N] highest visible K/V row, lower than kv_lo when the token sees nothing
+    const int32_t* kv_lo;   // [N] first K/V row that every token sees, or null: place_limits
+    const int32_t* kv_hi;   // [N] last one, lower than kv_lo where a token sees nothing
     int64_t N, Nk;
     int B, Hq, Hk, G, TPT;
     float scale_log2;
-    void* o;  int64_t o_sn, o_sh;     // [N, Hq, D]
-    float* lse;                       // [Hq, N] log2 units
+    void* o;                // [N, Hq, D] contiguous
+    float* lse;             // [Hq, N] log2 units
     int* status;
-};
-
-// Up to three problems in one launch (blockIdx.z): branches of a layer that do not wait for one another.  A short prompt has fewer tiles
-// than the SMs hold CTAs, and each launch of its own left most of them empty (517 tokens, 32 / 8 heads: 3 x 11 us, together 19: prefill 158 -> 138 us).
-constexpr int kRdProblems = 3;
-struct RangeDenseLaunch {
-    CUtensorMap q[kRdProblems], k[kRdProblems], v[kRdProblems], o[kRdProblems];
-    RangeDenseParams p[kRdProblems];
 };
 
 // First and last K/V row that token `tok` of a sequence sees, and its place, without documents.  The sequence has the rows [k0, k1); its last token is
@@ -40,10 +32,9 @@ __device__ __forceinline__ Sees place_limits(int tok, int k0, int k1, int q1, in
     return x;
 }
 
-// Attention with changed scores: the same problem, one a launch.
 struct BiasedFwdLaunch {
     CUtensorMap q, k, v;
-    RangeDenseParams p;     // (o_sn and o_sh are not used: o is contiguous; kv_lo null: place_limits)
+    BiasedFwdParams p;
     ScoreMod mod;
     int window;                     // -1: none
     const int32_t* prefix_lens;     // [B] or null
@@ -56,5 +47,12 @@ struct BiasedFwdLaunch {
 };
 // which: kModCap, kModBias; split: with kModSplit.  l.p.TPT tokens a tile, max_tiles tiles at most.
 cudaError_t launch_biased_fwd(int D, int dtype, int which, bool split, const BiasedFwdLaunch& l, int max_tiles, cudaStream_t stream);
+
+struct RangeKvPlan;      // range_bwd.cuh
+// The backward, a.bd's limits given; as parts of a chain of dependent launches, the second beside the first.
+cudaError_t launch_biased_bwd_dq(int dtype, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap, const CUtensorMap& vmap, int* status,
+                                 const ScoreMod& mod, int which, cudaStream_t stream);
+cudaError_t launch_biased_bwd_dkdv(int dtype, const RangeKvPlan& plan, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                                   int* status, const ScoreMod& mod, int which, cudaStream_t stream);
 
 }  // namespace fsa

@@ -1,10 +1,10 @@
 // Attention with changed scores (capped by a tanh, biased by distance) under causal, window, document and prefix masks, packed
 // sequences: the limits of every token and the entry points.  Under each of these masks a token sees one stretch of
-// K/V rows.  Forward: biased_fwd.cu; backward: the kernels of range attention (range_dense.cu, range_bwd_dkdv.cu) compiled for changed scores.
+// K/V rows.  Forward: biased_fwd.cu; backward: biased_bwd_dq.cu and biased_bwd_dkdv.cu, on the plan of range_bwd_dkdv.cu.
 #include "../../include/fsa_sm100.h"
 
 #include "range_bwd.cuh"
-#include "range_fwd.cuh"
+#include "biased.cuh"
 
 namespace fsa {
 
@@ -164,7 +164,7 @@ extern "C" int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, 
     cudaStream_t stream = (cudaStream_t)stream_;
     const BiasedLimits lim(limits, N);
     cudaError_t e;
-    RangeDenseParams& p = l.p;
+    BiasedFwdParams& p = l.p;
     if ((e = biased_status_word(&p.status)) != cudaSuccess) return cuda_failed(e);
     p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k;
     l.window = window; l.prefix_lens = prefix_lens;
@@ -205,6 +205,7 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     if (!q || !k || !v || !o || !lse || !d_o || !cu_seqlens_q || !cu_seqlens_k || !dq || !dk || !dv || !limits || !scratch || Nk == 0) return FSA_ERR_BAD_ARG;
     for (const void* x : {q, k, v, o, d_o, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)limits, (const void*)scratch})
         if (!aligned16(x)) return FSA_ERR_BAD_ARG;
+    if (((uintptr_t)dq & 31) || ((uintptr_t)dk & 31) || ((uintptr_t)dv & 31)) return FSA_ERR_BAD_ARG;
     if ((q_sn % 8) || (q_sh % 8) || (k_sn % 8) || (v_sn % 8) || (do_sn % 8) || (do_sh % 8) || k_sn < (int64_t)Hk * D || v_sn < (int64_t)Hk * D) return FSA_ERR_BAD_ARG;
     int64_t need = 0;
     if ((rc = fsa_biased_attn_bwd_bytes(N, Nk, B, Hq, Hk, D, &need))) return rc;
@@ -242,8 +243,9 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     if (e == cudaSuccess) e = biased_status_word(&status);
     if (e == cudaSuccess) e = launch_range_bwd_plan(plan, a, nullptr, stream, true);
     if (e == cudaSuccess) e = launch_sel_bwd_delta(dtype, a, s, stream);
-    if (e == cudaSuccess) e = launch_range_bwd_dq(dtype, a, s, kmap, vmap, status, stream, &mod, which);
-    if (e == cudaSuccess) e = launch_range_bwd_dkdv(dtype, plan, a, s, kmap, vmap, status, stream, &mod, which);
+    if (e == cudaSuccess) e = launch_biased_bwd_dq(dtype, a, s, kmap, vmap, status, mod, which, stream);
+    if (e == cudaSuccess) e = launch_biased_bwd_dkdv(dtype, plan, a, s, kmap, vmap, status, mod, which, stream);
+    if (e == cudaSuccess) e = launch_range_dkdv_reduce(dtype, plan, a.slabs, dk, dv, sm_count(), stream);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
 }
 

@@ -9,7 +9,7 @@
 // Both write partial results (unnormalised o, maximum, sum) side by side; the last kernel merges them.
 #include "../../include/fsa_sm100.h"
 
-#include "range_fwd.cuh"
+#include "biased.cuh"
 
 namespace fsa {
 
@@ -406,7 +406,7 @@ struct DecodeCut {
         if (groups > 0) {
             // (a group's last tile has one sequence at least; a place in the grid that no tile takes would hold up one that does)
             mtiles = B > groups ? (B - groups) / TPT + groups : B > 0 ? B : 1;
-            const int64_t blocks = max_shared < 1 ? 1 : (max_shared + kRdBK - 1) / kRdBK;
+            const int64_t blocks = max_shared < 1 ? 1 : (max_shared + kBiasedBK - 1) / kBiasedBK;
             int64_t n = 2 * sms / ((int64_t)mtiles * Hk);
             if (n < 1) n = 1;
             if (n > (blocks + 1) / 2) n = (blocks + 1) / 2;
@@ -492,9 +492,9 @@ extern "C" int fsa_biased_decode(const void* q, const void* k, const void* v, in
     if (has_shared) {
         BiasedFwdLaunch l = {};
         if ((rc = make_tile_map_3d_box(&l.q, q, dtype, D, B, Hq, (int64_t)Hq * D, D, TPT, G))) return rc;
-        if ((rc = make_tile_map(&l.k, shared_k, dtype, shared_rows, packed, shared_k_stride_n, kRdBK))) return rc;
-        if ((rc = make_tile_map(&l.v, shared_v, dtype, shared_rows, packed, shared_v_stride_n, kRdBK))) return rc;
-        RangeDenseParams& r = l.p;
+        if ((rc = make_tile_map(&l.k, shared_k, dtype, shared_rows, packed, shared_k_stride_n, kBiasedBK))) return rc;
+        if ((rc = make_tile_map(&l.v, shared_v, dtype, shared_rows, packed, shared_v_stride_n, kBiasedBK))) return rc;
+        BiasedFwdParams& r = l.p;
         r.cu_q = cu_group; r.cu_k = cu_shared;
         r.N = B; r.Nk = shared_rows; r.B = num_groups; r.Hq = Hq; r.Hk = Hk; r.G = G; r.TPT = TPT;
         r.scale_log2 = sm_scale * kLog2e;

@@ -18,7 +18,7 @@
 #include "../../include/fsa_sm100.h"
 #include <climits>
 
-#include "range_fwd.cuh"
+#include "biased.cuh"
 
 namespace fsa {
 
@@ -36,7 +36,7 @@ template <typename ET> constexpr float kBfLazy = ElemTraits<ET>::kIsBF16 ? 64.f 
 
 template <int D, int MOD, typename ET>
 __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constant__ BiasedFwdLaunch launch) {
-    constexpr int BK = kRdBK, KH = D / 64;
+    constexpr int BK = kBiasedBK, KH = D / 64;
     constexpr int kQ = kTileRows * D * 2;
     constexpr int kSlabQ = kTileRows * 128;          // 64 columns of the Q tile
     constexpr int kKt = BK * D * 2;                  // one K (or V) tile
@@ -67,7 +67,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
     int* status = reinterpret_cast<int*>(bars + 32) + 1;     // of this CTA
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-    const RangeDenseParams& p = launch.p;
+    const BiasedFwdParams& p = launch.p;
     const uint32_t limit = wait_limit(p.status);
     const int G = p.G, TPT = p.TPT;
     // First and last K/V row that a token sees, and its place.  kModSplit: a token is a sequence of the batch, whose own rows follow the shared ones.
@@ -503,7 +503,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
 
 template <int D, int MOD, typename ET>
 static cudaError_t launch_bf(const BiasedFwdLaunch& l, int max_tiles, cudaStream_t stream) {
-    constexpr int smem = kTileRows * D * 2 + (2 + kBfV) * kRdBK * D * 2 + 512;
+    constexpr int smem = kTileRows * D * 2 + (2 + kBfV) * kBiasedBK * D * 2 + 512;
     auto kern = biased_fwd<D, MOD, ET>;
     const cudaError_t e = allow_smem((const void*)kern, smem);
     if (e != cudaSuccess) return e;

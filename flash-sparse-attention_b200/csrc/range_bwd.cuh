@@ -1,6 +1,5 @@
 // Shared by the range-attention backward's kernels (range_bwd_dkdv.cu) and their callers (fsa_api.cu, sel_bwd.cu).
 #pragma once
-#include "score.cuh"
 #include "sel_launch.cuh"
 
 namespace fsa {
@@ -37,7 +36,9 @@ inline int64_t range_kv_slab_bytes(const SelShape& s) { return range_kv_max_cut(
 
 // dependent: as part of a chain of dependent launches, which leaves the status word (may be null) alone
 cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream, bool dependent = false);
+// dk / dv rows of the K/V tiles that were cut, as part of such a chain; head_dim 64 or 128
+cudaError_t launch_range_dkdv_reduce(int dtype, const RangeKvPlan& p, const float* slabs, void* dk, void* dv, int sms, cudaStream_t stream);
 cudaError_t launch_range_bwd_dkdv(int dtype, const RangeKvPlan& p, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap,
-                                  const CUtensorMap& vmap, int* status, cudaStream_t stream, const ScoreMod* mod = nullptr, int which = 0);
+                                  const CUtensorMap& vmap, int* status, cudaStream_t stream);
 
 }  // namespace fsa

@@ -36,6 +36,7 @@ int device_sm_count(int* out);
 
 constexpr int kRkThreads = 384;
 constexpr int kRkUnits = 5;             // Q / dO tiles in the ring
+constexpr int kRkTile = kTileRows * 128 * 2;
 
 // ------------------------------------------------------------------------------------------------ plan
 // Tokens that see a row of a K/V tile: [first, last] over the tokens of its sequence (a CTA per tile; the ranges need not be
@@ -171,9 +172,8 @@ struct RangeKvParams {
     const float* lse;       // [Hq, N] log2 units
     const float* delta;     // [Hq, N]
     float4* slabs;
-    void *dk, *dv;          // [Nk, Hk, D] contiguous
+    void *dk, *dv;          // [Nk, Hk, 128] contiguous
     int* status;
-    ScoreMod mod;
 };
 
 // One work item: K/V rows [key0, key0 + nkeys) of head h, n row tiles of TPT tokens from tok0 on, tokens up to tok_last.
@@ -193,12 +193,18 @@ __device__ __forceinline__ RkItem rk_item(const RangeKvPlan& p, int w) {
     return m;
 }
 
-template <int D, int MOD, typename ET>
+__device__ __forceinline__ float rk_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+template <typename ET>
 __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvParams p, const __grid_constant__ CUtensorMap qmap,
                                                                const __grid_constant__ CUtensorMap domap,
                                                                const __grid_constant__ CUtensorMap kmap,
                                                                const __grid_constant__ CUtensorMap vmap) {
-    constexpr int KH = D / 64, kRkTile = kTileRows * D * 2;
+    constexpr int D = 128;
     constexpr int kSlab = kTileRows * 128;           // 64 columns of a tile
     constexpr int cS = 0, cP = 128, cDV = 256, cDK = 384;
     extern __shared__ __align__(1024) uint8_t smem[];
@@ -228,7 +234,7 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
     uint64_t* p_read = s_full + 12;     // [2 halves] dV(i) has read P
     uint64_t* ds_read = s_full + 14;    // [2] dK(i) has read dS
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(s_full + 16);
-    int* s_masked = reinterpret_cast<int*>(s_full + 16) + 2;              // [2] some row of the tile does not see all K/V rows; 2: or sees none
+    int* s_masked = reinterpret_cast<int*>(s_full + 16) + 2;              // [2] some row of the tile does not see all K/V rows
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int* status = p.status;
@@ -249,7 +255,7 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
     }
     // rows past G * TPT of a Q or dO tile are never loaded, but they are multiplied (by P = dS = 0)
     for (int i = p.G * p.plan.TPT * 8 + tid; i < kTileRows * 8; i += kRkThreads)
-        for (int u = 0; u < KH * kRkUnits; ++u) reinterpret_cast<uint4*>(sU + u * kSlab)[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int u = 0; u < 2 * kRkUnits; ++u) reinterpret_cast<uint4*>(sU + u * kSlab)[i] = make_uint4(0u, 0u, 0u, 0u);
     fence_async_smem();
     if (warp == 0) tmem_alloc(&tmem_slot, 512);
     tc_fence_before();
@@ -264,7 +270,7 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
         if (lane == 0) {
             bool ok = true;
             int u = 0, qi = 0;             // Q / dO tiles and non-empty items so far
-            const uint32_t unit_bytes = (uint32_t)(KH * 128 * TPT * p.G);
+            const uint32_t unit_bytes = (uint32_t)(2 * 128 * TPT * p.G);
             for (int w = blockIdx.x; w < nitems && ok; w += gridDim.x) {
                 const RkItem m = rk_item(p.plan, w);
                 if (m.n == 0) continue;
@@ -274,7 +280,7 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
                     if (!ok) return;
                     mbar_expect_tx(&u_full[st], unit_bytes);
 #pragma unroll
-                    for (int b = 0; b < KH; ++b) tma_load_3d(smem_u32(sU + st * kRkTile + b * kSlab), map, b * 64, tok, m.h * p.G, &u_full[st]);
+                    for (int b = 0; b < 2; ++b) tma_load_3d(smem_u32(sU + st * kRkTile + b * kSlab), map, b * 64, tok, m.h * p.G, &u_full[st]);
                     ++u;
                 };
                 auto load_kv = [&](const CUtensorMap* map, uint8_t* dst, uint64_t* full, uint64_t* empty) {
@@ -282,7 +288,7 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
                     if (!ok) return;
                     mbar_expect_tx(full, (uint32_t)kRkTile);
 #pragma unroll
-                    for (int b = 0; b < KH; ++b)
+                    for (int b = 0; b < 2; ++b)
 #pragma unroll
                         for (int r = 0; r < 2; ++r)
                             tma_load_2d(smem_u32(dst + b * kSlab + r * (kSlab / 2)), map, m.h * D + b * 64, m.key0 + r * 64, full);
@@ -392,20 +398,18 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
                         hi[j] = __ldg(p.plan.kv_hi + tok);
                     }
                 }
-                bool masked = false, unseen = false;
+                bool masked = false;
                 int vis[4][2];
 #pragma unroll
                 for (int j = 0; j < 4; ++j) {
                     const int l = max(lo[j] - m.key0, 0), u = min(hi[j] - m.key0, kTileRows - 1);
                     const bool sees = u >= l && lse[j] > -INFINITY && lse[j] < INFINITY;     // a row that saw nothing in the forward sees nothing here
                     masked |= sees && (l > 0 || u < m.nkeys - 1);
-                    unseen |= !sees && g[j] < p.G;
                     if (!sees) { lse[j] = INFINITY; del[j] = 0.f; }                          // exp2(s - inf) = 0
                     vis[j][0] = sees ? l : kTileRows - 1;
                     vis[j][1] = sees ? u | 128 : 128;
                 }
                 masked = __any_sync(0xffffffffu, masked);
-                if constexpr (MOD & kModGuard) unseen = __any_sync(0xffffffffu, unseen);
                 const int b = c & 1;
                 ok = ok && mbar_wait(&st_empty[b], ((c >> 1) & 1) ^ 1, status);
 #pragma unroll
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
                     sVis[b * 256 + lane + 32 * j] = (uint8_t)vis[j][0];
                     sVis[b * 256 + 128 + lane + 32 * j] = (uint8_t)vis[j][1];
                 }
-                if (lane == 0) s_masked[b] = (MOD & kModGuard) && unseen ? 2 : masked;
+                if (lane == 0) s_masked[b] = masked;
                 mbar_arrive(&st_full[b]);
             }
         }
@@ -426,15 +430,10 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
         const int key = quarter * 32 + lane;
         const uint32_t lane_off = (uint32_t)(quarter * 32) << 16;
         const uint32_t tS = tbase + lane_off + cS + grp * 64, tP = tbase + lane_off + cP + grp * 64;
-        const NearTanh near(p.mod, 1.f);
-        bool far = false;               // the tile before had scores near the cap
-        const int g_first = grp * 64 / TPT, e_first = grp * 64 - g_first * TPT;      // head and token of the group's first column
         bool ok = true;
         int c = 0, qi = 0;
         for (int w = blockIdx.x; w < nitems && warp_stays(ok); w += gridDim.x) {
             const RkItem m = rk_item(p.plan, w);
-            // place of this K/V row before (negative) or behind the item's first token
-            const int key_rel = (MOD & kModBias) && m.n > 0 ? m.key0 + key - __ldg(p.mod.pos + m.tok0) : 0;
             for (int i = 0; i < m.n && warp_stays(ok); ++i, ++c) {
                 const int b = c & 1;
                 ok = ok && mbar_wait(&st_full[b], (c >> 1) & 1, status);
@@ -448,75 +447,15 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
                 tmem_ld32(tS + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
                 tmem_ld_wait();
                 uint32_t pk[32];
-                if constexpr (MOD != 0) {
-                    // v: P (1 - tanh^2), what dS takes; pk: P.  NEAR: products whose tanh is near's (looked at afterwards), else v has been changed
-                    // already
-                    const float to_log2 = (MOD & kModCap) ? p.mod.cap_log2 : p.scale_log2;
-                    const uint64_t s2 = f32x2(to_log2, to_log2), one2 = f32x2(1.f, 1.f);
-                    float big[2] = {0.f, 0.f};
-                    auto pairs = [&](auto is_near) {
-                        int e4 = e_first, g4 = g_first;
-#pragma unroll
-                        for (int j = 0; j < 16; ++j) {
-                            const float4 l = lse4[j];
-                            float c[4] = {-l.x, -l.y, -l.z, -l.w};
-                            if constexpr (MOD & kModBias) {
-                                // four columns: consecutive tokens of one head
-                                const float slope = __ldg(p.mod.slopes + m.h * p.G + min(g4, p.G - 1)) * kLog2e, d = (float)(key_rel - i * TPT - e4);
-#pragma unroll
-                                for (int q = 0; q < 4; ++q) c[q] = p.mod.ahead ? fmaf(-slope, fabsf(d - (float)q), c[q]) : fmaf(slope, d - (float)q, c[q]);
-                                e4 += 4;
-                                if (e4 == TPT) { e4 = 0; ++g4; }
-                            }
-#pragma unroll
-                            for (int q = 0; q < 4; q += 2) {
-                                const int k = 4 * j + q;
-                                uint64_t x = f32x2(__uint_as_float(v[k]), __uint_as_float(v[k + 1]));
-                                if constexpr (decltype(is_near)::on) {
-                                    big[(k >> 1) & 1] = max3_abs(big[(k >> 1) & 1], __uint_as_float(v[k]), __uint_as_float(v[k + 1]));
-                                    x = mul_f32x2(x, near.slope(x));
-                                }
-                                const float2 s = f32x2_get(fma_f32x2(x, s2, f32x2(c[q], c[q + 1])));
-                                float2 pr = make_float2(ex2_approx(s.x), ex2_approx(s.y));
-                                pk[k >> 1] = ElemTraits<ET>::pack2(pr.x, pr.y);
-                                if constexpr (MOD & kModCap) {
-                                    const float2 th = f32x2_get(x);
-                                    pr = f32x2_get(mul_f32x2(f32x2(pr.x, pr.y), fma_f32x2(f32x2(-th.x, -th.y), x, one2)));
-                                }
-                                v[k] = __float_as_uint(pr.x);
-                                v[k + 1] = __float_as_uint(pr.y);
-                            }
-                        }
-                    };
-                    if constexpr (MOD & kModCap) {
-                        bool is_far = far;
-                        if (!is_far) {
-                            pairs(Flag<true>{});
-                            is_far = __any_sync(0xffffffffu, !(fmaxf(big[0], big[1]) <= p.mod.near_v));
-                            if (is_far) {
-                                tmem_ld32(tS, *reinterpret_cast<uint32_t (*)[32]>(&v[0]));
-                                tmem_ld32(tS + 32, *reinterpret_cast<uint32_t (*)[32]>(&v[32]));
-                                tmem_ld_wait();
-                            }
-                        }
-                        if (is_far) {
-                            far = cap_scores(v, p.mod.x_scale, p.mod.near_v);
-                            pairs(Flag<false>{});
-                        }
-                    } else {
-                        pairs(Flag<false>{});
-                    }
-                } else {
 #pragma unroll
                 for (int j = 0; j < 16; ++j) {
                     const float4 l = lse4[j];
-                    float x0 = ex2_approx(fmaf(__uint_as_float(v[4 * j]), p.scale_log2, -l.x));
-                    float x1 = ex2_approx(fmaf(__uint_as_float(v[4 * j + 1]), p.scale_log2, -l.y));
-                    float x2 = ex2_approx(fmaf(__uint_as_float(v[4 * j + 2]), p.scale_log2, -l.z));
-                    float x3 = ex2_approx(fmaf(__uint_as_float(v[4 * j + 3]), p.scale_log2, -l.w));
+                    float x0 = rk_ex2(fmaf(__uint_as_float(v[4 * j]), p.scale_log2, -l.x));
+                    float x1 = rk_ex2(fmaf(__uint_as_float(v[4 * j + 1]), p.scale_log2, -l.y));
+                    float x2 = rk_ex2(fmaf(__uint_as_float(v[4 * j + 2]), p.scale_log2, -l.z));
+                    float x3 = rk_ex2(fmaf(__uint_as_float(v[4 * j + 3]), p.scale_log2, -l.w));
                     v[4 * j] = __float_as_uint(x0); v[4 * j + 1] = __float_as_uint(x1);
                     v[4 * j + 2] = __float_as_uint(x2); v[4 * j + 3] = __float_as_uint(x3);
-                }
                 }
                 if (masked) {
                     // four rows at a time: bit 7 of a byte of (128 | key) - first says key >= first, of (128 | last) - key that key <= last
@@ -530,33 +469,11 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
                                                   ((key4 | 0x80808080u) - f.z) & (l.z - key4), ((key4 | 0x80808080u) - f.w) & (l.w - key4)};
 #pragma unroll
                         for (int q = 0; q < 16; ++q)
-                            if (!(seen[q >> 2] & (0x80u << ((q & 3) * 8)))) {
-                                v[16 * j + q] = 0u;
-                                if (MOD != 0) pk[8 * j + (q >> 1)] &= (q & 1) ? 0x0000ffffu : 0xffff0000u;
-                            }
-                    }
-                }
-                if constexpr (MOD & kModGuard) {
-                    // Q and dO rows that see nothing here are multiplied by dS = P = 0: zeros take the place of what may be NaN.  The group's
-                    // half of S and dP is done; every thread has half of one of its 64 rows.
-                    if (s_masked[b] == 2) {
-                        ok = ok && mbar_wait(&dp_full[grp], c & 1, status);
-                        tc_fence_after();
-                        const int row = grp * 64 + (key & 63);
-                        if (ok && sLse[b * 128 + row] == INFINITY)
-#pragma unroll 1
-                            for (int u = 2 * c; u < 2 * c + 2; ++u)
-#pragma unroll
-                                for (int n = 0; n < D / 16; ++n) {
-                                    const int chunk = (key >> 6) * (D / 16) + n;
-                                    *reinterpret_cast<uint4*>(sU + (u % kRkUnits) * kRkTile + (chunk >> 3) * kSlab + sw128_chunk_off(row, chunk & 7)) =
-                                        make_uint4(0u, 0u, 0u, 0u);
-                                }
-                        fence_async_smem();
+                            if (!(seen[q >> 2] & (0x80u << ((q & 3) * 8)))) v[16 * j + q] = 0u;
                     }
                 }
 #pragma unroll
-                for (int j = 0; j < (MOD ? 0 : 32); ++j) pk[j] = ElemTraits<ET>::pack2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
+                for (int j = 0; j < 32; ++j) pk[j] = ElemTraits<ET>::pack2(__uint_as_float(v[2 * j]), __uint_as_float(v[2 * j + 1]));
                 tmem_st32(tS, pk);
                 tmem_st_wait();
                 tc_fence_before();
@@ -568,25 +485,6 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
                     uint32_t d[32], dd[16];
                     tmem_ld32(tP + hf * 32, d);
                     tmem_ld_wait();
-                    if constexpr (MOD != 0) {
-                        const uint64_t g2 = f32x2(p.scale, p.scale);
-#pragma unroll
-                        for (int j = 0; j < 8; ++j) {
-                            const float4 dl = del4[hf * 8 + j];
-                            const int k4 = hf * 32 + 4 * j;
-                            const float2 x = f32x2_get(mul_f32x2(f32x2(__uint_as_float(v[k4]), __uint_as_float(v[k4 + 1])),
-                                                                 fma_f32x2(f32x2(__uint_as_float(d[4 * j]), __uint_as_float(d[4 * j + 1])), g2, f32x2(-dl.x, -dl.y))));
-                            const float2 y = f32x2_get(mul_f32x2(f32x2(__uint_as_float(v[k4 + 2]), __uint_as_float(v[k4 + 3])),
-                                                                 fma_f32x2(f32x2(__uint_as_float(d[4 * j + 2]), __uint_as_float(d[4 * j + 3])), g2, f32x2(-dl.z, -dl.w))));
-                            dd[2 * j] = ElemTraits<ET>::pack2(x.x, x.y);
-                            dd[2 * j + 1] = ElemTraits<ET>::pack2(y.x, y.y);
-                        }
-                        if (masked) {           // (dP may be NaN where nothing is seen)
-#pragma unroll
-                            for (int j = 0; j < 16; ++j)
-                                dd[j] &= (v[hf * 32 + 2 * j] ? 0x0000ffffu : 0u) | (v[hf * 32 + 2 * j + 1] ? 0xffff0000u : 0u);
-                        }
-                    } else {
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float4 dl = del4[hf * 8 + j];
@@ -595,7 +493,6 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
                                                           __uint_as_float(v[k4 + 1]) * fmaf(__uint_as_float(d[4 * j + 1]), p.scale, -dl.y));
                         dd[2 * j + 1] = ElemTraits<ET>::pack2(__uint_as_float(v[k4 + 2]) * fmaf(__uint_as_float(d[4 * j + 2]), p.scale, -dl.z),
                                                               __uint_as_float(v[k4 + 3]) * fmaf(__uint_as_float(d[4 * j + 3]), p.scale, -dl.w));
-                    }
                     }
                     tmem_st16(tP + hf * 16, dd);
                 }
@@ -611,7 +508,7 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
             }
             const bool write = ok && key < m.nkeys;
             ET* dst = reinterpret_cast<ET*>(grp ? p.dk : p.dv) + ((int64_t)(m.key0 + key) * p.plan.Hk + m.h) * D;
-            float4* slab = p.slabs + ((int64_t)m.slab * p.plan.Hk + m.h) * (2 * (D / 4) * 128) + grp * ((D / 4) * 128) + key;
+            float4* slab = p.slabs + ((int64_t)m.slab * p.plan.Hk + m.h) * (2 * 32 * 128) + grp * (32 * 128) + key;
 #pragma unroll
             for (int c0 = 0; c0 < D; c0 += 32) {
                 uint32_t a[32];
@@ -647,7 +544,6 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
     tc_fence_before();
     __syncthreads();
     if (warp == 0) tmem_dealloc(tbase, 512);
-    if constexpr (MOD != 0) follow_late();      // it runs beside the dQ kernel, of which it needs nothing
 }
 
 cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream, bool dependent) {
@@ -660,60 +556,49 @@ cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int
     return cudaGetLastError();
 }
 
-template <int D, int MOD, typename ET>
-static cudaError_t launch_rk(const RangeKvParams& p, const CUtensorMap* maps, int sms, int64_t max_items, cudaStream_t stream) {
-    constexpr int smem = (2 + kRkUnits) * (kTileRows * D * 2) + 2 * 128 * (4 + 4 + 2) + 512;
-    auto kern = range_bwd_dkdv<D, MOD, ET>;
+template <int D, typename ET>
+static cudaError_t launch_reduce(const RangeKvPlan& p, const float* slabs, void* dk, void* dv, int sms, cudaStream_t stream) {
+    const cudaError_t e = prefer_l1((const void*)range_dkdv_reduce<D, ET>);
+    if (e != cudaSuccess) return e;
+    return launch_dependent(range_dkdv_reduce<D, ET>, dim3((unsigned)(4 * sms)), 256, 0, stream, 1, p, (const float4*)slabs, (ET*)dk, (ET*)dv);
+}
+
+cudaError_t launch_range_dkdv_reduce(int dtype, const RangeKvPlan& p, const float* slabs, void* dk, void* dv, int sms, cudaStream_t stream) {
+    if (p.D == 128) return dtype == kBF16 ? launch_reduce<128, __nv_bfloat16>(p, slabs, dk, dv, sms, stream) : launch_reduce<128, __half>(p, slabs, dk, dv, sms, stream);
+    return dtype == kBF16 ? launch_reduce<64, __nv_bfloat16>(p, slabs, dk, dv, sms, stream) : launch_reduce<64, __half>(p, slabs, dk, dv, sms, stream);
+}
+
+template <typename ET>
+static cudaError_t launch_rk(const RangeKvParams& p, const CUtensorMap& qmap, const CUtensorMap& domap, const CUtensorMap& kmap, const CUtensorMap& vmap,
+                             int sms, int64_t max_items, cudaStream_t stream) {
+    constexpr int smem = (2 + kRkUnits) * kRkTile + 2 * 128 * (4 + 4 + 2) + 512;
+    auto kern = range_bwd_dkdv<ET>;
     cudaError_t e = allow_smem((const void*)kern, smem);
     if (e != cudaSuccess) return e;
-    const unsigned grid = (unsigned)(max_items < sms ? max_items : sms);
-    if constexpr (MOD != 0) {
-        e = launch_dependent(kern, dim3(grid), kRkThreads, smem, stream, 1, p, maps[0], maps[1], maps[2], maps[3]);
-        if (e == cudaSuccess) e = prefer_l1((const void*)range_dkdv_reduce<D, ET>);
-        if (e != cudaSuccess) return e;
-        return launch_dependent(range_dkdv_reduce<D, ET>, dim3((unsigned)(4 * sms)), 256, 0, stream, 1, p.plan, (const float4*)p.slabs, (ET*)p.dk, (ET*)p.dv);
-    }
     prof_begin(FSA_KERNEL_SEL_BWD_MAIN, stream);
-    kern<<<grid, kRkThreads, smem, stream>>>(p, maps[0], maps[1], maps[2], maps[3]);
+    kern<<<(unsigned)(max_items < sms ? max_items : sms), kRkThreads, smem, stream>>>(p, qmap, domap, kmap, vmap);
     prof_end(FSA_KERNEL_SEL_BWD_MAIN, stream);
-    e = prefer_l1((const void*)range_dkdv_reduce<D, ET>);
+    e = prefer_l1((const void*)range_dkdv_reduce<128, ET>);
     if (e != cudaSuccess) return e;
-    range_dkdv_reduce<D, ET><<<(unsigned)(4 * sms), 256, 0, stream>>>(p.plan, (const float4*)p.slabs, (ET*)p.dk, (ET*)p.dv);
+    range_dkdv_reduce<128, ET><<<(unsigned)(4 * sms), 256, 0, stream>>>(p.plan, (const float4*)p.slabs, (ET*)p.dk, (ET*)p.dv);
     return cudaGetLastError();
 }
 
-template <int D, typename ET>
-static cudaError_t launch_rk_mod(int mod, const RangeKvParams& p, const CUtensorMap* maps, int sms, int64_t max_items, cudaStream_t stream) {
-    switch (mod) {
-        case 0: return launch_rk<D, kModGuard, ET>(p, maps, sms, max_items, stream);
-        case 1: return launch_rk<D, 1 | kModGuard, ET>(p, maps, sms, max_items, stream);
-        case 2: return launch_rk<D, 2 | kModGuard, ET>(p, maps, sms, max_items, stream);
-        case 3: return launch_rk<D, 3 | kModGuard, ET>(p, maps, sms, max_items, stream);
-        default: return cudaErrorInvalidValue;
-    }
-}
-
 cudaError_t launch_range_bwd_dkdv(int dtype, const RangeKvPlan& plan, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap,
-                                  const CUtensorMap& vmap, int* status, cudaStream_t stream, const ScoreMod* mod, int which) {
-    const int D = mod ? s.D : 128;
-    CUtensorMap maps[4];        // Q, dO, K, V
-    if (make_tile_map_3d_box(&maps[0], a.q, dtype, D, s.N, s.Hq, a.q_sn, a.q_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
-    if (make_tile_map_3d_box(&maps[1], a.d_o, dtype, D, s.N, s.Hq, a.do_sn, a.do_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
-    maps[2] = kmap; maps[3] = vmap;
+                                  const CUtensorMap& vmap, int* status, cudaStream_t stream) {
+    CUtensorMap qmap, domap;
+    if (make_tile_map_3d_box(&qmap, a.q, dtype, 128, s.N, s.Hq, a.q_sn, a.q_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
+    if (make_tile_map_3d_box(&domap, a.d_o, dtype, 128, s.N, s.Hq, a.do_sn, a.do_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
     RangeKvParams p;
     p.plan = plan;
     p.Hq = s.Hq; p.G = s.G;
     p.scale = a.sm_scale; p.scale_log2 = a.sm_scale * 1.4426950408889634f;
     p.lse = a.lse; p.delta = a.delta; p.slabs = (float4*)a.slabs; p.dk = a.dk; p.dv = a.dv; p.status = status;
-    p.mod = mod ? *mod : ScoreMod{};
     int sms = 0;
     if (device_sm_count(&sms) != 0 || sms <= 0) return cudaErrorInvalidValue;
     const int64_t max_items = (range_kv_max_tiles(s) + range_kv_max_cut(s)) * s.Hk;
-    const bool bf16 = dtype == kBF16;
-    if (!mod) return bf16 ? launch_rk<128, 0, __nv_bfloat16>(p, maps, sms, max_items, stream) : launch_rk<128, 0, __half>(p, maps, sms, max_items, stream);
-    if (D == 128)
-        return bf16 ? launch_rk_mod<128, __nv_bfloat16>(which, p, maps, sms, max_items, stream) : launch_rk_mod<128, __half>(which, p, maps, sms, max_items, stream);
-    return bf16 ? launch_rk_mod<64, __nv_bfloat16>(which, p, maps, sms, max_items, stream) : launch_rk_mod<64, __half>(which, p, maps, sms, max_items, stream);
+    return dtype == kBF16 ? launch_rk<__nv_bfloat16>(p, qmap, domap, kmap, vmap, sms, max_items, stream)
+                          : launch_rk<__half>(p, qmap, domap, kmap, vmap, sms, max_items, stream);
 }
 
 }  // namespace fsa

@@ -22,8 +22,7 @@
 #include "../../include/fsa_sm100.h"
 #include <climits>
 
-#include "range_bwd.cuh"
-#include "range_fwd.cuh"
+#include "sel_launch.cuh"
 
 namespace fsa {
 
@@ -32,8 +31,36 @@ int make_tile_map_3d_box(CUtensorMap* map, const void* base, int dtype, int64_t 
                          int64_t stride2, int box1, int box2);
 int device_sm_count(int* out);
 
+struct RangeDenseParams {
+    const int32_t* cu_q;    // [B + 1]
+    const int32_t* cu_k;    // [B + 1] first K/V row of every sequence
+    const int32_t* kv_lo;   // [N] lowest visible K/V row of every token, or null (the sequence's first row)
+    const int32_t* kv_hi;   // [N] highest visible K/V row, lower than kv_lo when the token sees nothing
+    int64_t N, Nk;
+    int B, Hq, Hk, G, TPT;
+    float scale_log2;
+    void* o;  int64_t o_sn, o_sh;     // [N, Hq, D]
+    float* lse;                       // [Hq, N] log2 units
+    int* status;
+};
+
+// Up to three problems in one launch (blockIdx.z): branches of a layer that do not wait for one another.  A short prompt has fewer tiles
+// than the SMs hold CTAs, and each launch of its own left most of them empty (517 tokens, 32 / 8 heads: 3 x 11 us, together 19: prefill 158 -> 138 us).
+constexpr int kRdProblems = 3;
+struct RangeDenseLaunch {
+    CUtensorMap q[kRdProblems], k[kRdProblems], v[kRdProblems], o[kRdProblems];
+    RangeDenseParams p[kRdProblems];
+};
+
 constexpr int kRdThreads = 192;
+constexpr int kRdBK = 64;
 constexpr float kRdLazy = 8.0f;       // raise a row's reference max only when exceeded by more than this (log2 units)
+
+__device__ __forceinline__ float rd_ex2(float x) {
+    float y;
+    asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
 
 // One item: a tile of tokens x one KV head of problem z.
 struct RdItem {
@@ -318,7 +345,7 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 float alpha = 1.f;
                 const bool raise = m_blk > m_ref + kRdLazy;     // false when m_blk is -inf; true when m_ref is -inf and m_blk finite
                 if (raise) {
-                    alpha = m_ref == -INFINITY ? 0.f : ex2_approx(m_ref - m_blk);
+                    alpha = m_ref == -INFINITY ? 0.f : rd_ex2(m_ref - m_blk);
                     m_ref = m_blk;
                 }
                 // accumulator rows already hold products (j > 0): rescale them when any row of the warp changes reference
@@ -343,10 +370,10 @@ __global__ void __launch_bounds__(kRdThreads, 2) range_fwd_dense(const __grid_co
                 uint32_t pk[BK / 2];
 #pragma unroll
                 for (int i = 0; i < BK; i += 4) {
-                    const float p0 = ex2_approx(fmaf(__uint_as_float(v[i]), scale_log2, -m_use));
-                    const float p1 = ex2_approx(fmaf(__uint_as_float(v[i + 1]), scale_log2, -m_use));
-                    const float p2 = ex2_approx(fmaf(__uint_as_float(v[i + 2]), scale_log2, -m_use));
-                    const float p3 = ex2_approx(fmaf(__uint_as_float(v[i + 3]), scale_log2, -m_use));
+                    const float p0 = rd_ex2(fmaf(__uint_as_float(v[i]), scale_log2, -m_use));
+                    const float p1 = rd_ex2(fmaf(__uint_as_float(v[i + 1]), scale_log2, -m_use));
+                    const float p2 = rd_ex2(fmaf(__uint_as_float(v[i + 2]), scale_log2, -m_use));
+                    const float p3 = rd_ex2(fmaf(__uint_as_float(v[i + 3]), scale_log2, -m_use));
                     ls[0] += p0; ls[1] += p1; ls[2] += p2; ls[3] += p3;
                     pk[i >> 1] = ElemTraits<ET>::pack2(p0, p1);
                     pk[(i >> 1) + 1] = ElemTraits<ET>::pack2(p2, p3);
@@ -467,7 +494,6 @@ struct RangeDqParams {
     const float* delta;     // [Hq, N] sum_d o dO
     void* dq;               // [N, Hq, D] contiguous
     int* status;
-    ScoreMod mod;
 };
 
 constexpr int kDqThreads = 384;     // producer, S/dP issuer, 8 row warps, dQ issuer, item warp
@@ -480,17 +506,16 @@ static_assert(kMaxTokens / kRdBK * kDqTileClocks + FSA_WAIT_CLOCKS < (int64_t)1 
 
 // One work item of the dQ kernel: a tile of tokens x one KV head.
 struct DqItem {
-    int seq, tok0, ne, row_lo, nblk, h, row_hi;
+    int seq, tok0, ne, row_lo, nblk, h;
 };
 
 // Work item w of the list (heaviest tiles first).  Warp-collective: all 32 lanes call it and get the same answer.
-template <int MOD>
 __device__ __forceinline__ DqItem dq_item(const RangeDqParams& p, int ntiles, int w, int lane) {
     DqItem m;
     m.h = w % p.Hk;
-    m.row_lo = 0; m.nblk = 0; m.row_hi = -1;
-    if constexpr (MOD != 0) find_ranked_tile(p.cu_q, p.cu_k, p.B, p.TPT, w / p.Hk, lane, m.seq, m.tok0, m.ne);
-    else find_seq_tile(p.cu_q, p.B, p.TPT, ntiles - 1 - w / p.Hk, lane, m.seq, m.tok0, m.ne);
+    const int want = ntiles - 1 - w / p.Hk;
+    m.row_lo = 0; m.nblk = 0;
+    find_seq_tile(p.cu_q, p.B, p.TPT, want, lane, m.seq, m.tok0, m.ne);
     if (m.seq < 0) return m;
     int lo = INT_MAX, hi = -1;
     const int k0 = __ldg(p.cu_k + m.seq);
@@ -506,18 +531,18 @@ __device__ __forceinline__ DqItem dq_item(const RangeDqParams& p, int ntiles, in
     }
     lo = max(lo, 0);
     hi = min(hi, (int)p.Nk - 1);
-    m.row_lo = lo; m.row_hi = hi;
+    m.row_lo = lo;
     m.nblk = hi >= lo ? (hi - lo) / kRdBK + 1 : 0;
     return m;
 }
 
-template <int D, int MOD, typename ET>
+template <typename ET>
 __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeDqParams p, const __grid_constant__ CUtensorMap qmap,
                                                                    const __grid_constant__ CUtensorMap domap,
                                                                    const __grid_constant__ CUtensorMap kmap,
                                                                    const __grid_constant__ CUtensorMap vmap,
                                                                    const __grid_constant__ CUtensorMap dqmap) {
-    constexpr int BK = kRdBK, KH = D / 64;
+    constexpr int D = 128, BK = kRdBK, KH = D / 64;
     constexpr int kQ = kTileRows * D * 2;            // Q tile, same for dO
     constexpr int kKt = BK * D * 2;
     constexpr int kOut = kTileRows * 128;            // 64 columns of the dQ tile on their way out
@@ -546,7 +571,6 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     int* status = p.status;
-    if constexpr (MOD != 0) follow_late();
     if (tid == 0) {
         mbar_init(qd_full, 1); mbar_init(qd_empty, 256);
         for (int i = 0; i < kDqStages; ++i) { mbar_init(&kv_full[i], 1); mbar_init(&kv_empty[i], 1); }
@@ -568,7 +592,6 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
     __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tmem_slot;
-    if constexpr (MOD != 0) let_next_start();
     const int ntiles = count_seq_tiles(p.cu_q, p.B, p.TPT, lane);
     const int nitems = ntiles * p.Hk;
     // Entry n of this CTA's items: every warp but the one that fills the ring takes each of them once, in order.
@@ -578,7 +601,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
         ok = warp_ok(ok);
         if (lane == 0) mbar_arrive(&it_empty[n % kDqItems]);
         DqItem m;
-        m.seq = x.x; m.tok0 = x.y; m.ne = x.z; m.row_lo = x.w; m.nblk = y.x; m.h = y.y; m.row_hi = y.z;
+        m.seq = x.x; m.tok0 = x.y; m.ne = x.z; m.row_lo = x.w; m.nblk = y.x; m.h = y.y;
         if (!ok) m.ne = m.nblk = 0;
         return m;
     };
@@ -588,13 +611,13 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
         bool ok = true;
         int n = 0, longest = 0;
         for (int w = blockIdx.x; w < nitems && ok; w += gridDim.x, ++n) {
-            const DqItem m = dq_item<MOD>(p, ntiles, w, lane);
+            const DqItem m = dq_item(p, ntiles, w, lane);
             ok = ok && mbar_wait(&it_empty[n % kDqItems], ((n / kDqItems) & 1) ^ 1, status, FSA_WAIT_CLOCKS + longest * kDqTileClocks);
             ok = warp_ok(ok);
             longest = max(longest, m.nblk);
             if (ok && lane == 0) {
                 s_item[(n % kDqItems) * 2] = make_int4(m.seq, m.tok0, m.ne, m.row_lo);
-                s_item[(n % kDqItems) * 2 + 1] = make_int4(m.nblk, m.h, m.row_hi, 0);
+                s_item[(n % kDqItems) * 2 + 1] = make_int4(m.nblk, m.h, 0, 0);
                 mbar_arrive(&it_full[n % kDqItems]);
             }
         }
@@ -724,36 +747,30 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
             ok = ok && mbar_wait(qd_full, qi & 1, status);
             ++qi;
             const uint8_t* src = sb ? sDO : sQ;
-            uint32_t x[KH][32];
+            uint32_t x[2][32];
 #pragma unroll
             for (int i = 0; i < D / 8; ++i)
                 *reinterpret_cast<uint4*>(&x[i >> 3][(i & 7) * 4]) = *reinterpret_cast<const uint4*>(src + (i >> 3) * (kTileRows * 128) + sw128_chunk_off(r, i & 7));
-#pragma unroll
-            for (int b = 0; b < KH; ++b) tmem_st32(tbase + lane_off + (sb ? cDO : cQ) + b * 32, x[b]);
+            tmem_st32(tbase + lane_off + (sb ? cDO : cQ), x[0]);
+            tmem_st32(tbase + lane_off + (sb ? cDO : cQ) + 32, x[1]);
             tmem_st_wait();
             tc_fence_before();
             mbar_arrive(qd_empty);
             mbar_arrive(qt_full);
         };
         // This row's numbers, loaded an item ahead: item numbers and loads of their own between two items were a third of the kernel.
-        struct Row { int lo, hi; float lse, delta, slope; int pos; };
+        struct Row { int lo, hi; float lse, delta; };
         auto load_numbers = [&](const DqItem& m) {
-            Row x = {0, -1, 0.f, 0.f, 0.f, 0};
+            Row x = {0, -1, 0.f, 0.f};
             if (g < p.G && e < m.ne) {
                 x.lo = p.kv_lo ? __ldg(p.kv_lo + m.tok0 + e) : __ldg(p.cu_k + m.seq);
                 x.hi = __ldg(p.kv_hi + m.tok0 + e);
                 const int64_t idx = (int64_t)(m.h * p.G + g) * p.N + m.tok0 + e;
                 x.lse = __ldg(p.lse + idx);
-                x.delta = MOD ? __ldcg(p.delta + idx) : __ldg(p.delta + idx);        // (MOD: the kernel before wrote it)
-                if constexpr (MOD & kModBias) {
-                    x.slope = __ldg(p.mod.slopes + m.h * p.G + g) * kLog2e;
-                    x.pos = __ldg(p.mod.pos + m.tok0 + e);
-                }
+                x.delta = __ldg(p.delta + idx);
             }
             return x;
         };
-        const NearTanh near(p.mod, 1.f);
-        bool far = false;               // the tile before had scores near the cap
         DqItem m;
         m.nblk = m.ne = 0;
         int n = 0;
@@ -767,8 +784,7 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
             const bool row_valid = g < p.G && e < m.ne;
             const int tok = m.tok0 + e;
             const int lo_r = row.lo;
-            const float lse_r = row.lse, delta_s = row.delta * p.scale, slope_r = row.slope;
-            const int pos_r = row.pos;
+            const float lse_r = row.lse, delta_s = row.delta * p.scale;
             int hi_r = min(row.hi, (int)p.Nk - 1);              // rows past the end of K/V do not exist
             if (!(lse_r > -INFINITY)) hi_r = lo_r - 1;          // a row that saw nothing in the forward sees nothing here
             DqItem next;
@@ -792,67 +808,22 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
                     tc_fence_before();
                     mbar_arrive(&sdp_free[b]);       // both rows are in registers: the buffer may take tile c + 2
                     if (j + 1 == m.nblk && next.nblk > 0) take_row();      // the next item's S / dP run under this item's end
-                    // bit i: column cb + i is seen
-                    const int v_lo = min(max(c_lo - cb, 0), HC), v_hi = min(max(c_hi - cb, 0), HC);
-                    const uint32_t vis = v_hi > v_lo ? (0xffffffffu >> (HC - v_hi + v_lo)) << v_lo : 0u;
-                    if constexpr (MOD != 0) {
-                        const float to_log2 = (MOD & kModCap) ? p.mod.cap_log2 : p.scale_log2;
-                        const uint64_t s2 = f32x2(to_log2, to_log2), g2 = f32x2(p.scale, p.scale), d2 = f32x2(-delta_s, -delta_s), one2 = f32x2(1.f, 1.f);
-                        const float rel = (float)(pos_r - R0 - cb);
-                        const float base = (MOD & kModBias) ? fmaf(-slope_r, rel, -lse_r) : -lse_r;
-                        float big[2] = {0.f, 0.f};
-                        // dS of the columns, two at a time.  NEAR: products whose tanh is near's (looked at afterwards), else sv has been changed
-                        // already; BOTH: keys behind the token's place are seen too; ALL: no mask
-                        auto pairs = [&](auto is_near, auto both, auto all) {
-#pragma unroll
-                            for (int i = 0; i < 32; i += 2) {
-                                float b0 = base, b1 = base;
-                                if constexpr (MOD & kModBias) {
-                                    b0 = decltype(both)::on ? fmaf(-slope_r, fabsf(rel - (float)i), -lse_r) : fmaf(slope_r, (float)i, base);
-                                    b1 = decltype(both)::on ? fmaf(-slope_r, fabsf(rel - (float)(i + 1)), -lse_r) : fmaf(slope_r, (float)(i + 1), base);
-                                }
-                                uint64_t x = f32x2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-                                if constexpr (decltype(is_near)::on) {
-                                    big[(i >> 1) & 1] = max3_abs(big[(i >> 1) & 1], __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
-                                    x = mul_f32x2(x, near.slope(x));
-                                }
-                                const float2 s = f32x2_get(fma_f32x2(x, s2, f32x2(b0, b1)));
-                                uint64_t gr = fma_f32x2(f32x2(__uint_as_float(dv[i]), __uint_as_float(dv[i + 1])), g2, d2);
-                                // d tanh(x) = 1 - tanh(x)^2
-                                if constexpr (MOD & kModCap) {
-                                    const float2 th = f32x2_get(x);
-                                    gr = mul_f32x2(gr, fma_f32x2(f32x2(-th.x, -th.y), x, one2));
-                                }
-                                const float2 ds = f32x2_get(mul_f32x2(f32x2(ex2_approx(s.x), ex2_approx(s.y)), gr));
-                                dd[i >> 1] = decltype(all)::on ? ElemTraits<ET>::pack2(ds.x, ds.y)
-                                                               : ElemTraits<ET>::pack2(vis >> i & 1u ? ds.x : 0.f, vis >> (i + 1) & 1u ? ds.y : 0.f);
-                            }
-                        };
-                        const bool both = (MOD & kModBias) && p.mod.ahead && __any_sync(0xffffffffu, hi_r > pos_r);
-                        bool is_far = both || far;
-                        if (!is_far) {
-                            if (all_visible) pairs(Flag<(MOD & kModCap) != 0>{}, Flag<false>{}, Flag<true>{});
-                            else pairs(Flag<(MOD & kModCap) != 0>{}, Flag<false>{}, Flag<false>{});
-                            if constexpr (MOD & kModCap) is_far = __any_sync(0xffffffffu, !(fmaxf(big[0], big[1]) <= p.mod.near_v));
-                        }
-                        if (is_far) {
-                            if constexpr (MOD & kModCap) far = cap_scores(sv, p.mod.x_scale, p.mod.near_v);
-                            if (both) pairs(Flag<false>{}, Flag<true>{}, Flag<false>{});
-                            else pairs(Flag<false>{}, Flag<false>{}, Flag<false>{});
-                        }
-                    } else if (all_visible) {
+                    if (all_visible) {
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
-                            const float p0 = ex2_approx(fmaf(__uint_as_float(sv[i]), p.scale_log2, -lse_r));
-                            const float p1 = ex2_approx(fmaf(__uint_as_float(sv[i + 1]), p.scale_log2, -lse_r));
+                            const float p0 = rd_ex2(fmaf(__uint_as_float(sv[i]), p.scale_log2, -lse_r));
+                            const float p1 = rd_ex2(fmaf(__uint_as_float(sv[i + 1]), p.scale_log2, -lse_r));
                             dd[i >> 1] = ElemTraits<ET>::pack2(p0 * fmaf(__uint_as_float(dv[i]), p.scale, -delta_s),
                                                                p1 * fmaf(__uint_as_float(dv[i + 1]), p.scale, -delta_s));
                         }
                     } else {
+                        // bit i: column cb + i is seen
+                        const int v_lo = min(max(c_lo - cb, 0), HC), v_hi = min(max(c_hi - cb, 0), HC);
+                        const uint32_t vis = v_hi > v_lo ? (0xffffffffu >> (HC - v_hi + v_lo)) << v_lo : 0u;
 #pragma unroll
                         for (int i = 0; i < 32; i += 2) {
-                            const float p0 = ex2_approx(fmaf(__uint_as_float(sv[i]), p.scale_log2, -lse_r));
-                            const float p1 = ex2_approx(fmaf(__uint_as_float(sv[i + 1]), p.scale_log2, -lse_r));
+                            const float p0 = rd_ex2(fmaf(__uint_as_float(sv[i]), p.scale_log2, -lse_r));
+                            const float p1 = rd_ex2(fmaf(__uint_as_float(sv[i + 1]), p.scale_log2, -lse_r));
                             const float d0 = (vis >> i & 1u) && p0 > 0.f ? p0 * fmaf(__uint_as_float(dv[i]), p.scale, -delta_s) : 0.f;
                             const float d1 = (vis >> (i + 1) & 1u) && p1 > 0.f ? p1 * fmaf(__uint_as_float(dv[i + 1]), p.scale, -delta_s) : 0.f;
                             dd[i >> 1] = ElemTraits<ET>::pack2(d0, d1);
@@ -861,44 +832,26 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
                 }
                 tmem_st16(tbase + lane_off + b * 128 + BK + cb, dd);
                 tmem_st_wait();
-                if constexpr (MOD & kModGuard) {
-                    // K rows that no row of the item sees are multiplied by dS = 0: zeros take the place of what may be NaN (the tile's S is
-                    // done).  Every thread has a quarter of one of the 64 rows.
-                    const int kr = R0 + (r & (BK - 1)), part = sb * 2 + (r >> 6);
-                    const bool unseen = kr > m.row_hi || (p.mod.key_ids && __ldg(p.mod.key_ids + kr) < 0);
-                    if (__any_sync(0xffffffffu, unseen)) {
-                        if (unseen && ok)
-#pragma unroll
-                            for (int i = 0; i < D / 32; ++i) {
-                                const int chunk = part * (D / 32) + i;
-                                *reinterpret_cast<uint4*>(sKV + (c % kDqStages) * 2 * kKt + (chunk >> 3) * (BK * 128) + sw128_chunk_off(r & (BK - 1), chunk & 7)) =
-                                    make_uint4(0u, 0u, 0u, 0u);
-                            }
-                        fence_async_smem();
-                    }
-                }
                 tc_fence_before();
                 mbar_arrive(&ds_full[b]);
             }
             if (m.nblk == 0 && next.nblk > 0) take_row();
             // ---- epilogue of the item: this group's 64 of the 128 dQ columns
-            // (at head size 64 a group has 32 columns, whose 64 bytes a row go out as plain stores)
-            constexpr int kOwn = D / 2;
-            const bool full_tile = D == 128 && m.ne == p.TPT && p.G * p.TPT == kTileRows && m.nblk > 0;
+            const bool full_tile = m.ne == p.TPT && p.G * p.TPT == kTileRows && m.nblk > 0;
             if (m.nblk > 0) {
                 ok = ok && mbar_wait(&ds_empty[(c - 1) & 1], ((c - 1) >> 1) & 1, status);      // the item's last dQ product is done
                 tc_fence_after();
             }
-            ET* drow = reinterpret_cast<ET*>(p.dq) + ((int64_t)tok * p.Hq + (m.h * p.G + g)) * D + sb * kOwn;
+            ET* drow = reinterpret_cast<ET*>(p.dq) + ((int64_t)tok * p.Hq + (m.h * p.G + g)) * D + sb * 64;
             uint8_t* stage = sOut + sb * kOut;
             // the slab of the item before has left its place; and the four warps go on, or give up, together
             if (quarter == 0 && lane == 0) bulk_wait_read0();
             ok = bar_all(1 + sb, 128, ok);
 #pragma unroll
-            for (int c0 = 0; c0 < kOwn; c0 += 32) {
+            for (int c0 = 0; c0 < 64; c0 += 32) {
                 uint32_t a[32];
                 if (m.nblk > 0) {
-                    tmem_ld32(tbase + lane_off + cDQ + sb * kOwn + c0, a);
+                    tmem_ld32(tbase + lane_off + cDQ + sb * 64 + c0, a);
                     tmem_ld_wait();
                 } else {
 #pragma unroll
@@ -941,53 +894,40 @@ __global__ void __launch_bounds__(kDqThreads, 1) range_bwd_dq_dense(const RangeD
     if (warp == 0) tmem_dealloc(tbase, kCols);
 }
 
-template <int D, int MOD, typename ET>
-static cudaError_t launch_dq(const RangeDqParams& p, const CUtensorMap* maps, unsigned grid, cudaStream_t stream) {
-    constexpr int smem = 2 * kTileRows * D * 2 + kDqStages * 2 * kRdBK * D * 2 + 2 * kTileRows * kRdBK * 2 + 256 + kDqItems * 32;
-    auto kern = range_bwd_dq_dense<D, MOD, ET>;
-    const cudaError_t e = allow_smem((const void*)kern, smem);
-    if (e != cudaSuccess) return e;
-    if constexpr (MOD != 0) return launch_dependent(kern, dim3(grid), kDqThreads, smem, stream, 1, p, maps[0], maps[1], maps[2], maps[3], maps[4]);
-    prof_begin(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
-    kern<<<grid, kDqThreads, smem, stream>>>(p, maps[0], maps[1], maps[2], maps[3], maps[4]);
-    prof_end(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
-    return cudaGetLastError();
-}
-
-template <int D, typename ET>
-static cudaError_t launch_dq_mod(int mod, const RangeDqParams& p, const CUtensorMap* maps, unsigned grid, cudaStream_t stream) {
-    switch (mod) {
-        case 0: return launch_dq<D, kModGuard, ET>(p, maps, grid, stream);
-        case 1: return launch_dq<D, 1 | kModGuard, ET>(p, maps, grid, stream);
-        case 2: return launch_dq<D, 2 | kModGuard, ET>(p, maps, grid, stream);
-        case 3: return launch_dq<D, 3 | kModGuard, ET>(p, maps, grid, stream);
-        default: return cudaErrorInvalidValue;
-    }
-}
-
-// dQ of a range-attention backward.  q / dO strided, dq contiguous [N, Hq, D].  mod null: plain scores, head_dim 128.
+// dQ of a range-attention backward (head_dim 128).  q / dO strided, dq contiguous [N, Hq, 128].
 cudaError_t launch_range_bwd_dq(int dtype, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap, const CUtensorMap& vmap,
-                                int* status, cudaStream_t stream, const ScoreMod* mod, int which) {
-    const int D = mod ? s.D : 128;
-    CUtensorMap maps[5];        // Q, dO, K, V, dQ
-    if (make_tile_map_3d_box(&maps[0], a.q, dtype, D, s.N, s.Hq, a.q_sn, a.q_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
-    if (make_tile_map_3d_box(&maps[1], a.d_o, dtype, D, s.N, s.Hq, a.do_sn, a.do_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
-    maps[2] = kmap; maps[3] = vmap;
-    if (make_tile_map_3d_box(&maps[4], a.dq, dtype, D, s.N, s.Hq, (int64_t)s.Hq * D, D, s.TPT, s.G)) return cudaErrorInvalidValue;
+                                int* status, cudaStream_t stream) {
+    CUtensorMap qmap, domap, dqmap;
+    if (make_tile_map_3d_box(&qmap, a.q, dtype, 128, s.N, s.Hq, a.q_sn, a.q_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
+    if (make_tile_map_3d_box(&domap, a.d_o, dtype, 128, s.N, s.Hq, a.do_sn, a.do_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
+    if (make_tile_map_3d_box(&dqmap, a.dq, dtype, 128, s.N, s.Hq, (int64_t)s.Hq * 128, 128, s.TPT, s.G)) return cudaErrorInvalidValue;
     RangeDqParams p;
     p.cu_q = a.cu; p.cu_k = a.bd.cu_k ? a.bd.cu_k : a.cu; p.kv_lo = a.bd.kv_lo; p.kv_hi = a.bd.kv_hi;
     p.N = s.N; p.Nk = s.Nk; p.B = s.B; p.Hq = s.Hq; p.Hk = s.Hk; p.G = s.G; p.TPT = s.TPT;
     p.scale = a.sm_scale; p.scale_log2 = a.sm_scale * 1.4426950408889634f;
     p.lse = a.lse; p.delta = a.delta; p.dq = a.dq; p.status = status;
-    p.mod = mod ? *mod : ScoreMod{};
+    constexpr int smem = 2 * kTileRows * 128 * 2 + kDqStages * 2 * kRdBK * 128 * 2 + 2 * kTileRows * kRdBK * 2 + 256 + kDqItems * 32;
     const int64_t max_items = ((s.N + s.TPT - 1) / s.TPT + s.B) * (int64_t)s.Hk;
     int sms = 0;
     if (device_sm_count(&sms) != 0 || sms <= 0) return cudaErrorInvalidValue;
     const unsigned grid = (unsigned)(max_items < sms ? max_items : sms);
-    const bool bf16 = dtype == kBF16;
-    if (!mod) return bf16 ? launch_dq<128, 0, __nv_bfloat16>(p, maps, grid, stream) : launch_dq<128, 0, __half>(p, maps, grid, stream);
-    if (D == 128) return bf16 ? launch_dq_mod<128, __nv_bfloat16>(which, p, maps, grid, stream) : launch_dq_mod<128, __half>(which, p, maps, grid, stream);
-    return bf16 ? launch_dq_mod<64, __nv_bfloat16>(which, p, maps, grid, stream) : launch_dq_mod<64, __half>(which, p, maps, grid, stream);
+    cudaError_t e;
+    if (dtype == kBF16) {
+        auto kern = range_bwd_dq_dense<__nv_bfloat16>;
+        e = allow_smem((const void*)kern, smem);
+        if (e != cudaSuccess) return e;
+        prof_begin(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
+        kern<<<grid, kDqThreads, smem, stream>>>(p, qmap, domap, kmap, vmap, dqmap);
+        prof_end(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
+    } else {
+        auto kern = range_bwd_dq_dense<__half>;
+        e = allow_smem((const void*)kern, smem);
+        if (e != cudaSuccess) return e;
+        prof_begin(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
+        kern<<<grid, kDqThreads, smem, stream>>>(p, qmap, domap, kmap, vmap, dqmap);
+        prof_end(FSA_KERNEL_SEL_BWD_DQ_REDUCE, stream);
+    }
+    return cudaGetLastError();
 }
 
 }  // namespace fsa

@@ -40,7 +40,6 @@ cudaError_t dispatch_sel_fwd(int dtype, const SelFwdArgs& a, const SelShape& s, 
                              cudaStream_t stream);
 
 struct RangeKvPlan;      // range_bwd.cuh
-struct ScoreMod;         // score.cuh
 
 struct SelBwdArgs {
     const void *q, *d_o, *o;
@@ -80,10 +79,9 @@ cudaError_t launch_sel_bwd_wide(int dtype, const SelBwdArgs& a, const SelShape& 
                                 const CUtensorMap& vmap, const CUtensorMap& dqmap, int num_sms, cudaStream_t stream);
 
 // dQ of a range-attention backward as one query-tile-major kernel (range_dense.cu; head_dim 128): the accumulator stays
-// in TMEM across the K/V tiles a tile of tokens sees (dK and dV: range_bwd_dkdv.cu).  mod: changed scores (score.cuh), `which` of
-// kModCap and kModBias, head_dim 64 or 128
+// in TMEM across the K/V tiles a tile of tokens sees (dK and dV: range_bwd_dkdv.cu)
 cudaError_t launch_range_bwd_dq(int dtype, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap, const CUtensorMap& vmap,
-                                int* status, cudaStream_t stream, const ScoreMod* mod = nullptr, int which = 0);
+                                int* status, cudaStream_t stream);
 
 // a.delta = sum_d o dO, as part of a chain of dependent launches
 cudaError_t launch_sel_bwd_delta(int dtype, const SelBwdArgs& a, const SelShape& s, cudaStream_t stream);
