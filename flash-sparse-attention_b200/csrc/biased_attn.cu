@@ -56,11 +56,12 @@ __device__ __forceinline__ int document_start(const int32_t* __restrict__ ids, i
 }
 
 // One thread per token.  Tokens of one sequence stand at consecutive K/V rows.  Documents: a token whose row does not begin one sees from where the
-// token before it does, so a warp scans its tokens and searches only for those that no such token precedes in it.
+// token before it does, so a CTA scans its tokens.  What is searched for backwards is the beginning for a sequence's first token (with rows in
+// front of it), by its warp, and for the CTA's first token, by the whole CTA, 4096 ids a step.
 __global__ void __launch_bounds__(kLimThreads) biased_limits(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k,
-                                                             const int32_t* __restrict__ doc_ids, const int32_t* __restrict__ prefix_lens, int B, int64_t N,
-                                                             int window, BiasedLimits out) {
-    const int tid = threadIdx.x, lane = tid & 31;
+                                                             const int32_t* __restrict__ doc_ids, int B, int64_t N, int window, BiasedLimits out) {
+    __shared__ int s_start[kLimThreads / 32], s_seq[kLimThreads / 32], s_found[kLimThreads / 32], s_first[4];
+    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
     const int64_t n = (int64_t)blockIdx.x * kLimThreads + tid;
     follow();
     const int used = __ldcg(cu_q + B);
@@ -69,38 +70,162 @@ __global__ void __launch_bounds__(kLimThreads) biased_limits(const int32_t* __re
     if (n < used && n < N) {
         seq = find_seq<true>(cu_q, B, (int)n);
         k0 = __ldcg(cu_k + seq);
-        x = place_limits((int)n, k0, __ldcg(cu_k + seq + 1), __ldcg(cu_q + seq + 1), window, prefix_lens ? __ldcg(prefix_lens + seq) : 0);
+        x = place_limits((int)n, k0, __ldcg(cu_k + seq + 1), __ldcg(cu_q + seq + 1), window, 0);
     }
-    if (doc_ids) {
-        const bool in = x.hi >= 0;
-        const int id = in ? __ldcg(doc_ids + x.pos) : -1;
-        const bool begins = !in || x.pos == k0 || __ldcg(doc_ids + x.pos - 1) != id;
-        const int seq_before = __shfl_up_sync(0xffffffffu, seq, 1);
-        int start = begins ? x.pos : -1;                // of the document, where it is known
-        const bool head = lane == 0 || seq_before != seq;
-        for (unsigned todo = __ballot_sync(0xffffffffu, head && !begins); todo; todo &= todo - 1) {
-            const int src = __ffs(todo) - 1;
-            const int found = document_start(doc_ids, __shfl_sync(0xffffffffu, k0, src), __shfl_sync(0xffffffffu, x.pos, src), lane);
-            if (lane == src) start = found;
-        }
-        // the nearest lane at or below this one that knows
-        const unsigned known = __ballot_sync(0xffffffffu, start >= 0) & (0xffffffffu >> (31 - lane));
-        start = __shfl_sync(0xffffffffu, start, known ? 31 - __clz(known) : lane);
-        if (in) {
-            if (id < 0) x.hi = -1;
-            else x.lo = max(x.lo, start);
+    const bool in = x.hi >= 0;
+    const int id = in ? __ldcg(doc_ids + x.pos) : -1;
+    const bool begins = !in || x.pos == k0 || __ldcg(doc_ids + x.pos - 1) != id;
+    if (lane == 31) s_seq[warp] = seq;
+    // the CTA's first token
+    if (tid == 0) { s_first[0] = begins; s_first[1] = k0; s_first[2] = x.pos; s_first[3] = id; }
+    __syncthreads();
+    int first = s_first[2];
+    if (!s_first[0]) {
+        const int from = s_first[1], want = s_first[3];
+        first = from;
+        for (int end = s_first[2]; end > from; end -= 16 * kLimThreads) {      // rows [end - 4096, end) are looked at
+            int found = -1;
+#pragma unroll
+            for (int i = 0; i < 16; ++i) {
+                const int j = end - 1 - (i * kLimThreads + tid);
+                if (j >= from && __ldcg(doc_ids + j) != want) found = max(found, j);
+            }
+            found = __reduce_max_sync(0xffffffffu, found);
+            if (lane == 0) s_found[warp] = found;
+            __syncthreads();
+            found = __reduce_max_sync(0xffffffffu, lane < kLimThreads / 32 ? s_found[lane] : -1);
+            __syncthreads();
+            if (found >= 0) { first = found + 1; break; }
         }
     }
+    int seq_before = __shfl_up_sync(0xffffffffu, seq, 1);
+    if (lane == 0) seq_before = warp ? s_seq[warp - 1] : seq;
+    // of the document, where it is known (a token before the first row stands at a negative place and sees nothing)
+    int start = begins ? max(x.pos, 0) : tid == 0 ? first : -1;
+    for (unsigned todo = __ballot_sync(0xffffffffu, start < 0 && seq_before != seq); todo; todo &= todo - 1) {
+        const int src = __ffs(todo) - 1;
+        const int found = document_start(doc_ids, __shfl_sync(0xffffffffu, k0, src), __shfl_sync(0xffffffffu, x.pos, src), lane);
+        if (lane == src) start = found;
+    }
+    // the nearest lane at or below this one that knows, or the end of a warp before
+    const unsigned known = __ballot_sync(0xffffffffu, start >= 0) & (0xffffffffu >> (31 - lane));
+    start = __shfl_sync(0xffffffffu, start, known ? 31 - __clz(known) : lane);
+    if (lane == 31) s_start[warp] = start;
+    __syncthreads();
+    for (int w = warp - 1; start < 0; --w) start = s_start[w];              // (warp 0 knows all of its)
     if (n < N) {
-        out.lo[n] = x.hi >= 0 ? x.lo : 0;
-        out.hi[n] = x.hi;
+        const bool sees = in && id >= 0;
+        out.lo[n] = sees ? max(x.lo, start) : 0;
+        out.hi[n] = sees ? x.hi : -1;
         out.pos[n] = x.pos;
     }
 }
 
-static cudaError_t launch_limits(const int32_t* cu_q, const int32_t* cu_k, const int32_t* doc_ids, const int32_t* prefix_lens, int B, int64_t N, int window,
-                                 const BiasedLimits& out, cudaStream_t stream) {
-    return launch_dependent(biased_limits, dim3((unsigned)((N + kLimThreads - 1) / kLimThreads)), kLimThreads, 0, stream, 1, cu_q, cu_k, doc_ids, prefix_lens, B, N, window, out);
+static cudaError_t launch_limits(const int32_t* cu_q, const int32_t* cu_k, const int32_t* doc_ids, int B, int64_t N, int window, const BiasedLimits& out,
+                                 cudaStream_t stream) {
+    return launch_dependent(biased_limits, dim3((unsigned)((N + kLimThreads - 1) / kLimThreads)), kLimThreads, 0, stream, 1, cu_q, cu_k, doc_ids, B, N, window, out);
+}
+
+// ------------------------------------------------------------------------------------------------ what the backward's kernels need
+// One launch: CTA 0 plans the items of dK / dV, the others work out delta = sum_d o dO, without documents the limits, and clear what lies behind the last
+// sequences.  Without documents the stretch of tokens that sees a tile of K/V rows follows from the rule: from the token at the tile's first
+// row (with a prefix that the tile is part of: the sequence's first) to the one at its last row (with a window: that far behind).
+struct BiasedPrep {
+    RangeKvPlan plan;
+    BiasedLimits lim;
+    const int32_t* prefix_lens;
+    int window, docs;               // docs: plan.tiles and the limits are there
+    const void *o, *d_o;            // [N, Hq, D], o contiguous
+    int64_t do_sn, do_sh;
+    int Hq;
+    float* delta;                   // [Hq, N]
+    uint4 *dq, *dk, *dv;
+};
+constexpr int kPrThreads = 512;
+
+template <int D, typename ET>
+__global__ void __launch_bounds__(kPrThreads) biased_prep(const BiasedPrep p) {
+    constexpr int L = D / 8, R = kPrThreads / L, U = 4;         // lanes a row, rows of a turn, turns in flight
+    const int tid = threadIdx.x, lane = tid & 31;
+    const int64_t N = p.plan.N;
+    const int B = p.plan.B;
+    follow();
+    if (blockIdx.x == 0) {
+        if (!p.docs) {
+            for (int i = tid >> 5; i < p.plan.max_tiles; i += kPrThreads / 32) {
+                int seq, key0, nkeys;
+                find_seq_tile<true>(p.plan.cu_k, B, kTileRows, i, lane, seq, key0, nkeys);
+                if (lane == 0) {
+                    int4 t = make_int4(0, 0, 0, -1);
+                    if (seq >= 0) {
+                        const int t0 = __ldcg(p.plan.cu_q + seq), t1 = __ldcg(p.plan.cu_q + seq + 1), k0 = __ldcg(p.plan.cu_k + seq), k1 = __ldcg(p.plan.cu_k + seq + 1);
+                        const int to_tok = t1 - k1;         // from a row to the token that stands there
+                        const bool shared = p.prefix_lens && key0 < k0 + __ldcg(p.prefix_lens + seq);
+                        // (with fewer rows than tokens the first tokens stand before row k0 and see nothing)
+                        const int first = max(max(t0, k0 + to_tok), shared ? t0 : key0 + to_tok);
+                        const int last = p.window >= 0 ? (int)min((int64_t)t1 - 1, (int64_t)key0 + nkeys - 1 + to_tok + p.window) : t1 - 1;
+                        t = make_int4(key0, nkeys, last >= first ? first : 0, last >= first ? last : -1);
+                    }
+                    p.plan.tiles[i] = t;
+                }
+            }
+            __syncthreads();
+        }
+        plan_items<kPrThreads>(p.plan);
+        return;
+    }
+    const int64_t ctas = gridDim.x - 1, me = (int64_t)(blockIdx.x - 1) * kPrThreads + tid, all = ctas * kPrThreads;
+    if (!p.docs)
+        for (int64_t n = me; n < N; n += all) {
+            Sees x = {0, -1, 0};
+            if (n < __ldcg(p.plan.cu_q + B)) {
+                const int seq = find_seq<true>(p.plan.cu_q, B, (int)n);
+                x = place_limits((int)n, __ldcg(p.plan.cu_k + seq), __ldcg(p.plan.cu_k + seq + 1), __ldcg(p.plan.cu_q + seq + 1), p.window,
+                                 p.prefix_lens ? __ldcg(p.prefix_lens + seq) : 0);
+            }
+            p.lim.lo[n] = x.hi >= 0 ? x.lo : 0;
+            p.lim.hi[n] = x.hi;
+            p.lim.pos[n] = x.pos;
+        }
+    const int64_t row16 = (int64_t)p.plan.Hk * L, qrow16 = (int64_t)p.Hq * L;
+    for (int64_t i = (int64_t)__ldcg(p.plan.cu_k + B) * row16 + me; i < p.plan.Nk * row16; i += all) p.dk[i] = p.dv[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int64_t i = (int64_t)__ldcg(p.plan.cu_q + B) * qrow16 + me; i < N * qrow16; i += all) p.dq[i] = make_uint4(0u, 0u, 0u, 0u);
+    // delta: L lanes a row of one head, U rows of a thread in flight
+    const int part = tid % L;
+    const uint32_t rows = (uint32_t)(N * p.Hq);
+    for (int64_t r0 = (int64_t)(blockIdx.x - 1) * (R * U) + tid / L; r0 - tid / L < rows; r0 += ctas * (R * U)) {
+        uint4 a[U], b[U];
+        uint32_t n[U], h[U];
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t r = min((uint32_t)r0 + u * R, rows - 1);
+            n[u] = r / (uint32_t)p.Hq;
+            h[u] = r - n[u] * (uint32_t)p.Hq;
+            a[u] = __ldcs(reinterpret_cast<const uint4*>(reinterpret_cast<const ET*>(p.o) + ((int64_t)n[u] * p.Hq + h[u]) * D) + part);
+            b[u] = __ldcg(reinterpret_cast<const uint4*>(reinterpret_cast<const ET*>(p.d_o) + (int64_t)n[u] * p.do_sn + (int64_t)h[u] * p.do_sh) + part);
+        }
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            const uint32_t *x = &a[u].x, *y = &b[u].x;
+            float acc = 0.f;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float2 v = ElemTraits<ET>::unpack2(x[i]), w = ElemTraits<ET>::unpack2(y[i]);
+                acc = fmaf(v.x, w.x, acc);
+                acc = fmaf(v.y, w.y, acc);
+            }
+#pragma unroll
+            for (int d = L / 2; d; d >>= 1) acc += __shfl_xor_sync(0xffffffffu, acc, d);
+            if (part == 0 && r0 + u * R < rows) p.delta[(int64_t)h[u] * N + n[u]] = acc;
+        }
+    }
+}
+
+template <int D, typename ET>
+static cudaError_t launch_prep(const BiasedPrep& p, cudaStream_t stream) {
+    constexpr int per = kPrThreads / (D / 8) * 4;
+    const int64_t want = (p.plan.N * p.Hq + per - 1) / per, most = 4 * (int64_t)sm_count();
+    return launch_dependent(biased_prep<D, ET>, dim3((unsigned)(1 + (want < most ? want : most))), kPrThreads, 0, stream, 1, p);
 }
 
 static int biased_shape(int64_t N, int64_t Nk, int B, int Hq, int Hk, int D, SelShape* s) {
@@ -169,7 +294,7 @@ extern "C" int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, 
     p.cu_q = cu_seqlens_q; p.cu_k = cu_seqlens_k;
     l.window = window; l.prefix_lens = prefix_lens;
     if (doc_ids) {          // (else the kernel works them out for itself)
-        if ((e = launch_limits(cu_seqlens_q, cu_seqlens_k, doc_ids, nullptr, B, N, window, lim, stream)) != cudaSuccess) return cuda_failed(e);
+        if ((e = launch_limits(cu_seqlens_q, cu_seqlens_k, doc_ids, B, N, window, lim, stream)) != cudaSuccess) return cuda_failed(e);
         p.kv_lo = lim.lo; p.kv_hi = lim.hi;
         l.mod.pos = lim.pos;
     }
@@ -230,22 +355,25 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     plan.cu_q = cu_seqlens_q; plan.cu_k = cu_seqlens_k; plan.kv_lo = lim.lo; plan.kv_hi = lim.hi;
     plan.N = N; plan.Nk = Nk; plan.B = B; plan.Hk = Hk; plan.TPT = s.TPT; plan.aim = range_kv_items();
     plan.max_tiles = (int)range_kv_max_tiles(s);
-    plan.D = D; plan.Hq = Hq; plan.dq = (uint4*)dq;
+    plan.D = D;
     plan.counts = (int*)sp;
     plan.tiles = (int4*)(sp + 256);
     plan.multi = plan.tiles + plan.max_tiles;
     plan.items = plan.multi + plan.max_tiles;
     sp += align_up(range_kv_plan_bytes(s), 1024);
     a.slabs = (float*)sp;
-    // with documents the forward has left the limits
-    cudaError_t e = doc_ids ? cudaSuccess : launch_limits(cu_seqlens_q, cu_seqlens_k, nullptr, prefix_lens, B, N, window, lim, stream);
     int* status = nullptr;
-    if (e == cudaSuccess) e = biased_status_word(&status);
-    if (e == cudaSuccess) e = launch_range_bwd_plan(plan, a, nullptr, stream, true);
-    if (e == cudaSuccess) e = launch_sel_bwd_delta(dtype, a, s, stream);
+    cudaError_t e = biased_status_word(&status);
+    BiasedPrep prep = {plan, lim, prefix_lens, window, doc_ids != nullptr, o, d_o, do_sn, do_sh, Hq, a.delta, (uint4*)dq, (uint4*)dk, (uint4*)dv};
+    // with documents the forward has left the limits, and the stretches are looked for
+    if (e == cudaSuccess && doc_ids) e = launch_range_key_tiles(plan, a, stream);
+    const bool bf16 = dtype == FSA_DTYPE_BF16;
+    if (e == cudaSuccess && D == 128) e = bf16 ? launch_prep<128, __nv_bfloat16>(prep, stream) : launch_prep<128, __half>(prep, stream);
+    if (e == cudaSuccess && D == 64) e = bf16 ? launch_prep<64, __nv_bfloat16>(prep, stream) : launch_prep<64, __half>(prep, stream);
     if (e == cudaSuccess) e = launch_biased_bwd_dq(dtype, a, s, kmap, vmap, status, mod, which, stream);
     if (e == cudaSuccess) e = launch_biased_bwd_dkdv(dtype, plan, a, s, kmap, vmap, status, mod, which, stream);
-    if (e == cudaSuccess) e = launch_range_dkdv_reduce(dtype, plan, a.slabs, dk, dv, sm_count(), stream);
+    // (no stretch of so few row tiles is cut)
+    if (e == cudaSuccess && N > (int64_t)kRkMinTiles * s.TPT) e = launch_range_dkdv_reduce(dtype, plan, a.slabs, dk, dv, sm_count(), stream);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
 }
 

@@ -492,7 +492,7 @@ static int sel_bwd_impl(const SelBounds& bd, int64_t Nk, const float* delta, con
         plan.cu_q = cu_seqlens; plan.cu_k = bd.cu_k ? bd.cu_k : cu_seqlens; plan.kv_lo = bd.kv_lo; plan.kv_hi = bd.kv_hi;
         plan.N = N; plan.Nk = Nk; plan.B = B; plan.Hk = Hk; plan.TPT = s.TPT; plan.aim = range_kv_items();
         plan.max_tiles = (int)range_kv_max_tiles(s);
-        plan.D = D; plan.Hq = Hq; plan.dq = nullptr;
+        plan.D = D;
         plan.counts = (int*)sp;
         plan.tiles = (int4*)(sp + 256);
         plan.multi = plan.tiles + plan.max_tiles;

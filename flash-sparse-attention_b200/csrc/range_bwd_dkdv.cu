@@ -53,9 +53,6 @@ __global__ void __launch_bounds__(512) range_key_tiles(const RangeKvPlan p, uint
             dk[i] = make_uint4(0u, 0u, 0u, 0u);
             dv[i] = make_uint4(0u, 0u, 0u, 0u);
         }
-        const int64_t qrow16 = (int64_t)p.Hq * p.D / 8;
-        if (p.dq)
-            for (int64_t i = (int64_t)__ldg(p.cu_q + p.B) * qrow16 + tid; i < p.N * qrow16; i += blockDim.x) p.dq[i] = make_uint4(0u, 0u, 0u, 0u);
         return;
     }
     int seq, key0, nkeys;
@@ -89,53 +86,9 @@ __global__ void __launch_bounds__(512) range_key_tiles(const RangeKvPlan p, uint
     }
 }
 
-// Work items from the stretches (one CTA): a tile of n row tiles becomes ceil(n / C) items of about equal length, C the
-// smallest length that leaves about p.aim items (times heads), and at least kRkMinTiles: below that an item's epilogue weighs
-// more than an idle SM.
 __global__ void __launch_bounds__(1024) range_plan_items(const RangeKvPlan p) {
-    __shared__ int wa[32], wb[32], wc[32];
-    __shared__ long long total;
-    const int tid = threadIdx.x, lane = tid & 31, warp = tid >> 5;
-    auto row_tiles = [&](const int4& t) { return t.w >= 0 ? (t.w - t.z + p.TPT) / p.TPT : 0; };
-    if (tid == 0) total = 0;
     follow();
-    __syncthreads();
-    int mine = 0;
-    for (int i = tid; i < p.max_tiles; i += 1024) mine += row_tiles(p.tiles[i]);
-    mine = __reduce_add_sync(0xffffffffu, mine);
-    if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&total), (unsigned long long)mine);
-    __syncthreads();
-    const int C = max(kRkMinTiles, (int)((total * p.Hk + p.aim - 1) / p.aim));
-    int items = 0, slabs = 0, multi = 0;              // so far
-    for (int base = 0; base < p.max_tiles; base += 1024) {
-        const int i = base + tid;
-        const int4 t = i < p.max_tiles ? p.tiles[i] : make_int4(0, 0, 0, -1);
-        const int n = row_tiles(t);
-        const int nch = t.y > 0 ? max(1, (n + C - 1) / C) : 0;
-        const int a = nch, b = nch > 1 ? nch : 0, c = nch > 1;
-        int sa = a, sb = b, sc = c;
-#pragma unroll
-        for (int o = 1; o < 32; o <<= 1) {
-            const int ta = __shfl_up_sync(0xffffffffu, sa, o), tb = __shfl_up_sync(0xffffffffu, sb, o), tc = __shfl_up_sync(0xffffffffu, sc, o);
-            if (lane >= o) { sa += ta; sb += tb; sc += tc; }
-        }
-        if (lane == 31) { wa[warp] = sa; wb[warp] = sb; wc[warp] = sc; }
-        __syncthreads();
-        const int va = wa[lane], vb = wb[lane], vc = wc[lane];
-        const int first = items + __reduce_add_sync(0xffffffffu, lane < warp ? va : 0) + sa - a;
-        const int slab = slabs + __reduce_add_sync(0xffffffffu, lane < warp ? vb : 0) + sb - b;
-        const int list = multi + __reduce_add_sync(0xffffffffu, lane < warp ? vc : 0) + sc - c;
-        for (int j = 0; j < nch; ++j) {
-            const int r0 = (int)((int64_t)n * j / nch), r1 = (int)((int64_t)n * (j + 1) / nch);
-            p.items[first + j] = make_int4(i, r0, r1 - r0, nch > 1 ? slab + j : -1);
-        }
-        if (nch > 1) p.multi[list] = make_int4(t.x, t.y, slab, nch);
-        items += __reduce_add_sync(0xffffffffu, va);
-        slabs += __reduce_add_sync(0xffffffffu, vb);
-        multi += __reduce_add_sync(0xffffffffu, vc);
-        __syncthreads();
-    }
-    if (tid == 0) { p.counts[0] = items; p.counts[1] = multi; }
+    plan_items<1024>(p);
 }
 
 // dk / dv rows of the K/V tiles that were cut: the sum of the slabs in order.  Slab: [dV, dK][column / 4][row] float4.
@@ -546,11 +499,11 @@ __global__ void __launch_bounds__(kRkThreads, 1) range_bwd_dkdv(const RangeKvPar
     if (warp == 0) tmem_dealloc(tbase, 512);
 }
 
-cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream, bool dependent) {
-    if (dependent) {
-        const cudaError_t e = launch_dependent(range_key_tiles, dim3((unsigned)p.max_tiles + 1), 512, 0, stream, 1, p, (uint4*)a.dk, (uint4*)a.dv, status);
-        return e == cudaSuccess ? launch_dependent(range_plan_items, dim3(1), 1024, 0, stream, 1, p) : e;
-    }
+cudaError_t launch_range_key_tiles(const RangeKvPlan& p, const SelBwdArgs& a, cudaStream_t stream) {
+    return launch_dependent(range_key_tiles, dim3((unsigned)p.max_tiles + 1), 512, 0, stream, 1, p, (uint4*)a.dk, (uint4*)a.dv, (int*)nullptr);
+}
+
+cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream) {
     range_key_tiles<<<(unsigned)p.max_tiles + 1, 512, 0, stream>>>(p, (uint4*)a.dk, (uint4*)a.dv, status);
     range_plan_items<<<1, 1024, 0, stream>>>(p);
     return cudaGetLastError();

@@ -345,7 +345,6 @@ template <typename ET>
 __global__ void __launch_bounds__(256) sel_bwd_delta(const ET* __restrict__ o, int64_t o_sn, int64_t o_sh,
                                                      const ET* __restrict__ d_o, int64_t do_sn, int64_t do_sh,
                                                      int64_t N, int Hq, int D, float* __restrict__ delta) {
-    follow();
     const int tpr = D >> 3;                                  // threads per row: 8, 16 or 32 (a power of two)
     const int rpc = 256 / tpr;                               // rows per pass of the CTA
     const int part = threadIdx.x & (tpr - 1), rloc = threadIdx.x / tpr;
@@ -555,22 +554,6 @@ __global__ void __launch_bounds__(256) sel_bwd_convert(const float* __restrict__
 
 constexpr int64_t kReduceFew = 24000;      // output rows up to which both reductions go in one launch (more: resident merges take dq)
 
-template <typename ET>
-static cudaError_t launch_delta(const SelBwdArgs& a, const SelShape& s, cudaStream_t stream, bool dependent = false) {
-    const int64_t rows = s.N * s.Hq, rows_per_cta = 2 * (256 / (s.D / 8));
-    const cudaError_t e = prefer_l1((const void*)sel_bwd_delta<ET>);
-    if (e != cudaSuccess) return e;
-    const unsigned grid = (unsigned)((rows + rows_per_cta - 1) / rows_per_cta);
-    if (dependent)
-        return launch_dependent(sel_bwd_delta<ET>, dim3(grid), 256, 0, stream, 1, (const ET*)a.o, a.o_sn, a.o_sh, (const ET*)a.d_o, a.do_sn, a.do_sh, s.N, s.Hq, s.D, a.delta);
-    sel_bwd_delta<ET><<<grid, 256, 0, stream>>>((const ET*)a.o, a.o_sn, a.o_sh, (const ET*)a.d_o, a.do_sn, a.do_sh, s.N, s.Hq, s.D, a.delta);
-    return cudaGetLastError();
-}
-
-cudaError_t launch_sel_bwd_delta(int dtype, const SelBwdArgs& a, const SelShape& s, cudaStream_t stream) {
-    return dtype == kBF16 ? launch_delta<__nv_bfloat16>(a, s, stream, true) : launch_delta<__half>(a, s, stream, true);
-}
-
 template <int D, typename ET>
 static cudaError_t launch_sel_bwd(const SelBwdArgs& a, const SelShape& s, const SelIndex& ix, const CUtensorMap& kmap,
                                   const CUtensorMap& vmap, int num_sms, cudaStream_t stream) {
@@ -590,7 +573,14 @@ static cudaError_t launch_sel_bwd(const SelBwdArgs& a, const SelShape& s, const 
         e = cudaMemsetAsync(a.dk_acc, 0, kv_elems * 4 * 2, stream);   // dk_acc and dv_acc are adjacent
         if (e != cudaSuccess) return e;
     }
-    if (rows > 0 && !a.have_delta && (e = launch_delta<ET>(a, s, stream)) != cudaSuccess) return e;
+    if (rows > 0 && !a.have_delta) {
+        const int64_t rows_per_cta = 2 * (256 / (D / 8));
+        unsigned grid = (unsigned)((rows + rows_per_cta - 1) / rows_per_cta);
+        e = prefer_l1((const void*)sel_bwd_delta<ET>);
+        if (e != cudaSuccess) return e;
+        sel_bwd_delta<ET><<<grid, 256, 0, stream>>>((const ET*)a.o, a.o_sn, a.o_sh, (const ET*)a.d_o, a.do_sn, a.do_sh,
+                                                    s.N, s.Hq, D, a.delta);
+    }
     if (a.plan) {
         e = launch_range_bwd_dq(dt, a, s, kmap, vmap, ix.header, stream);
         return e == cudaSuccess ? launch_range_bwd_dkdv(dt, *a.plan, a, s, kmap, vmap, ix.header, stream) : e;

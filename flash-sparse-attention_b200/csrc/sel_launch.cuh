@@ -83,9 +83,6 @@ cudaError_t launch_sel_bwd_wide(int dtype, const SelBwdArgs& a, const SelShape& 
 cudaError_t launch_range_bwd_dq(int dtype, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                 int* status, cudaStream_t stream);
 
-// a.delta = sum_d o dO, as part of a chain of dependent launches
-cudaError_t launch_sel_bwd_delta(int dtype, const SelBwdArgs& a, const SelShape& s, cudaStream_t stream);
-
 cudaError_t dispatch_sel_bwd(int dtype, const SelBwdArgs& a, const SelShape& s, const SelIndex& ix,
                              const CUtensorMap& kmap, const CUtensorMap& vmap, int num_sms, cudaStream_t stream);
 
