@@ -28,7 +28,7 @@ __device__ __forceinline__ Sees place_limits(int tok, int k0, int k1, int q1, in
     x.pos = tok + k1 - q1;
     const bool in = x.pos >= k0;            // (else the sequence has fewer keys than queries, and this one precedes them)
     x.lo = in && window >= 0 ? max(k0, x.pos - window) : k0;
-    x.hi = in ? max(x.pos, min(k0 + prefix, k1) - 1) : -1;
+    x.hi = in ? max(x.pos, k0 + min(prefix, k1 - k0) - 1) : -1;
     return x;
 }
 

@@ -134,7 +134,7 @@ struct BiasedPrep {
     RangeKvPlan plan;
     BiasedLimits lim;
     const int32_t* prefix_lens;
-    int window, docs;               // docs: plan.tiles and the limits are there
+    int window, docs;               // docs: plan.tiles and the limits are there, dk's and dv's last rows cleared
     const void *o, *d_o;            // [N, Hq, D], o contiguous
     int64_t do_sn, do_sh;
     int Hq;
@@ -152,30 +152,48 @@ __global__ void __launch_bounds__(kPrThreads) biased_prep(const BiasedPrep p) {
     follow();
     if (blockIdx.x == 0) {
         if (!p.docs) {
-            for (int i = tid >> 5; i < p.plan.max_tiles; i += kPrThreads / 32) {
-                int seq, key0, nkeys;
-                find_seq_tile<true>(p.plan.cu_k, B, kTileRows, i, lane, seq, key0, nkeys);
-                if (lane == 0) {
-                    int4 t = make_int4(0, 0, 0, -1);
-                    if (seq >= 0) {
-                        const int t0 = __ldcg(p.plan.cu_q + seq), t1 = __ldcg(p.plan.cu_q + seq + 1), k0 = __ldcg(p.plan.cu_k + seq), k1 = __ldcg(p.plan.cu_k + seq + 1);
-                        const int to_tok = t1 - k1;         // from a row to the token that stands there
-                        const bool shared = p.prefix_lens && key0 < k0 + __ldcg(p.prefix_lens + seq);
-                        // (with fewer rows than tokens the first tokens stand before row k0 and see nothing)
-                        const int first = max(max(t0, k0 + to_tok), shared ? t0 : key0 + to_tok);
-                        const int last = p.window >= 0 ? (int)min((int64_t)t1 - 1, (int64_t)key0 + nkeys - 1 + to_tok + p.window) : t1 - 1;
-                        t = make_int4(key0, nkeys, last >= first ? first : 0, last >= first ? last : -1);
-                    }
-                    p.plan.tiles[i] = t;
+            // as many sequences as threads at a time: their tiles are counted, and a tile finds its sequence among the counts
+            __shared__ int s_first[kPrThreads + 1], s_sum[kPrThreads / 32];
+            int done = 0;
+            for (int b0 = 0; b0 < B; b0 += kPrThreads) {
+                const int rows = b0 + tid < B ? __ldcg(p.plan.cu_k + b0 + tid + 1) - __ldcg(p.plan.cu_k + b0 + tid) : 0;
+                int incl = (rows + kTileRows - 1) / kTileRows;
+#pragma unroll
+                for (int d = 1; d < 32; d <<= 1) {
+                    const int up = __shfl_up_sync(0xffffffffu, incl, d);
+                    if (lane >= d) incl += up;
                 }
+                if (lane == 31) s_sum[tid >> 5] = incl;
+                __syncthreads();
+                s_first[tid + 1] = incl + __reduce_add_sync(0xffffffffu, lane < tid >> 5 ? s_sum[lane] : 0);
+                if (tid == 0) s_first[0] = 0;
+                __syncthreads();
+                const int total = min(s_first[kPrThreads], p.plan.max_tiles - done);
+                for (int i = tid; i < total; i += kPrThreads) {
+                    int s = 0;                              // the last one that begins at or before tile i
+#pragma unroll
+                    for (int step = kPrThreads / 2; step; step >>= 1) s += s_first[s + step] <= i ? step : 0;
+                    const int seq = b0 + s, t0 = __ldcg(p.plan.cu_q + seq), t1 = __ldcg(p.plan.cu_q + seq + 1), k0 = __ldcg(p.plan.cu_k + seq), k1 = __ldcg(p.plan.cu_k + seq + 1);
+                    const int key0 = k0 + (i - s_first[s]) * kTileRows, nkeys = min(kTileRows, k1 - key0);
+                    const int to_tok = t1 - k1;             // from a row to the token that stands there
+                    const bool shared = p.prefix_lens && key0 - k0 < __ldcg(p.prefix_lens + seq);
+                    // (with fewer rows than tokens the first tokens stand before row k0 and see nothing)
+                    const int first = max(max(t0, k0 + to_tok), shared ? t0 : key0 + to_tok);
+                    const int last = p.window >= 0 ? (int)min((int64_t)t1 - 1, (int64_t)key0 + nkeys - 1 + to_tok + p.window) : t1 - 1;
+                    p.plan.tiles[done + i] = make_int4(key0, nkeys, last >= first ? first : 0, last >= first ? last : -1);
+                }
+                done += total;
+                __syncthreads();
             }
+            for (int i = done + tid; i < p.plan.max_tiles; i += kPrThreads) p.plan.tiles[i] = make_int4(0, 0, 0, -1);
             __syncthreads();
         }
         plan_items<kPrThreads>(p.plan);
         return;
     }
     const int64_t ctas = gridDim.x - 1, me = (int64_t)(blockIdx.x - 1) * kPrThreads + tid, all = ctas * kPrThreads;
-    if (!p.docs)
+    const int64_t row16 = (int64_t)p.plan.Hk * L, qrow16 = (int64_t)p.Hq * L;
+    if (!p.docs) {
         for (int64_t n = me; n < N; n += all) {
             Sees x = {0, -1, 0};
             if (n < __ldcg(p.plan.cu_q + B)) {
@@ -187,8 +205,8 @@ __global__ void __launch_bounds__(kPrThreads) biased_prep(const BiasedPrep p) {
             p.lim.hi[n] = x.hi;
             p.lim.pos[n] = x.pos;
         }
-    const int64_t row16 = (int64_t)p.plan.Hk * L, qrow16 = (int64_t)p.Hq * L;
-    for (int64_t i = (int64_t)__ldcg(p.plan.cu_k + B) * row16 + me; i < p.plan.Nk * row16; i += all) p.dk[i] = p.dv[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int64_t i = (int64_t)__ldcg(p.plan.cu_k + B) * row16 + me; i < p.plan.Nk * row16; i += all) p.dk[i] = p.dv[i] = make_uint4(0u, 0u, 0u, 0u);
+    }
     for (int64_t i = (int64_t)__ldcg(p.plan.cu_q + B) * qrow16 + me; i < N * qrow16; i += all) p.dq[i] = make_uint4(0u, 0u, 0u, 0u);
     // delta: L lanes a row of one head, U rows of a thread in flight
     const int part = tid % L;
@@ -244,11 +262,7 @@ static int biased_mod(float sm_scale, float softcap, const float* slopes, const 
     if (!(sm_scale > 0.f) || !(softcap >= 0.f)) return FSA_ERR_BAD_ARG;
     *which = (softcap > 0.f ? kModCap : 0) | (slopes ? kModBias : 0);
     *m = ScoreMod{};
-    if (softcap > 0.f) {
-        m->x_scale = sm_scale / softcap;
-        m->cap_log2 = softcap * kLog2e;
-        near_coefficients(m);
-    }
+    if (softcap > 0.f && !set_cap(m, sm_scale, softcap)) return FSA_ERR_BAD_ARG;
     m->slopes = slopes; m->key_ids = doc_ids; m->ahead = ahead;
     return FSA_OK;
 }
@@ -353,7 +367,9 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     a.dq = dq; a.dk = dk; a.dv = dv;
     RangeKvPlan plan = {};
     plan.cu_q = cu_seqlens_q; plan.cu_k = cu_seqlens_k; plan.kv_lo = lim.lo; plan.kv_hi = lim.hi;
-    plan.N = N; plan.Nk = Nk; plan.B = B; plan.Hk = Hk; plan.TPT = s.TPT; plan.aim = range_kv_items();
+    plan.N = N; plan.Nk = Nk; plan.B = B; plan.Hk = Hk; plan.TPT = s.TPT;
+    // (2 x 4096 tokens of documents: 636 us a pass with 5 items an SM, 653 with 8, whose slabs take longer to join; 2 x 8192 capped: 1339 and 1366)
+    plan.aim = 5 * sm_count();
     plan.max_tiles = (int)range_kv_max_tiles(s);
     plan.D = D;
     plan.counts = (int*)sp;

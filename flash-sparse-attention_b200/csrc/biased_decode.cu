@@ -271,12 +271,12 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
 }
 
 // o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, lse = M + log2 of the latter, over the P partials of every row; 0 and -inf for a row that saw
-// nothing.  A sequence behind the last group (*grouped is their number) has no shared partials.  WARPS warps a row: what it takes is round trips to L2, so
+// nothing.  A sequence in front of the first or behind the last group has no shared partials.  WARPS warps a row: what it takes is round trips to L2, so
 // all maxima and sums, and the first 16 partials of every warp, are asked for at once (1 x 8191 tokens, 32 heads, 64 partials a row: 12 us with
 // a round trip for every four partials of a warp).
 constexpr int kMgThreads = 128, kMgAhead = 16;
 template <int D, int WARPS, typename ET>
-__global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const float* o_part, const float2* ml, int64_t rows, int Hq, int P, int nshared, const int32_t* grouped,
+__global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const float* o_part, const float2* ml, int64_t rows, int Hq, int P, int nshared, const int32_t* cu_group, int groups,
                                                                   ET* __restrict__ o, float* __restrict__ lse) {
     constexpr int V = D / 32;           // columns of a lane
     __shared__ float s_m[4], s_l[4];
@@ -286,7 +286,7 @@ __global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const float* o
     const int64_t row = (int64_t)blockIdx.x * (4 / WARPS) + warp / WARPS;
     follow();
     if (row >= rows) return;            // (with WARPS = 4 there is no such CTA)
-    const int first = nshared > 0 && row / Hq >= *grouped ? nshared : 0;
+    const int b = (int)(row / Hq), first = nshared > 0 && (b < __ldcg(cu_group) || b >= __ldcg(cu_group + groups)) ? nshared : 0;
     const float2* mlr = ml + row * P;
     const float* src = o_part + row * P * D + lane * V;
     auto load = [&](int i, float (&x)[4]) {
@@ -376,12 +376,12 @@ static cudaError_t launch_bd_which(int which, const BiasedDecodeParams& p, const
 }
 
 template <int D, typename ET>
-static cudaError_t launch_merge(const float* o_part, const float2* ml, int64_t rows, int Hq, int P, int nshared, const int32_t* grouped, void* o, float* lse,
+static cudaError_t launch_merge(const float* o_part, const float2* ml, int64_t rows, int Hq, int P, int nshared, const int32_t* cu_group, int groups, void* o, float* lse,
                                 cudaStream_t stream) {
     // a CTA per row while all of them still run at once
     if (rows <= 4 * sm_count())
-        return launch_dependent(biased_decode_merge<D, 4, ET>, dim3((unsigned)rows), kMgThreads, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, grouped, (ET*)o, lse);
-    return launch_dependent(biased_decode_merge<D, 1, ET>, dim3((unsigned)((rows + 3) / 4)), kMgThreads, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, grouped, (ET*)o,
+        return launch_dependent(biased_decode_merge<D, 4, ET>, dim3((unsigned)rows), kMgThreads, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, cu_group, groups, (ET*)o, lse);
+    return launch_dependent(biased_decode_merge<D, 1, ET>, dim3((unsigned)((rows + 3) / 4)), kMgThreads, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, cu_group, groups, (ET*)o,
                             lse);
 }
 
@@ -429,7 +429,7 @@ extern "C" int fsa_biased_decode_bytes(int batch, int num_q_heads, int num_kv_he
     if (!bytes_out || batch < 0 || num_kv_heads <= 0 || num_q_heads <= 0 || num_q_heads % num_kv_heads || num_groups < 0 || max_len < 0 || max_shared < 0)
         return FSA_ERR_BAD_ARG;
     const int G = num_q_heads / num_kv_heads;
-    if ((head_dim != 64 && head_dim != 128) || G > 32) return FSA_ERR_UNSUPPORTED;
+    if ((head_dim != 64 && head_dim != 128) || G > 32 || max_len >= ((int64_t)1 << 30) || max_shared >= kMaxTokens) return FSA_ERR_UNSUPPORTED;
     const DecodeCut cut(batch, num_kv_heads, G, (kTileRows / G) & ~3, num_groups, max_len, max_shared, window);
     const int64_t rows = (int64_t)batch * num_q_heads * cut.partials();
     *bytes_out = align_up(rows * head_dim * 4, 256) + align_up(rows * 8, 256);
@@ -469,11 +469,7 @@ extern "C" int fsa_biased_decode(const void* q, const void* k, const void* v, in
     float2* ml = (float2*)((char*)scratch + align_up(rows * P * D * 4, 256));
     ScoreMod mod = {};
     const int which = (softcap > 0.f ? kModCap : 0) | (slopes ? kModBias : 0);
-    if (softcap > 0.f) {
-        mod.x_scale = sm_scale / softcap;
-        mod.cap_log2 = softcap * kLog2e;
-        near_coefficients(&mod);
-    }
+    if (softcap > 0.f && !set_cap(&mod, sm_scale, softcap)) return FSA_ERR_BAD_ARG;
     mod.slopes = slopes;
     cudaError_t e;
     BiasedDecodeParams p = {};
@@ -505,8 +501,7 @@ extern "C" int fsa_biased_decode(const void* q, const void* k, const void* v, in
         e = launch_biased_fwd(D, dtype, which, true, l, cut.mtiles, stream);
         if (e != cudaSuccess) return cuda_failed(e);
     }
-    const int32_t* grouped = has_shared ? cu_group + num_groups : nullptr;
-    auto merge = [&](auto run) { return run(o_part, ml, rows, Hq, P, cut.nshared, grouped, o, lse, stream); };
+    auto merge = [&](auto run) { return run(o_part, ml, rows, Hq, P, cut.nshared, cu_group, num_groups, o, lse, stream); };
     if (D == 128) e = bf16 ? merge(launch_merge<128, __nv_bfloat16>) : merge(launch_merge<128, __half>);
     else e = bf16 ? merge(launch_merge<64, __nv_bfloat16>) : merge(launch_merge<64, __half>);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);

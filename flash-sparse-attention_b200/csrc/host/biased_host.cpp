@@ -61,6 +61,8 @@ static Tensor check_slopes(const MaybeTensor& s, const Tensor& q) {
 static void check_scores(const Tensor& q, double scale, double cap) {
     TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "sm_scale has to be above 0 and finite, got ", scale);
     TORCH_CHECK_VALUE(cap >= 0 && std::isfinite(cap), "softcap has to be above 0 and finite (or None), got ", cap);
+    TORCH_CHECK_VALUE(cap == 0 || (cap > 1e-30 && cap < 1e30 && scale / cap > 1e-30 && scale / cap < 1e30),
+                      "softcap and sm_scale / softcap have to be between 1e-30 and 1e30, got ", cap, " and ", scale / cap);
     TORCH_CHECK_VALUE(q.is_cuda(), "the sm_100a kernels need CUDA tensors (no CPU fallback)");
 }
 

@@ -2,6 +2,8 @@
 //   s = scale q.k;   s = cap tanh(s / cap);   s = s - slope_h |t - j|        (t, j: places of the token and the key)
 // and what the kernels of range attention need besides.  A kernel's MOD says what it is compiled with; 0 is the plain product.
 #pragma once
+#include <cfloat>
+
 #include "sm100_prims.cuh"
 
 namespace fsa {
@@ -104,6 +106,13 @@ inline void near_coefficients(ScoreMod* m) {
     m->near_v = (float)(0.5 / x);
     double pow = x;
     for (int i = 0; i < 4; ++i, pow *= x * x) m->near[i] = (float)(c[i] * pow);
+}
+// The cap's numbers; false where they leave the normal ones.
+inline bool set_cap(ScoreMod* m, float sm_scale, float softcap) {
+    m->x_scale = sm_scale / softcap;
+    m->cap_log2 = softcap * kLog2e;
+    near_coefficients(m);
+    return m->x_scale >= FLT_MIN && m->x_scale <= FLT_MAX / 4 && m->cap_log2 >= FLT_MIN && m->cap_log2 <= FLT_MAX;
 }
 
 // v <- scale v - slope |rel - i|, N scores of a row against keys i = 0, 1, ... of a tile; rel: the token's place among them.  both (the

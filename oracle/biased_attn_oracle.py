@@ -20,9 +20,9 @@ def visible(Lq, Lk, window=None, ids=None, prefix=None):
         seen = seen | ((j < prefix) & (t >= 0))
     if window is not None:
         seen = seen & (j >= t - window)
-    if ids is not None:
+    if ids is not None and Lk:
         # stretches of equal ids
-        run = torch.cumsum(torch.cat([torch.zeros(1, dtype=torch.long), (ids[1:] != ids[:-1]).long()]), 0) if Lk else ids.long()
+        run = torch.cumsum(torch.cat([torch.zeros(1, dtype=torch.long), (ids[1:] != ids[:-1]).long()]), 0)
         at = t[:, 0].clamp(min=0)
         seen = seen & (run[at][:, None] == run[None, :]) & (ids[at] >= 0)[:, None]
     return seen, (t - j).abs().double()

@@ -1,0 +1,234 @@
+"""Attention with changed scores at lengths where a kernel's blocks take several pieces of work each, with many sequences, at the ends of
+its arguments' ranges, and in calls side by side.
+
+Allowances as in test_biased_attn_gpu.py, with a slack of 1.2 instead of 1.05 for sums of up to n = 6000 terms: in 32 bits these are off by
+n 2^-24 = 2^-11.4 of their terms' sizes at most, 0.18 of the half step 2^-9 that the allowance counts for every bf16 term."""
+import math
+import os
+import subprocess
+import sys
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from fsa.ops import biased_attention
+from fsa_preview.ops import biased_decode_attention, shared_prefix_decode_attention
+from oracle import biased_attn_oracle as orc
+from test_biased_attn_gpu import BF16, DEV, check, cu_of, inputs, near, near_lse, slopes_of
+from test_biased_decode_gpu import cache_of, i32
+
+INT_MAX = 2 ** 31 - 1
+
+
+def roomy(got, ref, off, name):
+    err = (got.double() - ref).abs()
+    room = 1.2 * off + 2.0 ** -20 * float(ref.abs().max())
+    assert bool((err <= room).all()), f"{name}: {float((err - room).max()):.3e} over the allowance"
+
+
+@pytest.mark.parametrize("Hk,G,d,cap,alibi,how", [
+    (8, 1, 128, 30.0, False, {}),                     # 47 K/V tiles and 8 heads: several pieces of work an SM, tiles cut
+    (4, 4, 64, None, True, {}),
+    (8, 2, 128, None, False, {"window": 700}),
+    (4, 2, 128, 50.0, True, {"docs": 900}),
+    (4, 1, 64, 20.0, True, {"prefix": 2500}),
+])
+def test_long(Hk, G, d, cap, alibi, how):
+    N, Hq = 6000, Hk * G
+    q, k, v, do = (x.to(DEV) for x in inputs([N], [N], Hk, G, d, BF16, N + G))
+    ids = torch.div(torch.arange(N, dtype=torch.int32), how["docs"], rounding_mode="floor").int() if "docs" in how else None
+    sl = slopes_of(Hq) if alibi else None
+    leaves = [x.clone().requires_grad_() for x in (q, k, v)]
+    o, lse = biased_attention(*leaves, i32([0, N]), softcap=cap, alibi_slopes=None if sl is None else sl.to(DEV), window_size=how.get("window"),
+                              doc_ids=None if ids is None else ids.to(DEV), prefix_lens=i32([how["prefix"]]) if "prefix" in how else None)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do)
+    seen, dist = (x.to(DEV) for x in orc.visible(N, N, how.get("window"), ids, how.get("prefix")))
+    half = torch.finfo(BF16).eps / 2
+    tiny = torch.finfo(BF16).smallest_normal * half
+    for kh in range(Hk):
+        sums = [0.0] * 4
+        for h in range(kh * G, kh * G + G):
+            ref, off = orc.one_head(*(x.double() for x in (q[:, h], k[:, kh], v[:, kh])), seen, dist, d ** -0.5, cap or 0.0, float(sl[h]) if alibi else 0.0,
+                                    do[:, h].double(), half, tiny)
+            roomy(o[:, h], ref[0], off[0], f"o of head {h}")
+            near_lse(lse[h], ref[1].cpu())
+            roomy(dq[:, h], ref[2], off[1], f"dq of head {h}")
+            sums = [a + b for a, b in zip(sums, (ref[3], ref[4], off[2], off[3]))]
+        # (dk and dv: the heads of a group are added in 32 bits, the sum is rounded once)
+        roomy(dk[:, kh], sums[0], sums[2] + half * sums[0].abs(), f"dk of head {kh}")
+        roomy(dv[:, kh], sums[1], sums[3] + half * sums[1].abs(), f"dv of head {kh}")
+
+
+@pytest.mark.parametrize("how", [{}, {"window": 40}, {"docs": True}, {"prefix": True}])
+def test_many_sequences(how):
+    """More sequences than a block has threads, some without tokens, some with more keys than queries and the other way round."""
+    lens = [3, 0, 130, 1, 17] * 130
+    klens = [5, 2, 130, 0, 200] * 130
+    q, k, v, do = inputs(lens, klens, 1, 2, 64, BF16, 9)
+    ids = torch.div(torch.arange(sum(klens), dtype=torch.int32), 50, rounding_mode="floor").int() if "docs" in how else None
+    prefix = torch.tensor([b % 140 for b in range(len(lens))], dtype=torch.int32) if "prefix" in how else None
+    check(q, k, v, do, lens, klens, 20.0, slopes_of(2), window=how.get("window"), ids=ids, prefix=prefix)
+
+
+@pytest.mark.parametrize("lens,klens", [([150, 40], [150, 40]), ([100, 20], [300, 10])])
+def test_the_largest_window_and_prefix(lens, klens):
+    """(The second sequence begins behind row 0: its first row and such a prefix are more than an int holds.)"""
+    q, k, v, do = inputs(lens, klens, 1, 2, 128, BF16, 2)
+    check(q, k, v, do, lens, klens, 20.0, None, window=INT_MAX)
+    check(q, k, v, do, lens, klens, 20.0, None, prefix=torch.tensor([INT_MAX, INT_MAX], dtype=torch.int32))
+    check(q, k, v, do, lens, klens, 20.0, None, prefix=torch.tensor([-1, -INT_MAX - 1], dtype=torch.int32))
+
+
+@pytest.mark.parametrize("cap,scale", [(1e8, 0.1), (30.0, 1e-12), (1e20, 0.1)])
+def test_caps_far_above_the_scores(cap, scale):
+    lens = [90, 33]
+    q, k, v, do = inputs(lens, lens, 1, 2, 64, BF16, 3)
+    check(q, k, v, do, lens, lens, cap, scale=scale)
+
+
+def test_a_cap_far_below_the_scores():
+    """All scores are at the cap: their gradients are 0 but for the error of the tanh, 6e-7, which 1 - t^2 doubles: 2^-19 sm_scale sum_j p |dP - delta| |k|, and
+    |dP - delta| is at most twice the largest |dP|, the sum over the p of a row is 1, and a key has up to 90 of them."""
+    lens, scale = [90, 33], 0.1
+    q, k, v, do = inputs(lens, lens, 1, 2, 64, BF16, 3)
+    leaves = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    o, lse = biased_attention(*leaves, cu_of(lens).to(DEV), softcap=1e-6, sm_scale=scale)
+    ref, off = orc.packed(q, k, v, cu_of(lens), cu_of(lens), scale, 1e-6, do=do, dtype=BF16)
+    near(o.detach(), ref[0], off[0], "o")
+    near_lse(lse, ref[1])
+    dq, dk, dv = (x.double().cpu() for x in torch.autograd.grad(o, leaves, do.to(DEV)))
+    most = 2.0 ** -18 * scale * float(torch.einsum("nhd,md->nhm", do.double(), v[:, 0].double()).abs().max())
+    assert bool(((dq - ref[2]).abs() <= most * float(k.abs().max())).all())
+    assert bool(((dk - ref[3]).abs() <= 2 * 90 * most * float(q.abs().max())).all())
+    near(dv, ref[4], off[3], "dv")
+
+
+def test_documents_with_fewer_keys_than_queries():
+    """Tokens in front of a sequence's first row stand at negative places, in the first block's first row as well."""
+    lens, klens = [400, 300, 5], [90, 350, 0]
+    q, k, v, do = inputs(lens, klens, 1, 2, 64, BF16, 4)
+    ids = torch.cat([torch.full((n,), i, dtype=torch.int32) for n, i in ((60, 3), (200, 1), (100, -1), (80, 1))])
+    check(q, k, v, do, lens, klens, 20.0, slopes_of(2), ids=ids)
+
+
+def test_sequences_in_front_of_the_first_group():
+    """cu_group that begins behind 0: the sequences before it have no prefix either."""
+    lens, prefixes = [70, 5, 300, 1, 40], [333, 64]
+    q, k, v, row0 = cache_of(lens, 2, 2, 128, BF16, 6)
+    g = torch.Generator().manual_seed(7)
+    pk, pv = (torch.randn(sum(prefixes), 2, 128, generator=g).to(BF16) for _ in range(2))
+    o, lse = shared_prefix_decode_attention(q.to(DEV), k.to(DEV), v.to(DEV), i32(lens), i32(row0), pk.to(DEV), pv.to(DEV), i32([0, 333, 397]),
+                                            i32([1, 3, 4]), max_len=300, softcap=20.0)
+    none, a, b = (pk[:0], pv[:0]), (pk[:333], pv[:333]), (pk[333:], pv[333:])
+    ref, off = orc.decoded(q, k, v, lens, row0, 128 ** -0.5, 20.0, None, None, [none, a, a, b, none], BF16)
+    near(o, ref[0], off, "o")
+    near_lse(lse, ref[1])
+
+
+def test_a_million_token_hint():
+    """max_len far above what the cache holds: more chunks, the same rows."""
+    lens = [200, 31]
+    q, k, v, row0 = cache_of(lens, 1, 2, 64, BF16, 8)
+    args = [q.to(DEV), k.to(DEV), v.to(DEV), i32(lens), i32(row0)]
+    ref, off = orc.decoded(q, k, v, lens, row0, 64 ** -0.5, 0.0, None, None, None, BF16)
+    for hint in (0, 1 << 20):
+        o, lse = biased_decode_attention(*args, max_len=hint)
+        near(o, ref[0], off, "o")
+        near_lse(lse, ref[1])
+    with pytest.raises(ValueError, match="not supported"):
+        biased_decode_attention(*args, max_len=1 << 30)
+
+
+def test_two_graphs_replayed_at_once():
+    """Two captured training steps, each on its own stream, replayed together."""
+    lens, Hk, G, d = [900, 333], 2, 2, 128
+    cu = cu_of(lens).to(DEV)
+    steps, graphs, held = [], [], []
+    for seed in (1, 2):
+        *leaves, do = (x.to(DEV) for x in inputs(lens, lens, Hk, G, d, BF16, seed))
+        leaves = [x.requires_grad_() for x in leaves]
+
+        def step(leaves=leaves, do=do):
+            o, lse = biased_attention(*leaves, cu, softcap=30.0)
+            return [o.detach(), lse, *torch.autograd.grad(o, leaves, do)]
+
+        steps.append(step)
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            step()
+        torch.cuda.current_stream().wait_stream(side)
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            held.append(step())
+    want = [s() for s in steps]
+    streams = [torch.cuda.Stream() for _ in graphs]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for x in held[0] + held[1]:
+            x.zero_()
+        torch.cuda.synchronize()
+        for st, g in zip(streams, graphs):
+            with torch.cuda.stream(st):
+                g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for h, w in zip(held, want) for a, b in zip(h, w))
+
+
+def test_steps_one_behind_another_on_one_stream():
+    """Layers in a row without a pause, each writing where the one before it was read: what a kernel that starts early may not overtake."""
+    lens = [1500, 40]
+    cu = cu_of(lens).to(DEV)
+    q, k, v, do = (x.to(DEV) for x in inputs(lens, lens, 2, 2, 64, BF16, 5))
+
+    def run():
+        x, out = q, []
+        for i in range(6):
+            leaves = [t.detach().requires_grad_() for t in (x, k, v)]
+            o, _ = biased_attention(*leaves, cu, softcap=10.0 + i)
+            dq, dk, dv = torch.autograd.grad(o, leaves, do)
+            out += [dq, dk, dv]
+            x = (o.detach() * 2 + dq).contiguous()
+        return out
+
+    first = run()
+    torch.cuda.synchronize()
+    for _ in range(5):
+        assert all(torch.equal(a, b) for a, b in zip(first, run()))
+
+
+def test_gradients_need_not_be_asked_for_all():
+    lens = [100]
+    q, k, v, do = (x.to(DEV) for x in inputs(lens, lens, 1, 2, 64, BF16, 1))
+    cu = cu_of(lens).to(DEV)
+    kk = k.clone().requires_grad_()
+    o, _ = biased_attention(q, kk, v, cu, softcap=5.0)
+    every = [x.clone().requires_grad_() for x in (q, k, v)]
+    o2, _ = biased_attention(*every, cu, softcap=5.0)
+    assert torch.equal(torch.autograd.grad(o, kk, do)[0], torch.autograd.grad(o2, every, do)[1])
+    with torch.no_grad():
+        assert torch.equal(biased_attention(*every, cu, softcap=5.0)[0], o)
+
+
+_WITH_CHECKS = """
+import torch
+from fsa.ops import biased_attention
+from fsa_preview.ops import biased_decode_attention
+x = [torch.randn(70, 2, 64, device="cuda").bfloat16().requires_grad_() for _ in range(3)]
+cu = torch.tensor([0, 70], dtype=torch.int32, device="cuda")
+o, lse = biased_attention(*x, cu, softcap=5.0)
+o.float().sum().backward()
+n = torch.tensor([70], dtype=torch.int32, device="cuda")
+d, _ = biased_decode_attention(x[0][-1:].detach(), x[1].detach(), x[2].detach(), n, n * 0, max_len=70, softcap=5.0)
+assert (d[0] - o[-1]).abs().max() <= 2 ** -6 * o.abs().max()
+print("read")
+"""
+
+
+def test_with_status_checks():
+    """FSA_CHECK_STATUS=1: the status word is read behind every call."""
+    root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "flash-sparse-attention_b200")
+    r = subprocess.run([sys.executable, "-c", _WITH_CHECKS], env={**os.environ, "FSA_CHECK_STATUS": "1", "PYTHONPATH": root}, capture_output=True, text=True, timeout=120)
+    assert r.returncode == 0 and "read" in r.stdout, r.stderr[-2000:]
