@@ -6,6 +6,7 @@
 namespace fsa {
 
 constexpr int kBiasedBK = 64;       // K/V rows of a tile
+constexpr int kBiasedLeast = 4;     // K/V tiles of a chunk (an item's beginning and end are as long as 4 to 5 of them)
 
 struct BiasedFwdParams {
     const int32_t* cu_q;    // [B + 1]
@@ -38,15 +39,32 @@ struct BiasedFwdLaunch {
     ScoreMod mod;
     int window;                     // -1: none
     const int32_t* prefix_lens;     // [B] or null
-    // kModSplit: rows that several sequences share, a "token" is a sequence of the batch (kv_lo and kv_hi are not used).  The K/V rows of every
-    // tile are cut into nchunk chunks (blockIdx.y) of `chunk` tiles; chunk c of a row writes partial c of P
-    const int32_t* seq_len; // [N] own tokens of every sequence, the new one among them
+    // kModSplit: the K/V rows of every tile are cut into nchunk chunks (blockIdx.y) of `chunk` tiles (0: an equal share, at least kBiasedLeast);
+    // chunk c of a row writes partial c of P.
+    // seq_len: rows that several sequences share, a "token" is a sequence of the batch (kv_lo and kv_hi are not used), and the kernel runs beside the
+    // one before it
+    const int32_t* seq_len; // [N] own tokens of every sequence, the new one among them; or null
     float* o_part;          // [N, Hq, P, D] unnormalised
     float2* ml;             // [N, Hq, P] reference maximum (log2 units) and sum
     int P, nchunk, chunk;
 };
 // which: kModCap, kModBias; split: with kModSplit.  l.p.TPT tokens a tile, max_tiles tiles at most.
 cudaError_t launch_biased_fwd(int D, int dtype, int which, bool split, const BiasedFwdLaunch& l, int max_tiles, cudaStream_t stream);
+
+// o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, lse = M + log2 of the latter, of rows = tokens x Hq over their P partials.  The first nshared
+// partials of tokens outside [cu[0], cu[groups]) are left out.  lse[token * lse_sn + head * lse_sh].  (biased_decode.cu)
+struct BiasedMerge {
+    const float* o_part;
+    const float2* ml;
+    int64_t rows;
+    int Hq, P, nshared;
+    const int32_t* cu;
+    int groups;
+    void* o;
+    float* lse;
+    int64_t lse_sn, lse_sh;
+};
+cudaError_t launch_biased_merge(int D, int dtype, const BiasedMerge& m, cudaStream_t stream);
 
 struct RangeKvPlan;      // range_bwd.cuh
 // The backward, a.bd's limits given; as parts of a chain of dependent launches, the second beside the first.

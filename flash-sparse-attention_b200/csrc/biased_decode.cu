@@ -270,14 +270,12 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
     }
 }
 
-// o = sum_i 2^(m_i - M) o_i / sum_i 2^(m_i - M) l_i, lse = M + log2 of the latter, over the P partials of every row; 0 and -inf for a row that saw
-// nothing.  A sequence in front of the first or behind the last group has no shared partials.  WARPS warps a row: what it takes is round trips to L2, so
+// BiasedMerge; 0 and -inf for a row that saw nothing.  WARPS warps a row: what it takes is round trips to L2, so
 // all maxima and sums, and the first 16 partials of every warp, are asked for at once (1 x 8191 tokens, 32 heads, 64 partials a row: 12 us with
 // a round trip for every four partials of a warp).
-constexpr int kMgThreads = 128, kMgAhead = 16;
-template <int D, int WARPS, typename ET>
-__global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const float* o_part, const float2* ml, int64_t rows, int Hq, int P, int nshared, const int32_t* cu_group, int groups,
-                                                                  ET* __restrict__ o, float* __restrict__ lse) {
+constexpr int kMgThreads = 128;
+template <int D, int WARPS, int AHEAD, typename ET>
+__global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const BiasedMerge a) {
     constexpr int V = D / 32;           // columns of a lane
     __shared__ float s_m[4], s_l[4];
     __shared__ float4 s_acc[4][32];
@@ -285,18 +283,19 @@ __global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const float* o
     const int w = warp % WARPS;
     const int64_t row = (int64_t)blockIdx.x * (4 / WARPS) + warp / WARPS;
     follow();
-    if (row >= rows) return;            // (with WARPS = 4 there is no such CTA)
-    const int b = (int)(row / Hq), first = nshared > 0 && (b < __ldcg(cu_group) || b >= __ldcg(cu_group + groups)) ? nshared : 0;
-    const float2* mlr = ml + row * P;
-    const float* src = o_part + row * P * D + lane * V;
+    if (row >= a.rows) return;            // (with WARPS = 4 there is no such CTA)
+    const int P = a.P, b = (int)((uint32_t)row / (uint32_t)a.Hq);
+    const int first = a.nshared > 0 && (b < __ldcg(a.cu) || b >= __ldcg(a.cu + a.groups)) ? a.nshared : 0;
+    const float2* mlr = a.ml + row * P;
+    const float* src = a.o_part + row * P * D + lane * V;
     auto load = [&](int i, float (&x)[4]) {
         x[2] = x[3] = 0.f;
         if constexpr (V == 4) *reinterpret_cast<float4*>(x) = __ldcg(reinterpret_cast<const float4*>(src + (int64_t)i * D));
         else *reinterpret_cast<float2*>(x) = __ldcg(reinterpret_cast<const float2*>(src + (int64_t)i * D));
     };
-    float x[kMgAhead][4];
+    float x[AHEAD][4];
 #pragma unroll
-    for (int j = 0; j < kMgAhead; ++j)
+    for (int j = 0; j < AHEAD; ++j)
         if (first + w + WARPS * j < P) load(first + w + WARPS * j, x[j]);
     float M = -INFINITY, L = 0.f;
     for (int i = first + w * 32 + lane; i < P; i += 32 * WARPS) {
@@ -331,9 +330,9 @@ __global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const float* o
         }
     };
 #pragma unroll
-    for (int j = 0; j < kMgAhead; ++j)
+    for (int j = 0; j < AHEAD; ++j)
         if (first + w + WARPS * j < P) add(first + w + WARPS * j, x[j]);
-    for (int i = first + w + WARPS * kMgAhead; i < P; i += WARPS) {
+    for (int i = first + w + WARPS * AHEAD; i < P; i += WARPS) {
         float y[4];
         load(i, y);
         add(i, y);
@@ -349,10 +348,10 @@ __global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const float* o
         }
     }
     const float inv = L > 0.f ? 1.f / L : 0.f;
-    ET* dst = o + row * D + lane * V;
+    ET* dst = (ET*)a.o + row * D + lane * V;
     if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(ElemTraits<ET>::pack2(acc[0] * inv, acc[1] * inv), ElemTraits<ET>::pack2(acc[2] * inv, acc[3] * inv));
     else *reinterpret_cast<uint32_t*>(dst) = ElemTraits<ET>::pack2(acc[0] * inv, acc[1] * inv);
-    if (lane == 0) lse[row] = L > 0.f ? M + log2f(L) : -INFINITY;
+    if (lane == 0) a.lse[b * a.lse_sn + (row - (int64_t)b * a.Hq) * a.lse_sh] = L > 0.f ? M + log2f(L) : -INFINITY;
 }
 
 template <int D, bool HI, int MOD, typename ET>
@@ -376,13 +375,17 @@ static cudaError_t launch_bd_which(int which, const BiasedDecodeParams& p, const
 }
 
 template <int D, typename ET>
-static cudaError_t launch_merge(const float* o_part, const float2* ml, int64_t rows, int Hq, int P, int nshared, const int32_t* cu_group, int groups, void* o, float* lse,
-                                cudaStream_t stream) {
+static cudaError_t launch_merge(const BiasedMerge& m, cudaStream_t stream) {
     // a CTA per row while all of them still run at once
-    if (rows <= 4 * sm_count())
-        return launch_dependent(biased_decode_merge<D, 4, ET>, dim3((unsigned)rows), kMgThreads, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, cu_group, groups, (ET*)o, lse);
-    return launch_dependent(biased_decode_merge<D, 1, ET>, dim3((unsigned)((rows + 3) / 4)), kMgThreads, 0, stream, 1, o_part, ml, rows, Hq, P, nshared, cu_group, groups, (ET*)o,
-                            lse);
+    if (m.rows <= 4 * sm_count()) return launch_dependent(biased_decode_merge<D, 4, 16, ET>, dim3((unsigned)m.rows), kMgThreads, 0, stream, 1, m);
+    const dim3 grid((unsigned)((m.rows + 3) / 4));
+    if (m.P <= 4) return launch_dependent(biased_decode_merge<D, 1, 4, ET>, grid, kMgThreads, 0, stream, 1, m);
+    return launch_dependent(biased_decode_merge<D, 1, 16, ET>, grid, kMgThreads, 0, stream, 1, m);
+}
+
+cudaError_t launch_biased_merge(int D, int dtype, const BiasedMerge& m, cudaStream_t stream) {
+    if (D == 128) return dtype == kBF16 ? launch_merge<128, __nv_bfloat16>(m, stream) : launch_merge<128, __half>(m, stream);
+    return dtype == kBF16 ? launch_merge<64, __nv_bfloat16>(m, stream) : launch_merge<64, __half>(m, stream);
 }
 
 // How a decode call is cut: partials of the shared rows, of the own ones.  Own rows: as many chunks as run at once, two CTAs an SM, and chunks of up to
@@ -501,8 +504,6 @@ extern "C" int fsa_biased_decode(const void* q, const void* k, const void* v, in
         e = launch_biased_fwd(D, dtype, which, true, l, cut.mtiles, stream);
         if (e != cudaSuccess) return cuda_failed(e);
     }
-    auto merge = [&](auto run) { return run(o_part, ml, rows, Hq, P, cut.nshared, cu_group, num_groups, o, lse, stream); };
-    if (D == 128) e = bf16 ? merge(launch_merge<128, __nv_bfloat16>) : merge(launch_merge<128, __half>);
-    else e = bf16 ? merge(launch_merge<64, __nv_bfloat16>) : merge(launch_merge<64, __half>);
+    e = launch_biased_merge(D, dtype, BiasedMerge{o_part, ml, rows, Hq, P, cut.nshared, cu_group, num_groups, o, lse, Hq, 1}, stream);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
 }

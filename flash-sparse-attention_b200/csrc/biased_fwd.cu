@@ -70,10 +70,11 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
     const BiasedFwdParams& p = launch.p;
     const uint32_t limit = wait_limit(p.status);
     const int G = p.G, TPT = p.TPT;
-    // First and last K/V row that a token sees, and its place.  kModSplit: a token is a sequence of the batch, whose own rows follow the shared ones.
+    // First and last K/V row that a token sees, and its place.  kModSplit: with shared rows a token is a sequence of the batch, whose own rows
+    // follow them.
     auto limits = [&](int seq, int tok) {
         Sees x;
-        if constexpr (kSplit) {
+        if (kSplit && launch.seq_len) {
             const int k0 = __ldcg(p.cu_k + seq), k1 = __ldcg(p.cu_k + seq + 1), len = __ldcg(launch.seq_len + tok);
             x.pos = k1 + len - 1;
             x.lo = launch.window >= 0 ? max(k0, x.pos - launch.window) : k0;
@@ -88,7 +89,8 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
         }
         return x;
     };
-    if constexpr (!kSplit) follow_late();
+    const bool beside = kSplit && launch.seq_len;        // it needs nothing of the kernel before it
+    if (!beside) follow_late();
     if (tid == 0) {
         *status = kStatusOk;
         mbar_init(q_full, 1); mbar_init(q_empty, 1);
@@ -109,7 +111,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
         tc_fence_before();
         asm volatile("bar.sync 2, 192;" ::: "memory");
         tc_fence_after();
-        if constexpr (!kSplit) let_next_start();
+        if (!beside) let_next_start();
     }
     const uint32_t tbase = warp ? tmem_slot : 0u;
     // Item n of this CTA.  Each of the five other warps takes every item once, in order; z < 0 ends the list.
@@ -155,9 +157,10 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                 hi = min(__reduce_max_sync(0xffffffffu, hi), (int)p.Nk - 1);
                 int nblk = hi >= lo ? (hi - lo) / BK + 1 : 0;
                 if constexpr (kSplit) {
-                    // chunks of one size (the last one takes what is left), so that long shared rows are cut more often than short ones
-                    const int b0 = min(z * launch.chunk, nblk);
-                    nblk = z + 1 < launch.nchunk ? min(launch.chunk, nblk - b0) : nblk - b0;
+                    // chunks of one size (the last one takes what is left), so that long shared rows are cut more often than short ones, or equal ones
+                    const int size = launch.chunk ? launch.chunk : max(kBiasedLeast, (nblk + launch.nchunk - 1) / launch.nchunk);
+                    const int b0 = min(z * size, nblk);
+                    nblk = z + 1 < launch.nchunk ? min(size, nblk - b0) : nblk - b0;
                     lo += b0 * BK;
                     hi = min(hi, lo + nblk * BK - 1);
                 }
@@ -497,7 +500,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
     tc_fence_before();
     __syncthreads();
     if (warp == 1) tmem_dealloc(tbase, kCols);
-    if constexpr (kSplit) follow_late();
+    if (beside) follow_late();
     if (tid == 0 && *status != kStatusOk && p.status) atomicMax(p.status, *status);
 }
 
@@ -507,7 +510,7 @@ static cudaError_t launch_bf(const BiasedFwdLaunch& l, int max_tiles, cudaStream
     auto kern = biased_fwd<D, MOD, ET>;
     const cudaError_t e = allow_smem((const void*)kern, smem);
     if (e != cudaSuccess) return e;
-    // (kModSplit: beside the kernel before it, which is the one of the own rows, biased_decode.cu)
+    // (shared rows: beside the kernel before it, which is the one of the own rows, biased_decode.cu)
     return launch_dependent(kern, dim3((unsigned)max_tiles * (unsigned)l.p.Hk, (MOD & kModSplit) ? (unsigned)l.nchunk : 1u), kBfThreads, smem, stream, 1, l);
 }
 

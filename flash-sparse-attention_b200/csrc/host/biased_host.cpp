@@ -88,11 +88,14 @@ static std::tuple<Tensor, Tensor, Tensor> biased_fwd(const Tensor& q_, const Ten
         return {at::zeros({N, Hq, D}, q_.options().requires_grad(false)),
                 at::full({Hq, N}, -INFINITY, q_.options().dtype(at::kFloat).requires_grad(false)), limits};
     const Rows3 q(q_, false), k(k_, true), v(v_, true);
-    Tensor o = fresh({N, Hq, D}, q_), lse = f32({Hq, N}, q_);
+    Tensor o = fresh({N, Hq, D}, q_), lse = f32({Hq, N}, q_), scratch;
+    const int B = (int)a.cu_q.size(0) - 1;
+    check(fsa_biased_attn_fwd_bytes(N, Nk, B, (int)Hq, (int)Hk, (int)D, (int)a.window, &nb), "fsa_biased_attn_fwd_bytes");
+    if (nb > 0) scratch = bytes(nb, q_);
     check(fsa_biased_attn_fwd(ptr(q.t), ptr(k.t), ptr(v.t), iptr(a.cu_q), iptr(a.cu_k), iptr(a.docs), iptr(a.prefix),
-                              a.slopes.defined() ? a.slopes.data_ptr<float>() : nullptr, N, Nk, (int)a.cu_q.size(0) - 1, (int)Hq, (int)Hk, (int)D,
+                              a.slopes.defined() ? a.slopes.data_ptr<float>() : nullptr, N, Nk, B, (int)Hq, (int)Hk, (int)D,
                               dtype_code(q_), q.sn, q.sh, k.sn, v.sn, (float)a.scale, (float)a.cap, (int)a.window, ptr(o), lse.data_ptr<float>(), ptr(limits),
-                              limits.numel(), stream_of(q_)),
+                              limits.numel(), ptr(scratch), nb, stream_of(q_)),
           "fsa_biased_attn_fwd");
     check_biased_status("fsa_biased_attn_fwd status");
     return {o, lse, limits};

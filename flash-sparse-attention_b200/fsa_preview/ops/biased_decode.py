@@ -83,8 +83,8 @@ def shared_prefix_decode_attention(
         seq_len: ``[batch]`` int32: every sequence's OWN tokens, behind its prefix, the new one included.  0: an idle place
         prefix_k, prefix_v: the prefixes' rows, one prefix after the other ``[rows, num_kv_heads, head_dim]``
         cu_prefix: ``[num_prefixes + 1]`` int32: where the prefixes begin in prefix_k
-        cu_group: ``[num_prefixes + 1]`` int32: sequences ``cu_group[i] .. cu_group[i + 1] - 1`` continue prefix i (sequences behind the
-            last group have no prefix)
+        cu_group: ``[num_prefixes + 1]`` int32: sequences ``cu_group[i] .. cu_group[i + 1] - 1`` continue prefix i (sequences in front of
+            the first and behind the last group have no prefix)
         max_prefix: how long the longest prefix is (host integer; all of prefix_k's rows, if not given)
     Distances, and window_size, count from the beginning of the prefix: the new token stands at place
     ``len(prefix) + seq_len[b] - 1``.

@@ -212,17 +212,20 @@ int fsa_range_attn_bwd_indexed(int head_dim);
  *   prefix_lens      (int32 per sequence; not with window or doc_ids) and the sequence's first prefix_lens[b] keys besides.
  * k, v: head stride head_dim.  o [N, Hq, D] contiguous, lse [Hq, N] (log2 units); rows behind the last sequence become 0 / -inf.  K/V
  * rows that no token sees, and q and d_o rows of tokens that see nothing, may hold anything, NaN included.  limits: workspace of
- * fsa_biased_attn_limits_bytes bytes, kept for the backward.
+ * fsa_biased_attn_limits_bytes bytes, kept for the backward.  scratch: 32-byte aligned, of fsa_biased_attn_fwd_bytes bytes for the same sizes (0: none).
  * head_dim 64 or 128, up to 32 query heads a kv head, fewer than 2^25 tokens and K/V rows, N * num_q_heads below 2^31. */
 int fsa_biased_attn_limits_bytes(int64_t total_tokens, int64_t* bytes_out);
+int fsa_biased_attn_fwd_bytes(int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window,
+                              int64_t* bytes_out);
 int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, const int32_t* cu_seqlens_q, const int32_t* cu_seqlens_k,
                         const int32_t* doc_ids, const int32_t* prefix_lens, const float* slopes, int64_t total_tokens, int64_t total_kv_rows, int batch,
                         int num_q_heads, int num_kv_heads, int head_dim, int dtype, int64_t q_stride_n, int64_t q_stride_h, int64_t k_stride_n,
-                        int64_t v_stride_n, float sm_scale, float softcap, int window, void* o, float* lse, void* limits, int64_t limits_bytes, void* stream);
+                        int64_t v_stride_n, float sm_scale, float softcap, int window, void* o, float* lse, void* limits, int64_t limits_bytes, void* scratch,
+                        int64_t scratch_bytes, void* stream);
 /* The same scores for one new token of every sequence, the last of its seq_len[b] tokens, which the cache rows seq_row0[b] .. hold (next to
  * fsa_decode_attn_partial).  Sequences may follow rows that they share: group i is the sequences cu_group[i] .. cu_group[i + 1] - 1, in front of
  * whose own tokens stand the rows cu_shared[i] .. cu_shared[i + 1] - 1 of shared_k / shared_v, read once for all of them (num_groups 0: none; sequences
- * behind the last group share nothing).  window: keys at least seq's length - 1 - window.  seq_len[b] <= 0: an idle place, o = 0, lse = -inf.
+ * in front of the first group and behind the last share nothing).  window: keys at least seq's length - 1 - window.  seq_len[b] <= 0: an idle place, o = 0, lse = -inf.
  * q, o [B, Hq, D] contiguous, lse [B, Hq].  max_len, max_shared: how long the longest are, by which the work is cut; longer ones are
  * read all the same.  Rows behind a sequence may hold anything.  scratch 32-byte aligned, of fsa_biased_decode_bytes bytes for the same sizes.
  * Limits as above (batch, shared_rows and num_groups below 2^25, cache rows below 2^31). */

@@ -232,3 +232,66 @@ def test_with_status_checks():
     root = os.path.join(os.path.dirname(os.path.abspath(__file__)), "..", "flash-sparse-attention_b200")
     r = subprocess.run([sys.executable, "-c", _WITH_CHECKS], env={**os.environ, "FSA_CHECK_STATUS": "1", "PYTHONPATH": root}, capture_output=True, text=True, timeout=120)
     assert r.returncode == 0 and "read" in r.stdout, r.stderr[-2000:]
+
+
+def cut_bytes(q, k, cu, window):
+    """Workspace of a forward whose K/V rows are cut into chunks; 0: they are not."""
+    import ctypes
+
+    from fsa._lib import lib
+
+    n = ctypes.c_int64(-1)
+    assert lib().fsa_biased_attn_fwd_bytes(q.shape[0], k.shape[0], cu.numel() - 1, q.shape[1], k.shape[1], q.shape[2], -1 if window is None else window,
+                                           ctypes.byref(n)) == 0
+    return n.value
+
+
+@pytest.mark.parametrize("score", [(None, False), (20.0, False), (None, True), (50.0, True)])
+@pytest.mark.parametrize("lens,klens,Hk,G,d,dtype,how", [
+    ([1], [3001], 1, 1, 128, BF16, {}),                                # one query
+    ([5, 0, 33], [2500, 700, 3100], 2, 4, 128, BF16, {}),              # a sequence without queries
+    ([40, 3, 100], [4000, 2, 60], 1, 3, 64, torch.float16, {}),        # chunks without rows; fewer keys than queries
+    ([17, 64], [3000, 2000], 1, 8, 128, BF16, {"window": 1500}),
+    ([130, 20], [2500, 1500], 1, 2, 64, BF16, {"docs": True}),
+    ([300, 70], [2500, 2200], 1, 4, 128, BF16, {"prefix": [2400, 2199]}),
+    ([1900], [1900], 1, 1, 128, BF16, {"prefix": [1500]}),
+])
+def test_few_queries_over_many_keys(score, lens, klens, Hk, G, d, dtype, how):
+    """Forward with the K/V rows cut into chunks: masks that leave chunks empty, padding of NaN in the middle."""
+    cap, alibi = score
+    q, k, v, do = inputs(lens, klens, Hk, G, d, dtype, sum(klens))
+    assert cut_bytes(q, k, cu_of(lens), how.get("window")) > 0
+    ids = None
+    if "docs" in how:
+        ids = torch.cat([torch.full((n,), i, dtype=torch.int32) for i, n in ((1, 300), (-1, 100), (2, 2100), (4, 700), (-3, 90), (5, 710))])
+        k[ids < 0], v[ids < 0] = math.nan, math.inf
+    prefix = torch.tensor(how["prefix"], dtype=torch.int32) if "prefix" in how else None
+    check(q, k, v, do, lens, klens, cap, slopes_of(Hk * G) if alibi else None, window=how.get("window"), ids=ids, prefix=prefix)
+
+
+def test_chunks_and_rows_behind_the_last_sequence():
+    lens, klens, spare = [30, 11], [2600, 2100], 50
+    q, k, v, _ = inputs(lens, klens, 2, 2, 128, BF16, 1)
+    pad = lambda x: torch.cat([x, torch.full((spare, *x.shape[1:]), math.nan, dtype=x.dtype)]).to(DEV)  # noqa: E731
+    qc, kc, vc = pad(q), pad(k), pad(v)
+    assert cut_bytes(qc, kc, cu_of(lens), None) > 0
+    o, lse = biased_attention(qc, kc, vc, cu_of(lens).to(DEV), cu_seqlens_k=cu_of(klens).to(DEV), softcap=30.0)
+    ref, off = orc.packed(q, k, v, cu_of(lens), cu_of(klens), 128 ** -0.5, 30.0, dtype=BF16)
+    n = sum(lens)
+    near(o[:n], ref[0], off[0], "o")
+    near_lse(lse[:, :n], ref[1])
+    assert bool((o[n:] == 0).all()) and bool((lse[:, n:] == -math.inf).all())
+    again = biased_attention(qc, kc, vc, cu_of(lens).to(DEV), cu_seqlens_k=cu_of(klens).to(DEV), softcap=30.0)
+    assert torch.equal(again[0], o) and torch.equal(again[1], lse)
+
+
+def test_a_verification_step_agrees_with_single_tokens():
+    """Four drafted tokens after a cache in one call, and the same tokens one at a time over the cache: the rows agree to what P's rounding and o's make."""
+    Hk, G, d, L = 2, 4, 128, 5000
+    q, k, v, _ = (x.to(DEV) for x in inputs([4], [L], Hk, G, d, BF16, 12))
+    o, lse = biased_attention(q, k, v, i32([0, 4]), cu_seqlens_k=i32([0, L]), softcap=40.0, alibi_slopes=slopes_of(8).to(DEV))
+    for i in range(4):
+        o1, lse1 = biased_decode_attention(q[i : i + 1], k, v, i32([L - 3 + i]), i32([0]), max_len=L, softcap=40.0, alibi_slopes=slopes_of(8).to(DEV))
+        # each side: half a step 2^-9 of P (sums of |p v|, at most max |v|), and 2^-9 of o
+        assert float((o[i] - o1[0]).abs().max()) <= 2 * 2.0 ** -8 * float(v.abs().max())
+        assert float((lse[:, i] - lse1[0]).abs().max()) <= 2.0 ** -15
