@@ -55,7 +55,7 @@ __device__ __forceinline__ BqItem bq_item(const BiasedDqParams& p, int w, int la
     if (m.seq < 0) return m;
     int lo = INT_MAX, hi = -1;
     for (int e = lane; e < m.ne; e += 32) {
-        const int l = __ldg(p.kv_lo + m.tok0 + e), u = __ldg(p.kv_hi + m.tok0 + e);
+        const int l = __ldcg(p.kv_lo + m.tok0 + e), u = __ldcg(p.kv_hi + m.tok0 + e);
         if (u >= l) { lo = min(lo, l); hi = max(hi, u); }
     }
     m.row_lo = max(__reduce_min_sync(0xffffffffu, lo), 0);
@@ -294,14 +294,14 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
         auto load_numbers = [&](const BqItem& m) {
             Row x = {0, -1, 0.f, 0.f, 0.f, 0};
             if (g < p.G && e < m.ne) {
-                x.lo = __ldg(p.kv_lo + m.tok0 + e);
-                x.hi = __ldg(p.kv_hi + m.tok0 + e);
+                x.lo = __ldcg(p.kv_lo + m.tok0 + e);
+                x.hi = __ldcg(p.kv_hi + m.tok0 + e);
                 const int64_t idx = (int64_t)(m.h * p.G + g) * p.N + m.tok0 + e;
-                x.lse = __ldg(p.lse + idx);
+                x.lse = __ldcg(p.lse + idx);
                 x.delta = __ldcg(p.delta + idx);        // (the kernel before wrote it)
                 if constexpr (MOD & kModBias) {
-                    x.slope = __ldg(p.mod.slopes + m.h * p.G + g) * kLog2e;
-                    x.pos = __ldg(p.mod.pos + m.tok0 + e);
+                    x.slope = __ldcg(p.mod.slopes + m.h * p.G + g) * kLog2e;
+                    x.pos = __ldcg(p.mod.pos + m.tok0 + e);
                 }
             }
             return x;
