@@ -270,9 +270,9 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
     }
 }
 
-// BiasedMerge; 0 and -inf for a row that saw nothing.  WARPS warps a row: what it takes is round trips to L2, so
-// all maxima and sums, and the first 16 partials of every warp, are asked for at once (1 x 8191 tokens, 32 heads, 64 partials a row: 12 us with
-// a round trip for every four partials of a warp).
+// BiasedMerge; 0 and -inf for a row that saw nothing.  WARPS warps a row: what it takes is round trips to L2,
+// so all maxima and sums, and the first AHEAD partials of every warp, are asked for at once (1 x 8191 tokens, 32 heads, 64 partials a row: 12 us with
+// a round trip for every four partials of a warp).  Of few partials many rows: AHEAD 4, whose registers leave room for more warps (16544 rows of 2: 8 us less).
 constexpr int kMgThreads = 128;
 template <int D, int WARPS, int AHEAD, typename ET>
 __global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const BiasedMerge a) {

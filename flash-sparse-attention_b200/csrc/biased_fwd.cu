@@ -1,20 +1,21 @@
 // Forward of attention with changed scores (score.cuh) for sm_100a: every token attends one stretch of K/V rows, its scores capped by a tanh
-// and / or biased by distance.  Also its form with the K/V rows cut into chunks (kModSplit), whose partial results are merged afterwards: the
-// rows that many sequences of a batch share.
+// and / or biased by distance.  Also its form with the K/V rows cut into chunks (kModSplit), whose partial results are merged afterwards
+// (biased_decode.cu): few queries over many rows, and rows that many sequences of a decoded batch share.
 //
 // An item is a tile of <= 128 rows (query head of a GQA group, TPT consecutive tokens of one sequence) x one KV head, as in range_dense.cu; the
 // CTA walks the K/V tiles that the rows see, 64 rows each, from the nearest to the furthest, with the accumulator in TMEM, and writes o and
-// lse once.  Two CTAs share an SM (96 KB of shared memory, 256 TMEM columns each).
+// lse once.  Two CTAs share an SM (113 KB of shared memory at D = 128, 256 TMEM columns each).
 //   warp 0      finds the items (cluster launch control: a running CTA takes over those whose CTA has not started); TMA producer
-//   warp 1      one elected thread issues S = Q K^T for two K/V tiles at a time (N = 128), then O (+)= P V tile by tile
+//   warp 1      one elected thread issues S = Q K^T of the next K/V tile into the other of two TMEM buffers, then O (+)= P V of this one
 //   warps 2..5  one row per thread: changed scores, running maximum and sum, P -> TMEM over S; epilogue
-// Tiles two at a time, because a product of 128 x 64 keys reads its left operand from shared memory as well, 48 KB where the tensor cores take 256
-// cycles and shared memory 384; with 128 keys it is 64 KB in 512 cycles, what the tensor cores take.
+// (S of two K/V tiles at a time, N = 128, reads Q from shared memory half as often, but waits for two tiles: 314 us for what takes 280, capped.)
 // The row threads do their arithmetic in one pass over a tile: it takes the rows' references for given and the tanh's arguments for near,
-// so that the polynomial and the sums run under the exp2 (16 a cycle and SM, 512 cycles a tile: what bounds the kernel beside the products,
-// 512).  What it assumed is looked at afterwards; where it does not hold (a row's first tile, a maximum far above the reference, scores near
-// the cap, keys that some row does not see) the tile takes three passes: scores, maximum, exp2.  The nearest tile comes first because a distance
-// bias sets the reference there (furthest first, every tile raised it: 676 us for what now takes 255).
+// so that the polynomial and the sums run under the exp2 (16 a cycle and SM, 512 cycles a tile, like the products).  What it assumed is looked
+// at afterwards; where it does not hold (a row's first tile, a maximum far above the reference, scores near the cap, keys that some row
+// does not see) the tile takes three passes: scores, maximum, exp2.  The nearest tile comes first because a distance bias sets the reference
+// there (furthest first, every tile raised it: 676 us for what now takes 245).
+// 2 x 8192 tokens, 8 / 4 heads of 128: 237 us plain, 279 capped (985 TFLOP/s), 245 with a distance bias, 280 with both.  Capped, the tensor cores' queue
+// is 64 % busy, exp2 49 %, issue 49 %: two row warps a scheduler do not hide each other's loads from TMEM and chains of arithmetic altogether.
 #include "../../include/fsa_sm100.h"
 #include <climits>
 
