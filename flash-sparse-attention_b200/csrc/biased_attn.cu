@@ -278,22 +278,26 @@ extern "C" int fsa_biased_attn_limits_bytes(int64_t N, int64_t* bytes_out) {
     return FSA_OK;
 }
 
-// How the forward is cut.  While its items leave SMs idle (two run on one), a tile's K/V rows are cut into as many chunks as run at once, whose
-// partial results are merged, where that is expected to gain: 0.75 us for every K/V tile that an item has fewer, against 4 us of the second launch and
-// the partials' way to memory and back.  16 tokens, 32 / 8 heads of 128, after 65536 in the cache: 80 us with 36 chunks, 799 uncut; 2000 tokens of
-// 8 / 2 heads: 36 us with 2 chunks, 32 uncut.
+// How the forward is cut.  While its items leave SMs idle (two run on one), a tile's K/V rows are cut into chunks, no more than run at once, whose
+// partial results are merged, where that is expected to gain: 0.75 us for every K/V tile that the longest item has fewer, against 4 us of the second
+// launch and the partials' way to memory and back.  How long the longest is the host does not know: of several sequences, twice the mean.
+// 16 tokens, 32 / 8 heads of 128, after 65536 in the cache: 80 us with 36 chunks, 799 uncut; 2000 tokens of 8 / 2 heads: 36 us with 2 chunks, 32 uncut.
 struct ForwardCut {
     int nchunk = 1;
     ForwardCut(const SelShape& s, int window) {
         if (s.N == 0) return;
         const int64_t row_tiles = (s.N + s.TPT - 1) / s.TPT, items = (row_tiles > s.B ? row_tiles : s.B) * s.Hk;
-        int64_t keys = s.Nk / s.B - s.N / s.B / 2;          // that a token sees, about
-        if (window >= 0 && keys > (int64_t)window + s.TPT) keys = (int64_t)window + s.TPT;
+        int64_t most = s.Nk, keys = s.Nk / s.B - s.N / s.B / 2;         // that a token sees, at most and about
+        if (s.B > 1) keys *= 2;
+        if (window >= 0 && most > (int64_t)window + s.TPT) most = (int64_t)window + s.TPT;
+        if (keys > most) keys = most;
         int64_t n = 2 * sm_count() / items;
-        if (n > keys / (kBiasedBK * kBiasedLeast)) n = keys / (kBiasedBK * kBiasedLeast);
-        if (n < 2) return;
-        const double gain = 0.75 * (double)keys / kBiasedBK * (double)(n - 1) / (double)n, cost = 4.0 + (double)(s.N * s.Hq * n * s.D * 8) / 5e6;
-        if (gain > cost) nchunk = (int)n;
+        if (n > most / (kBiasedBK * kBiasedLeast)) n = most / (kBiasedBK * kBiasedLeast);
+        double best = 0.0;
+        for (; n >= 2; n /= 2) {
+            const double gain = 0.75 * (double)keys / kBiasedBK * (double)(n - 1) / (double)n - 4.0 - (double)(s.N * s.Hq * n * s.D * 8) / 5e6;
+            if (gain > best) { best = gain; nchunk = (int)n; }
+        }
     }
     int64_t bytes(const SelShape& s) const { return nchunk > 1 ? align_up(s.N * s.Hq * nchunk * s.D * 4, 256) + s.N * s.Hq * nchunk * 8 : 0; }
 };
