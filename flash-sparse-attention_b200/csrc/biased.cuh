@@ -66,10 +66,16 @@ struct BiasedMerge {
 };
 cudaError_t launch_biased_merge(int D, int dtype, const BiasedMerge& m, cudaStream_t stream);
 
+// Which of the items, longest first, is this CTA's n-th: forth and back, so that who has the longer item of one round has the shorter one of the next (always
+// forth, the first CTA has the longest of every round: 2 x 8192 tokens, 8 / 4 heads, dQ 437 us, dK / dV 568).
+__device__ __forceinline__ int forth_and_back(int n) { return n * (int)gridDim.x + (int)(n & 1 ? gridDim.x - 1 - blockIdx.x : blockIdx.x); }
+
 struct RangeKvPlan;      // range_bwd.cuh
-// The backward, a.bd's limits given; as parts of a chain of dependent launches, the second beside the first.
+// The backward, a.bd's limits given; as parts of a chain of dependent launches, dK / dV beside dQ.  nchunk > 1: dQ cut into chunks along the keys, part
+// [N, Hq, nchunk, D], which launch_biased_dq_sum joins after both.
 cudaError_t launch_biased_bwd_dq(int dtype, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap, const CUtensorMap& vmap, int* status,
-                                 const ScoreMod& mod, int which, cudaStream_t stream);
+                                 const ScoreMod& mod, int which, int nchunk, float* part, cudaStream_t stream);
+cudaError_t launch_biased_dq_sum(int dtype, const float* part, const SelBwdArgs& a, const SelShape& s, int nchunk, cudaStream_t stream);
 cudaError_t launch_biased_bwd_dkdv(int dtype, const RangeKvPlan& plan, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap, const CUtensorMap& vmap,
                                    int* status, const ScoreMod& mod, int which, cudaStream_t stream);
 

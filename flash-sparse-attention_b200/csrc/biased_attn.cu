@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kPrThreads) biased_prep(const BiasedPrep p) {
             for (int i = done + tid; i < p.plan.max_tiles; i += kPrThreads) p.plan.tiles[i] = make_int4(0, 0, 0, -1);
             __syncthreads();
         }
-        plan_items<kPrThreads>(p.plan);
+        plan_items<kPrThreads, true>(p.plan);
         return;
     }
     const int64_t ctas = gridDim.x - 1, me = (int64_t)(blockIdx.x - 1) * kPrThreads + tid, all = ctas * kPrThreads;
@@ -362,12 +362,36 @@ extern "C" int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, 
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
 }
 
-extern "C" int fsa_biased_attn_bwd_bytes(int64_t N, int64_t Nk, int B, int Hq, int Hk, int D, int64_t* bytes_out) {
+// The same for dQ, one item an SM.  An SM needs about 1 us a K/V tile and 3 an item; uncut, as long as the longest item if that is more than an even share
+// of all.  Cut, the parts' way to memory and back and 5 us of the launch that sums them come on top.  8192 tokens of one head: 41 us with four
+// chunks, 113 uncut; of four sequences of 1000 and four heads 27 with two chunks, 22 uncut.
+struct DqCut {
+    int nchunk = 1;
+    DqCut(const SelShape& s, int window) {
+        if (s.N == 0) return;
+        const int64_t row_tiles = (s.N + s.TPT - 1) / s.TPT, items = (row_tiles > s.B ? row_tiles : s.B) * s.Hk;
+        double longest = (double)(s.Nk / s.B), mean = (double)(s.Nk / s.B - s.N / s.B / 2);
+        if (s.B > 1) longest *= 1.25;           // (the host does not know)
+        if (window >= 0 && longest > (double)window + s.TPT) longest = (double)window + s.TPT;
+        if (mean > longest) mean = longest;
+        longest /= kBiasedBK;
+        const double shared = mean / kBiasedBK * (double)items / sm_count(), each = 3.0 * (double)items / sm_count();
+        double best = 0.0;
+        for (int n = 1; n == 1 || (n <= 64 && (double)n * kBiasedLeast <= longest); n *= 2) {
+            const double part = longest / n + 3.0, all = shared + n * each;
+            const double t = (part > all ? part : all) + (n > 1 ? 5.0 + (double)(s.N * s.Hq * n * s.D * 8) / 5e6 : 0.0);
+            if (n == 1 || t < best) { best = t; nchunk = n; }
+        }
+    }
+    int64_t bytes(const SelShape& s) const { return nchunk > 1 ? s.N * s.Hq * nchunk * s.D * 4 : 0; }
+};
+
+extern "C" int fsa_biased_attn_bwd_bytes(int64_t N, int64_t Nk, int B, int Hq, int Hk, int D, int window, int64_t* bytes_out) {
     SelShape s;
     const int rc = biased_shape(N, Nk, B, Hq, Hk, D, &s);
     if (rc) return rc;
     if (!bytes_out) return FSA_ERR_BAD_ARG;
-    *bytes_out = align_up(N * Hq * 4, 1024) + align_up(range_kv_plan_bytes(s), 1024) + range_kv_slab_bytes(s);
+    *bytes_out = align_up(N * Hq * 4, 1024) + align_up(range_kv_plan_bytes(s), 1024) + align_up(range_kv_slab_bytes(s), 1024) + DqCut(s, window).bytes(s);
     return FSA_OK;
 }
 
@@ -390,7 +414,7 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     if (((uintptr_t)dq & 31) || ((uintptr_t)dk & 31) || ((uintptr_t)dv & 31)) return FSA_ERR_BAD_ARG;
     if ((q_sn % 8) || (q_sh % 8) || (k_sn % 8) || (v_sn % 8) || (do_sn % 8) || (do_sh % 8) || k_sn < (int64_t)Hk * D || v_sn < (int64_t)Hk * D) return FSA_ERR_BAD_ARG;
     int64_t need = 0;
-    if ((rc = fsa_biased_attn_bwd_bytes(N, Nk, B, Hq, Hk, D, &need))) return rc;
+    if ((rc = fsa_biased_attn_bwd_bytes(N, Nk, B, Hq, Hk, D, window, &need))) return rc;
     if (limits_bytes < BiasedLimits::bytes(N) || scratch_bytes < need) return FSA_ERR_WORKSPACE;
     (void)cudaGetLastError();
     if ((rc = ensure_context())) return rc;
@@ -420,7 +444,9 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     plan.multi = plan.tiles + plan.max_tiles;
     plan.items = plan.multi + plan.max_tiles;
     sp += align_up(range_kv_plan_bytes(s), 1024);
-    a.slabs = (float*)sp;
+    a.slabs = (float*)sp;           sp += align_up(range_kv_slab_bytes(s), 1024);
+    float* part = (float*)sp;
+    const DqCut cut(s, window);
     int* status = nullptr;
     cudaError_t e = biased_status_word(&status);
     BiasedPrep prep = {plan, lim, prefix_lens, window, doc_ids != nullptr, o, d_o, do_sn, do_sh, Hq, a.delta, (uint4*)dq, (uint4*)dk, (uint4*)dv};
@@ -429,10 +455,11 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     const bool bf16 = dtype == FSA_DTYPE_BF16;
     if (e == cudaSuccess && D == 128) e = bf16 ? launch_prep<128, __nv_bfloat16>(prep, stream) : launch_prep<128, __half>(prep, stream);
     if (e == cudaSuccess && D == 64) e = bf16 ? launch_prep<64, __nv_bfloat16>(prep, stream) : launch_prep<64, __half>(prep, stream);
-    if (e == cudaSuccess) e = launch_biased_bwd_dq(dtype, a, s, kmap, vmap, status, mod, which, stream);
+    if (e == cudaSuccess) e = launch_biased_bwd_dq(dtype, a, s, kmap, vmap, status, mod, which, cut.nchunk, part, stream);
     if (e == cudaSuccess) e = launch_biased_bwd_dkdv(dtype, plan, a, s, kmap, vmap, status, mod, which, stream);
     // (no stretch of so few row tiles is cut)
     if (e == cudaSuccess && N > (int64_t)kRkMinTiles * s.TPT) e = launch_range_dkdv_reduce(dtype, plan, a.slabs, dk, dv, sm_count(), stream);
+    if (e == cudaSuccess && cut.nchunk > 1) e = launch_biased_dq_sum(dtype, part, a, s, cut.nchunk, stream);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
 }
 

@@ -123,7 +123,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                 bool ok = true;
                 int u = 0, qi = 0;             // Q / dO tiles and non-empty items so far
                 const uint32_t unit_bytes = (uint32_t)(KH * 128 * TPT * p.G);
-                for (int w = blockIdx.x; w < nitems && ok; w += gridDim.x) {
+                for (int round = 0, w; (w = forth_and_back(round)) < nitems && ok; ++round) {
                     const BkItem m = bk_item(p.plan, w);
                     if (m.n == 0) continue;
                     auto load_unit = [&](const CUtensorMap* map, int tok) {
@@ -194,7 +194,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                 }
                 __syncwarp();
             };
-            for (int w = blockIdx.x; w < nitems && ok; w += gridDim.x) {
+            for (int round = 0, w; (w = forth_and_back(round)) < nitems && ok; ++round) {
                 const BkItem m = bk_item(p.plan, w);
                 if (m.n == 0) continue;
                 ok = ok && mbar_wait(kv_full, qi & 1, status);
@@ -233,7 +233,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
             int g[4], e[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) { g[j] = (lane + 32 * j) / TPT; e[j] = lane + 32 * j - g[j] * TPT; }
-            for (int w = blockIdx.x; w < nitems && warp_stays(ok); w += gridDim.x) {
+            for (int round = 0, w; (w = forth_and_back(round)) < nitems && warp_stays(ok); ++round) {
                 const BkItem m = bk_item(p.plan, w);
                 float slope[4] = {0.f, 0.f, 0.f, 0.f};
                 int far = 0;            // from the item's first key to its first token's place
@@ -301,7 +301,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
         const int q_col = r0 + 4 * (lane & 7), q_g = min(q_col / TPT, p.G - 1), q_e = q_col - q_col / TPT * TPT;
         bool ok = true;
         int c = 0, qi = 0;
-        for (int w = blockIdx.x; w < nitems && warp_stays(ok); w += gridDim.x) {
+        for (int round = 0, w; (w = forth_and_back(round)) < nitems && warp_stays(ok); ++round) {
             const BkItem m = bk_item(p.plan, w);
             const float q_slope = (MOD & kModBias) ? __ldg(p.mod.slopes + m.h * p.G + q_g) * kLog2e : 0.f;
             // with keys behind a token's place: place of this K/V row before (negative) or behind the item's first token

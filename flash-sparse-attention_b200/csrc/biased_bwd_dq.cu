@@ -30,6 +30,8 @@ struct BiasedDqParams {
     const float* lse;       // [Hq, N] log2 units
     const float* delta;     // [Hq, N] sum_d o dO
     void* dq;               // [N, Hq, D] contiguous
+    int nchunk;             // the K/V tiles of an item are cut into so many chunks, whose dQ go to part, unless there is only one
+    float* part;            // [N, Hq, nchunk, D]
     int* status;
     ScoreMod mod;
 };
@@ -44,12 +46,14 @@ constexpr uint32_t kBqTileClocks = 4096;
 static_assert(kMaxTokens / kBiasedBK * kBqTileClocks + FSA_WAIT_CLOCKS < (int64_t)1 << 32, "the counter comes round");
 
 struct BqItem {
-    int seq, tok0, ne, row_lo, nblk, h, row_hi;
+    int seq, tok0, ne, row_lo, nblk, h, row_hi, z;     // z: chunk
 };
 
-// Work item w of the list.  All 32 lanes call it and get the same answer.
+// Work item w of the list.  (Chunks of equal size, kBiasedLeast tiles at least; the last ones may be empty.)  All 32 lanes call it and get the same answer.
 __device__ __forceinline__ BqItem bq_item(const BiasedDqParams& p, int w, int lane) {
     BqItem m;
+    m.z = w % p.nchunk;
+    w /= p.nchunk;
     m.h = w % p.Hk;
     m.row_lo = 0; m.nblk = 0; m.row_hi = -1;
     find_ranked_tile(p.cu_q, p.cu_k, p.B, p.TPT, w / p.Hk, lane, m.seq, m.tok0, m.ne);
@@ -62,6 +66,12 @@ __device__ __forceinline__ BqItem bq_item(const BiasedDqParams& p, int w, int la
     m.row_lo = max(__reduce_min_sync(0xffffffffu, lo), 0);
     m.row_hi = min(__reduce_max_sync(0xffffffffu, hi), (int)p.Nk - 1);
     m.nblk = m.row_hi >= m.row_lo ? (m.row_hi - m.row_lo) / kBiasedBK + 1 : 0;
+    if (p.nchunk > 1) {
+        const int size = max(kBiasedLeast, (m.nblk + p.nchunk - 1) / p.nchunk), first = min(m.z * size, m.nblk);
+        m.nblk = min(size, m.nblk - first);
+        m.row_lo += first * kBiasedBK;
+        m.row_hi = min(m.row_hi, m.row_lo + m.nblk * kBiasedBK - 1);
+    }
     return m;
 }
 
@@ -116,7 +126,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
     tc_fence_after();
     const uint32_t tbase = tmem_slot;
     let_next_start();
-    const int nitems = count_seq_tiles<true>(p.cu_q, p.B, p.TPT, lane) * p.Hk;
+    const int nitems = count_seq_tiles<true>(p.cu_q, p.B, p.TPT, lane) * p.Hk * p.nchunk;
     // Entry n of this CTA's items: every warp but the one that fills the ring takes each of them once, in order.
     auto take_item = [&](int n, bool& ok) {
         ok = ok && mbar_wait(&it_full[n % kBqItems], (n / kBqItems) & 1, status);
@@ -124,7 +134,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
         ok = warp_ok(ok);
         if (lane == 0) mbar_arrive(&it_empty[n % kBqItems]);
         BqItem m;
-        m.seq = x.x; m.tok0 = x.y; m.ne = x.z; m.row_lo = x.w; m.nblk = y.x; m.h = y.y; m.row_hi = y.z;
+        m.seq = x.x; m.tok0 = x.y; m.ne = x.z; m.row_lo = x.w; m.nblk = y.x; m.h = y.y; m.row_hi = y.z; m.z = y.w;
         if (!ok) m.ne = m.nblk = 0;
         return m;
     };
@@ -135,14 +145,14 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
             // -------------------------------------------------------------- items
             bool ok = true;
             int n = 0, longest = 0;
-            for (int w = blockIdx.x; w < nitems && ok; w += gridDim.x, ++n) {
+            for (int w; (w = forth_and_back(n)) < nitems && ok; ++n) {
                 const BqItem m = bq_item(p, w, lane);
                 ok = ok && mbar_wait(&it_empty[n % kBqItems], ((n / kBqItems) & 1) ^ 1, status, FSA_WAIT_CLOCKS + longest * kBqTileClocks);
                 ok = warp_ok(ok);
                 longest = max(longest, m.nblk);
                 if (ok && lane == 0) {
                     s_item[(n % kBqItems) * 2] = make_int4(m.seq, m.tok0, m.ne, m.row_lo);
-                    s_item[(n % kBqItems) * 2 + 1] = make_int4(m.nblk, m.h, m.row_hi, 0);
+                    s_item[(n % kBqItems) * 2 + 1] = make_int4(m.nblk, m.h, m.row_hi, m.z);
                     mbar_arrive(&it_full[n % kBqItems]);
                 }
             }
@@ -150,7 +160,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
             // -------------------------------------------------------------- TMA producer
             bool ok = true;
             int kvc = 0, qi = 0, n = 0;    // K/V tiles and non-empty items so far
-            for (int w = blockIdx.x; w < nitems && ok; w += gridDim.x, ++n) {
+            for (; forth_and_back(n) < nitems && ok; ++n) {
                 const BqItem m = take_item(n, ok);
                 if (m.nblk == 0) continue;
                 if (lane == 0) {
@@ -197,7 +207,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
             const uint32_t k_mn_lo = umma_desc_lo(smem_u32(sKV), BK * 128);
             bool ok = true;
             int c = 0, qi = 0, n = 0;
-            for (int w = blockIdx.x; w < nitems && ok; w += gridDim.x, ++n) {
+            for (; forth_and_back(n) < nitems && ok; ++n) {
                 const BqItem m = take_item(n, ok);
                 if (m.nblk == 0) continue;
                 if (warp == 1) {
@@ -311,12 +321,12 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
         BqItem m;
         m.nblk = m.ne = 0;
         int n = 0;
-        if ((int)blockIdx.x < nitems) {
+        if (forth_and_back(0) < nitems) {
             m = take_item(n, ok);
             if (m.nblk > 0) take_row();
         }
         Row row = load_numbers(m);
-        for (int w = blockIdx.x; w < nitems && warp_stays(ok); w += gridDim.x) {
+        while (forth_and_back(n) < nitems && warp_stays(ok)) {
             const bool row_valid = g < p.G && e < m.ne;
             const int tok = m.tok0 + e;
             const int lo_r = row.lo;
@@ -326,7 +336,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
             if (!(lse_r > -INFINITY)) hi_r = lo_r - 1;          // a row that saw nothing in the forward sees nothing here
             BqItem next;
             next.nblk = next.ne = 0;
-            if (w + (int)gridDim.x < nitems) next = take_item(++n, ok);
+            if (forth_and_back(++n) < nitems) next = take_item(n, ok);
             row = load_numbers(next);
             const int c0 = c;
             c += m.nblk;
@@ -440,24 +450,32 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
             }
             if (!warp_stays(ok)) break;
             constexpr int kOwn = D / 4;
-            ET* drow = reinterpret_cast<ET*>(p.dq) + ((int64_t)tok * p.Hq + (m.h * p.G + g)) * D + grp * kOwn;
-            uint32_t x[kOwn / 2];
+            const int64_t drow = (int64_t)tok * p.Hq + (m.h * p.G + g);
+            uint32_t a[kOwn];
             if (m.nblk > 0) {
-                uint32_t a[kOwn];
                 if constexpr (D == 128) tmem_ld32(tbase + lane_off + cDQ + grp * kOwn, a);
                 else tmem_ld16(tbase + lane_off + cDQ + grp * kOwn, a);
                 tmem_ld_wait();
                 tc_fence_before();
                 mbar_arrive(dq_free);            // the accumulator may take the next item
-#pragma unroll
-                for (int i = 0; i < kOwn / 2; ++i) x[i] = ElemTraits<ET>::pack2(__uint_as_float(a[2 * i]), __uint_as_float(a[2 * i + 1]));
             } else {
 #pragma unroll
-                for (int i = 0; i < kOwn / 2; ++i) x[i] = 0u;
+                for (int i = 0; i < kOwn; ++i) a[i] = 0u;
             }
-            if (row_valid) {
+            if (p.nchunk > 1) {
+                float* dst = p.part + (drow * p.nchunk + m.z) * D + grp * kOwn;
+                if (row_valid)
 #pragma unroll
-                for (int i = 0; i < kOwn; i += 16) st_global32(drow + i, &x[i / 2]);
+                    for (int i = 0; i < kOwn; i += 8) st_global32(dst + i, &a[i]);
+            } else if (row_valid) {
+                ET* dst = reinterpret_cast<ET*>(p.dq) + drow * D + grp * kOwn;
+#pragma unroll
+                for (int i = 0; i < kOwn; i += 16) {
+                    uint32_t x[8];
+#pragma unroll
+                    for (int j = 0; j < 8; ++j) x[j] = ElemTraits<ET>::pack2(__uint_as_float(a[i + 2 * j]), __uint_as_float(a[i + 2 * j + 1]));
+                    st_global32(dst + i, x);
+                }
             }
             m = next;
         }
@@ -465,6 +483,40 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
     tc_fence_before();
     __syncthreads();
     if (warp == 0) tmem_dealloc(tbase, kCols);
+}
+
+// dQ of the tokens of the sequences: the sum of the chunks in order, rounded once.  A thread has 8 columns of a row; bound by memory.
+constexpr int kDsThreads = 256;
+template <int D, typename ET>
+__global__ void __launch_bounds__(kDsThreads) biased_dq_sum(const float* part, const int32_t* cu_q, int B, int64_t rows, int Hq, int nchunk, ET* __restrict__ dq) {
+    constexpr int L = D / 8;
+    const int64_t i = (int64_t)blockIdx.x * kDsThreads + threadIdx.x, row = i / L;
+    follow();
+    if (row >= rows) return;
+    const int tok = (int)((uint32_t)row / (uint32_t)Hq);
+    if (tok < __ldcg(cu_q) || tok >= __ldcg(cu_q + B)) return;      // (the row is cleared)
+    const float* src = part + row * nchunk * D + i % L * 8;
+    float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
+#pragma unroll 4
+    for (int z = 0; z < nchunk; ++z) {
+        const float4 x = __ldcg(reinterpret_cast<const float4*>(src + z * D)), y = __ldcg(reinterpret_cast<const float4*>(src + z * D + 4));
+        acc[0] += x.x; acc[1] += x.y; acc[2] += x.z; acc[3] += x.w;
+        acc[4] += y.x; acc[5] += y.y; acc[6] += y.z; acc[7] += y.w;
+    }
+    *reinterpret_cast<uint4*>(dq + i * 8) = make_uint4(ElemTraits<ET>::pack2(acc[0], acc[1]), ElemTraits<ET>::pack2(acc[2], acc[3]),
+                                                       ElemTraits<ET>::pack2(acc[4], acc[5]), ElemTraits<ET>::pack2(acc[6], acc[7]));
+}
+
+template <int D, typename ET>
+static cudaError_t launch_sum(const float* part, const SelBwdArgs& a, const SelShape& s, int nchunk, cudaStream_t stream) {
+    const int64_t rows = s.N * s.Hq, blocks = (rows * (D / 8) + kDsThreads - 1) / kDsThreads;
+    return launch_dependent(biased_dq_sum<D, ET>, dim3((unsigned)blocks), kDsThreads, 0, stream, 1, part, a.cu, s.B, rows, s.Hq, nchunk, (ET*)a.dq);
+}
+
+cudaError_t launch_biased_dq_sum(int dtype, const float* part, const SelBwdArgs& a, const SelShape& s, int nchunk, cudaStream_t stream) {
+    const bool bf16 = dtype == kBF16;
+    if (s.D == 128) return bf16 ? launch_sum<128, __nv_bfloat16>(part, a, s, nchunk, stream) : launch_sum<128, __half>(part, a, s, nchunk, stream);
+    return bf16 ? launch_sum<64, __nv_bfloat16>(part, a, s, nchunk, stream) : launch_sum<64, __half>(part, a, s, nchunk, stream);
 }
 
 template <int D, int MOD, typename ET>
@@ -487,7 +539,7 @@ static cudaError_t launch_bq_which(int which, const BiasedDqParams& p, const CUt
 }
 
 cudaError_t launch_biased_bwd_dq(int dtype, const SelBwdArgs& a, const SelShape& s, const CUtensorMap& kmap, const CUtensorMap& vmap, int* status,
-                                 const ScoreMod& mod, int which, cudaStream_t stream) {
+                                 const ScoreMod& mod, int which, int nchunk, float* part, cudaStream_t stream) {
     CUtensorMap maps[4];        // Q, dO, K, V
     if (make_tile_map_3d_box(&maps[0], a.q, dtype, s.D, s.N, s.Hq, a.q_sn, a.q_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
     if (make_tile_map_3d_box(&maps[1], a.d_o, dtype, s.D, s.N, s.Hq, a.do_sn, a.do_sh, s.TPT, s.G)) return cudaErrorInvalidValue;
@@ -498,7 +550,9 @@ cudaError_t launch_biased_bwd_dq(int dtype, const SelBwdArgs& a, const SelShape&
     p.scale = a.sm_scale; p.scale_log2 = a.sm_scale * kLog2e;
     p.lse = a.lse; p.delta = a.delta; p.dq = a.dq; p.status = status;
     p.mod = mod;
-    const int64_t max_items = ((s.N + s.TPT - 1) / s.TPT + s.B) * (int64_t)s.Hk;
+    p.nchunk = nchunk; p.part = part;
+    const int64_t max_items = ((s.N + s.TPT - 1) / s.TPT + s.B) * (int64_t)s.Hk * nchunk;
+    if (max_items >= (int64_t)1 << 30) return cudaErrorInvalidValue;
     int sms = 0;
     if (device_sm_count(&sms) != 0 || sms <= 0) return cudaErrorInvalidValue;
     const unsigned grid = (unsigned)(max_items < sms ? max_items : sms);

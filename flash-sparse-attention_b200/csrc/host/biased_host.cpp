@@ -112,7 +112,7 @@ static std::tuple<Tensor, Tensor, Tensor> biased_bwd(const Tensor& q_, const Ten
     const Rows3 q(q_, false), k(k_, true), v(v_, true), dout(do_, false);
     int64_t nb = 0;
     const int B = (int)a.cu_q.size(0) - 1;
-    check(fsa_biased_attn_bwd_bytes(N, Nk, B, (int)Hq, (int)Hk, (int)D, &nb), "fsa_biased_attn_bwd_bytes");
+    check(fsa_biased_attn_bwd_bytes(N, Nk, B, (int)Hq, (int)Hk, (int)D, (int)a.window, &nb), "fsa_biased_attn_bwd_bytes");
     const Tensor scratch = bytes(nb, q_);
     Tensor dq = fresh({N, Hq, D}, q_), dk = fresh({Nk, Hk, D}, q_), dv = fresh_like(dk);
     check(fsa_biased_attn_bwd(ptr(q.t), ptr(k.t), ptr(v.t), ptr(o), lse.data_ptr<float>(), ptr(dout.t), iptr(a.cu_q), iptr(a.cu_k), iptr(a.docs),

@@ -34,8 +34,8 @@ inline int64_t range_kv_slab_bytes(const SelShape& s) { return range_kv_max_cut(
 
 // Work items from the stretches (one CTA of T threads): a tile of n row tiles becomes ceil(n / C) items of about equal length, C the
 // smallest length that leaves about p.aim items (times heads), and at least kRkMinTiles: below that an item's epilogue weighs
-// more than an idle SM.
-template <int T>
+// more than an idle SM.  SORT: longest items first, in 64 steps of length (in a step in no order; nothing that is computed depends on it).
+template <int T, bool SORT>
 __device__ __forceinline__ void plan_items(const RangeKvPlan& p) {
     __shared__ int wa[32], wb[32], wc[32];      // (of the T / 32 warps)
     __shared__ long long total;
@@ -49,12 +49,37 @@ __device__ __forceinline__ void plan_items(const RangeKvPlan& p) {
     if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&total), (unsigned long long)mine);
     __syncthreads();
     const int C = max(kRkMinTiles, (int)((total * p.Hk + p.aim - 1) / p.aim));
+    auto pieces = [&](const int4& t, int n) { return t.y > 0 ? max(1, (n + C - 1) / C) : 0; };
+    auto step = [&](int n, int nch) { return 63 - (int)((int64_t)((n + nch - 1) / nch) * 63 / C); };
+    __shared__ int place[64];                         // SORT: where the next item of this length goes
+    if constexpr (SORT) {
+        if (tid < 64) place[tid] = 0;
+        __syncthreads();
+        for (int i = tid; i < p.max_tiles; i += T) {
+            const int4 t = p.tiles[i];
+            const int n = row_tiles(t), nch = pieces(t, n);
+            if (nch) atomicAdd(&place[step(n, nch)], nch);
+        }
+        __syncthreads();
+        if (warp == 0) {
+            const int a = place[2 * lane], b = place[2 * lane + 1];
+            int incl = a + b;
+#pragma unroll
+            for (int d = 1; d < 32; d <<= 1) {
+                const int up = __shfl_up_sync(0xffffffffu, incl, d);
+                if (lane >= d) incl += up;
+            }
+            place[2 * lane] = incl - a - b;
+            place[2 * lane + 1] = incl - b;
+        }
+        __syncthreads();
+    }
     int items = 0, slabs = 0, multi = 0;              // so far
     for (int base = 0; base < p.max_tiles; base += T) {
         const int i = base + tid;
         const int4 t = i < p.max_tiles ? p.tiles[i] : make_int4(0, 0, 0, -1);
         const int n = row_tiles(t);
-        const int nch = t.y > 0 ? max(1, (n + C - 1) / C) : 0;
+        const int nch = pieces(t, n);
         const int a = nch, b = nch > 1 ? nch : 0, c = nch > 1;
         int sa = a, sb = b, sc = c;
 #pragma unroll
@@ -65,7 +90,8 @@ __device__ __forceinline__ void plan_items(const RangeKvPlan& p) {
         if (lane == 31) { wa[warp] = sa; wb[warp] = sb; wc[warp] = sc; }
         __syncthreads();
         const int va = lane < T / 32 ? wa[lane] : 0, vb = lane < T / 32 ? wb[lane] : 0, vc = lane < T / 32 ? wc[lane] : 0;
-        const int first = items + __reduce_add_sync(0xffffffffu, lane < warp ? va : 0) + sa - a;
+        int first = items + __reduce_add_sync(0xffffffffu, lane < warp ? va : 0) + sa - a;
+        if (SORT && nch) first = atomicAdd(&place[step(n, nch)], nch);
         const int slab = slabs + __reduce_add_sync(0xffffffffu, lane < warp ? vb : 0) + sb - b;
         const int list = multi + __reduce_add_sync(0xffffffffu, lane < warp ? vc : 0) + sc - c;
         for (int j = 0; j < nch; ++j) {

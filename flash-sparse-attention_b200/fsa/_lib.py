@@ -82,7 +82,7 @@ SIGNATURES = {
         [c_void_p] * 8 + [c_int64] * 2 + [c_int] * 5 + [c_int64] * 4 + [c_float] * 2 + [c_int] + [c_void_p] * 3
         + [c_int64, c_void_p, c_int64, c_void_p]),
     "fsa_biased_attn_fwd_bytes": (c_int, [c_int64] * 2 + [c_int] * 5 + [POINTER(c_int64)]),
-    "fsa_biased_attn_bwd_bytes": (c_int, [c_int64] * 2 + [c_int] * 4 + [POINTER(c_int64)]),
+    "fsa_biased_attn_bwd_bytes": (c_int, [c_int64] * 2 + [c_int] * 5 + [POINTER(c_int64)]),
     "fsa_biased_attn_bwd": (
         c_int,
         [c_void_p] * 11 + [c_int64] * 2 + [c_int] * 5 + [c_int64] * 6 + [c_float] * 2 + [c_int] + [c_void_p] * 4

@@ -239,7 +239,8 @@ int fsa_biased_decode(const void* q, const void* k, const void* v, int64_t kv_ro
 /* What the waits of these operators' kernels left on the current device: 0, or that one ran out (synchronises). */
 int fsa_biased_read_status(int* status_out);
 /* fsa_biased_attn_fwd's gradient.  dq, dk, dv contiguous; every row of them is written.  limits: what the forward left.  Bit-reproducible. */
-int fsa_biased_attn_bwd_bytes(int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads, int head_dim, int64_t* bytes_out);
+int fsa_biased_attn_bwd_bytes(int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window,
+                              int64_t* bytes_out);
 int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens_q,
                         const int32_t* cu_seqlens_k, const int32_t* doc_ids, const int32_t* prefix_lens, const float* slopes, int64_t total_tokens, int64_t total_kv_rows,
                         int batch, int num_q_heads, int num_kv_heads, int head_dim, int dtype, int64_t q_stride_n, int64_t q_stride_h, int64_t k_stride_n,

@@ -34,6 +34,10 @@ def roomy(got, ref, off, name):
     (8, 2, 128, None, False, {"window": 700}),
     (4, 2, 128, 50.0, True, {"docs": 900}),
     (4, 1, 64, 20.0, True, {"prefix": 2500}),
+    (1, 1, 128, 30.0, True, {}),                      # one head: o and dQ cut along the keys
+    (1, 2, 64, None, False, {}),
+    (1, 1, 64, 20.0, False, {"docs": 3500}),
+    (1, 1, 128, None, True, {"window": 2900}),
 ])
 def test_long(Hk, G, d, cap, alibi, how):
     N, Hq = 6000, Hk * G

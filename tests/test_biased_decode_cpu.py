@@ -85,5 +85,5 @@ def test_workspace_holds_the_partials_and_no_more_than_it_has_to():
     assert L.fsa_biased_decode_bytes(1, 3, 2, 128, 0, 1, 0, -1, byref(n)) == _lib.FSA_ERR_BAD_ARG
     assert L.fsa_biased_decode_bytes(1, 4, 2, 256, 0, 1, 0, -1, byref(n)) == _lib.FSA_ERR_UNSUPPORTED
     assert L.fsa_biased_decode_bytes(1, 66, 2, 128, 0, 1, 0, -1, byref(n)) == _lib.FSA_ERR_UNSUPPORTED
-    assert L.fsa_biased_attn_bwd_bytes(10, 10, 0, 4, 2, 128, byref(n)) == _lib.FSA_ERR_BAD_ARG
-    assert L.fsa_biased_attn_bwd_bytes(1 << 25, 10, 1, 4, 2, 128, byref(n)) == _lib.FSA_ERR_UNSUPPORTED
+    assert L.fsa_biased_attn_bwd_bytes(10, 10, 0, 4, 2, 128, -1, byref(n)) == _lib.FSA_ERR_BAD_ARG
+    assert L.fsa_biased_attn_bwd_bytes(1 << 25, 10, 1, 4, 2, 128, -1, byref(n)) == _lib.FSA_ERR_UNSUPPORTED
