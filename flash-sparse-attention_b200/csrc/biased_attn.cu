@@ -189,7 +189,7 @@ __global__ void __launch_bounds__(kPrThreads) biased_prep(const BiasedPrep p) {
             for (int i = done + tid; i < p.plan.max_tiles; i += kPrThreads) p.plan.tiles[i] = make_int4(0, 0, 0, -1);
             __syncthreads();
         }
-        plan_items<kPrThreads, true>(p.plan);
+        plan_items<kPrThreads>(p.plan);
         return;
     }
     const int64_t ctas = gridDim.x - 1, me = (int64_t)(blockIdx.x - 1) * kPrThreads + tid, all = ctas * kPrThreads;

@@ -88,6 +88,9 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
     uint64_t* p_read = s_full + 12;     // [2 halves] dV(i) has read P
     uint64_t* ds_read = s_full + 14;    // [2] dK(i) has read dS
     uint32_t& tmem_slot = *reinterpret_cast<uint32_t*>(s_full + 16);
+    uint64_t* it_full = s_full + 18;    // [2] the next item is known
+    uint64_t* it_empty = s_full + 20;   // [2] ... has been taken by the 19 other warps
+    int* s_it = reinterpret_cast<int*>(s_full + 22);                      // [2] its place in the list, -1: there are no more
     int* s_masked = reinterpret_cast<int*>(s_full + 16) + 2;              // [2] some row of the tile does not see all K/V rows; 2: or sees none
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -100,6 +103,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
             mbar_init(&s_full[i], 1); mbar_init(&p_full[i], 256); mbar_init(&dp_full[i], 1); mbar_init(&ds_full[i], 256);
             mbar_init(&p_read[i], 1); mbar_init(&ds_read[i], 1);
         }
+        for (int i = 0; i < 2; ++i) { mbar_init(&it_full[i], 1); mbar_init(&it_empty[i], kBkThreads / 32 - 1); }
         mbar_init(dv_done, 1); mbar_init(dk_done, 1); mbar_init(dv_free, 256); mbar_init(dk_free, 256);
         mbar_init_fence();
     }
@@ -114,6 +118,14 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
     const uint32_t tbase = tmem_slot;
     const int nitems = __ldg(p.plan.counts) * p.plan.Hk;
     const int TPT = p.plan.TPT;
+    // Item n of this CTA: every warp but the producer's takes each of them once, in order; below 0 ends the list.
+    auto take_item = [&](int n, bool& ok) {
+        ok = ok && mbar_wait(&it_full[n & 1], (n >> 1) & 1, status);
+        const int w = s_it[n & 1];
+        ok = warp_ok(ok);
+        if (lane == 0) mbar_arrive(&it_empty[n & 1]);
+        return ok ? w : -1;
+    };
 
     if (warp < 4) {
         reg_dec<64>();
@@ -123,7 +135,15 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                 bool ok = true;
                 int u = 0, qi = 0;             // Q / dO tiles and non-empty items so far
                 const uint32_t unit_bytes = (uint32_t)(KH * 128 * TPT * p.G);
-                for (int round = 0, w; (w = forth_and_back(round)) < nitems && ok; ++round) {
+                for (int n = 0;; ++n) {
+                    // the next item that nobody has: CTAs that start late, where a dQ CTA was at work, take fewer (every CTA its share of the list
+                    // beforehand: 641 us instead of 628 for a pass over 2 x 4096 tokens of documents; longest first: 655, their Q and dO meet less in L2)
+                    const int w = atomicAdd(p.plan.counts + 2, 1);
+                    ok = ok && mbar_wait(&it_empty[n & 1], ((n >> 1) & 1) ^ 1, status);
+                    if (!ok) break;
+                    s_it[n & 1] = w < nitems ? w : -1;
+                    mbar_arrive(&it_full[n & 1]);
+                    if (w >= nitems) break;
                     const BkItem m = bk_item(p.plan, w);
                     if (m.n == 0) continue;
                     auto load_unit = [&](const CUtensorMap* map, int tok) {
@@ -194,7 +214,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                 }
                 __syncwarp();
             };
-            for (int round = 0, w; (w = forth_and_back(round)) < nitems && ok; ++round) {
+            for (int n = 0, w; (w = take_item(n, ok)) >= 0; ++n) {
                 const BkItem m = bk_item(p.plan, w);
                 if (m.n == 0) continue;
                 ok = ok && mbar_wait(kv_full, qi & 1, status);
@@ -233,7 +253,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
             int g[4], e[4];
 #pragma unroll
             for (int j = 0; j < 4; ++j) { g[j] = (lane + 32 * j) / TPT; e[j] = lane + 32 * j - g[j] * TPT; }
-            for (int round = 0, w; (w = forth_and_back(round)) < nitems && warp_stays(ok); ++round) {
+            for (int n = 0, w; (w = take_item(n, ok)) >= 0 && warp_stays(ok); ++n) {
                 const BkItem m = bk_item(p.plan, w);
                 float slope[4] = {0.f, 0.f, 0.f, 0.f};
                 int far = 0;            // from the item's first key to its first token's place
@@ -301,7 +321,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
         const int q_col = r0 + 4 * (lane & 7), q_g = min(q_col / TPT, p.G - 1), q_e = q_col - q_col / TPT * TPT;
         bool ok = true;
         int c = 0, qi = 0;
-        for (int round = 0, w; (w = forth_and_back(round)) < nitems && warp_stays(ok); ++round) {
+        for (int n = 0, w; (w = take_item(n, ok)) >= 0 && warp_stays(ok); ++n) {
             const BkItem m = bk_item(p.plan, w);
             const float q_slope = (MOD & kModBias) ? __ldg(p.mod.slopes + m.h * p.G + q_g) * kLog2e : 0.f;
             // with keys behind a token's place: place of this K/V row before (negative) or behind the item's first token

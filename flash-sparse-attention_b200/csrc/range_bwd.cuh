@@ -16,7 +16,7 @@ struct RangeKvPlan {
     int B, Hk, TPT, max_tiles;
     int D;
     int aim;            // range_kv_items()
-    int* counts;        // [0] items, [1] tiles cut into several items
+    int* counts;        // [0] items, [1] tiles cut into several items, [2] items that have been taken (biased_bwd_dkdv.cu)
     int4* tiles;        // [max_tiles] first K/V row, rows, first and last token that see one of them
     int4* items;        // tile, first row tile of its stretch, row tiles, slab (-1: written in place)
     int4* multi;        // first K/V row, rows, first slab, slabs
@@ -34,8 +34,8 @@ inline int64_t range_kv_slab_bytes(const SelShape& s) { return range_kv_max_cut(
 
 // Work items from the stretches (one CTA of T threads): a tile of n row tiles becomes ceil(n / C) items of about equal length, C the
 // smallest length that leaves about p.aim items (times heads), and at least kRkMinTiles: below that an item's epilogue weighs
-// more than an idle SM.  SORT: longest items first, in 64 steps of length (in a step in no order; nothing that is computed depends on it).
-template <int T, bool SORT>
+// more than an idle SM.
+template <int T>
 __device__ __forceinline__ void plan_items(const RangeKvPlan& p) {
     __shared__ int wa[32], wb[32], wc[32];      // (of the T / 32 warps)
     __shared__ long long total;
@@ -49,37 +49,12 @@ __device__ __forceinline__ void plan_items(const RangeKvPlan& p) {
     if (lane == 0) atomicAdd(reinterpret_cast<unsigned long long*>(&total), (unsigned long long)mine);
     __syncthreads();
     const int C = max(kRkMinTiles, (int)((total * p.Hk + p.aim - 1) / p.aim));
-    auto pieces = [&](const int4& t, int n) { return t.y > 0 ? max(1, (n + C - 1) / C) : 0; };
-    auto step = [&](int n, int nch) { return 63 - (int)((int64_t)((n + nch - 1) / nch) * 63 / C); };
-    __shared__ int place[64];                         // SORT: where the next item of this length goes
-    if constexpr (SORT) {
-        if (tid < 64) place[tid] = 0;
-        __syncthreads();
-        for (int i = tid; i < p.max_tiles; i += T) {
-            const int4 t = p.tiles[i];
-            const int n = row_tiles(t), nch = pieces(t, n);
-            if (nch) atomicAdd(&place[step(n, nch)], nch);
-        }
-        __syncthreads();
-        if (warp == 0) {
-            const int a = place[2 * lane], b = place[2 * lane + 1];
-            int incl = a + b;
-#pragma unroll
-            for (int d = 1; d < 32; d <<= 1) {
-                const int up = __shfl_up_sync(0xffffffffu, incl, d);
-                if (lane >= d) incl += up;
-            }
-            place[2 * lane] = incl - a - b;
-            place[2 * lane + 1] = incl - b;
-        }
-        __syncthreads();
-    }
     int items = 0, slabs = 0, multi = 0;              // so far
     for (int base = 0; base < p.max_tiles; base += T) {
         const int i = base + tid;
         const int4 t = i < p.max_tiles ? p.tiles[i] : make_int4(0, 0, 0, -1);
         const int n = row_tiles(t);
-        const int nch = pieces(t, n);
+        const int nch = t.y > 0 ? max(1, (n + C - 1) / C) : 0;
         const int a = nch, b = nch > 1 ? nch : 0, c = nch > 1;
         int sa = a, sb = b, sc = c;
 #pragma unroll
@@ -90,8 +65,7 @@ __device__ __forceinline__ void plan_items(const RangeKvPlan& p) {
         if (lane == 31) { wa[warp] = sa; wb[warp] = sb; wc[warp] = sc; }
         __syncthreads();
         const int va = lane < T / 32 ? wa[lane] : 0, vb = lane < T / 32 ? wb[lane] : 0, vc = lane < T / 32 ? wc[lane] : 0;
-        int first = items + __reduce_add_sync(0xffffffffu, lane < warp ? va : 0) + sa - a;
-        if (SORT && nch) first = atomicAdd(&place[step(n, nch)], nch);
+        const int first = items + __reduce_add_sync(0xffffffffu, lane < warp ? va : 0) + sa - a;
         const int slab = slabs + __reduce_add_sync(0xffffffffu, lane < warp ? vb : 0) + sb - b;
         const int list = multi + __reduce_add_sync(0xffffffffu, lane < warp ? vc : 0) + sc - c;
         for (int j = 0; j < nch; ++j) {
@@ -104,7 +78,7 @@ __device__ __forceinline__ void plan_items(const RangeKvPlan& p) {
         multi += __reduce_add_sync(0xffffffffu, vc);
         __syncthreads();
     }
-    if (tid == 0) { p.counts[0] = items; p.counts[1] = multi; }
+    if (tid == 0) { p.counts[0] = items; p.counts[1] = multi; p.counts[2] = 0; }
 }
 
 cudaError_t launch_range_bwd_plan(const RangeKvPlan& p, const SelBwdArgs& a, int* status, cudaStream_t stream);

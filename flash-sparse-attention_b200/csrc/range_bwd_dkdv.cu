@@ -88,7 +88,7 @@ __global__ void __launch_bounds__(512) range_key_tiles(const RangeKvPlan p, uint
 
 __global__ void __launch_bounds__(1024) range_plan_items(const RangeKvPlan p) {
     follow();
-    plan_items<1024, false>(p);
+    plan_items<1024>(p);
 }
 
 // dk / dv rows of the K/V tiles that were cut: the sum of the slabs in order.  Slab: [dV, dK][column / 4][row] float4.
