@@ -126,7 +126,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
     tc_fence_after();
     const uint32_t tbase = tmem_slot;
     let_next_start();
-    const int nitems = count_seq_tiles<true>(p.cu_q, p.B, p.TPT, lane) * p.Hk * p.nchunk;
+    const int nitems = count_ranked_tiles(p.cu_q, p.B, p.TPT, lane) * p.Hk * p.nchunk;
     // Entry n of this CTA's items: every warp but the one that fills the ring takes each of them once, in order.
     auto take_item = [&](int n, bool& ok) {
         ok = ok && mbar_wait(&it_full[n % kBqItems], (n / kBqItems) & 1, status);

@@ -408,7 +408,7 @@ struct DecodeCut {
         tiles = nshared = mtiles = 0;
         if (groups > 0) {
             // (a group's last tile has one sequence at least; a place in the grid that no tile takes would hold up one that does)
-            mtiles = B > groups ? (B - groups) / TPT + groups : B > 0 ? B : 1;
+            mtiles = groups > kRankedSeqs ? B / TPT + groups : B > groups ? (B - groups) / TPT + groups : B > 0 ? B : 1;
             const int64_t blocks = max_shared < 1 ? 1 : (max_shared + kBiasedBK - 1) / kBiasedBK;
             int64_t n = 2 * sms / ((int64_t)mtiles * Hk);
             if (n < 1) n = 1;

@@ -206,7 +206,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                 }
                 c += nblk;
                 qi += nblk > 0;
-            } else if constexpr (!kSplit) {
+            } else if (!kSplit && ne == 0) {
                 // There are max_tiles >= N / TPT + B places in the list and at most used / TPT + B tiles: those left over clear the rows behind the
                 // last sequence, TPT tokens each.
                 const int64_t t0 = (int64_t)__ldcg(p.cu_q + p.B) + (int64_t)tok0 * TPT;

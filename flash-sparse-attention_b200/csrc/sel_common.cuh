@@ -238,7 +238,6 @@ __device__ __forceinline__ int count_seq_tiles(const int32_t* __restrict__ cu_q,
     return total;
 }
 // tile `want` of the list: its sequence (-1 if there is no such tile), first token and number of tokens
-template <bool CG = false>
 __device__ __forceinline__ void find_seq_tile(const int32_t* __restrict__ cu_q, int B, int TPT, int want, int lane, int& seq, int& tok0,
                                              int& ne) {
     seq = -1; tok0 = 0; ne = 0;
@@ -246,7 +245,7 @@ __device__ __forceinline__ void find_seq_tile(const int32_t* __restrict__ cu_q, 
     int acc = 0;
     for (int b0 = 0; b0 < B; b0 += 32) {
         const int b = b0 + lane;
-        const int s0 = b < B ? ld_cg<CG>(cu_q + b) : 0, L = b < B ? ld_cg<CG>(cu_q + b + 1) - s0 : 0;
+        const int s0 = b < B ? __ldg(cu_q + b) : 0, L = b < B ? __ldg(cu_q + b + 1) - s0 : 0;
         const int nt = (L + TPT - 1) / TPT;
         int incl = nt;                                   // inclusive prefix over the 32 sequences
 #pragma unroll
@@ -268,15 +267,32 @@ __device__ __forceinline__ void find_seq_tile(const int32_t* __restrict__ cu_q, 
     }
 }
 
-// The same list (behind its end: seq -1, tok0 how far), longest rows of keys first, for up to 32 sequences (others: from its end): a tile's tokens see about as many keys as precede
-// them in their sequence, cu_k's included, which is what tiles are ranked by.  Sequence after sequence, a long one that comes late in the list
-// is still at work when everybody else is done: two sequences of 8192 tokens, 8 / 4 heads, took 28 % longer a tile than one of 16384.
+// Such a list with the longest rows of keys first, for up to kRankedSeqs sequences (behind its end: seq -1, ne 0, tok0 how far): a tile's tokens see about
+// as many keys as precede them in their sequence, cu_k's included, which is what tiles are ranked by.  Sequence after sequence, a long one that comes
+// late in the list is still at work when everybody else is done: two sequences of 8192 tokens, 8 / 4 heads, took 28 % longer a tile than one of 16384.
+// More sequences: sequence b has the places from cu_q[b] / TPT + b on, some of which hold no tile (seq -1, ne -1), and a search among 32 at a time finds a
+// place's in two or three steps, where walking them took B / 32.
+constexpr int kRankedSeqs = 32;
+__device__ __forceinline__ int count_ranked_tiles(const int32_t* __restrict__ cu_q, int B, int TPT, int lane) {
+    return B > kRankedSeqs ? __ldcg(cu_q + B) / TPT + B : count_seq_tiles<true>(cu_q, B, TPT, lane);
+}
 __device__ __forceinline__ void find_ranked_tile(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, int B, int TPT, int rank, int lane,
                                                 int& seq, int& tok0, int& ne) {
-    if (B > 32) {
-        const int total = count_seq_tiles<true>(cu_q, B, TPT, lane);
-        find_seq_tile<true>(cu_q, B, TPT, total - 1 - rank, lane, seq, tok0, ne);
-        if (seq < 0) tok0 = rank - total;
+    if (B > kRankedSeqs) {
+        const int total = __ldcg(cu_q + B) / TPT + B, place = total - 1 - rank;      // (from the end: what comes late in a sequence sees most)
+        seq = -1; tok0 = -place - 1; ne = 0;
+        if (place < 0) return;
+        int lo = 0, hi = B;                     // first place of lo <= place < first place of hi
+        while (hi - lo > 1) {
+            const int step = (hi - lo + 31) / 32, b = min(lo + lane * step, hi);
+            const unsigned at_or_before = __ballot_sync(0xffffffffu, b < hi && __ldcg(cu_q + b) / TPT + b <= place);     // (a run of lanes from 0 on)
+            lo += (31 - __clz(at_or_before)) * step;
+            hi = min(hi, lo + step);
+        }
+        const int s0 = __ldcg(cu_q + lo), n = __ldcg(cu_q + lo + 1) - s0, first = (place - s0 / TPT - lo) * TPT;
+        tok0 = s0 + first;
+        ne = first < n ? min(TPT, n - first) : -1;
+        if (ne > 0) seq = lo;
         return;
     }
     const int s0 = lane < B ? __ldcg(cu_q + lane) : 0, s1 = lane < B ? __ldcg(cu_q + lane + 1) : 0;

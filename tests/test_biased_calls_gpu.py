@@ -17,7 +17,7 @@ from fsa.ops import biased_attention
 from fsa_preview.ops import biased_decode_attention, shared_prefix_decode_attention
 from oracle import biased_attn_oracle as orc
 from test_biased_attn_gpu import BF16, DEV, check, cu_of, inputs, near, near_lse, slopes_of
-from test_biased_decode_gpu import cache_of, i32
+from test_biased_decode_gpu import cache_of, check as check_decode, i32
 
 INT_MAX = 2 ** 31 - 1
 
@@ -299,3 +299,17 @@ def test_a_verification_step_agrees_with_single_tokens():
         # each side: half a step 2^-9 of P (sums of |p v|, at most max |v|), and 2^-9 of o
         assert float((o[i] - o1[0]).abs().max()) <= 2 * 2.0 ** -8 * float(v.abs().max())
         assert float((lse[:, i] - lse1[0]).abs().max()) <= 2.0 ** -15
+
+
+def test_many_groups():
+    """More shared prefixes than a warp has lanes, some with no sequence, some of no rows."""
+    prefixes = [100, 1, 0, 70, 333] * 9
+    groups = [1, 0, 3, 2, 40] * 9
+    lens = [(i * 7) % 50 + 1 for i in range(sum(groups) + 3)]
+    check_decode(lens, 2, 4, 64, BF16, "both", prefixes=prefixes, groups=groups)
+
+
+def test_many_sequences_of_one_token():
+    lens = [1] * 700 + [0] * 40 + [300] + [1] * 50
+    q, k, v, do = inputs(lens, lens, 2, 4, 64, BF16, 10)
+    check(q, k, v, do, lens, lens, 20.0, slopes_of(8))
