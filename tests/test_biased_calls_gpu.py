@@ -313,3 +313,23 @@ def test_many_sequences_of_one_token():
     lens = [1] * 700 + [0] * 40 + [300] + [1] * 50
     q, k, v, do = inputs(lens, lens, 2, 4, 64, BF16, 10)
     check(q, k, v, do, lens, lens, 20.0, slopes_of(8))
+
+
+@pytest.mark.parametrize("score", [(20.0, False), (50.0, True)])
+@pytest.mark.parametrize("lens,klens", [([400, 1, 250], [400, 1, 250]), ([60, 7, 300], [500, 90, 300])])
+@pytest.mark.parametrize("window", [0, 33, 150])
+def test_documents_within_a_window(score, lens, klens, window):
+    cap, alibi = score
+    q, k, v, do = inputs(lens, klens, 1, 4, 128, BF16, window + len(klens))
+    g = torch.Generator().manual_seed(window)
+    ids = torch.cumsum((torch.rand(sum(klens), generator=g) < 0.02).int(), 0).to(torch.int32)
+    ids[100:130] = -1
+    check(q, k, v, do, lens, klens, cap, slopes_of(4) if alibi else None, window=window, ids=ids)
+
+
+@pytest.mark.parametrize("prefix", [None, [300, 20]])
+def test_scores_that_grow_with_the_distance(prefix):
+    """Negative slopes: the furthest keys weigh most, so a row's maximum rises tile after tile."""
+    lens = [400, 130]
+    q, k, v, do = inputs(lens, lens, 2, 2, 64, BF16, 13)
+    check(q, k, v, do, lens, lens, None, torch.tensor([-0.05, 0.0, -0.01, 0.05]), prefix=None if prefix is None else torch.tensor(prefix, dtype=torch.int32))
