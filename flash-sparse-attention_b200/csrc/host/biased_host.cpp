@@ -43,6 +43,20 @@ static void check_biased_status(const char* what) {
     check(st == 0 ? FSA_OK : FSA_ERR_DEVICE_STATUS, what);
 }
 
+// Gradients of a leaf are added up on the stream that its first live graph was made on.  Where that is another than the capturing one, torch ends the capture, and the
+// process with it, in the backward pass: refused here, before anything is captured.
+static void check_capture(const Tensor& q, const Tensor& k, const Tensor& v) {
+    const auto stream = c10::cuda::getCurrentCUDAStream(q.device().index());
+    cudaStreamCaptureStatus capturing = cudaStreamCaptureStatusNone;
+    if (cudaStreamIsCapturing(stream.stream(), &capturing) != cudaSuccess || capturing == cudaStreamCaptureStatusNone) return;
+    for (const Tensor* t : {&q, &k, &v}) {
+        if (!t->requires_grad() || !t->is_leaf()) continue;
+        const auto sum = torch::autograd::impl::try_get_grad_accumulator(*t);
+        const auto on = sum ? sum->stream() : std::nullopt;
+        TORCH_CHECK(!on || *on == stream.unwrap(), "biased_attention: a graph made on another stream still holds a leaf of this capture: release what depends on it first");
+    }
+}
+
 static void check_lengths(const Tensor& t, const Tensor& q, int64_t n, const char* name) {
     TORCH_CHECK_TYPE(t.scalar_type() == at::kInt, name, " has to be int32, got ", t.scalar_type());
     TORCH_CHECK_VALUE(t.dim() == 1 && (n < 0 || t.size(0) == n), name, " has to have ", n, " entries, got a tensor of shape ", t.sizes());
@@ -160,6 +174,7 @@ std::tuple<Tensor, Tensor> biased_attention(const Tensor& q, const Tensor& k, co
     auto plain = [](const MaybeTensor& t) { return t ? t->contiguous() : Tensor(); };
     const Tensor cu = cu_q.contiguous(), cu_k = cu_k_ ? cu_k_->contiguous() : cu, docs = plain(docs_), prefix = plain(prefix_);
     if (wants_grad({&q, &k, &v})) {
+        check_capture(q, k, v);
         const auto r = BiasedAttention::apply(q, k, v, BiasedArgs{cu, cu_k, slopes, docs, prefix, scale, cap, window});
         return {r[0], r[1]};
     }

@@ -333,3 +333,25 @@ def test_scores_that_grow_with_the_distance(prefix):
     lens = [400, 130]
     q, k, v, do = inputs(lens, lens, 2, 2, 64, BF16, 13)
     check(q, k, v, do, lens, lens, None, torch.tensor([-0.05, 0.0, -0.01, 0.05]), prefix=None if prefix is None else torch.tensor(prefix, dtype=torch.int32))
+
+
+def test_capture_beside_a_live_graph_of_the_same_leaves():
+    """Refused before anything is captured; once the eager graph is gone, the capture holds forward and backward."""
+    lens = [100]
+    q, k, v, do = (x.to(DEV) for x in inputs(lens, lens, 1, 2, 64, BF16, 14))
+    cu = cu_of(lens).to(DEV)
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+    o, _ = biased_attention(*leaves, cu, softcap=5.0)
+    want = o.detach().clone()
+    graph = torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="leaf of this capture"):
+        with torch.cuda.graph(graph):
+            biased_attention(*leaves, cu, softcap=5.0)
+    del o
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o, _ = biased_attention(*leaves, cu, softcap=5.0)
+        grads = torch.autograd.grad(o, leaves, do)
+    graph.replay()
+    assert torch.equal(o.detach(), want) and all(bool(torch.isfinite(x).all()) for x in grads)
