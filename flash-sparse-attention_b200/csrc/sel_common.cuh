@@ -291,7 +291,7 @@ __device__ __forceinline__ void find_ranked_tile(const int32_t* __restrict__ cu_
         }
         const int s0 = __ldcg(cu_q + lo), n = __ldcg(cu_q + lo + 1) - s0, first = (place - s0 / TPT - lo) * TPT;
         tok0 = s0 + first;
-        ne = first < n ? min(TPT, n - first) : -1;
+        ne = first >= 0 && first < n ? min(TPT, n - first) : -1;        // (below 0: rows in front of the first sequence)
         if (ne > 0) seq = lo;
         return;
     }

@@ -309,6 +309,20 @@ def test_many_groups():
     check_decode(lens, 2, 4, 64, BF16, "both", prefixes=prefixes, groups=groups)
 
 
+def test_many_groups_behind_sequences_without_one():
+    lens, prefixes = [70, 5, 300, 1, 40] * 8, [90] * 36
+    q, k, v, row0 = cache_of(lens, 1, 4, 64, BF16, 6)
+    g = torch.Generator().manual_seed(7)
+    pk, pv = (torch.randn(sum(prefixes), 1, 64, generator=g).to(BF16) for _ in range(2))
+    cg = [3 + i for i in range(37)]         # sequences 3 .. 38, one a group
+    o, lse = shared_prefix_decode_attention(q.to(DEV), k.to(DEV), v.to(DEV), i32(lens), i32(row0), pk.to(DEV), pv.to(DEV), cu_of(prefixes).to(DEV), i32(cg),
+                                            max_len=300, softcap=20.0)
+    mine = [(pk[(b - 3) * 90 : (b - 2) * 90], pv[(b - 3) * 90 : (b - 2) * 90]) if 3 <= b < 39 else (pk[:0], pv[:0]) for b in range(len(lens))]
+    ref, off = orc.decoded(q, k, v, lens, row0, 64 ** -0.5, 20.0, None, None, mine, BF16)
+    near(o, ref[0], off, "o")
+    near_lse(lse, ref[1])
+
+
 def test_many_sequences_of_one_token():
     lens = [1] * 700 + [0] * 40 + [300] + [1] * 50
     q, k, v, do = inputs(lens, lens, 2, 4, 64, BF16, 10)
