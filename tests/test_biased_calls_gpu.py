@@ -369,3 +369,48 @@ def test_capture_beside_a_live_graph_of_the_same_leaves():
         grads = torch.autograd.grad(o, leaves, do)
     graph.replay()
     assert torch.equal(o.detach(), want) and all(bool(torch.isfinite(x).all()) for x in grads)
+
+
+def test_offsets_beyond_32_bits():
+    """2.3e9 elements of q: the last sequences get what they get alone, bit for bit.  dk and dv but for the order of their sums: alone, a K/V tile's 25 row tiles
+    are cut into four parts that are added up (items of 8 row tiles at least, 740 wanted), among 1400 sequences they are not.  Sums of n = 3200 terms in 32 bits in two orders differ by
+    2 n 2^-24 = 2^-11.4 of the sum of their sizes at most, which for terms of random signs is 0.8 n / 4 sqrt(n) = 11 times the largest of some thousand such sums: 2^-7.9
+    of that; and then by one step of bf16, 2^-7 of the value."""
+    L, B, Hk, G, d = 100, 1400, 4, 32, 128
+    N, Hq = L * B, Hk * G
+    assert N * Hq * d > 2 ** 31
+    g = torch.Generator(device=DEV).manual_seed(3)
+    mk = lambda h: torch.randn(N, h, d, device=DEV, dtype=BF16, generator=g)  # noqa: E731
+    q, k, v, do = mk(Hq), mk(Hk), mk(Hk), mk(Hq)
+    cu = torch.arange(B + 1, dtype=torch.int32, device=DEV) * L
+    sl = slopes_of(Hq).to(DEV)
+
+    def step(q, k, v, do, cu):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        o, lse = biased_attention(*leaves, cu, softcap=20.0, alibi_slopes=sl)
+        return [o.detach(), lse.T, *torch.autograd.grad(o, leaves, do)]
+
+    whole = step(q, k, v, do, cu)
+    n = 40 * L          # (more than 32 sequences: the same order of work)
+    alone = step(q[-n:], k[-n:], v[-n:], do[-n:], cu[:41])
+    for name, a, b in zip(("o", "lse", "dq", "dk", "dv"), whole, alone):
+        a = a[-n:]
+        if name in ("dk", "dv"):
+            x, y = a.double(), b.double()
+            assert bool(((x - y).abs() <= 2.0 ** -7 * y.abs() + 2.0 ** -7.9 * float(y.abs().max())).all()), name
+        else:
+            assert torch.equal(a, b), name
+
+
+def test_a_cache_beyond_32_bits():
+    rows, Hk, G, d, lens = 4_300_000, 4, 4, 128, [3000, 17]
+    assert rows * Hk * d > 2 ** 31
+    k = torch.zeros(rows, Hk, d, device=DEV, dtype=BF16)
+    v = torch.zeros_like(k)
+    qs, kc, vc, row0 = cache_of(lens, Hk, G, d, BF16, 15)
+    at = rows - kc.shape[0]
+    k[at:], v[at:] = kc.to(DEV), vc.to(DEV)
+    how = dict(max_len=3000, softcap=20.0)
+    far = biased_decode_attention(qs.to(DEV), k, v, i32(lens), i32([r + at for r in row0]), **how)
+    near_ = biased_decode_attention(qs.to(DEV), kc.to(DEV), vc.to(DEV), i32(lens), i32(row0), **how)
+    assert torch.equal(far[0], near_[0]) and torch.equal(far[1], near_[1]) and bool(torch.isfinite(far[0]).all())
