@@ -362,6 +362,10 @@ extern "C" int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, 
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);
 }
 
+// Items of dK / dV that the plan aims at.  (2 x 4096 tokens of documents: 636 us a pass with 5 an SM, 653 with 8, whose slabs take longer to join;
+// 2 x 8192 capped: 1339 and 1366)
+static int dkdv_items() { return 5 * sm_count(); }
+
 // The same for dQ, one item an SM.  An SM needs about 1 us a K/V tile and 3 an item; uncut, as long as the longest item if that is more than an even share
 // of all.  Cut, the parts' way to memory and back and 5 us of the launch that sums them come on top.  8192 tokens of one head: 41 us with four
 // chunks, 113 uncut; of four sequences of 1000 and four heads 27 with two chunks, 22 uncut.
@@ -391,7 +395,7 @@ extern "C" int fsa_biased_attn_bwd_bytes(int64_t N, int64_t Nk, int B, int Hq, i
     const int rc = biased_shape(N, Nk, B, Hq, Hk, D, &s);
     if (rc) return rc;
     if (!bytes_out) return FSA_ERR_BAD_ARG;
-    *bytes_out = align_up(N * Hq * 4, 1024) + align_up(range_kv_plan_bytes(s), 1024) + align_up(range_kv_slab_bytes(s), 1024) + DqCut(s, window).bytes(s);
+    *bytes_out = align_up(N * Hq * 4, 1024) + align_up(range_kv_plan_bytes(s, dkdv_items()), 1024) + align_up(range_kv_slab_bytes(s, dkdv_items()), 1024) + DqCut(s, window).bytes(s);
     return FSA_OK;
 }
 
@@ -435,16 +439,15 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     RangeKvPlan plan = {};
     plan.cu_q = cu_seqlens_q; plan.cu_k = cu_seqlens_k; plan.kv_lo = lim.lo; plan.kv_hi = lim.hi;
     plan.N = N; plan.Nk = Nk; plan.B = B; plan.Hk = Hk; plan.TPT = s.TPT;
-    // (2 x 4096 tokens of documents: 636 us a pass with 5 items an SM, 653 with 8, whose slabs take longer to join; 2 x 8192 capped: 1339 and 1366)
-    plan.aim = 5 * sm_count();
+    plan.aim = dkdv_items();
     plan.max_tiles = (int)range_kv_max_tiles(s);
     plan.D = D;
     plan.counts = (int*)sp;
     plan.tiles = (int4*)(sp + 256);
     plan.multi = plan.tiles + plan.max_tiles;
     plan.items = plan.multi + plan.max_tiles;
-    sp += align_up(range_kv_plan_bytes(s), 1024);
-    a.slabs = (float*)sp;           sp += align_up(range_kv_slab_bytes(s), 1024);
+    sp += align_up(range_kv_plan_bytes(s, dkdv_items()), 1024);
+    a.slabs = (float*)sp;           sp += align_up(range_kv_slab_bytes(s, dkdv_items()), 1024);
     float* part = (float*)sp;
     const DqCut cut(s, window);
     int* status = nullptr;

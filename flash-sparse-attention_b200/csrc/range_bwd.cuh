@@ -24,13 +24,13 @@ struct RangeKvPlan {
 
 // Sizes of the plan and the slabs: ceil(n / C) <= 2 n / C for a tile that is cut, so the cut tiles have at most 2 aim / Hk items.
 inline int64_t range_kv_max_tiles(const SelShape& s) { return (s.Nk + kTileRows - 1) / kTileRows + s.B; }
-inline int64_t range_kv_max_cut(const SelShape& s) {
+inline int64_t range_kv_max_cut(const SelShape& s, int64_t aim = range_kv_items()) {
     const int64_t row_tiles = range_kv_max_tiles(s) * ((s.N + s.TPT - 1) / s.TPT);
-    const int64_t a = 2 * (int64_t)range_kv_items() / s.Hk + 1, b = 2 * row_tiles / kRkMinTiles + 1;
+    const int64_t a = 2 * aim / s.Hk + 1, b = 2 * row_tiles / kRkMinTiles + 1;
     return a < b ? a : b;
 }
-inline int64_t range_kv_plan_bytes(const SelShape& s) { return 256 + 16 * (3 * range_kv_max_tiles(s) + range_kv_max_cut(s)); }
-inline int64_t range_kv_slab_bytes(const SelShape& s) { return range_kv_max_cut(s) * s.Hk * (2 * 128 * (int64_t)s.D * 4); }
+inline int64_t range_kv_plan_bytes(const SelShape& s, int64_t aim = range_kv_items()) { return 256 + 16 * (3 * range_kv_max_tiles(s) + range_kv_max_cut(s, aim)); }
+inline int64_t range_kv_slab_bytes(const SelShape& s, int64_t aim = range_kv_items()) { return range_kv_max_cut(s, aim) * s.Hk * (2 * 128 * (int64_t)s.D * 4); }
 
 // Work items from the stretches (one CTA of T threads): a tile of n row tiles becomes ceil(n / C) items of about equal length, C the
 // smallest length that leaves about p.aim items (times heads), and at least kRkMinTiles: below that an item's epilogue weighs
