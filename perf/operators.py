@@ -17,7 +17,6 @@ own = False
 
 DTYPES = {"bf16": torch.bfloat16, "fp16": torch.float16}
 LOG2E = 1.4426950408889634
-PACKAGE = os.path.join(os.getcwd(), "flash-sparse-attention_b200")
 
 
 def _attn(name, train, seqlens, Hk, G, d, dtype, cap=0.0, alibi=False, window=0, docs="", prefix="", cached=""):
@@ -179,6 +178,7 @@ def prepare(case, seed):
 
 def run(s):
     if own:
+        sys.path.insert(0, os.path.join(os.getcwd(), "flash-sparse-attention_b200"))
         return _run_own(s)
     if s["kind"] == "decode":
         return _plain_decode(s)
@@ -191,8 +191,6 @@ def run(s):
 
 
 def _run_own(s):
-    if PACKAGE not in sys.path:
-        sys.path.insert(0, PACKAGE)
     how = dict(sm_scale=s["scale"], softcap=s["cap"], alibi_slopes=s["slopes"], window_size=s["window"])
     if s["kind"] == "decode":
         from fsa_preview.ops import biased_decode_attention
