@@ -279,19 +279,21 @@ __device__ __forceinline__ int count_ranked_tiles(const int32_t* __restrict__ cu
 __device__ __forceinline__ void find_ranked_tile(const int32_t* __restrict__ cu_q, const int32_t* __restrict__ cu_k, int B, int TPT, int rank, int lane,
                                                 int& seq, int& tok0, int& ne) {
     if (B > kRankedSeqs) {
-        const int total = __ldcg(cu_q + B) / TPT + B, place = total - 1 - rank;      // (from the end: what comes late in a sequence sees most)
+        const int before = __ldcg(cu_q) / TPT, total = __ldcg(cu_q + B) / TPT + B, place = total - 1 - rank;      // (from the end: what comes late in a sequence sees most)
         seq = -1; tok0 = -place - 1; ne = 0;
         if (place < 0) return;
+        ne = -1;
+        if (place < before) return;             // rows in front of the first sequence: the search below has no sequence for them
         int lo = 0, hi = B;                     // first place of lo <= place < first place of hi
         while (hi - lo > 1) {
             const int step = (hi - lo + 31) / 32, b = min(lo + lane * step, hi);
-            const unsigned at_or_before = __ballot_sync(0xffffffffu, b < hi && __ldcg(cu_q + b) / TPT + b <= place);     // (a run of lanes from 0 on)
+            const unsigned at_or_before = __ballot_sync(0xffffffffu, b < hi && __ldcg(cu_q + b) / TPT + b <= place);     // (a run of lanes from 0 on, whose own place is lo's)
             lo += (31 - __clz(at_or_before)) * step;
             hi = min(hi, lo + step);
         }
         const int s0 = __ldcg(cu_q + lo), n = __ldcg(cu_q + lo + 1) - s0, first = (place - s0 / TPT - lo) * TPT;
         tok0 = s0 + first;
-        ne = first >= 0 && first < n ? min(TPT, n - first) : -1;        // (below 0: rows in front of the first sequence)
+        if (first < n) ne = min(TPT, n - first);
         if (ne > 0) seq = lo;
         return;
     }

@@ -1,0 +1,30 @@
+"""Attention with changed scores where a call is allowed but unusual.  Allowances as in test_biased_attn_gpu.py, where nothing else is said."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+from fsa_preview.ops import shared_prefix_decode_attention
+from oracle import biased_attn_oracle as orc
+from test_biased_attn_gpu import BF16, DEV, cu_of, near, near_lse
+from test_biased_decode_gpu import cache_of, i32
+
+
+@pytest.mark.parametrize("G,front,groups", [(32, 9, 36), (4, 70, 33), (32, 130, 400), (1, 260, 40)])
+def test_many_groups_behind_at_least_a_tile_of_sequences_without_one(G, front, groups):
+    """More groups than a warp has lanes, and so many sequences in front of the first one that whole tiles lie there."""
+    assert groups > 32 and front >= (128 // G) & ~3
+    P, d = 20, 64
+    lens = [1 + (7 * i) % 30 for i in range(front + groups + 2)]
+    q, k, v, row0 = cache_of(lens, 1, G, d, BF16, 6)
+    g = torch.Generator().manual_seed(7)
+    pk, pv = (torch.randn(P * groups, 1, d, generator=g).to(BF16) for _ in range(2))
+    o, lse = shared_prefix_decode_attention(q.to(DEV), k.to(DEV), v.to(DEV), i32(lens), i32(row0), pk.to(DEV), pv.to(DEV), cu_of([P] * groups).to(DEV),
+                                            i32([front + i for i in range(groups + 1)]), max_len=30, max_prefix=P, softcap=20.0)
+    mine = [(pk[P * (b - front) : P * (b - front + 1)], pv[P * (b - front) : P * (b - front + 1)]) if front <= b < front + groups else (pk[:0], pv[:0])
+            for b in range(len(lens))]
+    ref, off = orc.decoded(q, k, v, lens, row0, d ** -0.5, 20.0, None, None, mine, BF16)
+    near(o, ref[0], off, "o")
+    near_lse(lse, ref[1])
