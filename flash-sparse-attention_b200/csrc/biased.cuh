@@ -22,14 +22,14 @@ struct BiasedFwdParams {
 };
 
 // First and last K/V row that token `tok` of a sequence sees, and its place, without documents.  The sequence has the rows [k0, k1); its last token is
-// the one before q1 and stands at row k1 - 1.  window: -1 for none; prefix: rows at its beginning that all tokens see.
+// the one before q1 and stands at row k1 - 1.  window: -1 for none; prefix: rows at its beginning that all tokens see (below 0: none).
 struct Sees { int lo, hi, pos; };
 __device__ __forceinline__ Sees place_limits(int tok, int k0, int k1, int q1, int window, int prefix) {
     Sees x;
     x.pos = tok + k1 - q1;
     const bool in = x.pos >= k0;            // (else the sequence has fewer keys than queries, and this one precedes them)
     x.lo = in && window >= 0 ? max(k0, x.pos - window) : k0;
-    x.hi = in ? max(x.pos, k0 + min(prefix, k1 - k0) - 1) : -1;
+    x.hi = in ? max(x.pos, k0 + min(max(prefix, 0), k1 - k0) - 1) : -1;
     return x;
 }
 

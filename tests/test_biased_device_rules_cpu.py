@@ -147,3 +147,39 @@ def test_every_tile_of_many_sequences_is_found_once(search, lens, front, TPT):
 def test_every_tile_of_few_sequences_is_found_once(search, front, lens, klens, TPT):
     left = every_tile(search, front, lens, TPT, klens)
     assert left == list(range(len(left)))
+
+
+LIMITS = r"""
+extern "C" void limits(int tok, int k0, int k1, int q1, int window, int prefix, int* out) {
+    const Sees x = place_limits(tok, k0, k1, q1, window, prefix);
+    out[0] = x.lo; out[1] = x.hi; out[2] = x.pos;
+}
+"""
+
+
+@pytest.fixture(scope="module")
+def limits(tmp_path_factory):
+    text = "struct Sees { int lo, hi, pos; };\n" + function("biased.cuh", "__device__ __forceinline__ Sees place_limits(") + LIMITS
+    lib = build(tmp_path_factory.mktemp("limits"), text)
+
+    def call(*args):
+        out = (ctypes.c_int * 3)()
+        lib.limits(*args, out)
+        return tuple(out)
+
+    return call
+
+
+LARGEST = 2 ** 31 - 1
+
+
+@pytest.mark.parametrize("k0,k1,q1", [(0, 10, 10), (0, 10, 4), (5, 25, 10), (2 ** 25 - 40, 2 ** 25 - 1, 20), (3, 3, 10), (0, 4, 10)])
+@pytest.mark.parametrize("window,prefix", [(-1, 0), (-1, 3), (-1, 10), (-1, LARGEST), (-1, -1), (-1, -LARGEST), (-1, -LARGEST - 1), (0, 0), (4, 0), (LARGEST, 0)])
+def test_rows_that_a_token_sees(limits, k0, k1, q1, window, prefix):
+    """Of its own sequence's rows, whatever stands in prefix_lens and window_size."""
+    for tok in range(max(0, q1 - 8), q1):
+        pos = tok + k1 - q1
+        seen = [j for j in range(k0, k1) if pos >= k0 and (j <= pos or j - k0 < prefix) and (window < 0 or j >= pos - window)]
+        lo, hi, at = limits(tok, k0, k1, q1, window, prefix)
+        assert at == pos and list(range(lo, min(hi, lo + 10 ** 4) + 1)) == seen
+        assert hi < k1

@@ -8,7 +8,7 @@ pytestmark = pytest.mark.gpu
 
 from fsa_preview.ops import shared_prefix_decode_attention
 from oracle import biased_attn_oracle as orc
-from test_biased_attn_gpu import BF16, DEV, cu_of, near, near_lse
+from test_biased_attn_gpu import BF16, DEV, check, cu_of, inputs, near, near_lse
 from test_biased_decode_gpu import cache_of, i32
 
 
@@ -28,3 +28,12 @@ def test_many_groups_behind_at_least_a_tile_of_sequences_without_one(G, front, g
     ref, off = orc.decoded(q, k, v, lens, row0, d ** -0.5, 20.0, None, None, mine, BF16)
     near(o, ref[0], off, "o")
     near_lse(lse, ref[1])
+
+
+@pytest.mark.parametrize("Hk,G,d", [(1, 2, 64), (2, 1, 128)])
+def test_prefixes_below_zero(Hk, G, d):
+    """The smallest number in the sequence that begins at row 0: nobody sees the rows of another sequence."""
+    lens = [90, 40, 130]
+    q, k, v, do = inputs(lens, lens, Hk, G, d, BF16, 2)
+    for prefix in ([-2 ** 31] * 3, [-1, 7, -2 ** 31]):
+        check(q, k, v, do, lens, lens, 20.0, None, prefix=torch.tensor(prefix, dtype=torch.int32))
