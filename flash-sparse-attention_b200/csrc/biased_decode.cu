@@ -121,7 +121,7 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
         const float tanh_k = (MOD & kModCap) ? 2.f * kLog2e * p.mod.x_scale : 0.f;
         // score of a product (log2 units); dist: tokens between the key and the new token
         auto score = [&](float x, float sl, float dist) {
-            const float s = (MOD & kModCap) ? tanh_any(x, tanh_k) * p.mod.cap_log2 : x * p.scale_log2;
+            const float s = (MOD & kModCap) ? tanh_far(x, tanh_k) * p.mod.cap_log2 : x * p.scale_log2;
             return (MOD & kModBias) ? fmaf(-sl, dist, s) : s;
         };
 #pragma unroll

@@ -40,15 +40,16 @@ __device__ __forceinline__ float rcp_approx(float x) {
     return y;
 }
 
-// tanh(x) = 1 - 2 / (1 + e^2x) for any x (k = 2 log2(e) times what v is to be multiplied with): off by some 2e-7, which a cap of 50
-// makes 1e-5 of a score.  tanh.approx would take one special-function step instead of two, but is off by 5e-4 of the score.
-__device__ __forceinline__ float tanh_any(float v, float k) { return fmaf(-2.f, rcp_approx(1.f + ex2_approx(v * k)), 1.f); }
+// tanh(x) = 1 - 2 / (1 + e^2x) (k = 2 log2(e) times what v is to be multiplied with): off by some 2e-7, whatever the value: for |x| above 3/4, where that is
+// 3e-7 of it (a cap of 50 makes 1e-5 of a score).  tanh.approx would take one special-function step instead of two, but is off by 5e-4 of the score.
+__device__ __forceinline__ float tanh_far(float v, float k) { return fmaf(-2.f, rcp_approx(1.f + ex2_approx(v * k)), 1.f); }
 
 // tanh_near: of two values no larger than 3/4; cap_scores: v <- tanh(x_scale v), N scores of a row (all lanes of a warp
 // call it; whether some |v| was above near_v).  The special-function unit gives 16 results a cycle and SM, and the
 // softmax needs one for each score already; with two more the capped forward would be bound by it, three times as long as its products.
 // Where no |x| of the warp's 32 rows is above 3/4 (scores below 37 at a cap of 50), tanh(x) = x p(x^2) with p of degree 4: the
-// polynomial that is nearest to tanh(x) / x on [0, 9/16] in relative error, 6e-7 (fitted on Chebyshev points); two scores an instruction.
+// polynomial that is nearest to tanh(x) / x on [0, 9/16] in relative error, 6e-7 (fitted on Chebyshev points); two scores an instruction.  In other
+// warps every score takes the form for its size: the other one's error, times a cap far above a small score, can be as large as the score.
 constexpr float kTanhNear = 0.75f;
 __device__ __forceinline__ uint64_t tanh_near(uint64_t x) {
     constexpr float c[5] = {0.999999463558197f, -0.3332825005054474f, 0.13258983194828033f, -0.050056297332048416f, 0.012929627671837807f};
@@ -76,9 +77,15 @@ __device__ __forceinline__ bool cap_scores(uint32_t (&v)[N], float x_scale, floa
             v[i + 1] = __float_as_uint(t.y);
         }
     } else {
+        const uint64_t xs = f32x2(x_scale, x_scale);
         const float k = 2.f * kLog2e * x_scale;
 #pragma unroll
-        for (int i = 0; i < N; ++i) v[i] = __float_as_uint(tanh_any(__uint_as_float(v[i]), k));
+        for (int i = 0; i < N; i += 2) {
+            const float a = __uint_as_float(v[i]), b = __uint_as_float(v[i + 1]);
+            const float2 x = f32x2_get(mul_f32x2(f32x2(a, b), xs)), t = f32x2_get(tanh_near(f32x2(x.x, x.y)));
+            v[i] = __float_as_uint(fabsf(x.x) <= kTanhNear ? t.x : tanh_far(a, k));
+            v[i + 1] = __float_as_uint(fabsf(x.y) <= kTanhNear ? t.y : tanh_far(b, k));
+        }
     }
     return __any_sync(0xffffffffu, most > near_v);
 }

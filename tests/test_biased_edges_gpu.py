@@ -6,6 +6,7 @@ import torch
 
 pytestmark = pytest.mark.gpu
 
+from fsa.ops import biased_attention
 from fsa_preview.ops import shared_prefix_decode_attention
 from oracle import biased_attn_oracle as orc
 from test_biased_attn_gpu import BF16, DEV, check, cu_of, inputs, near, near_lse
@@ -37,3 +38,24 @@ def test_prefixes_below_zero(Hk, G, d):
     q, k, v, do = inputs(lens, lens, Hk, G, d, BF16, 2)
     for prefix in ([-2 ** 31] * 3, [-1, 7, -2 ** 31]):
         check(q, k, v, do, lens, lens, 20.0, None, prefix=torch.tensor(prefix, dtype=torch.int32))
+
+
+@pytest.mark.parametrize("cap", [1e4, 1e6, 1e8])
+@pytest.mark.parametrize("d,dtype", [(64, BF16), (128, BF16)])
+def test_a_cap_that_one_token_reaches(cap, d, dtype):
+    """One token's scores are as large as a cap far above all the others': those get what they get without it."""
+    lens, big = [130], 40
+    q, k, v, do = inputs(lens, lens, 1, 2, d, dtype, 3)
+    q[big], do[big] = q[big] * cap, 0.0
+    cu = cu_of(lens)
+    ref, off = orc.packed(q, k, v, cu, cu, d ** -0.5, cap, do=do, dtype=dtype)
+    leaves = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    o, lse = biased_attention(*leaves, cu.to(DEV), softcap=cap)
+    grads = torch.autograd.grad(o, leaves, do.to(DEV))
+    rest = [t for t in range(lens[0]) if t != big]
+    near(o.detach()[rest], ref[0][rest], off[0][rest], "o")
+    near_lse(lse[:, rest], ref[1][:, rest])
+    near(grads[0][rest], ref[2][rest], off[1][rest], "dq")
+    # (without a dO the large one has no share in these)
+    near(grads[1], ref[3], off[2], "dk")
+    near(grads[2], ref[4], off[3], "dv")
