@@ -118,12 +118,9 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
             slope[0] = gid < NG ? p.mod.slopes[h * p.G + g0 + gid] * kLog2e : 0.f;
             slope[1] = HI && gid + 8 < NG ? p.mod.slopes[h * p.G + g0 + gid + 8] * kLog2e : 0.f;
         }
-        const float tanh_k = (MOD & kModCap) ? 2.f * kLog2e * p.mod.x_scale : 0.f;
-        // score of a product (log2 units); dist: tokens between the key and the new token
-        auto score = [&](float x, float sl, float dist) {
-            const float s = (MOD & kModCap) ? tanh_far(x, tanh_k) * p.mod.cap_log2 : x * p.scale_log2;
-            return (MOD & kModBias) ? fmaf(-sl, dist, s) : s;
-        };
+        const float to_log2 = (MOD & kModCap) ? p.mod.cap_log2 : p.scale_log2;
+        // score (log2 units) of a product, or of its tanh; dist: tokens between the key and the new token
+        auto score = [&](float x, float sl, float dist) { return (MOD & kModBias) ? fmaf(-sl, dist, x * to_log2) : x * to_log2; };
 #pragma unroll
         for (int i = 0; i < NO; ++i) acc[i][0] = acc[i][1] = acc[i][2] = acc[i][3] = 0.f;
         const int lrow = lane & 7, lmat = lane >> 3;
@@ -148,6 +145,14 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
                         mma16816<ET>(sc[nt], qf[c0 / 2][0], qh[c0 / 2][0], qf[c0 / 2][1], qh[c0 / 2][1], r0, r1);
                         mma16816<ET>(sc[nt], qf[c0 / 2 + 1][0], qh[c0 / 2 + 1][0], qf[c0 / 2 + 1][1], qh[c0 / 2 + 1][1], r2, r3);
                     }
+                }
+                if constexpr (MOD & kModCap) {
+                    uint32_t x[HI ? 8 : 4];
+#pragma unroll
+                    for (int i = 0; i < (HI ? 8 : 4); ++i) x[i] = __float_as_uint(HI ? sc[i >> 2][i & 3] : sc[i >> 1][i & 1]);
+                    cap_scores(x, p.mod.x_scale, p.mod.near_v);
+#pragma unroll
+                    for (int i = 0; i < (HI ? 8 : 4); ++i) (HI ? sc[i >> 2][i & 3] : sc[i >> 1][i & 1]) = __uint_as_float(x[i]);
                 }
                 float tmax0 = -INFINITY, tmax1 = -INFINITY;
 #pragma unroll

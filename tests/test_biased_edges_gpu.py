@@ -7,7 +7,7 @@ import torch
 pytestmark = pytest.mark.gpu
 
 from fsa.ops import biased_attention
-from fsa_preview.ops import shared_prefix_decode_attention
+from fsa_preview.ops import biased_decode_attention, shared_prefix_decode_attention
 from oracle import biased_attn_oracle as orc
 from test_biased_attn_gpu import BF16, DEV, check, cu_of, inputs, near, near_lse
 from test_biased_decode_gpu import cache_of, i32
@@ -59,3 +59,25 @@ def test_a_cap_that_one_token_reaches(cap, d, dtype):
     # (without a dO the large one has no share in these)
     near(grads[1], ref[3], off[2], "dk")
     near(grads[2], ref[4], off[3], "dv")
+
+
+@pytest.mark.parametrize("cap,scale", [(1e4, 0.1), (1e6, 0.1), (1e8, 0.1), (30.0, 1e-12), (1e20, 0.1)])
+@pytest.mark.parametrize("d,G", [(64, 2), (128, 16)])
+def test_decode_with_caps_far_above_the_scores(cap, scale, d, G):
+    """Single tokens, behind shared rows too, and the same rows of a prefill: all of them right, so that they agree."""
+    lens, P = [300, 0, 70], 200
+    q, k, v, row0 = cache_of(lens, 1, G, d, BF16, 4)
+    g = torch.Generator().manual_seed(5)
+    pk, pv = (torch.randn(P, 1, d, generator=g).to(BF16) for _ in range(2))
+    args, how = [x.to(DEV) for x in (q, k, v)] + [i32(lens), i32(row0)], dict(max_len=300, softcap=cap, sm_scale=scale)
+    for mine, (o, lse) in ((None, biased_decode_attention(*args, **how)),
+                           ([(pk, pv)] * 3, shared_prefix_decode_attention(*args, pk.to(DEV), pv.to(DEV), i32([0, P]), i32([0, 3]), **how))):
+        ref, off = orc.decoded(q, k, v, lens, row0, scale, cap, None, None, mine, BF16)
+        near(o, ref[0], off, "o")
+        near_lse(lse, ref[1])
+    for b in (0, 2):
+        rows = slice(row0[b], row0[b] + lens[b])
+        o1, lse1 = biased_attention(q[b : b + 1].to(DEV), k[rows].to(DEV), v[rows].to(DEV), i32([0, 1]), cu_seqlens_k=i32([0, lens[b]]), softcap=cap, sm_scale=scale)
+        ref, off = orc.decoded(q, k, v, lens, row0, scale, cap, dtype=BF16)
+        near(o1[0], ref[0][b], off[b], "o of a prefill")
+        near_lse(lse1[:, 0], ref[1][b])
