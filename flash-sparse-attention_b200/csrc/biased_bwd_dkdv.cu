@@ -282,7 +282,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
 #pragma unroll
                     for (int j = 0; j < 4; ++j) {
                         const int l = max(lo[j] - m.key0, 0), u = min(hi[j] - m.key0, kTileRows - 1);
-                        const bool sees = u >= l && cc[j] > -INFINITY && cc[j] < INFINITY;     // a row that saw nothing in the forward sees nothing here
+                        const bool sees = u >= l && fabsf(cc[j]) != INFINITY;      // a row that saw nothing in the forward sees nothing here (one that saw NaN has NaN)
                         masked |= sees && (l > 0 || u < m.nkeys - 1);
                         unseen |= !sees && g[j] < p.G;
                         if (!sees) { cc[j] = -INFINITY; del[j] = 0.f; }                        // exp2(s - inf) = 0

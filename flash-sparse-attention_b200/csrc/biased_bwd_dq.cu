@@ -333,7 +333,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
             const float lse_r = row.lse, delta_s = row.delta * p.scale, slope_r = row.slope;
             const int pos_r = row.pos;
             int hi_r = min(row.hi, (int)p.Nk - 1);              // rows past the end of K/V do not exist
-            if (!(lse_r > -INFINITY)) hi_r = lo_r - 1;          // a row that saw nothing in the forward sees nothing here
+            if (lse_r == -INFINITY) hi_r = lo_r - 1;            // a row that saw nothing in the forward sees nothing here (one that saw NaN gets NaN)
             BqItem next;
             next.nblk = next.ne = 0;
             if (forth_and_back(++n) < nitems) next = take_item(n, ok);

@@ -175,8 +175,10 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
                     tmax1 = fmaxf(tmax1, __shfl_xor_sync(0xffffffffu, tmax1, 2));
                 }
                 const float mn0 = fmaxf(m0, tmax0), mn1 = HI ? fmaxf(m1, tmax1) : m1;
+                // (as long as all scores of a row are -inf, every p is exp2(-inf - 0) = 0)
+                const float u0 = mn0 == -INFINITY ? 0.f : mn0, u1 = HI && mn1 != -INFINITY ? mn1 : 0.f;
                 if (__any_sync(0xffffffffu, mn0 > m0 || (HI && mn1 > m1))) {
-                    const float a0 = ex2_approx(m0 - mn0), a1 = HI ? ex2_approx(m1 - mn1) : 1.f;
+                    const float a0 = ex2_approx(m0 - u0), a1 = HI ? ex2_approx(m1 - u1) : 1.f;
                     l0 *= a0;
                     l1 *= a1;
 #pragma unroll
@@ -189,12 +191,12 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
                 }
                 uint32_t pa[4];
                 {
-                    const float e00 = ex2_approx(sc[0][0] - m0), e01 = ex2_approx(sc[0][1] - m0), e10 = ex2_approx(sc[1][0] - m0), e11 = ex2_approx(sc[1][1] - m0);
+                    const float e00 = ex2_approx(sc[0][0] - u0), e01 = ex2_approx(sc[0][1] - u0), e10 = ex2_approx(sc[1][0] - u0), e11 = ex2_approx(sc[1][1] - u0);
                     l0 += e00 + e01 + e10 + e11;
                     pa[0] = ElemTraits<ET>::pack2(e00, e01);
                     pa[2] = ElemTraits<ET>::pack2(e10, e11);
                     if (HI) {
-                        const float f00 = ex2_approx(sc[0][2] - m1), f01 = ex2_approx(sc[0][3] - m1), f10 = ex2_approx(sc[1][2] - m1), f11 = ex2_approx(sc[1][3] - m1);
+                        const float f00 = ex2_approx(sc[0][2] - u1), f01 = ex2_approx(sc[0][3] - u1), f10 = ex2_approx(sc[1][2] - u1), f11 = ex2_approx(sc[1][3] - u1);
                         l1 += f00 + f01 + f10 + f11;
                         pa[1] = ElemTraits<ET>::pack2(f00, f01);
                         pa[3] = ElemTraits<ET>::pack2(f10, f11);
@@ -258,7 +260,7 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float mw = smm[w * 16 + g];
-            if (mw > -INFINITY) o += ex2_approx(mw - M) * so[(size_t)w * NG * D + i];
+            if (sll[w * 16 + g] != 0.f) o += ex2_approx(mw - M) * so[(size_t)w * NG * D + i];        // (0: a warp without keys)
         }
         p.o_part[(pbase + (int64_t)g * p.P) * D + (i - g * D)] = o;
     }
@@ -269,13 +271,13 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
             const float mw = smm[w * 16 + g];
-            if (mw > -INFINITY) L += ex2_approx(mw - M) * sll[w * 16 + g];
+            if (sll[w * 16 + g] != 0.f) L += ex2_approx(mw - M) * sll[w * 16 + g];
         }
         p.ml[pbase + (int64_t)g * p.P] = make_float2(M, L);
     }
 }
 
-// BiasedMerge; 0 and -inf for a row that saw nothing.  WARPS warps a row: what it takes is round trips to L2,
+// BiasedMerge; 0 and -inf for a row that saw nothing (partials whose sum is 0), NaN for one that saw NaN.  WARPS warps a row: what it takes is round trips to L2,
 // so all maxima and sums, and the first AHEAD partials of every warp, are asked for at once (1 x 8191 tokens, 32 heads, 64 partials a row: 12 us with
 // a round trip for every four partials of a warp).  Of few partials many rows: AHEAD 4, whose registers leave room for more warps (16544 rows of 2: 8 us less).
 constexpr int kMgThreads = 128;
@@ -305,7 +307,7 @@ __global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const BiasedMe
     float M = -INFINITY, L = 0.f;
     for (int i = first + w * 32 + lane; i < P; i += 32 * WARPS) {
         const float2 v = __ldcg(mlr + i);
-        if (v.y > 0.f) {
+        if (v.y != 0.f) {
             const float m = fmaxf(M, v.x);
             L = L * ex2_approx(M - m) + v.y * ex2_approx(v.x - m);
             M = m;
@@ -328,7 +330,7 @@ __global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const BiasedMe
     float acc[4] = {0.f, 0.f, 0.f, 0.f};
     auto add = [&](int i, const float (&y)[4]) {
         const float2 v = __ldcg(mlr + i);
-        if (v.y > 0.f) {                // (a partial without keys has no o)
+        if (v.y != 0.f) {               // (a partial without keys has no o)
             const float f = ex2_approx(v.x - M);
 #pragma unroll
             for (int k = 0; k < V; ++k) acc[k] = fmaf(f, y[k], acc[k]);
@@ -352,11 +354,11 @@ __global__ void __launch_bounds__(kMgThreads) biased_decode_merge(const BiasedMe
             acc[0] += y.x; acc[1] += y.y; acc[2] += y.z; acc[3] += y.w;
         }
     }
-    const float inv = L > 0.f ? 1.f / L : 0.f;
+    const float inv = L == 0.f ? 0.f : 1.f / L;
     ET* dst = (ET*)a.o + row * D + lane * V;
     if constexpr (V == 4) *reinterpret_cast<uint2*>(dst) = make_uint2(ElemTraits<ET>::pack2(acc[0] * inv, acc[1] * inv), ElemTraits<ET>::pack2(acc[2] * inv, acc[3] * inv));
     else *reinterpret_cast<uint32_t*>(dst) = ElemTraits<ET>::pack2(acc[0] * inv, acc[1] * inv);
-    if (lane == 0) a.lse[b * a.lse_sn + (row - (int64_t)b * a.Hq) * a.lse_sh] = L > 0.f ? M + log2f(L) : -INFINITY;
+    if (lane == 0) a.lse[b * a.lse_sn + (row - (int64_t)b * a.Hq) * a.lse_sh] = L == 0.f ? -INFINITY : M + log2f(L);
 }
 
 template <int D, bool HI, int MOD, typename ET>

@@ -460,10 +460,12 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
             ok = bar_all(1, 128, ok);
             const bool write = row_valid && ok;
             const int64_t head_row = (int64_t)tok * p.Hq + m.h * G + g;
-            const float inv_l = l_run > 0.f ? 1.f / l_run : 0.f;
+            // (a sum of 0: nothing was seen.  NaN, from NaN or infinity in what was seen, goes on into o and lse)
+            const bool none = l_run == 0.f;
+            const float inv_l = none ? 0.f : 1.f / l_run;
             if (write) {
-                if constexpr (kSplit) launch.ml[head_row * launch.P + m.z] = l_run > 0.f ? make_float2(m_ref, l_run) : make_float2(-INFINITY, 0.f);
-                else p.lse[(int64_t)(m.h * G + g) * p.N + tok] = l_run > 0.f ? m_ref + log2f(l_run) : -INFINITY;
+                if constexpr (kSplit) launch.ml[head_row * launch.P + m.z] = none ? make_float2(-INFINITY, 0.f) : make_float2(m_ref, l_run);
+                else p.lse[(int64_t)(m.h * G + g) * p.N + tok] = none ? -INFINITY : m_ref + log2f(l_run);
             }
 #pragma unroll 1
             for (int c0 = 0; c0 < D; c0 += 32) {
@@ -481,7 +483,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                 }
                 // every thread stores its own row, whole sectors of 32 bytes
                 if constexpr (kSplit) {
-                    if (write && l_run > 0.f)
+                    if (write && !none)
 #pragma unroll
                         for (int i = 0; i < 32; i += 8) st_global32(launch.o_part + (head_row * launch.P + m.z) * D + c0 + i, &a[i]);
                 } else {

@@ -52,7 +52,8 @@ def biased_attention(
         differentiable).  A token that sees nothing, and rows behind the last sequence, get 0 and -inf.
 
     k and v rows that no token sees, and q rows of tokens that see nothing (and their gradients), may hold anything, NaN
-    included.  Gradients are the same bit for bit from run to run.  A CUDA graph can hold the call and its backward; while one is
+    included.  What is seen and not a number goes on as in the formula: a token whose scores hold NaN (or +infinity) gets NaN in o and lse, and so
+    do the gradients that it has a share in.  Gradients are the same bit for bit from run to run.  A CUDA graph can hold the call and its backward; while one is
     captured, no graph made on another stream may hold q, k or v as a leaf (RuntimeError).
     """
     if window_size is not None and window_size < 0:

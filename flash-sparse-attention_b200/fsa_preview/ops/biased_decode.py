@@ -52,7 +52,7 @@ def biased_decode_attention(
     Returns:
         ``o [batch, num_q_heads, head_dim]`` and its log-sum-exp ``[batch, num_q_heads]`` in log2 units; 0 and -inf at idle places.
 
-    Rows behind a sequence may hold anything, NaN included.  No synchronisation: a CUDA graph can hold the call.
+    Rows behind a sequence may hold anything, NaN included; a NaN (or +infinity) among a sequence's scores gives NaN in o and lse.  No synchronisation: a CUDA graph can hold the call.
     """
     return host().biased_decode(q, k, v, seq_len, seq_row0, None, None, None, None, alibi_slopes, q.shape[-1] ** -0.5 if sm_scale is None else float(sm_scale),
                                 0.0 if softcap is None else float(softcap), _window(window_size), int(max_len), 0)

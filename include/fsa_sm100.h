@@ -211,7 +211,8 @@ int fsa_range_attn_bwd_indexed(int head_dim);
  *                    they see nothing (o = 0, lse = -inf) and nobody sees them;
  *   prefix_lens      (int32 per sequence; not with window or doc_ids) and the sequence's first prefix_lens[b] keys besides.
  * k, v: head stride head_dim.  o [N, Hq, D] contiguous, lse [Hq, N] (log2 units); rows behind the last sequence become 0 / -inf.  K/V
- * rows that no token sees, and q and d_o rows of tokens that see nothing, may hold anything, NaN included.  limits: workspace of
+ * rows that no token sees, and q and d_o rows of tokens that see nothing, may hold anything, NaN included; NaN or +infinity among the scores of
+ * what a token sees gives NaN in its o and lse, and in the gradients that it has a share in.  limits: workspace of
  * fsa_biased_attn_limits_bytes bytes, kept for the backward.  scratch: 32-byte aligned, of fsa_biased_attn_fwd_bytes bytes for the same sizes (0: none).
  * head_dim 64 or 128, up to 32 query heads a kv head, fewer than 2^25 tokens and K/V rows, N * num_q_heads below 2^31. */
 int fsa_biased_attn_limits_bytes(int64_t total_tokens, int64_t* bytes_out);

@@ -9,7 +9,7 @@ pytestmark = pytest.mark.gpu
 from fsa.ops import biased_attention
 from fsa_preview.ops import biased_decode_attention, shared_prefix_decode_attention
 from oracle import biased_attn_oracle as orc
-from test_biased_attn_gpu import BF16, DEV, check, cu_of, inputs, near, near_lse
+from test_biased_attn_gpu import BF16, DEV, check, cu_of, inputs, near, near_lse, slopes_of
 from test_biased_decode_gpu import cache_of, i32
 
 
@@ -81,3 +81,97 @@ def test_decode_with_caps_far_above_the_scores(cap, scale, d, G):
         ref, off = orc.decoded(q, k, v, lens, row0, scale, cap, dtype=BF16)
         near(o1[0], ref[0][b], off[b], "o of a prefill")
         near_lse(lse1[:, 0], ref[1][b])
+
+
+SCORES_OF = [(None, False), (20.0, False), (None, True), (50.0, True)]
+
+
+def same_where_finite(o, lse, ref, ref_lse, off):
+    """NaN where the definition has NaN, and only there; the rest as everywhere.  o [rows, heads, d], lse and ref_lse [rows, heads]."""
+    nan = torch.isnan(ref_lse)
+    o, lse = o.detach().cpu(), lse.detach().cpu()
+    assert torch.equal(torch.isnan(lse), nan), "lse"
+    assert torch.equal(torch.isnan(o).all(-1), nan) and torch.equal(torch.isnan(o).any(-1), nan), "o"
+    near(o[~nan], ref[~nan], off[~nan], "o")
+    near_lse(lse[~nan], ref_lse[~nan])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("cap,alibi", SCORES_OF)
+@pytest.mark.parametrize("lens,klens,at,d,dtype", [
+    ([200, 70], [200, 70], 130, 128, BF16),
+    ([200, 70], [200, 70], 131, 64, torch.float16),
+    ([6, 3], [3000, 2500], 1000, 128, BF16),             # cut along the keys: in one chunk of many
+    ([6, 3], [3000, 2500], 2998, 64, BF16),              # seen by the sequence's last tokens only
+])
+def test_what_is_seen_and_not_a_number(lens, klens, at, d, dtype, cap, alibi, bad):
+    """One number of a key that is seen: exactly the tokens whose softmax has no value get NaN, in o and lse, however the work is cut."""
+    Hk, G = 2, 2
+    q, k, v, _ = inputs(lens, klens, Hk, G, d, dtype, 9)
+    k[at, 1, 5] = bad
+    q[:, :, 5] = torch.where(q[:, :, 5] == 0, torch.ones_like(q[:, :, 5]), q[:, :, 5])
+    cu, cuk = cu_of(lens), cu_of(klens)
+    sl = slopes_of(Hk * G) if alibi else None
+    how = dict(softcap=cap, alibi_slopes=None if sl is None else sl.to(DEV), cu_seqlens_k=cuk.to(DEV))
+    o, lse = biased_attention(q.to(DEV), k.to(DEV), v.to(DEV), cu.to(DEV), **how)
+    ref, off = orc.packed(q, k, v, cu, cuk, d ** -0.5, cap or 0.0, sl, dtype=dtype)
+    if bad == bad and cap:                  # the cap makes numbers of infinite scores
+        assert not torch.isnan(ref[1]).any()
+    else:
+        assert torch.isnan(ref[1]).any() and not torch.isnan(ref[1][:G]).any()
+    same_where_finite(o, lse.T, ref[0], ref[1].T, off[0])
+
+
+@pytest.mark.parametrize("bad", [math.nan, math.inf])
+@pytest.mark.parametrize("cap,alibi", SCORES_OF)
+@pytest.mark.parametrize("where", ["own", "prefix", "q"])
+def test_decode_of_what_is_not_a_number(where, cap, alibi, bad):
+    Hk, G, d, P = 2, 4, 128, 200
+    lens = [700, 1, 130]
+    q, k, v, row0 = cache_of(lens, Hk, G, d, BF16, 8)
+    g = torch.Generator().manual_seed(5)
+    pk, pv = (torch.randn(P, Hk, d, generator=g).to(BF16) for _ in range(2))
+    if where == "own":
+        k[row0[0] + 400, 1, 5] = bad
+    elif where == "prefix":
+        pk[77, 1, 5] = bad
+    elif bad == bad:
+        return                              # (infinity in q: infinite scores of both signs)
+    else:
+        q[2, 3, 9] = bad
+    sl = slopes_of(Hk * G) if alibi else None
+    how = dict(max_len=700, softcap=cap, alibi_slopes=None if sl is None else sl.to(DEV))
+    args = [x.to(DEV) for x in (q, k, v)] + [i32(lens), i32(row0)]
+    for mine, (o, lse) in ((None, biased_decode_attention(*args, **how)),
+                           ([(pk, pv)] * 3, shared_prefix_decode_attention(*args, pk.to(DEV), pv.to(DEV), i32([0, P]), i32([0, 3]), **how))):
+        ref, off = orc.decoded(q, k, v, lens, row0, d ** -0.5, cap or 0.0, sl, None, mine, BF16)
+        same_where_finite(o, lse, ref[0], ref[1], off)
+
+
+@pytest.mark.parametrize("cap,alibi", SCORES_OF)
+@pytest.mark.parametrize("lens,d", [([300], 128), ([4000], 64)])
+def test_gradients_of_what_is_not_a_number(lens, d, cap, alibi):
+    """A NaN in one token's q reaches its own dq and the dk and dv of every key that it sees; the other tokens' dq are what they are without it (not bit for
+    bit: which of the two forms of the tanh, each off by 6e-7, a row takes its warp decides)."""
+    t0, n = 170, lens[0]
+    q, k, v, do = inputs(lens, lens, 1, 1, d, BF16, 10)
+    sl, cu = slopes_of(1) if alibi else None, cu_of(lens)
+    ref, off = orc.packed(q, k, v, cu, cu, d ** -0.5, cap or 0.0, sl, do=do, dtype=BF16)
+    q[t0, 0, 3] = math.nan
+    leaves = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    o, _ = biased_attention(*leaves, cu.to(DEV), softcap=cap, alibi_slopes=None if sl is None else sl.to(DEV))
+    dq, dk, dv = torch.autograd.grad(o, leaves, do.to(DEV))
+    assert bool(torch.isnan(dq[t0]).all()) and bool(torch.isnan(dk[: t0 + 1, 0, 3]).all()) and bool(torch.isnan(dv[: t0 + 1]).all())
+    rest = [t for t in range(n) if t != t0]
+    near(dq[rest], ref[2][rest], off[1][rest], "dq")
+    near(dv[t0 + 1 :], ref[4][t0 + 1 :], off[3][t0 + 1 :], "dv")
+
+
+def test_gradients_of_tokens_that_saw_a_key_that_is_not_a_number():
+    lens, at = [260], 130
+    q, k, v, do = inputs(lens, lens, 1, 2, 128, BF16, 11)
+    k[at, 0, 0] = math.nan
+    leaves = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    o, _ = biased_attention(*leaves, cu_of(lens).to(DEV), softcap=20.0)
+    dq, dk, dv = torch.autograd.grad(o, leaves, do.to(DEV))
+    assert bool(torch.isnan(dq[at:]).all()) and bool(torch.isnan(dk).all()) and bool(torch.isnan(dv).all())
