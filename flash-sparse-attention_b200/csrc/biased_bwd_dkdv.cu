@@ -1,7 +1,8 @@
 // dK and dV of attention with changed scores (score.cuh), key-tile-major, for sm_100a: the plan and the products of range_bwd_dkdv.cu (which sums the
 // parts of the K/V tiles that were cut, too).  An item is a tile of 128 K/V rows of one sequence x one KV head x a stretch of tokens, walked in
 // tiles of <= 128 rows (query head of the GQA group, token); a TMEM lane is a K/V row:
-//   S^T = K Q^T, dP^T = V dO^T, P = exp2(s - lse), dS = scale P (dP - delta) ds/dx, dV += P^T dO, dK += dS^T Q.
+//   S^T = K Q^T, dP^T = V dO^T, P = exp2(s - lse), dS = P (dP - delta) ds/dx, dV += P^T dO, dK += scale dS^T Q
+// with the scale in the epilogue, as in biased_bwd_dq.cu.
 // One CTA per SM, 640 threads:
 //   warp 0       TMA producer: K and V of an item, and Q, dO, Q, dO, ... through a ring of five tiles
 //   warp 1       issues S(i) and dV(i)            warp 2    issues dP(i) and dK(i)
@@ -66,7 +67,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
     uint8_t* sV = sK + kTile;
     uint8_t* sU = sV + kTile;                        // [kBkUnits] Q, dO, Q, dO, ...
     float* sC = reinterpret_cast<float*>(sU + kBkUnits * kTile);          // [2][128] what a score gets besides: -lse and the bias at the item's first key
-    float* sDel = sC + 2 * 128;                                           // [2][128] scale * delta
+    float* sDel = sC + 2 * 128;                                           // [2][128] delta
     uint8_t* sVis = reinterpret_cast<uint8_t*>(sDel + 2 * 128);           // [2][2][128] first visible row; last one | 128
     uint64_t* bars = reinterpret_cast<uint64_t*>(sVis + 4 * 128);
     uint64_t* k_full = bars;            // K of an item has landed
@@ -272,7 +273,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                         if (g[j] < p.G && tok <= m.tok_last) {
                             const int64_t idx = (int64_t)(m.h * p.G + g[j]) * p.plan.N + tok;
                             cc[j] = -__ldg(p.lse + idx);
-                            del[j] = __ldg(p.delta + idx) * p.scale;
+                            del[j] = __ldg(p.delta + idx);
                             lo[j] = __ldg(p.plan.kv_lo + tok);
                             hi[j] = __ldg(p.plan.kv_hi + tok);
                         }
@@ -436,15 +437,14 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                     uint32_t d[32];
                     tmem_ld32(tP, d);
                     tmem_ld_wait();
-                    const uint64_t g2 = f32x2(p.scale, p.scale);
 #pragma unroll
                     for (int j = 0; j < 8; ++j) {
                         const float4 dl = del4[j];
                         const int k = 4 * j;
                         const float2 x = f32x2_get(mul_f32x2(f32x2(__uint_as_float(v[k]), __uint_as_float(v[k + 1])),
-                                                             fma_f32x2(f32x2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), g2, f32x2(-dl.x, -dl.y))));
+                                                             add_f32x2(f32x2(__uint_as_float(d[k]), __uint_as_float(d[k + 1])), f32x2(-dl.x, -dl.y))));
                         const float2 y = f32x2_get(mul_f32x2(f32x2(__uint_as_float(v[k + 2]), __uint_as_float(v[k + 3])),
-                                                             fma_f32x2(f32x2(__uint_as_float(d[k + 2]), __uint_as_float(d[k + 3])), g2, f32x2(-dl.z, -dl.w))));
+                                                             add_f32x2(f32x2(__uint_as_float(d[k + 2]), __uint_as_float(d[k + 3])), f32x2(-dl.z, -dl.w))));
                         pk[2 * j] = ElemTraits<ET>::pack2(x.x, x.y);
                         pk[2 * j + 1] = ElemTraits<ET>::pack2(y.x, y.y);
                     }
@@ -483,6 +483,10 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                 if (c0 + 32 == kOwn && m.n > 0) {
                     tc_fence_before();
                     mbar_arrive(half ? dk_free : dv_free);            // the accumulator may take the next item
+                }
+                if (half) {
+#pragma unroll
+                    for (int j = 0; j < 32; ++j) a[j] = __float_as_uint(__uint_as_float(a[j]) * p.scale);
                 }
                 if (write && m.slab >= 0) {
 #pragma unroll

@@ -1,6 +1,8 @@
 // dQ of attention with changed scores (score.cuh), query-tile-major, for sm_100a: the tiling of the forward (biased_fwd.cu), per K/V tile of 64 rows
-//   S = Q K^T, dP = dO V^T, P = exp2(s - lse), dS = scale P (dP - delta) ds/dx, dQ (+)= dS K
-// with ds/dx = 1 - tanh^2 under a cap; dQ accumulated in TMEM over the tiles and written once.  One CTA per SM, 640 threads:
+//   S = Q K^T, dP = dO V^T, P = exp2(s - lse), dS = P (dP - delta) ds/dx, dQ (+)= dS K
+// with ds/dx = 1 - tanh^2 under a cap; dQ accumulated in TMEM over the tiles, multiplied with the scale and written once.  (dS without the scale: 1 / 11 of it
+// at head size 128, it would lose three bits more of small gradients to fp16's subnormal numbers: dq over 4096 keys, dO of size 1e-3, was off by 9.1e-7 and is by less than 1.8e-7.
+// The other end of fp16: P (dP - delta) up to 65504.)  One CTA per SM, 640 threads:
 //   warp 0       TMA producer: Q and dO tiles of every item, (K, V) tiles through a ring of kBqStages
 //   warp 1       one elected thread issues S and dP (two TMEM buffers)      warp 2    ... dQ
 //   warp 3       finds the items, up to four ahead, longest first
@@ -330,7 +332,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
             const bool row_valid = g < p.G && e < m.ne;
             const int tok = m.tok0 + e;
             const int lo_r = row.lo;
-            const float lse_r = row.lse, delta_s = row.delta * p.scale, slope_r = row.slope;
+            const float lse_r = row.lse, delta_r = row.delta, slope_r = row.slope;
             const int pos_r = row.pos;
             int hi_r = min(row.hi, (int)p.Nk - 1);              // rows past the end of K/V do not exist
             if (lse_r == -INFINITY) hi_r = lo_r - 1;            // a row that saw nothing in the forward sees nothing here (one that saw NaN gets NaN)
@@ -359,7 +361,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
                     // bit i: column cb + i is seen
                     const int v_lo = min(max(c_lo - cb, 0), HC), v_hi = min(max(c_hi - cb, 0), HC);
                     const uint32_t vis = v_hi > v_lo ? (0xffffffffu >> (HC - v_hi + v_lo)) << v_lo : 0u;
-                    const uint64_t s2 = f32x2(to_log2, to_log2), g2 = f32x2(p.scale, p.scale), d2 = f32x2(-delta_s, -delta_s), one2 = f32x2(1.f, 1.f);
+                    const uint64_t s2 = f32x2(to_log2, to_log2), d2 = f32x2(-delta_r, -delta_r), one2 = f32x2(1.f, 1.f);
                     const float rel = (float)(pos_r - R0 - cb);
                     const float base = (MOD & kModBias) ? fmaf(-slope_r, rel, -lse_r) : -lse_r;
                     // dS of the columns, two at a time.  NEAR: products whose tanh is near's, else sv has been changed already; BOTH: keys behind the token's
@@ -375,7 +377,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
                             uint64_t x = f32x2(__uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
                             if constexpr (decltype(is_near)::on) x = mul_f32x2(x, near.slope(x));
                             const float2 s = f32x2_get(fma_f32x2(x, s2, f32x2(b0, b1)));
-                            uint64_t gr = fma_f32x2(f32x2(__uint_as_float(dv[i]), __uint_as_float(dv[i + 1])), g2, d2);
+                            uint64_t gr = add_f32x2(f32x2(__uint_as_float(dv[i]), __uint_as_float(dv[i + 1])), d2);
                             // d tanh(x) = 1 - tanh(x)^2
                             if constexpr (MOD & kModCap) {
                                 const float2 th = f32x2_get(x);
@@ -458,6 +460,8 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
                 tmem_ld_wait();
                 tc_fence_before();
                 mbar_arrive(dq_free);            // the accumulator may take the next item
+#pragma unroll
+                for (int i = 0; i < kOwn; ++i) a[i] = __float_as_uint(__uint_as_float(a[i]) * p.scale);
             } else {
 #pragma unroll
                 for (int i = 0; i < kOwn; ++i) a[i] = 0u;

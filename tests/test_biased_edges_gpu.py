@@ -175,3 +175,43 @@ def test_gradients_of_tokens_that_saw_a_key_that_is_not_a_number():
     o, _ = biased_attention(*leaves, cu_of(lens).to(DEV), softcap=20.0)
     dq, dk, dv = torch.autograd.grad(o, leaves, do.to(DEV))
     assert bool(torch.isnan(dq[at:]).all()) and bool(torch.isnan(dk).all()) and bool(torch.isnan(dv).all())
+
+
+def spread(x, dtype):
+    """Variance of a value's rounding error, at most: uniform within half a step each way, which below the normal numbers is that of the smallest one."""
+    half = torch.finfo(dtype).eps / 2
+    return (half * x.abs()).clamp(min=torch.finfo(dtype).smallest_normal * half) ** 2 / 3
+
+
+@pytest.mark.parametrize("size", [1e-2, 1e-3, 1e-4])
+@pytest.mark.parametrize("cap", [None, 20.0])
+@pytest.mark.parametrize("d", [64, 128])
+def test_small_gradients_in_fp16(d, cap, size):
+    """300 tokens over 4096 keys, dO as small as without loss scaling: dS = P (dP - delta) lies among fp16's subnormal numbers.  Its rounding, P's, o's and the results'
+    are independent of one another: their variances add up through the sums, and what is measured over some 40000 numbers may be 1.25 times the root of that."""
+    dtype, lens, klens, G, scale = torch.float16, [300], [4096], 2, d ** -0.5
+    q, k, v, do = inputs(lens, klens, 1, G, d, dtype, 12)
+    do = (do.double() * size).to(dtype)
+    leaves = [x.to(DEV).requires_grad_() for x in (q, k, v)]
+    o, _ = biased_attention(*leaves, cu_of(lens).to(DEV), cu_seqlens_k=cu_of(klens).to(DEV), softcap=cap)
+    got = [x.double() for x in torch.autograd.grad(o, leaves, do.to(DEV))]
+    q, k, v, do = (x.double().to(DEV) for x in (q, k[:, 0], v[:, 0], do))
+    seen, dist = (x.to(DEV) for x in orc.visible(300, 4096))
+    sums = [0.0] * 4
+    for h in range(G):
+        _, lse, dq, dk, dv = orc.one_head(q[:, h], k, v, seen, dist, scale, cap or 0.0, do=do[:, h])[0]
+        x = scale * (q[:, h] @ k.T)
+        th = torch.tanh(x / cap) if cap else torch.zeros_like(x)
+        p = torch.exp2((cap * th if cap else x) / math.log(2.0) - lse[:, None]).masked_fill(~seen, 0.0)
+        inner = p * (1 - th * th)
+        out = p @ v
+        ds = inner * (do[:, h] @ v.T - (out * do[:, h]).sum(1, keepdim=True))
+        of_o = spread(p, dtype) * seen @ v ** 2 + spread(out, dtype)
+        of_delta = (of_o * do[:, h] ** 2).sum(1, keepdim=True)
+        of_ds = spread(ds, dtype) * seen
+        of_dq = scale ** 2 * (of_ds @ k ** 2 + of_delta * (inner @ k) ** 2) + spread(dq, dtype)
+        assert float((got[0][:, h] - dq).square().mean().sqrt()) <= 1.25 * float(of_dq.mean().sqrt()), f"dq of head {h}"
+        sums = [a + b for a, b in zip(sums, (dk, dv, scale ** 2 * (of_ds.T @ q[:, h] ** 2 + (inner ** 2).T @ (of_delta * q[:, h] ** 2)),
+                                             (spread(p, dtype) * seen).T @ do[:, h] ** 2))]
+    for name, x, ref, of in zip(("dk", "dv"), got[1:], sums[:2], sums[2:]):
+        assert float((x[:, 0] - ref).square().mean().sqrt()) <= 1.25 * float((of + spread(ref, dtype)).mean().sqrt()), name
