@@ -38,14 +38,16 @@ struct BiasedKvParams {
     ScoreMod mod;
 };
 
+// (Plan, limits and delta are from the kernel before dQ, which every dQ CTA has waited for before it let this kernel start; this one waits at its end
+// only.  They are read through L2: the non-coherent path need not see what was written while a kernel before ran.)
 // One work item: K/V rows [key0, key0 + nkeys) of head h, n row tiles of TPT tokens from tok0 on, tokens up to tok_last.
 struct BkItem {
     int h, key0, nkeys, tok0, tok_last, n, slab;
 };
 __device__ __forceinline__ BkItem bk_item(const RangeKvPlan& p, int w) {
     BkItem m;
-    const int4 it = __ldg(p.items + w / p.Hk);
-    const int4 t = __ldg(p.tiles + it.x);
+    const int4 it = __ldcg(p.items + w / p.Hk);
+    const int4 t = __ldcg(p.tiles + it.x);
     m.h = w % p.Hk;
     m.key0 = t.x; m.nkeys = t.y;
     m.tok0 = t.z + it.y * p.TPT;
@@ -117,7 +119,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
     __syncthreads();
     tc_fence_after();
     const uint32_t tbase = tmem_slot;
-    const int nitems = __ldg(p.plan.counts) * p.plan.Hk;
+    const int nitems = __ldcg(p.plan.counts) * p.plan.Hk;
     const int TPT = p.plan.TPT;
     // Item n of this CTA: every warp but the producer's takes each of them once, in order; below 0 ends the list.
     auto take_item = [&](int n, bool& ok) {
@@ -259,9 +261,9 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                 float slope[4] = {0.f, 0.f, 0.f, 0.f};
                 int far = 0;            // from the item's first key to its first token's place
                 if ((MOD & kModBias) && m.n > 0 && !p.mod.ahead) {
-                    far = __ldg(p.mod.pos + m.tok0) - m.key0;
+                    far = __ldcg(p.mod.pos + m.tok0) - m.key0;
 #pragma unroll
-                    for (int j = 0; j < 4; ++j) slope[j] = g[j] < p.G ? __ldg(p.mod.slopes + m.h * p.G + g[j]) * kLog2e : 0.f;
+                    for (int j = 0; j < 4; ++j) slope[j] = g[j] < p.G ? __ldcg(p.mod.slopes + m.h * p.G + g[j]) * kLog2e : 0.f;
                 }
                 for (int i = 0; i < m.n && warp_stays(ok); ++i, ++c) {
                     float cc[4], del[4];
@@ -272,10 +274,10 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                         cc[j] = -INFINITY; del[j] = 0.f; lo[j] = 0; hi[j] = -1;
                         if (g[j] < p.G && tok <= m.tok_last) {
                             const int64_t idx = (int64_t)(m.h * p.G + g[j]) * p.plan.N + tok;
-                            cc[j] = -__ldg(p.lse + idx);
-                            del[j] = __ldg(p.delta + idx);
-                            lo[j] = __ldg(p.plan.kv_lo + tok);
-                            hi[j] = __ldg(p.plan.kv_hi + tok);
+                            cc[j] = -__ldcg(p.lse + idx);
+                            del[j] = __ldcg(p.delta + idx);
+                            lo[j] = __ldcg(p.plan.kv_lo + tok);
+                            hi[j] = __ldcg(p.plan.kv_hi + tok);
                         }
                     }
                     bool masked = false, unseen = false;
@@ -324,9 +326,9 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
         int c = 0, qi = 0;
         for (int n = 0, w; (w = take_item(n, ok)) >= 0 && warp_stays(ok); ++n) {
             const BkItem m = bk_item(p.plan, w);
-            const float q_slope = (MOD & kModBias) ? __ldg(p.mod.slopes + m.h * p.G + q_g) * kLog2e : 0.f;
+            const float q_slope = (MOD & kModBias) ? __ldcg(p.mod.slopes + m.h * p.G + q_g) * kLog2e : 0.f;
             // with keys behind a token's place: place of this K/V row before (negative) or behind the item's first token
-            const int key_rel = (MOD & kModBias) && p.mod.ahead && m.n > 0 ? m.key0 + key - __ldg(p.mod.pos + m.tok0) : 0;
+            const int key_rel = (MOD & kModBias) && p.mod.ahead && m.n > 0 ? m.key0 + key - __ldcg(p.mod.pos + m.tok0) : 0;
             for (int i = 0; i < m.n && warp_stays(ok); ++i, ++c) {
                 const int b = c & 1;
                 ok = ok && mbar_wait(&st_full[b], (c >> 1) & 1, status);

@@ -420,7 +420,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
                     // K rows that no row of the item sees are multiplied by dS = 0: zeros take the place of what may be NaN (the tile's S is
                     // done).  Every thread of the buffer's two groups has a quarter of one of the 64 rows.
                     const int kr = R0 + (r & (BK - 1)), part = sb * 2 + (r >> 6);
-                    const bool unseen = kr > m.row_hi || (p.mod.key_ids && __ldg(p.mod.key_ids + kr) < 0);
+                    const bool unseen = kr > m.row_hi || (p.mod.key_ids && __ldcg(p.mod.key_ids + kr) < 0);
                     if (__any_sync(0xffffffffu, unseen)) {
                         if (unseen && ok)
 #pragma unroll

@@ -49,19 +49,19 @@ __global__ void __launch_bounds__(512) range_key_tiles(const RangeKvPlan p, uint
     if (blockIdx.x == gridDim.x - 1) {
         if (tid == 0 && status) *status = kStatusOk;
         const int64_t row16 = (int64_t)p.Hk * p.D / 8;
-        for (int64_t i = (int64_t)__ldg(p.cu_k + p.B) * row16 + tid; i < p.Nk * row16; i += blockDim.x) {
+        for (int64_t i = (int64_t)__ldcg(p.cu_k + p.B) * row16 + tid; i < p.Nk * row16; i += blockDim.x) {
             dk[i] = make_uint4(0u, 0u, 0u, 0u);
             dv[i] = make_uint4(0u, 0u, 0u, 0u);
         }
         return;
     }
     int seq, key0, nkeys;
-    find_seq_tile(p.cu_k, p.B, kTileRows, (int)blockIdx.x, lane, seq, key0, nkeys);
+    find_seq_tile<true>(p.cu_k, p.B, kTileRows, (int)blockIdx.x, lane, seq, key0, nkeys);
     if (seq < 0) {
         if (tid == 0) p.tiles[blockIdx.x] = make_int4(0, 0, 0, -1);
         return;
     }
-    const int t0 = __ldg(p.cu_q + seq), t1 = __ldg(p.cu_q + seq + 1), k0 = __ldg(p.cu_k + seq), key1 = key0 + nkeys - 1;
+    const int t0 = __ldcg(p.cu_q + seq), t1 = __ldcg(p.cu_q + seq + 1), k0 = __ldcg(p.cu_k + seq), key1 = key0 + nkeys - 1;
     int first = INT_MAX, last = -1;
     for (int base = t0 + tid; base < t1; base += 512 * 8) {
         int l[8], u[8];
@@ -96,10 +96,10 @@ template <int D, typename ET>
 __global__ void __launch_bounds__(256) range_dkdv_reduce(const RangeKvPlan p, const float4* __restrict__ slabs, ET* __restrict__ dk, ET* __restrict__ dv) {
     follow();
     constexpr int kChunks = D / 8, kParts = 2 * kChunks * 128 / 256;
-    const int64_t units = (int64_t)__ldg(p.counts + 1) * p.Hk * kParts;       // 2 x kChunks x 128 chunks of 8 columns per tile and head, 256 a CTA
+    const int64_t units = (int64_t)__ldcg(p.counts + 1) * p.Hk * kParts;       // 2 x kChunks x 128 chunks of 8 columns per tile and head, 256 a CTA
     for (int64_t w = blockIdx.x; w < units; w += gridDim.x) {
         const int part = (int)(w % kParts), h = (int)(w / kParts % p.Hk);
-        const int4 m = __ldg(p.multi + w / kParts / p.Hk);
+        const int4 m = __ldcg(p.multi + w / kParts / p.Hk);
         const int u = part * 256 + threadIdx.x, key = u & 127, chunk = (u >> 7) % kChunks, which = (u >> 7) / kChunks;
         if (key >= m.y) continue;
         float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};

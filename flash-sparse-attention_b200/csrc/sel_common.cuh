@@ -238,6 +238,7 @@ __device__ __forceinline__ int count_seq_tiles(const int32_t* __restrict__ cu_q,
     return total;
 }
 // tile `want` of the list: its sequence (-1 if there is no such tile), first token and number of tokens
+template <bool CG = false>
 __device__ __forceinline__ void find_seq_tile(const int32_t* __restrict__ cu_q, int B, int TPT, int want, int lane, int& seq, int& tok0,
                                              int& ne) {
     seq = -1; tok0 = 0; ne = 0;
@@ -245,7 +246,7 @@ __device__ __forceinline__ void find_seq_tile(const int32_t* __restrict__ cu_q, 
     int acc = 0;
     for (int b0 = 0; b0 < B; b0 += 32) {
         const int b = b0 + lane;
-        const int s0 = b < B ? __ldg(cu_q + b) : 0, L = b < B ? __ldg(cu_q + b + 1) - s0 : 0;
+        const int s0 = b < B ? ld_cg<CG>(cu_q + b) : 0, L = b < B ? ld_cg<CG>(cu_q + b + 1) - s0 : 0;
         const int nt = (L + TPT - 1) / TPT;
         int incl = nt;                                   // inclusive prefix over the 32 sequences
 #pragma unroll

@@ -183,3 +183,18 @@ def test_rows_that_a_token_sees(limits, k0, k1, q1, window, prefix):
         lo, hi, at = limits(tok, k0, k1, q1, window, prefix)
         assert at == pos and list(range(lo, min(hi, lo + 10 ** 4) + 1)) == seen
         assert hi < k1
+
+
+@pytest.mark.parametrize("name,kernels", [
+    ("biased_attn.cu", None), ("biased_fwd.cu", None), ("biased_bwd_dq.cu", None), ("biased_bwd_dkdv.cu", None), ("biased_decode.cu", None),
+    ("range_bwd_dkdv.cu", ["range_key_tiles(const", "range_plan_items(const", "range_dkdv_reduce(const"]),
+])
+def test_kernels_that_start_early_read_nothing_by_the_non_coherent_path(name, kernels):
+    """Such a load may be moved before the wait for the kernels before, or be answered from what was there while one of them still ran.  (A breach shows only in a
+    run that a load wins by chance.)"""
+    with open(os.path.join(CSRC, name)) as f:
+        text = re.sub(r"//[^\n]*", "", f.read())
+    for part in [text] if kernels is None else [function(name, head) for head in kernels]:
+        part = re.sub(r"//[^\n]*", "", part)
+        assert "__ldg(" not in part and "ld.global.nc" not in part
+        assert not re.findall(r"find_seq\(|find_seq_tile\(|count_seq_tiles\(", part)       # (they load that way unless told otherwise)
