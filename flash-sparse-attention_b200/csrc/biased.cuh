@@ -8,6 +8,26 @@ namespace fsa {
 constexpr int kBiasedBK = 64;       // K/V rows of a tile
 constexpr int kBiasedLeast = 4;     // K/V tiles of a chunk (an item's beginning and end are as long as 4 to 5 of them)
 
+// The operators' status word (one a device): what a wait that ran out left, and above it when that was, in units of 2^30 ns of the device's timer.
+// The later CTAs of a launch that has failed are not to take 0.2 s each for their waits: up to two units after a failure waits are short.  What
+// failed before that is over, whoever has read it or not.  (biased_bwd_dq and _dkdv, whose CTAs all run at once, leave the time out.)
+constexpr int kStampBits = 22;
+__device__ __forceinline__ int now_stamp() {
+    uint64_t t;
+    asm volatile("mov.u64 %0, %%globaltimer;" : "=l"(t));
+    return (int)(t >> 30) & ((1 << kStampBits) - 1);
+}
+__device__ __forceinline__ void stamp_status(int* word, int status) { atomicMax(word, now_stamp() << 8 | status); }
+__device__ __forceinline__ uint32_t stamped_wait_limit(const int* word) {
+    const int failed = *reinterpret_cast<const volatile int*>(word);
+    return failed && ((now_stamp() - (failed >> 8)) & ((1 << kStampBits) - 1)) < 2 ? FSA_WAIT_CLOCKS / 64 : FSA_WAIT_CLOCKS;
+}
+__device__ __forceinline__ bool mbar_wait_stamped(uint64_t* bar, uint32_t parity, int* word, uint32_t limit) {
+    if (mbar_poll(bar, parity, limit)) return true;
+    stamp_status(word, kStatusWaitTimeout);
+    return false;
+}
+
 struct BiasedFwdParams {
     const int32_t* cu_q;    // [B + 1]
     const int32_t* cu_k;    // [B + 1] first K/V row of every sequence

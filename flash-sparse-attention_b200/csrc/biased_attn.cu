@@ -13,7 +13,7 @@ int make_tile_map_3d_box(CUtensorMap* map, const void* base, int dtype, int64_t 
                          int64_t stride2, int box1, int box2);
 int cuda_failed(cudaError_t e);
 
-// Set (atomicMax) by a kernel of these operators whose bounded wait ran out; read with fsa_biased_read_status.
+// Set (biased.cuh) by a kernel of these operators whose bounded wait ran out; read, and cleared, with fsa_biased_read_status.
 static __device__ int g_biased_status;
 
 // Its address on the current device (once per thread and device: a driver call).
@@ -468,5 +468,33 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
 
 extern "C" int fsa_biased_read_status(int* status_out) {
     if (!status_out) return FSA_ERR_BAD_ARG;
-    return cudaMemcpyFromSymbol(status_out, g_biased_status, sizeof(int)) == cudaSuccess ? FSA_OK : FSA_ERR_CUDA;
+    // (of all streams: torch's own do not wait for the legacy one, which the copies go through)
+    int word = 0;
+    const int none = 0;
+    cudaError_t e = cudaDeviceSynchronize();
+    if (e == cudaSuccess) e = cudaMemcpyFromSymbol(&word, g_biased_status, sizeof(int));
+    if (e == cudaSuccess && word) e = cudaMemcpyToSymbol(g_biased_status, &none, sizeof(int));
+    *status_out = word & 255;
+    return e == cudaSuccess ? FSA_OK : cuda_failed(e);
+}
+
+// A wait of these operators that runs out, harmlessly: nobody arrives at the barrier.
+static __global__ void biased_wait_timeout_probe(int* word) {
+    __shared__ uint64_t bar;
+    if (threadIdx.x == 0) {
+        mbar_init(&bar, 1);
+        mbar_init_fence();
+        mbar_wait_stamped(&bar, 0, word, stamped_wait_limit(word));
+    }
+}
+
+extern "C" int fsa_biased_debug_wait_timeout(void* stream_) {
+    (void)cudaGetLastError();
+    int* word = nullptr;
+    cudaError_t e = biased_status_word(&word);
+    if (e == cudaSuccess) {
+        biased_wait_timeout_probe<<<1, 32, 0, (cudaStream_t)stream_>>>(word);
+        e = cudaGetLastError();
+    }
+    return e == cudaSuccess ? FSA_OK : cuda_failed(e);
 }

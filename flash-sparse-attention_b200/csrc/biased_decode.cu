@@ -49,7 +49,7 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
     constexpr int NK = D / 16;                           // k-steps of Q K^T
     constexpr int NO = D / 8;                            // 8-column output tiles of P V
     unsigned char* base = reinterpret_cast<unsigned char*>((reinterpret_cast<uintptr_t>(dsm_raw) + 1023) & ~uintptr_t(1023));
-    const uint32_t limit = wait_limit(p.status);
+    const uint32_t limit = stamped_wait_limit(p.status);
     uint64_t* full = reinterpret_cast<uint64_t*>(base + (size_t)kBdStages * STAGE_BYTES);
     uint64_t* empty = full + kBdStages;
     float* smm = reinterpret_cast<float*>(empty + kBdStages);    // [4][16]
@@ -90,7 +90,7 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
             const int row = p.row0[b] + lo;
             for (int it = 0; it * kBdKT < n; ++it) {
                 const int s = it % kBdStages;
-                if (it >= kBdStages && !mbar_wait(&empty[s], ((it / kBdStages) - 1) & 1, p.status, limit)) break;
+                if (it >= kBdStages && !mbar_wait_stamped(&empty[s], ((it / kBdStages) - 1) & 1, p.status, limit)) break;
                 mbar_expect_tx(&full[s], STAGE_BYTES);
                 const uint32_t kb = sbase + s * STAGE_BYTES;
 #pragma unroll
@@ -127,7 +127,7 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
         bool ok = true;
         for (int it = 0; it * kBdKT < n; ++it) {
             const int s = it % kBdStages;
-            ok = mbar_wait(&full[s], (it / kBdStages) & 1, p.status, limit);
+            ok = mbar_wait_stamped(&full[s], (it / kBdStages) & 1, p.status, limit);
             if (!warp_stays(ok)) break;
             const int k0 = it * kBdKT + warp * 16;               // first key of this warp's tile
             if (k0 < n) {

@@ -69,7 +69,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
 
     const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
     const BiasedFwdParams& p = launch.p;
-    const uint32_t limit = wait_limit(p.status);
+    const uint32_t limit = stamped_wait_limit(p.status);
     const int G = p.G, TPT = p.TPT;
     // First and last K/V row that a token sees, and its place.  kModSplit: with shared rows a token is a sequence of the batch, whose own rows
     // follow them.
@@ -504,7 +504,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
     __syncthreads();
     if (warp == 1) tmem_dealloc(tbase, kCols);
     if (beside) follow_late();
-    if (tid == 0 && *status != kStatusOk && p.status) atomicMax(p.status, *status);
+    if (tid == 0 && *status != kStatusOk) stamp_status(p.status, *status);
 }
 
 template <int D, int MOD, typename ET>

@@ -93,6 +93,7 @@ SIGNATURES = {
         [c_void_p] * 3 + [c_int64] * 3 + [c_void_p] * 4 + [c_int64] * 3 + [c_void_p] * 2 + [c_int, c_void_p] + [c_int] * 5 + [c_float] * 2
         + [c_int] + [c_int64] * 2 + [c_void_p] * 3 + [c_int64, c_void_p]),
     "fsa_biased_read_status": (c_int, [POINTER(c_int)]),
+    "fsa_biased_debug_wait_timeout": (c_int, [c_void_p]),
     "fsa_linear_compress_fwd": (
         c_int, [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p, c_void_p, c_void_p]),
     "fsa_compress_bias_scratch_bytes": (c_int64, [c_int, c_int]),

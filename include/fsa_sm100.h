@@ -237,8 +237,10 @@ int fsa_biased_decode(const void* q, const void* k, const void* v, int64_t kv_ro
                       int64_t shared_v_stride_n, const int32_t* cu_shared, const int32_t* cu_group, int num_groups, const float* slopes, int batch,
                       int num_q_heads, int num_kv_heads, int head_dim, int dtype, float sm_scale, float softcap, int window, int64_t max_len,
                       int64_t max_shared, void* o, float* lse, void* scratch, int64_t scratch_bytes, void* stream);
-/* What the waits of these operators' kernels left on the current device: 0, or that one ran out (synchronises). */
+/* What the waits of these operators' kernels have left on the current device since the last call: 0, or that one ran out (waits for the device). */
 int fsa_biased_read_status(int* status_out);
+/* For tests: a kernel whose wait runs out after 0.2 s (3 ms up to two seconds after another one that did), on the same status word. */
+int fsa_biased_debug_wait_timeout(void* stream);
 /* fsa_biased_attn_fwd's gradient.  dq, dk, dv contiguous; every row of them is written.  limits: what the forward left.  Bit-reproducible. */
 int fsa_biased_attn_bwd_bytes(int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window,
                               int64_t* bytes_out);
