@@ -127,8 +127,8 @@ static cudaError_t launch_limits(const int32_t* cu_q, const int32_t* cu_k, const
 }
 
 // ------------------------------------------------------------------------------------------------ what the backward's kernels need
-// One launch: CTA 0 plans the items of dK / dV, the others work out delta = sum_d o dO, without documents the limits, and clear what lies behind the
-// last sequences.  Without documents the stretch of tokens that sees a tile of K/V rows follows from the rule: from the token at the tile's first row
+// One launch: CTA 0 plans the items of dK / dV, the others work out delta = sum_d o dO, without documents the limits, and clear what lies outside of the
+// sequences.  Without documents the stretch of tokens that sees a tile of K/V rows follows from the rule: from the token at the tile's first row
 // (with a prefix that the tile is part of: the sequence's first) to the one at its last row (with a window: that far behind).  2 x 8192 tokens, 8 heads
 // of 128: 15 us, bound by memory (67 MB of o and dO); delta alone took 20, limits, stretches and plan a launch each besides.
 struct BiasedPrep {
@@ -208,6 +208,8 @@ __global__ void __launch_bounds__(kPrThreads) biased_prep(const BiasedPrep p) {
         }
         for (int64_t i = (int64_t)__ldcg(p.plan.cu_k + B) * row16 + me; i < p.plan.Nk * row16; i += all) p.dk[i] = p.dv[i] = make_uint4(0u, 0u, 0u, 0u);
     }
+    // (K/V rows in front of the first sequence: where cu_seqlens_k is a part of a longer one)
+    for (int64_t i = me; i < (int64_t)__ldcg(p.plan.cu_k) * row16; i += all) p.dk[i] = p.dv[i] = make_uint4(0u, 0u, 0u, 0u);
     for (int64_t i = (int64_t)__ldcg(p.plan.cu_q + B) * qrow16 + me; i < N * qrow16; i += all) p.dq[i] = make_uint4(0u, 0u, 0u, 0u);
     // delta: L lanes a row of one head, U rows of a thread in flight
     const int part = tid % L;

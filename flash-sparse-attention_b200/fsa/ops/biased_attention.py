@@ -37,7 +37,7 @@ def biased_attention(
         q: ``[total_len, num_q_heads, head_dim]`` bf16/fp16, head_dim 64 or 128
         k, v: ``[total_kv_len, num_kv_heads, head_dim]``, up to 32 query heads a kv head
         cu_seqlens: ``[batch + 1]`` int32, 0 first, where the sequences begin in q (and in k and v, unless cu_seqlens_k is given)
-        cu_seqlens_k: ``[batch + 1]`` int32: where they begin in k and v.  The queries of a sequence are its last tokens, as in
+        cu_seqlens_k: ``[batch + 1]`` int32: where they begin in k and v (rows in front of the first are nobody's).  The queries of a sequence are its last tokens, as in
             a chunked prefill: query i of Lq stands at place ``t = Lk - Lq + i`` of the Lk keys (and sees none where t < 0)
         sm_scale: defaults to ``1/sqrt(head_dim)``
         softcap: cap of the scores; None (or 0): none

@@ -210,7 +210,7 @@ int fsa_range_attn_bwd_indexed(int head_dim);
  *   doc_ids          (int32 per K/V row) those of its document: the stretch of equal ids around t.  Rows with a negative id are padding:
  *                    they see nothing (o = 0, lse = -inf) and nobody sees them;
  *   prefix_lens      (int32 per sequence; not with window or doc_ids) and the sequence's first prefix_lens[b] keys besides.
- * k, v: head stride head_dim.  o [N, Hq, D] contiguous, lse [Hq, N] (log2 units); rows behind the last sequence become 0 / -inf.  K/V
+ * k, v: head stride head_dim.  cu_seqlens_q[0] is 0.  o [N, Hq, D] contiguous, lse [Hq, N] (log2 units); rows behind the last sequence become 0 / -inf.  K/V
  * rows that no token sees, and q and d_o rows of tokens that see nothing, may hold anything, NaN included; NaN or +infinity among the scores of
  * what a token sees gives NaN in its o and lse, and in the gradients that it has a share in.  limits: workspace of
  * fsa_biased_attn_limits_bytes bytes, kept for the backward.  scratch: 32-byte aligned, of fsa_biased_attn_fwd_bytes bytes for the same sizes (0: none).

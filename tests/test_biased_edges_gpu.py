@@ -215,3 +215,27 @@ def test_small_gradients_in_fp16(d, cap, size):
                                              (spread(p, dtype) * seen).T @ do[:, h] ** 2))]
     for name, x, ref, of in zip(("dk", "dv"), got[1:], sums[:2], sums[2:]):
         assert float((x[:, 0] - ref).square().mean().sqrt()) <= 1.25 * float((of + spread(ref, dtype)).mean().sqrt()), name
+
+
+@pytest.mark.parametrize("how", [{}, {"docs": True}, {"window": 40}, {"prefix": [60, 3]}])
+@pytest.mark.parametrize("lens,klens", [([100, 30], [300, 90]), ([7, 2], [3000, 2100])])
+def test_keys_in_front_of_the_first_sequence(lens, klens, how):
+    """cu_seqlens_k as a part of a longer one: the rows in front of it, of NaN, belong to nobody, and their gradients are 0."""
+    front, Hk, G, d = 333, 1, 2, 128
+    q, k, v, do = inputs(lens, klens, Hk, G, d, BF16, 3)
+    ids = torch.div(torch.arange(sum(klens), dtype=torch.int32), 50, rounding_mode="floor").int() if "docs" in how else None
+    prefix = torch.tensor(how["prefix"], dtype=torch.int32) if "prefix" in how else None
+    ref, off = orc.packed(q, k, v, cu_of(lens), cu_of(klens), d ** -0.5, 20.0, None, how.get("window"), ids, prefix, do, BF16)
+    ahead = lambda x, fill: torch.cat([torch.full((front, *x.shape[1:]), fill, dtype=x.dtype), x]).to(DEV)  # noqa: E731
+    dirt = [torch.full((front + sum(klens), Hk, d), math.nan, dtype=BF16, device=DEV) for _ in range(4)]
+    del dirt                                # (memory for the gradients that does not happen to hold zeros)
+    leaves = [x.requires_grad_() for x in (q.to(DEV), ahead(k, math.nan), ahead(v, math.nan))]
+    o, lse = biased_attention(*leaves, cu_of(lens).to(DEV), cu_seqlens_k=(cu_of(klens) + front).to(DEV), softcap=20.0, window_size=how.get("window"),
+                              doc_ids=None if ids is None else ahead(ids, 0), prefix_lens=None if prefix is None else prefix.to(DEV))
+    near(o.detach(), ref[0], off[0], "o")
+    near_lse(lse, ref[1])
+    dq, dk, dv = torch.autograd.grad(o, leaves, do.to(DEV))
+    near(dq, ref[2], off[1], "dq")
+    for name, got, r, e in (("dk", dk, ref[3], off[2]), ("dv", dv, ref[4], off[3])):
+        near(got[front:], r, e, name)
+        assert bool((got[:front] == 0).all()), name
