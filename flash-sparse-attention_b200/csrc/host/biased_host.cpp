@@ -63,12 +63,19 @@ static void check_lengths(const Tensor& t, const Tensor& q, int64_t n, const cha
     TORCH_CHECK_VALUE(t.device() == q.device(), name, " is on ", t.device(), ", q on ", q.device());
 }
 
+// Forward-mode tangents would be lost where no gradient is asked for (autograd refuses them itself where one is).
+static void check_no_tangents(const char* what, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        TORCH_CHECK_NOT_IMPLEMENTED(!t->defined() || !t->_fw_grad(0).defined(), what, " has no forward-mode derivative: give tensors without tangents");
+}
+
 static Tensor check_slopes(const MaybeTensor& s, const Tensor& q) {
     if (!s) return Tensor();
     TORCH_CHECK_TYPE(s->scalar_type() == at::kFloat, "alibi_slopes has to be float32, got ", s->scalar_type());
     TORCH_CHECK_VALUE(s->dim() == 1 && s->size(0) == q.size(1), "alibi_slopes has to have one entry for each of the ", q.size(1), " query heads, got ", s->sizes());
     TORCH_CHECK_VALUE(s->device() == q.device(), "alibi_slopes is on ", s->device(), ", q on ", q.device());
     TORCH_CHECK_VALUE(!s->requires_grad(), "alibi_slopes has no gradient here: give slopes that need none");
+    check_no_tangents("alibi_slopes", {&*s});
     return s->contiguous();
 }
 
@@ -160,6 +167,7 @@ struct BiasedAttention : torch::autograd::Function<BiasedAttention> {
 std::tuple<Tensor, Tensor> biased_attention(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& cu_q, const MaybeTensor& cu_k_, const MaybeTensor& slopes_,
                                             const MaybeTensor& docs_, const MaybeTensor& prefix_, double scale, double cap, int64_t window) {
     check_qkv(q, k, v);
+    check_no_tangents("biased_attention", {&q, &k, &v});
     TORCH_CHECK_VALUE(cu_q.dim() == 1 && cu_q.size(0) >= 2, "cu_seqlens has to have an entry more than there are sequences, and there is one at least");
     const int64_t B = cu_q.size(0) - 1;
     check_lengths(cu_q, q, -1, "cu_seqlens");
@@ -194,12 +202,14 @@ std::tuple<Tensor, Tensor> biased_decode(const Tensor& q_, const Tensor& k, cons
                                          const MaybeTensor& pv, const MaybeTensor& cu_prefix, const MaybeTensor& cu_group, const MaybeTensor& slopes_, double scale,
                                          double cap, int64_t window, int64_t max_len, int64_t max_prefix) {
     check_qkv(q_, k, v);
+    check_no_tangents("decode", {&q_, &k, &v});
     const int64_t B = q_.size(0), Hq = q_.size(1), D = q_.size(2), Hk = k.size(1);
     check_lengths(seq_len, q_, B, "seq_len");
     check_lengths(row0, q_, B, "seq_row0");
     int64_t groups = 0, prefix_rows = 0;
     if (pk) {
         check_qkv(q_, *pk, *pv);
+        check_no_tangents("decode", {&*pk, &*pv});
         TORCH_CHECK_VALUE(pk->size(1) == Hk, "prefix_k has ", pk->size(1), " heads, k ", Hk);
         TORCH_CHECK_VALUE(cu_prefix->dim() == 1 && cu_prefix->size(0) >= 2, "cu_prefix has to have an entry more than there are prefixes, and there is one at least");
         groups = cu_prefix->size(0) - 1;
