@@ -1,6 +1,9 @@
 // Attention with changed scores (capped, biased by distance) and masks: checks, workspaces, launches and the autograd function.
 #include "host_common.h"
 
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/functions/utils.h>
+
 #include <cmath>
 #include <optional>
 
@@ -157,9 +160,16 @@ struct BiasedAttention : torch::autograd::Function<BiasedAttention> {
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
         const auto t = ctx->get_saved_variables();
+        const bool again = at::GradMode::is_enabled();          // (create_graph)
+        at::NoGradGuard plain;
         auto [dq, dk, dv] = biased_bwd(t[0], t[1], t[2], t[3], t[4], g[0], t[5],
                                        {t[6], t[7], t[8], t[9], t[10], ctx->saved_data["scale"].toDouble(), ctx->saved_data["cap"].toDouble(),
                                         ctx->saved_data["window"].toInt()});
+        if (!again) return {dq, dk, dv, Tensor()};
+        // Their own derivative is not there: whoever asks for it, on the way to what they are made of, is told so instead of getting a gradient that lacks it.
+        const auto none = std::make_shared<torch::autograd::Error>("biased_attention has no second derivative",
+                                                                   torch::autograd::collect_next_edges(t[0], t[1], t[2], g[0]));
+        for (const Tensor& x : {dq, dk, dv}) torch::autograd::set_history(x, none);
         return {dq, dk, dv, Tensor()};
     }
 };

@@ -31,7 +31,7 @@ def biased_attention(
     doc_ids: Optional[torch.Tensor] = None,
     prefix_lens: Optional[torch.Tensor] = None,
 ) -> Tuple[torch.Tensor, torch.Tensor]:
-    """Attention with changed scores, differentiable in q, k and v (in backward mode; forward-mode tangents are refused).
+    """Attention with changed scores, differentiable in q, k and v (once, in backward mode: forward-mode tangents and second derivatives are refused).
 
     Args:
         q: ``[total_len, num_q_heads, head_dim]`` bf16/fp16, head_dim 64 or 128

@@ -239,3 +239,21 @@ def test_keys_in_front_of_the_first_sequence(lens, klens, how):
     for name, got, r, e in (("dk", dk, ref[3], off[2]), ("dv", dv, ref[4], off[3])):
         near(got[front:], r, e, name)
         assert bool((got[:front] == 0).all()), name
+
+
+def test_second_derivatives_are_refused():
+    """create_graph works for the gradients themselves; what depends on them in turn is refused instead of being left out."""
+    lens = [90]
+    q, k, v, do = (x.to(DEV) for x in inputs(lens, lens, 1, 2, 64, BF16, 1))
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+
+    def first(**how):
+        o, _ = biased_attention(*leaves, cu_of(lens).to(DEV), softcap=5.0)
+        return torch.autograd.grad(o, leaves, do, **how)
+
+    want, got = first(), first(create_graph=True)
+    assert all(torch.equal(a, b.detach()) for a, b in zip(want, got))
+    for i in range(3):
+        with pytest.raises(RuntimeError, match="no second derivative"):
+            torch.autograd.grad(got[i].float().square().sum() + sum(x.float().sum() for x in leaves), leaves, retain_graph=True)
+    torch.autograd.grad(first(retain_graph=True)[0].float().sum() + leaves[0].float().sum(), leaves[0])
