@@ -413,7 +413,7 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                             }
                     }
                 }
-                if ((MOD & kModGuard) && masked == 2) {
+                if (masked == 2) {
                     // Q and dO rows that see nothing here are multiplied by dS = P = 0: zeros take the place of what may be NaN.  The half's S and dP
                     // are done; every thread of its two groups has a quarter of one of its 64 rows.
                     ok = ok && mbar_wait(&dp_full[half], c & 1, status);
@@ -524,7 +524,7 @@ static cudaError_t launch_bk(const BiasedKvParams& p, const CUtensorMap* maps, u
 template <int D, typename ET>
 static cudaError_t launch_bk_which(int which, const BiasedKvParams& p, const CUtensorMap* maps, unsigned grid, cudaStream_t stream) {
     switch (which) {
-#define FSA_CASE(M) case M: return launch_bk<D, (M) | kModGuard, ET>(p, maps, grid, stream);
+#define FSA_CASE(M) case M: return launch_bk<D, M, ET>(p, maps, grid, stream);
         FSA_CASE(0) FSA_CASE(kModCap) FSA_CASE(kModBias) FSA_CASE(kModCap | kModBias)
 #undef FSA_CASE
         default: return cudaErrorInvalidValue;

@@ -416,7 +416,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
                 }
                 tmem_st16(tDS, dd);
                 tmem_st_wait();
-                if ((MOD & kModGuard) && (p.mod.key_ids || j + 1 == m.nblk)) {
+                if (p.mod.key_ids || j + 1 == m.nblk) {
                     // K rows that no row of the item sees are multiplied by dS = 0: zeros take the place of what may be NaN (the tile's S is
                     // done).  Every thread of the buffer's two groups has a quarter of one of the 64 rows.
                     const int kr = R0 + (r & (BK - 1)), part = sb * 2 + (r >> 6);
@@ -535,7 +535,7 @@ static cudaError_t launch_bq(const BiasedDqParams& p, const CUtensorMap* maps, u
 template <int D, typename ET>
 static cudaError_t launch_bq_which(int which, const BiasedDqParams& p, const CUtensorMap* maps, unsigned grid, cudaStream_t stream) {
     switch (which) {
-#define FSA_CASE(M) case M: return launch_bq<D, (M) | kModGuard, ET>(p, maps, grid, stream);
+#define FSA_CASE(M) case M: return launch_bq<D, M, ET>(p, maps, grid, stream);
         FSA_CASE(0) FSA_CASE(kModCap) FSA_CASE(kModBias) FSA_CASE(kModCap | kModBias)
 #undef FSA_CASE
         default: return cudaErrorInvalidValue;

@@ -425,7 +425,7 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                 l_run += l2.x + l2.y;
                 tmem_st32(tS, pk);
                 tmem_st_wait();
-                if ((MOD & kModGuard) && (launch.mod.key_ids || t == nblk - 1)) {
+                if (launch.mod.key_ids || t == nblk - 1) {
                     // V rows that no row of the item sees are multiplied by p = 0, but 0 x NaN is NaN: zeros take their place.  Every thread
                     // has half of one of the 64 rows.
                     const int kr = m.row_lo + t * BK + (r & (BK - 1));
@@ -520,7 +520,7 @@ static cudaError_t launch_bf(const BiasedFwdLaunch& l, int max_tiles, cudaStream
 template <int D, typename ET>
 static cudaError_t launch_which(int mod, const BiasedFwdLaunch& l, int max_tiles, cudaStream_t stream) {
     switch (mod) {
-#define FSA_CASE(M) case M: return launch_bf<D, (M) | kModGuard, ET>(l, max_tiles, stream);
+#define FSA_CASE(M) case M: return launch_bf<D, M, ET>(l, max_tiles, stream);
         FSA_CASE(0) FSA_CASE(kModCap) FSA_CASE(kModBias) FSA_CASE(kModCap | kModBias)
         FSA_CASE(kModSplit) FSA_CASE(kModSplit | kModCap) FSA_CASE(kModSplit | kModBias) FSA_CASE(kModSplit | kModCap | kModBias)
 #undef FSA_CASE

@@ -10,9 +10,7 @@ namespace fsa {
 
 constexpr int kModCap = 1;       // tanh cap
 constexpr int kModBias = 2;      // distance bias
-constexpr int kModGuard = 4;     // rows that nobody sees (padding, rows behind a sequence) may hold anything, NaN included
-constexpr int kModSplit = 8;     // K/V rows cut into chunks, unnormalised partial results (forward)
-constexpr int kModScore = kModCap | kModBias;
+constexpr int kModSplit = 4;     // K/V rows cut into chunks, unnormalised partial results (forward)
 
 struct ScoreMod {
     float x_scale;              // scale / cap: from a product to the argument of the tanh

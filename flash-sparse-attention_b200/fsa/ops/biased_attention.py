@@ -3,8 +3,8 @@
 
     s = sm_scale q.k;   s = softcap tanh(s / softcap);   s = s - slope_h |t - j|;   o = softmax(s over the visible j) v
 
-The reference has no such operator; it stands next to the sliding-window branch (``fsa.ops.range_attention``), whose kernels
-are compiled for it too.  One token of every sequence over a K/V cache: ``fsa_preview.ops.biased_decode``.
+The reference has no such operator; it stands next to the sliding-window branch (``fsa.ops.range_attention``), with kernels of
+its own.  One token of every sequence over a K/V cache: ``fsa_preview.ops.biased_decode``.
 """
 from __future__ import annotations
 
