@@ -83,7 +83,8 @@ static Tensor check_slopes(const MaybeTensor& s, const Tensor& q) {
 }
 
 static void check_scores(const Tensor& q, double scale, double cap) {
-    TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale), "sm_scale has to be above 0 and finite, got ", scale);
+    const float log2 = (float)scale * 1.44269504f;         // (as the kernels take it)
+    TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale) && std::isnormal(log2), "sm_scale has to be above 0 and finite, in 32 bits too, got ", scale);
     TORCH_CHECK_VALUE(cap >= 0 && std::isfinite(cap), "softcap has to be above 0 and finite (or None), got ", cap);
     TORCH_CHECK_VALUE(cap == 0 || (cap > 1e-30 && cap < 1e30 && scale / cap > 1e-30 && scale / cap < 1e30),
                       "softcap and sm_scale / softcap have to be between 1e-30 and 1e30, got ", cap, " and ", scale / cap);

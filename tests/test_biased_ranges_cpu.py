@@ -27,3 +27,12 @@ def test_lengths_that_no_cache_has(max_len, max_shared):
     out = ctypes.c_int64(-7)
     assert lib().fsa_biased_decode_bytes(4, 8, 2, 64, 2, max_len, max_shared, -1, ctypes.byref(out)) == FSA_ERR_UNSUPPORTED
     assert out.value == -7
+
+
+@pytest.mark.parametrize("scale", [1e39, 3e38, 1e-50, 1e-40])
+def test_scales_that_leave_32_bits(scale):
+    x = torch.zeros(4, 2, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match="sm_scale"):
+        biased_attention(x, x, x, torch.tensor([0, 4], dtype=torch.int32), sm_scale=scale)
+    with pytest.raises(ValueError, match="sm_scale"):
+        biased_decode_attention(x, x, x, torch.ones(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32), max_len=4, sm_scale=scale)
