@@ -7,6 +7,9 @@ namespace fsa {
 
 constexpr int kBiasedBK = 64;       // K/V rows of a tile
 constexpr int kBiasedLeast = 4;     // K/V tiles of a chunk (an item's beginning and end are as long as 4 to 5 of them)
+// Tiles of `tokens` tokens in B sequences, at most; of all kv heads there are fewer than kBiasedMaxPlaces (32-bit numbers of items and CTAs, some to spare).
+inline int64_t biased_places(int64_t tokens, int TPT, int64_t B) { return (tokens + TPT - 1) / TPT + B; }
+constexpr int64_t kBiasedMaxPlaces = (int64_t)1 << 30;
 
 // The operators' status word (one a device): what a wait that ran out left, and above it when that was, in units of 2^30 ns of the device's timer.
 // The later CTAs of a launch that has failed are not to take 0.2 s each for their waits: up to two units after a failure waits are short.  What

@@ -256,7 +256,8 @@ static int biased_shape(int64_t N, int64_t Nk, int B, int Hq, int Hk, int D, Sel
     *s = SelShape{};
     s->N = N; s->Nk = Nk; s->B = B; s->Hq = Hq; s->Hk = Hk; s->G = Hq / Hk; s->D = D;
     s->TPT = (kTileRows / s->G) & ~3;
-    return FSA_OK;
+    // (places in the kernels' lists of tiles)
+    return (biased_places(N, s->TPT, B) * Hk >= kBiasedMaxPlaces) ? FSA_ERR_UNSUPPORTED : FSA_OK;
 }
 
 static bool aligned16(const void* p) { return ((uintptr_t)p & 15) == 0; }
@@ -358,7 +359,7 @@ extern "C" int fsa_biased_attn_fwd(const void* q, const void* k, const void* v, 
         l.ml = (float2*)((char*)scratch + align_up(N * Hq * cut.nchunk * D * 4, 256));
         l.P = l.nchunk = cut.nchunk;
     }
-    e = launch_biased_fwd(D, dtype, which, cut.nchunk > 1, l, (int)((N + s.TPT - 1) / s.TPT) + B, stream);
+    e = launch_biased_fwd(D, dtype, which, cut.nchunk > 1, l, (int)biased_places(N, s.TPT, B), stream);
     if (e == cudaSuccess && cut.nchunk > 1)     // (tokens outside the sequences have no partials)
         e = launch_biased_merge(D, dtype, BiasedMerge{l.o_part, l.ml, N * Hq, Hq, cut.nchunk, cut.nchunk, cu_seqlens_q, B, o, lse, 1, N}, stream);
     return e == cudaSuccess ? FSA_OK : cuda_failed(e);

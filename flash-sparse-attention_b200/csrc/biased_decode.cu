@@ -440,6 +440,7 @@ extern "C" int fsa_biased_decode_bytes(int batch, int num_q_heads, int num_kv_he
         return FSA_ERR_BAD_ARG;
     const int G = num_q_heads / num_kv_heads;
     if ((head_dim != 64 && head_dim != 128) || G > 32 || max_len >= ((int64_t)1 << 30) || max_shared >= kMaxTokens) return FSA_ERR_UNSUPPORTED;
+    if (biased_places(batch, (kTileRows / G) & ~3, num_groups) * num_kv_heads >= kBiasedMaxPlaces) return FSA_ERR_UNSUPPORTED;
     const DecodeCut cut(batch, num_kv_heads, G, (kTileRows / G) & ~3, num_groups, max_len, max_shared, window);
     const int64_t rows = (int64_t)batch * num_q_heads * cut.partials();
     *bytes_out = align_up(rows * head_dim * 4, 256) + align_up(rows * 8, 256);

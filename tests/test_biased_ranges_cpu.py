@@ -36,3 +36,13 @@ def test_scales_that_leave_32_bits(scale):
         biased_attention(x, x, x, torch.tensor([0, 4], dtype=torch.int32), sm_scale=scale)
     with pytest.raises(ValueError, match="sm_scale"):
         biased_decode_attention(x, x, x, torch.ones(4, dtype=torch.int32), torch.zeros(4, dtype=torch.int32), max_len=4, sm_scale=scale)
+
+
+@pytest.mark.parametrize("batch,kv_heads,fits", [(1 << 20, 8, True), (1 << 24, 64, False), (1 << 24, 256, False), (1 << 23, 127, True)])
+def test_more_places_than_a_grid_has(batch, kv_heads, fits):
+    """Sequences without tokens take a place in the list of tiles too: their number times the kv heads stays in 32 bits."""
+    out = ctypes.c_int64(-7)
+    want = 0 if fits else FSA_ERR_UNSUPPORTED
+    for size in (lib().fsa_biased_attn_fwd_bytes, lib().fsa_biased_attn_bwd_bytes):
+        assert size(5, 1000, batch, kv_heads, kv_heads, 64, -1, ctypes.byref(out)) == want
+    assert lib().fsa_biased_decode_bytes(4, kv_heads, kv_heads, 64, batch, 100, 100, -1, ctypes.byref(out)) == want
