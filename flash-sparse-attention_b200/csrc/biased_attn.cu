@@ -414,7 +414,14 @@ extern "C" int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, 
     ScoreMod mod;
     int which;
     if ((rc = biased_mod(sm_scale, softcap, slopes, doc_ids, prefix_lens != nullptr, &mod, &which))) return rc;
-    if (N == 0) return FSA_OK;
+    if (N == 0) {           // nobody sees the keys
+        if (Nk > 0 && (!dk || !dv)) return FSA_ERR_BAD_ARG;
+        (void)cudaGetLastError();
+        cudaError_t e = cudaSuccess;
+        for (void* x : {dk, dv})
+            if (e == cudaSuccess && Nk > 0) e = cudaMemsetAsync(x, 0, (size_t)(Nk * Hk * D * 2), (cudaStream_t)stream_);
+        return e == cudaSuccess ? FSA_OK : cuda_failed(e);
+    }
     if (!q || !k || !v || !o || !lse || !d_o || !cu_seqlens_q || !cu_seqlens_k || !dq || !dk || !dv || !limits || !scratch || Nk == 0) return FSA_ERR_BAD_ARG;
     for (const void* x : {q, k, v, o, d_o, (const void*)dq, (const void*)dk, (const void*)dv, (const void*)limits, (const void*)scratch})
         if (!aligned16(x)) return FSA_ERR_BAD_ARG;

@@ -214,7 +214,8 @@ int fsa_range_attn_bwd_indexed(int head_dim);
  * rows that no token sees, and q and d_o rows of tokens that see nothing, may hold anything, NaN included; NaN or +infinity among the scores of
  * what a token sees gives NaN in its o and lse, and in the gradients that it has a share in.  limits: workspace of
  * fsa_biased_attn_limits_bytes bytes, kept for the backward.  scratch: 32-byte aligned, of fsa_biased_attn_fwd_bytes bytes for the same sizes (0: none).
- * head_dim 64 or 128, up to 32 query heads a kv head, fewer than 2^25 tokens and K/V rows, N * num_q_heads below 2^31. */
+ * head_dim 64 or 128, up to 32 query heads a kv head, fewer than 2^25 tokens and K/V rows (one of these at least where there are tokens), N * num_q_heads
+ * below 2^31. */
 int fsa_biased_attn_limits_bytes(int64_t total_tokens, int64_t* bytes_out);
 int fsa_biased_attn_fwd_bytes(int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window,
                               int64_t* bytes_out);
@@ -241,7 +242,7 @@ int fsa_biased_decode(const void* q, const void* k, const void* v, int64_t kv_ro
 int fsa_biased_read_status(int* status_out);
 /* For tests: a kernel whose wait runs out after 0.2 s (3 ms up to two seconds after another one that did), on the same status word. */
 int fsa_biased_debug_wait_timeout(void* stream);
-/* fsa_biased_attn_fwd's gradient.  dq, dk, dv contiguous; every row of them is written.  limits: what the forward left.  Bit-reproducible. */
+/* fsa_biased_attn_fwd's gradient.  dq, dk, dv contiguous; every row of them is written (without tokens too: dk and dv are 0).  limits: what the forward left.  Bit-reproducible. */
 int fsa_biased_attn_bwd_bytes(int64_t total_tokens, int64_t total_kv_rows, int batch, int num_q_heads, int num_kv_heads, int head_dim, int window,
                               int64_t* bytes_out);
 int fsa_biased_attn_bwd(const void* q, const void* k, const void* v, const void* o, const float* lse, const void* d_o, const int32_t* cu_seqlens_q,

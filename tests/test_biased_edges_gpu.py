@@ -257,3 +257,16 @@ def test_second_derivatives_are_refused():
         with pytest.raises(RuntimeError, match="no second derivative"):
             torch.autograd.grad(got[i].float().square().sum() + sum(x.float().sum() for x in leaves), leaves, retain_graph=True)
     torch.autograd.grad(first(retain_graph=True)[0].float().sum() + leaves[0].float().sum(), leaves[0])
+
+
+def test_backward_without_tokens_writes_dk_and_dv():
+    """Through the C ABI: keys that no token is there to see."""
+    from fsa import _lib
+
+    cu = torch.zeros(2, dtype=torch.int32, device=DEV)
+    dk, dv = (torch.full((50, 2, 64), math.nan, dtype=BF16, device=DEV) for _ in range(2))
+    none, p = None, _lib.ptr
+    args = [none] * 6 + [p(cu), p(cu)] + [none] * 3 + [0, 50, 1, 4, 2, 64, _lib.DTYPE_CODE[BF16], 256, 64, 128, 128, 256, 64, 0.1, 0.0, -1, none, p(dk), p(dv)]
+    args += [none, 0, none, 0, _lib.current_stream(torch.device(DEV))]
+    assert _lib.lib().fsa_biased_attn_bwd(*args) == 0
+    assert bool((dk == 0).all()) and bool((dv == 0).all())
