@@ -194,10 +194,11 @@ __global__ void __launch_bounds__(kPrThreads) biased_prep(const BiasedPrep p) {
     }
     const int64_t ctas = gridDim.x - 1, me = (int64_t)(blockIdx.x - 1) * kPrThreads + tid, all = ctas * kPrThreads;
     const int64_t row16 = (int64_t)p.plan.Hk * L, qrow16 = (int64_t)p.Hq * L;
+    const int k_first = __ldcg(p.plan.cu_k), k_end = __ldcg(p.plan.cu_k + B), q_end = __ldcg(p.plan.cu_q + B);
     if (!p.docs) {
         for (int64_t n = me; n < N; n += all) {
             Sees x = {0, -1, 0};
-            if (n < __ldcg(p.plan.cu_q + B)) {
+            if (n < q_end) {
                 const int seq = find_seq<true>(p.plan.cu_q, B, (int)n);
                 x = place_limits((int)n, __ldcg(p.plan.cu_k + seq), __ldcg(p.plan.cu_k + seq + 1), __ldcg(p.plan.cu_q + seq + 1), p.window,
                                  p.prefix_lens ? __ldcg(p.prefix_lens + seq) : 0);
@@ -206,11 +207,11 @@ __global__ void __launch_bounds__(kPrThreads) biased_prep(const BiasedPrep p) {
             p.lim.hi[n] = x.hi;
             p.lim.pos[n] = x.pos;
         }
-        for (int64_t i = (int64_t)__ldcg(p.plan.cu_k + B) * row16 + me; i < p.plan.Nk * row16; i += all) p.dk[i] = p.dv[i] = make_uint4(0u, 0u, 0u, 0u);
+        for (int64_t i = k_end * row16 + me; i < p.plan.Nk * row16; i += all) p.dk[i] = p.dv[i] = make_uint4(0u, 0u, 0u, 0u);
     }
     // (K/V rows in front of the first sequence: where cu_seqlens_k is a part of a longer one)
-    for (int64_t i = me; i < (int64_t)__ldcg(p.plan.cu_k) * row16; i += all) p.dk[i] = p.dv[i] = make_uint4(0u, 0u, 0u, 0u);
-    for (int64_t i = (int64_t)__ldcg(p.plan.cu_q + B) * qrow16 + me; i < N * qrow16; i += all) p.dq[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int64_t i = me; i < k_first * row16; i += all) p.dk[i] = p.dv[i] = make_uint4(0u, 0u, 0u, 0u);
+    for (int64_t i = q_end * qrow16 + me; i < N * qrow16; i += all) p.dq[i] = make_uint4(0u, 0u, 0u, 0u);
     // delta: L lanes a row of one head, U rows of a thread in flight
     const int part = tid % L;
     const uint32_t rows = (uint32_t)(N * p.Hq);

@@ -96,10 +96,10 @@ template <int D, typename ET>
 __global__ void __launch_bounds__(256) range_dkdv_reduce(const RangeKvPlan p, const float4* __restrict__ slabs, ET* __restrict__ dk, ET* __restrict__ dv) {
     follow();
     constexpr int kChunks = D / 8, kParts = 2 * kChunks * 128 / 256;
-    const int64_t units = (int64_t)__ldcg(p.counts + 1) * p.Hk * kParts;       // 2 x kChunks x 128 chunks of 8 columns per tile and head, 256 a CTA
+    const int64_t units = (int64_t)p.counts[1] * p.Hk * kParts;       // 2 x kChunks x 128 chunks of 8 columns per tile and head, 256 a CTA
     for (int64_t w = blockIdx.x; w < units; w += gridDim.x) {
         const int part = (int)(w % kParts), h = (int)(w / kParts % p.Hk);
-        const int4 m = __ldcg(p.multi + w / kParts / p.Hk);
+        const int4 m = p.multi[w / kParts / p.Hk];
         const int u = part * 256 + threadIdx.x, key = u & 127, chunk = (u >> 7) % kChunks, which = (u >> 7) / kChunks;
         if (key >= m.y) continue;
         float acc[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};
