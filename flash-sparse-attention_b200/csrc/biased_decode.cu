@@ -83,7 +83,7 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
     __syncthreads();
     const uint32_t sbase = smem_u32(base);
     float acc[NO][4];
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+    float m0 = -FLT_MAX, m1 = -FLT_MAX, l0 = 0.f, l1 = 0.f;      // (not -inf: as long as all scores of a row are that, every p is exp2(-inf) = 0)
 
     if (warp == 4) {
         if (elect_one()) {
@@ -175,10 +175,8 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
                     tmax1 = fmaxf(tmax1, __shfl_xor_sync(0xffffffffu, tmax1, 2));
                 }
                 const float mn0 = fmaxf(m0, tmax0), mn1 = HI ? fmaxf(m1, tmax1) : m1;
-                // (as long as all scores of a row are -inf, every p is exp2(-inf - 0) = 0)
-                const float u0 = mn0 == -INFINITY ? 0.f : mn0, u1 = HI && mn1 != -INFINITY ? mn1 : 0.f;
                 if (__any_sync(0xffffffffu, mn0 > m0 || (HI && mn1 > m1))) {
-                    const float a0 = ex2_approx(m0 - u0), a1 = HI ? ex2_approx(m1 - u1) : 1.f;
+                    const float a0 = ex2_approx(m0 - mn0), a1 = HI ? ex2_approx(m1 - mn1) : 1.f;
                     l0 *= a0;
                     l1 *= a1;
 #pragma unroll
@@ -191,12 +189,12 @@ __global__ void __launch_bounds__(kBdThreads) biased_decode_partial(const Biased
                 }
                 uint32_t pa[4];
                 {
-                    const float e00 = ex2_approx(sc[0][0] - u0), e01 = ex2_approx(sc[0][1] - u0), e10 = ex2_approx(sc[1][0] - u0), e11 = ex2_approx(sc[1][1] - u0);
+                    const float e00 = ex2_approx(sc[0][0] - m0), e01 = ex2_approx(sc[0][1] - m0), e10 = ex2_approx(sc[1][0] - m0), e11 = ex2_approx(sc[1][1] - m0);
                     l0 += e00 + e01 + e10 + e11;
                     pa[0] = ElemTraits<ET>::pack2(e00, e01);
                     pa[2] = ElemTraits<ET>::pack2(e10, e11);
                     if (HI) {
-                        const float f00 = ex2_approx(sc[0][2] - u1), f01 = ex2_approx(sc[0][3] - u1), f10 = ex2_approx(sc[1][2] - u1), f11 = ex2_approx(sc[1][3] - u1);
+                        const float f00 = ex2_approx(sc[0][2] - m1), f01 = ex2_approx(sc[0][3] - m1), f10 = ex2_approx(sc[1][2] - m1), f11 = ex2_approx(sc[1][3] - m1);
                         l1 += f00 + f01 + f10 + f11;
                         pa[1] = ElemTraits<ET>::pack2(f00, f01);
                         pa[3] = ElemTraits<ET>::pack2(f10, f11);

@@ -124,7 +124,7 @@ def test_what_is_seen_and_not_a_number(lens, klens, at, d, dtype, cap, alibi, ba
 
 @pytest.mark.parametrize("bad", [math.nan, math.inf])
 @pytest.mark.parametrize("cap,alibi", SCORES_OF)
-@pytest.mark.parametrize("where", ["own", "prefix", "q"])
+@pytest.mark.parametrize("where", ["own", "many", "prefix", "q"])
 def test_decode_of_what_is_not_a_number(where, cap, alibi, bad):
     Hk, G, d, P = 2, 4, 128, 200
     lens = [700, 1, 130]
@@ -133,6 +133,8 @@ def test_decode_of_what_is_not_a_number(where, cap, alibi, bad):
     pk, pv = (torch.randn(P, Hk, d, generator=g).to(BF16) for _ in range(2))
     if where == "own":
         k[row0[0] + 400, 1, 5] = bad
+    elif where == "many":                   # all keys of some warps and chunks: with infinity, scores of -infinity for the heads whose q is negative there
+        k[row0[0] + 100 : row0[0] + 690, 1, 5] = bad
     elif where == "prefix":
         pk[77, 1, 5] = bad
     elif bad == bad:
