@@ -10,7 +10,7 @@
 //   warps 4..19  one K/V row per thread and a quarter of the tile's rows: P and dS; epilogue: dV the first two groups, dK the others, half the
 //                columns each.
 // A tile's products read 256 KB of shared memory and its loads write 64 KB, 2560 cycles (D = 128); sixteen row warps instead of eight, because with
-// eight the capped scores took 4050 cycles and a distance bias 3860.  2 x 8192 tokens, 8 / 4 heads of 128, capped: 568 us (968 TFLOP/s of the four
+// eight the capped scores took 4050 cycles and a distance bias 3860.  2 x 8192 tokens, 8 / 4 heads of 128, capped: 529 us (1039 TFLOP/s of the four
 // products), the tensor cores' queue 72 % busy, issue 53 %.
 #include "../../include/fsa_sm100.h"
 

@@ -12,7 +12,7 @@
 // The left operand of every product comes from TMEM (in shared memory it would be read at every tile, 48 KB a product of 256 cycles).  The products
 // take 768 cycles a tile at D = 128, exp2 512.  What bounds the tile is the row threads' chain of loads, arithmetic and stores: with eight row warps in
 // step on one tile (range_dense.cu) it takes 1540 cycles, capped 1990; sixteen on two tiles hide one another's latencies.  2 x 8192 tokens, 8 / 4 heads of
-// 128, capped: 401 us (1028 TFLOP/s of the three products); the tensor cores 51 % busy, issue 52 % before the items went forth and back.
+// 128, capped: 397 us (1039 TFLOP/s of the three products); the tensor cores 51 % busy, issue 52 % before the items went forth and back.
 #include "../../include/fsa_sm100.h"
 #include <climits>
 

@@ -8,13 +8,13 @@
 //   warp 0      finds the items (cluster launch control: a running CTA takes over those whose CTA has not started); TMA producer
 //   warp 1      one elected thread issues S = Q K^T of the next K/V tile into the other of two TMEM buffers, then O (+)= P V of this one
 //   warps 2..5  one row per thread: changed scores, running maximum and sum, P -> TMEM over S; epilogue
-// (S of two K/V tiles at a time, N = 128, reads Q from shared memory half as often, but waits for two tiles: 314 us for what takes 280, capped.)
+// (S of two K/V tiles at a time, N = 128, reads Q from shared memory half as often, but waits for two tiles: 314 us for what takes 281, capped.)
 // The row threads do their arithmetic in one pass over a tile: it takes the rows' references for given and the tanh's arguments for near,
 // so that the polynomial and the sums run under the exp2 (16 a cycle and SM, 512 cycles a tile, like the products).  What it assumed is looked
 // at afterwards; where it does not hold (a row's first tile, a maximum far above the reference, scores near the cap, keys that some row
 // does not see) the tile takes three passes: scores, maximum, exp2.  The nearest tile comes first because a distance bias sets the reference
-// there (furthest first, every tile raised it: 676 us for what now takes 245).
-// 2 x 8192 tokens, 8 / 4 heads of 128: 237 us plain, 279 capped (985 TFLOP/s), 245 with a distance bias, 280 with both.  Capped, the tensor cores' queue
+// there (furthest first, every tile raised it: 676 us for what now takes 248).
+// 2 x 8192 tokens, 8 / 4 heads of 128: 240 us plain, 281 capped (978 TFLOP/s), 248 with a distance bias, 299 with both.  Capped, the tensor cores' queue
 // is 64 % busy, exp2 49 %, issue 49 %: two row warps a scheduler do not hide each other's loads from TMEM and chains of arithmetic altogether.
 #include "../../include/fsa_sm100.h"
 #include <climits>
