@@ -122,6 +122,9 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
         mbar_init(dq_free, kBqRows); mbar_init(qt_full, kBqRows);
         mbar_init_fence();
     }
+    // rows past G * TPT of the Q and dO tiles are never loaded, but have a part in their warp's choice of a tanh (biased_fwd.cu)
+    for (int i = p.G * p.TPT * 8 + tid; i < kTileRows * 8; i += kBqThreads)
+        for (int b = 0; b < KH; ++b) reinterpret_cast<uint4*>(sQ + b * (kTileRows * 128))[i] = reinterpret_cast<uint4*>(sDO + b * (kTileRows * 128))[i] = make_uint4(0u, 0u, 0u, 0u);
     if (warp == 0) tmem_alloc(&tmem_slot, kCols);
     tc_fence_before();
     __syncthreads();

@@ -108,6 +108,11 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
         __syncwarp();
         asm volatile("bar.arrive 2, 192;" ::: "memory");
     } else {
+        // Rows past G * TPT of the Q tile are never loaded, and their scores go nowhere; but they have a part in their warp's choice of the way through a tile, and with
+        // what a kernel before left there the other rows' last bits changed from run to run.
+        for (int i = G * TPT * 8 + tid - 32; i < kTileRows * 8; i += kBfThreads - 32)
+            for (int b = 0; b < KH; ++b) reinterpret_cast<uint4*>(sQ + b * kSlabQ)[i] = make_uint4(0u, 0u, 0u, 0u);
+        fence_async_smem();
         if (warp == 1) tmem_alloc(&tmem_slot, kCols);
         tc_fence_before();
         asm volatile("bar.sync 2, 192;" ::: "memory");

@@ -272,3 +272,35 @@ def test_backward_without_tokens_writes_dk_and_dv():
     args += [none, 0, none, 0, _lib.current_stream(torch.device(DEV))]
     assert _lib.lib().fsa_biased_attn_bwd(*args) == 0
     assert bool((dk == 0).all()) and bool((dv == 0).all())
+
+
+@pytest.mark.parametrize("G", [3, 7, 11, 31])
+@pytest.mark.parametrize("d", [64, 128])
+def test_the_same_bits_whatever_a_kernel_before_left(G, d):
+    """Groups whose heads do not fill a tile's 128 rows: what stands in the other rows' shared memory, zeros or numbers far above every cap, changes no bit."""
+    lens, P = [150, 33], 300
+    q, k, v, do = (x.to(DEV) for x in inputs(lens, lens, 2, G, d, BF16, G))
+    cu, sl = cu_of(lens).to(DEV), slopes_of(2 * G).to(DEV)
+    big = [torch.ones(9000, h, d, dtype=BF16, device=DEV) for h in (4, 1, 1, 4)]
+    n, pre = i32([2, 5, 1, 9]), [k[:P], v[:P], i32([0, 150, 183]), i32([0, 3, 4])]
+    k2, v2 = (x.repeat(2, 1, 1) for x in (k, v))
+    r0 = i32([0, 10, 20, 30])
+
+    def fill(value):
+        """Every SM's shared memory, by the same kernels on tiles that are full."""
+        leaves = [(x * value).requires_grad_() for x in big[:3]]
+        o, _ = biased_attention(*leaves, i32([0, 9000]), softcap=5.0)
+        torch.autograd.grad(o, leaves, big[3] * value)
+
+    def run(cap, alibi):
+        leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+        o, lse = biased_attention(*leaves, cu, softcap=cap, alibi_slopes=sl if alibi else None)
+        return [o.detach(), lse, *torch.autograd.grad(o, leaves, do),
+                *shared_prefix_decode_attention(q[:4], k2, v2, n, r0, *pre, max_len=9, softcap=cap, alibi_slopes=sl if alibi else None)]
+
+    for cap, alibi in SCORES_OF:
+        fill(0.0)
+        want = run(cap, alibi)
+        for value in (1e3, -1e3):
+            fill(value)
+            assert all(torch.equal(a, b) for a, b in zip(want, run(cap, alibi))), (cap, alibi, value)
