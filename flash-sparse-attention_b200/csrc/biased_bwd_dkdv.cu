@@ -386,7 +386,8 @@ __global__ void __launch_bounds__(kBkThreads, 1) biased_bwd_dkdv(const BiasedKvP
                             big[0] = max3_abs(big[0], __uint_as_float(v[j]), __uint_as_float(v[j + 1]));
                             big[1] = max3_abs(big[1], __uint_as_float(v[j + 2]), __uint_as_float(v[j + 3]));
                         }
-                        is_far = __any_sync(0xffffffffu, !(fmaxf(big[0], big[1]) <= p.mod.near_v));
+                        // (what decides: scores of tokens with keys that they see, as in the forward; a K/V row past the item's may be another sequence's or nobody's)
+                        is_far = masked || __any_sync(0xffffffffu, key < m.nkeys && !(fmaxf(big[0], big[1]) <= p.mod.near_v));
                     }
                     if (!is_far) {
                         pairs(Flag<kCap>{});

@@ -12,7 +12,7 @@
 // The left operand of every product comes from TMEM (in shared memory it would be read at every tile, 48 KB a product of 256 cycles).  The products
 // take 768 cycles a tile at D = 128, exp2 512.  What bounds the tile is the row threads' chain of loads, arithmetic and stores: with eight row warps in
 // step on one tile (range_dense.cu) it takes 1540 cycles, capped 1990; sixteen on two tiles hide one another's latencies.  2 x 8192 tokens, 8 / 4 heads of
-// 128, capped: 397 us (1039 TFLOP/s of the three products); the tensor cores 51 % busy, issue 52 % before the items went forth and back.
+// 128, capped: 392 us (1051 TFLOP/s of the three products); the tensor cores 51 % busy, issue 52 % before the items went forth and back.
 #include "../../include/fsa_sm100.h"
 #include <climits>
 
@@ -308,7 +308,7 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
         // This row's numbers, loaded an item ahead.
         struct Row { int lo, hi; float lse, delta, slope; int pos; };
         auto load_numbers = [&](const BqItem& m) {
-            Row x = {0, -1, 0.f, 0.f, 0.f, 0};
+            Row x = {0, INT_MAX, 0.f, 0.f, 0.f, INT_MAX};       // (a place without a token sees everything: its row goes nowhere)
             if (g < p.G && e < m.ne) {
                 x.lo = __ldcg(p.kv_lo + m.tok0 + e);
                 x.hi = __ldcg(p.kv_hi + m.tok0 + e);
@@ -393,7 +393,8 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
                     };
                     const bool both = (MOD & kModBias) && p.mod.ahead && __any_sync(0xffffffffu, hi_r > pos_r);
                     constexpr bool kCap = (MOD & kModCap) != 0;
-                    bool is_far = both;
+                    // (what decides: scores of tokens with keys that they see, as in the forward)
+                    bool is_far = both || (kCap && !all_visible);
                     if constexpr (kCap) {       // (before, not afterwards as in the forward: the products would have to be kept beside the dS)
                         float big[2] = {0.f, 0.f};
 #pragma unroll
@@ -401,11 +402,11 @@ __global__ void __launch_bounds__(kBqThreads, 1) biased_bwd_dq(const BiasedDqPar
                             big[0] = max3_abs(big[0], __uint_as_float(sv[i]), __uint_as_float(sv[i + 1]));
                             big[1] = max3_abs(big[1], __uint_as_float(sv[i + 2]), __uint_as_float(sv[i + 3]));
                         }
-                        is_far |= __any_sync(0xffffffffu, !(fmaxf(big[0], big[1]) <= p.mod.near_v));
+                        is_far |= __any_sync(0xffffffffu, row_valid && !(fmaxf(big[0], big[1]) <= p.mod.near_v));
                     }
                     if (!is_far) {
-                        if (all_visible) pairs(Flag<kCap>{}, Flag<false>{}, Flag<true>{});
-                        else pairs(Flag<kCap>{}, Flag<false>{}, Flag<false>{});
+                        if (kCap || all_visible) pairs(Flag<kCap>{}, Flag<false>{}, Flag<true>{});
+                        else pairs(Flag<false>{}, Flag<false>{}, Flag<false>{});
                     } else {
                         if constexpr (kCap) cap_scores(sv, p.mod.x_scale, p.mod.near_v);
                         if (both) pairs(Flag<false>{}, Flag<true>{}, Flag<false>{});

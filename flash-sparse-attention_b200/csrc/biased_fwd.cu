@@ -8,13 +8,13 @@
 //   warp 0      finds the items (cluster launch control: a running CTA takes over those whose CTA has not started); TMA producer
 //   warp 1      one elected thread issues S = Q K^T of the next K/V tile into the other of two TMEM buffers, then O (+)= P V of this one
 //   warps 2..5  one row per thread: changed scores, running maximum and sum, P -> TMEM over S; epilogue
-// (S of two K/V tiles at a time, N = 128, reads Q from shared memory half as often, but waits for two tiles: 314 us for what takes 281, capped.)
+// (S of two K/V tiles at a time, N = 128, reads Q from shared memory half as often, but waits for two tiles: 314 us for what takes 282, capped.)
 // The row threads do their arithmetic in one pass over a tile: it takes the rows' references for given and the tanh's arguments for near,
 // so that the polynomial and the sums run under the exp2 (16 a cycle and SM, 512 cycles a tile, like the products).  What it assumed is looked
 // at afterwards; where it does not hold (a row's first tile, a maximum far above the reference, scores near the cap, keys that some row
 // does not see) the tile takes three passes: scores, maximum, exp2.  The nearest tile comes first because a distance bias sets the reference
 // there (furthest first, every tile raised it: 676 us for what now takes 248).
-// 2 x 8192 tokens, 8 / 4 heads of 128: 240 us plain, 281 capped (978 TFLOP/s), 248 with a distance bias, 299 with both.  Capped, the tensor cores' queue
+// 2 x 8192 tokens, 8 / 4 heads of 128: 240 us plain, 282 capped (975 TFLOP/s), 248 with a distance bias, 299 with both.  Capped, the tensor cores' queue
 // is 64 % busy, exp2 49 %, issue 49 %: two row warps a scheduler do not hide each other's loads from TMEM and chains of arithmetic altogether.
 #include "../../include/fsa_sm100.h"
 #include <climits>
@@ -333,7 +333,9 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
             const float slope_r = row.slope;
             const int pos_r = row.pos - m.row_lo;
             const int nblk = m.nblk;
-            float m_ref = -INFINITY, l_run = 0.f;
+            // What decides on a warp's way through a tile, and with it on last bits, are scores of its tokens with keys that they see: not those of places without
+            // a token, whose reference is infinite, and none of a tile that is not seen whole (rows of other sequences or of none, which may hold anything).
+            float m_ref = g < G && e < m.ne ? -INFINITY : INFINITY, l_run = 0.f;
             // tiles that all rows of the warp see whole (and none of them behind a token's place): [whole_lo, whole_hi]
             const int whole_lo = __reduce_max_sync(0xffffffffu, (max(lo_r, 0) + BK - 1) / BK);
             const int whole_hi = __reduce_min_sync(0xffffffffu, (((MOD & kModBias) && launch.mod.ahead ? min(hi_r, pos_r) : hi_r) + 1 >> 6) - 1);
@@ -371,12 +373,12 @@ __global__ void __launch_bounds__(kBfThreads, 2) biased_fwd(const __grid_constan
                         top[(i >> 1) & 1] = max3(top[(i >> 1) & 1], y.x, y.y);
                         two(i, x);
                     }
-                    passes = __any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) <= kBfLazy<ET>) || ((MOD & kModCap) && !(fmaxf(big[0], big[1]) <= launch.mod.near_v)) || !ok);
+                    passes = __any_sync(0xffffffffu, !(fmaxf(top[0], top[1]) <= kBfLazy<ET>) || ((MOD & kModCap) && !(fmaxf(big[0], big[1]) <= launch.mod.near_v) && m_ref < INFINITY) || !ok);
                 }
                 if (passes) {
                     if (!warp_stays(ok)) break;
                     const int c_lo = max(0, lo_r - t * BK), c_hi = min(BK, hi_r - t * BK + 1);      // visible columns [c_lo, c_hi)
-                    if constexpr (MOD & kModCap) far = cap_scores(v, launch.mod.x_scale, launch.mod.near_v);
+                    if constexpr (MOD & kModCap) far = cap_scores(v, launch.mod.x_scale, launch.mod.near_v, m_ref < INFINITY) && t >= whole_lo && t <= whole_hi;
                     if constexpr (MOD & kModBias)
                         bias_scores(v, to_log2, slope_r, rel, launch.mod.ahead && __any_sync(0xffffffffu, t * BK + c_hi - 1 > pos_r));
                     if (c_lo > 0 || c_hi < BK) {

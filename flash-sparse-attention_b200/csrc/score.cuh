@@ -43,7 +43,7 @@ __device__ __forceinline__ float rcp_approx(float x) {
 __device__ __forceinline__ float tanh_far(float v, float k) { return fmaf(-2.f, rcp_approx(1.f + ex2_approx(v * k)), 1.f); }
 
 // tanh_near: of two values no larger than 3/4; cap_scores: v <- tanh(x_scale v), N scores of a row (all lanes of a warp
-// call it; whether some |v| was above near_v).  The special-function unit gives 16 results a cycle and SM, and the
+// call it; whether some |v| of the lanes that count was above near_v).  The special-function unit gives 16 results a cycle and SM, and the
 // softmax needs one for each score already; with two more the capped forward would be bound by it, three times as long as its products.
 // Where no |x| of the warp's 32 rows is above 3/4 (scores below 37 at a cap of 50), tanh(x) = x p(x^2) with p of degree 4: the
 // polynomial that is nearest to tanh(x) / x on [0, 9/16] in relative error, 6e-7 (fitted on Chebyshev points); two scores an instruction.  In other
@@ -58,7 +58,7 @@ __device__ __forceinline__ uint64_t tanh_near(uint64_t x) {
     return mul_f32x2(x, p);
 }
 template <int N>
-__device__ __forceinline__ bool cap_scores(uint32_t (&v)[N], float x_scale, float near_v) {
+__device__ __forceinline__ bool cap_scores(uint32_t (&v)[N], float x_scale, float near_v, bool counts = true) {
     float a[2] = {0.f, 0.f};
 #pragma unroll
     for (int i = 0; i < N; i += 4) {        // (a NaN stays out of a maximum: it is masked, or makes the row NaN either way)
@@ -85,7 +85,7 @@ __device__ __forceinline__ bool cap_scores(uint32_t (&v)[N], float x_scale, floa
             v[i + 1] = __float_as_uint(fabsf(x.y) <= kTanhNear ? t.y : tanh_far(b, k));
         }
     }
-    return __any_sync(0xffffffffu, most > near_v);
+    return __any_sync(0xffffffffu, counts && most > near_v);
 }
 
 // Of products no larger than near_v, half a cap: tanh(x_scale v) = v p(v^2), p of degree 3 with the scale in its coefficients (host: near_coefficients);

@@ -304,3 +304,37 @@ def test_the_same_bits_whatever_a_kernel_before_left(G, d):
         for value in (1e3, -1e3):
             fill(value)
             assert all(torch.equal(a, b) for a, b in zip(want, run(cap, alibi))), (cap, alibi, value)
+
+
+@pytest.mark.parametrize("G,d", [(2, 128), (3, 64), (1, 64)])
+@pytest.mark.parametrize("how", [{}, {"docs": True}, {"window": 70}])
+def test_the_same_bits_whatever_nobodys_rows_hold(G, d, how):
+    """Rows in front of, behind and (as padding) within the sequences: zeros, numbers far above every cap, NaN.  No bit of the others' results changes."""
+    lens, klens, front, behind = [150, 90, 33], [300, 90, 200], 77, 50
+    q, k, v, do = inputs(lens, klens, 2, G, d, BF16, 20 + G)
+    ids = None
+    if "docs" in how:
+        ids = torch.cat([torch.full((n,), i, dtype=torch.int32) for n, i in ((200, 1), (70, -1), (90, 2), (60, 3), (100, -2), (70, 4))])
+    sl, cu, cuk = slopes_of(2 * G).to(DEV), cu_of(lens).to(DEV), (cu_of(klens) + front).to(DEV)
+
+    def run(value, cap, alibi):
+        def pad(x, a, b):
+            y = torch.full((a + x.shape[0] + b, *x.shape[1:]), value, dtype=x.dtype)
+            y[a : a + x.shape[0]] = x
+            return y
+
+        kk, vv, qq, dd = pad(k, front, behind), pad(v, front, behind), pad(q, 0, behind), pad(do, 0, behind)
+        if ids is not None:
+            nobody = torch.nonzero(ids < 0)[:, 0]
+            kk[front + nobody], vv[front + nobody] = value, value
+            at = torch.cat([torch.arange(c, c + n) for c, n in ((150, 150), (300, 90), (557, 33))])       # keys at which the tokens stand
+            qq[: len(at)][ids[at] < 0], dd[: len(at)][ids[at] < 0] = value, value
+        leaves = [x.to(DEV).requires_grad_() for x in (qq, kk, vv)]
+        docs = None if ids is None else torch.cat([torch.zeros(front, dtype=torch.int32), ids, torch.zeros(behind, dtype=torch.int32)]).to(DEV)
+        o, lse = biased_attention(*leaves, cu, cu_seqlens_k=cuk, softcap=cap, alibi_slopes=sl if alibi else None, doc_ids=docs, window_size=how.get("window"))
+        return [o.detach(), lse, *torch.autograd.grad(o, leaves, dd.to(DEV))]
+
+    for cap, alibi in SCORES_OF:
+        want = run(0.0, cap, alibi)
+        for value in (1e3, -1e4, math.nan):
+            assert all(torch.equal(a, b) for a, b in zip(want, run(value, cap, alibi))), (cap, alibi, value)
