@@ -338,3 +338,63 @@ def test_the_same_bits_whatever_nobodys_rows_hold(G, d, how):
         want = run(0.0, cap, alibi)
         for value in (1e3, -1e4, math.nan):
             assert all(torch.equal(a, b) for a, b in zip(want, run(value, cap, alibi))), (cap, alibi, value)
+
+
+@pytest.mark.parametrize("how", [{}, {"docs": True}, {"window": 50}, {"prefix": True}])
+def test_a_captured_step_with_other_lengths(how):
+    """Lengths, documents and prefixes are read on the device: a captured step is replayed with others, and gives what an eager one gives for them."""
+    n, B = 700, 3
+    q, k, v, do = (x.to(DEV) for x in inputs([n], [n], 2, 2, 64, BF16, 30))
+    cu, cuk, ids, prefix = i32([0, 300, 500, n]), i32([0, 300, 500, n]), i32([t // 90 for t in range(n)]), i32([10, 0, 50])
+    leaves = [x.requires_grad_() for x in (q, k, v)]
+
+    def step():
+        o, lse = biased_attention(*leaves, cu, cu_seqlens_k=cuk, softcap=30.0, doc_ids=ids if "docs" in how else None, window_size=how.get("window"),
+                                  prefix_lens=prefix if "prefix" in how else None)
+        return [o.detach(), lse, *torch.autograd.grad(o, leaves, do)]
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        held = step()
+    for lens, klens in (([1, 0, 600], [500, 100, 100]), ([0, 0, 0], [0, 0, 0]), ([233, 233, 234], [233, 233, 234]), ([700, 0, 0], [100, 300, 200])):
+        assert len(lens) == B
+        cu.copy_(cu_of(lens))
+        cuk.copy_(cu_of(klens))
+        ids.copy_(torch.div(torch.arange(n, dtype=torch.int32), 7 + lens[0] % 50, rounding_mode="floor").int() % 5 - 1)
+        prefix.copy_(torch.tensor([lens[0] // 2, -4, 1000], dtype=torch.int32))
+        graph.replay()
+        want = step()
+        assert all(torch.equal(a, b) for a, b in zip(held, want)), (lens, klens)
+
+
+def test_memory_that_calls_find_changes_no_bit():
+    """Workspaces and results lie where something else was: all bits set, or zeros."""
+    lens, klens = [400, 1, 90, 33], [900, 300, 90, 200]
+    q, k, v, do = (x.to(DEV) for x in inputs(lens, klens, 1, 4, 128, BF16, 31))
+    cu, cuk, ids = cu_of(lens).to(DEV), cu_of(klens).to(DEV), i32([t // 60 for t in range(sum(klens))])
+    n, r0, pre = i32([5, 0, 300, 1]), i32([0, 10, 400, 800]), [k[:260], v[:260], i32([0, 200, 260]), i32([1, 2, 3])]
+
+    def run():
+        out = []
+        for how in ({}, {"doc_ids": ids}, {"window_size": 100}):
+            leaves = [x.detach().requires_grad_() for x in (q, k, v)]
+            o, lse = biased_attention(*leaves, cu, cu_seqlens_k=cuk, softcap=30.0, **how)
+            out += [o.detach(), lse, *torch.autograd.grad(o, leaves, do)]
+        one = [x.detach().requires_grad_() for x in (q[:400, :1], k, v)]            # few items: o and dQ cut along the keys
+        o, lse = biased_attention(*one, i32([0, 400]), cu_seqlens_k=i32([0, sum(klens)]), softcap=30.0)
+        out += [o.detach(), lse, *torch.autograd.grad(o, one, do[:400, :1])]
+        out += biased_decode_attention(q[:4], k, v, n, r0, max_len=300)
+        return out + list(shared_prefix_decode_attention(q[:4], k, v, n, r0, *pre, max_len=300))
+
+    want = run()
+    for byte in (0, 255):
+        for size in [1 << i for i in range(9, 27)] * 3:
+            torch.full((size,), byte, dtype=torch.uint8, device=DEV)
+        held = [torch.full((size,), byte, dtype=torch.uint8, device=DEV) for size in [1 << i for i in range(9, 26)] * 4]
+        del held
+        assert all(torch.equal(a, b) for a, b in zip(want, run())), byte
